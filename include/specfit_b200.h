@@ -33,6 +33,7 @@
  *   sf_linear_bf16        F.linear (q|k|v, o, lm_head, drafter)  transformers/...:Qwen3MoeAttention.forward,
  *                                                               Qwen3MoeForCausalLM.forward (lm_head)
  *                                                               (candidate-pool expansion)
+ *   sf_kv8_*, sf_kv_keep_heaviest   (none: the reference keeps every key and value in bf16)
  */
 #ifndef SPECFIT_B200_H_
 #define SPECFIT_B200_H_
@@ -763,6 +764,92 @@ SF_API int sf_qk_norm_rope(const void* qkv, int64_t batch, int64_t tokens, int n
                            void* q_out, void* k_cache, void* v_cache, int64_t kv_batch_stride,
                            int64_t kv_head_stride, int64_t row0, const int64_t* row0_device,
                            void* stream);
+
+/*
+ * The 8-bit KV cache of a layer.  Keys and values of the first `sealed`
+ * tokens are e4m3 codes [batch, num_kv_heads, sealed, head_dim] (rows
+ * head_dim bytes apart) with one fp32 scale per block of `block_tokens`
+ * tokens and head; the `tail` rows after them are bf16 (rows head_dim
+ * elements apart).  Strides in elements.  scale = 2^e, e the least integer
+ * >= -100 with max |x| of the block <= 448 * 2^e, code = x / scale rounded to
+ * nearest even; a block that holds a NaN or an infinity has a NaN scale and
+ * zero codes.  head_dim: a multiple of 16 up to 128; block_tokens: 32, 64 or
+ * 128; codes and tails 16-byte aligned, their strides too.
+ */
+typedef struct sf_kv8_rows {
+  int batch, num_kv_heads, head_dim, block_tokens;
+  int64_t sealed, tail;
+  void *k_codes, *v_codes;
+  int64_t code_batch_stride, code_head_stride;
+  float *k_scale, *v_scale;
+  int64_t scale_batch_stride, scale_head_stride;
+  void *k_tail, *v_tail;
+  int64_t tail_batch_stride, tail_head_stride;
+} sf_kv8_rows;
+
+/*
+ * Seals `blocks` blocks of bf16 rows k, v [batch, num_kv_heads, blocks *
+ * block_tokens, head_dim] (strides in elements, multiples of 8) into the
+ * cache's blocks first_block, first_block + 1, ...; rows->sealed is the number
+ * of tokens its code buffers hold.
+ */
+SF_API int sf_kv8_seal(const void* k, const void* v, int64_t batch_stride, int64_t head_stride,
+                       int64_t row_stride, const sf_kv8_rows* rows, int64_t first_block, int64_t blocks,
+                       void* stream);
+/* Rows [first, first + count) of the cache as bf16 (exact), rows head_dim apart. */
+SF_API int sf_kv8_read(const sf_kv8_rows* rows, int64_t first, int64_t count, void* k_out, void* v_out,
+                       int64_t out_batch_stride, int64_t out_head_stride, void* stream);
+/*
+ * sf_tree_attention over an 8-bit cache, `rows->batch` requests in one call:
+ * q [batch, num_heads, q_len, head_dim] bf16; keys before prefix_len are
+ * visible to every row, key prefix_len + j to rows with bit j set in
+ * tree_bits [batch, q_len, bit_words].  out [batch, q_len, num_heads,
+ * head_dim] bf16; lse (nullable) [batch, num_heads, q_len]: the natural
+ * log-sum-exp of a row's scaled scores.  A row that sees no key answers zeros
+ * and -infinity.  A key with a NaN (or, in its value row, an infinity)
+ * answers NaN to the rows that see it and to no other.  workspace (16-byte
+ * aligned): sf_kv8_attention_workspace_bytes(...) bytes, 0 where one key range
+ * is enough.
+ */
+SF_API size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim,
+                                               int64_t q_len, int64_t kv_len);
+SF_API int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride,
+                                 int64_t q_row_stride, int num_heads, int64_t q_len, const sf_kv8_rows* rows,
+                                 const uint32_t* tree_bits, int bit_words, int64_t bits_batch_stride,
+                                 int64_t prefix_len, float scale, void* out, int64_t out_batch_stride,
+                                 float* lse, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * Adds to mass [batch, num_kv_heads, >= sealed + tail] (fp32) the attention
+ * weight that each cached token received in a pass: the sum over the query
+ * heads of its KV head and the rows that see it of exp(scale * q . k - lse),
+ * lse [batch, num_heads, q_len] as sf_kv8_tree_attention returned it.  Rows
+ * with lse -infinity add nothing.  Only the key side of `rows` is read.
+ */
+SF_API int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int64_t q_head_stride,
+                                 int64_t q_row_stride, int num_heads, int64_t q_len, const float* lse,
+                                 const sf_kv8_rows* rows, const uint32_t* tree_bits, int bit_words,
+                                 int64_t bits_batch_stride, int64_t prefix_len, float scale, float* mass,
+                                 int64_t mass_batch_stride, int64_t mass_head_stride, void* stream);
+/*
+ * The tokens an eviction keeps: keep [batch, num_kv_heads, budget] int32,
+ * ascending: the first `sinks`, the last `recent`, and the heaviest of the
+ * others by mass (ties: the earlier token; NaN: the least).
+ * sinks + recent <= budget <= length.
+ */
+SF_API int sf_kv_keep_heaviest(const float* mass, int64_t mass_batch_stride, int64_t mass_head_stride,
+                               int batch, int num_kv_heads, int64_t length, int64_t budget, int64_t sinks,
+                               int64_t recent, int32_t* keep, void* stream);
+/*
+ * Moves rows keep[b, h, 0 .. n) of `rows` into the cache `out` (buffers of its
+ * own; out->sealed = n / block_tokens * block_tokens, out->tail = the rest):
+ * whole blocks are sealed anew, the last n % block_tokens rows become its bf16
+ * tail.  mass / mass_out (nullable, both or neither): the kept tokens' mass
+ * moves along.  An index outside the cache moves a row of zeros.
+ */
+SF_API int sf_kv8_compact(const sf_kv8_rows* rows, const int32_t* keep, int64_t n, const sf_kv8_rows* out,
+                          const float* mass, int64_t mass_batch_stride, int64_t mass_head_stride,
+                          float* mass_out, int64_t mass_out_batch_stride, int64_t mass_out_head_stride,
+                          void* stream);
 
 #ifdef __cplusplus
 }

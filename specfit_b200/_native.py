@@ -96,6 +96,19 @@ class SfCacheFill(ctypes.Structure):
     _fields_ = [("expert", _i32), ("slot", _i32), ("generation", _u32), ("done", _i32),
                 ("submission", _i64), ("ready_event", _u64)]
 
+
+class Kv8RowsStruct(ctypes.Structure):
+    """``sf_kv8_rows`` (include/specfit_b200.h)."""
+
+    _fields_ = [("batch", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("block_tokens", _i32),
+                ("sealed", _i64), ("tail", _i64), ("k_codes", _vp), ("v_codes", _vp),
+                ("code_batch_stride", _i64), ("code_head_stride", _i64), ("k_scale", _vp), ("v_scale", _vp),
+                ("scale_batch_stride", _i64), ("scale_head_stride", _i64), ("k_tail", _vp), ("v_tail", _vp),
+                ("tail_batch_stride", _i64), ("tail_head_stride", _i64)]
+
+
+_kv8_p = ctypes.POINTER(Kv8RowsStruct)
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "sf_last_error": (ctypes.c_char_p, []),
@@ -197,6 +210,15 @@ SIGNATURES = {
     "sf_add_rmsnorm": (_i32, [_vp, _vp, _vp, _vp, _f32, _i64, _i32, _vp, _vp]),
     "sf_qk_norm_rope": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp,
                                _vp, _i64, _i64, _i64, _vp, _vp]),
+    "sf_kv8_seal": (_i32, [_vp, _vp, _i64, _i64, _i64, _kv8_p, _i64, _i64, _vp]),
+    "sf_kv8_read": (_i32, [_kv8_p, _i64, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "sf_kv8_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64, _i64]),
+    "sf_kv8_tree_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i64, _kv8_p, _vp, _i32, _i64, _i64, _f32, _vp,
+                                     _i64, _vp, _vp, _sz, _vp]),
+    "sf_kv8_attention_mass": (_i32, [_vp, _i64, _i64, _i64, _i32, _i64, _vp, _kv8_p, _vp, _i32, _i64, _i64, _f32,
+                                     _vp, _i64, _i64, _vp]),
+    "sf_kv_keep_heaviest": (_i32, [_vp, _i64, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "sf_kv8_compact": (_i32, [_kv8_p, _vp, _i64, _kv8_p, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
 }
 
 

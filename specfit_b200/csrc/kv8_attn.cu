@@ -1,0 +1,585 @@
+// Tree-masked GQA attention over the 8-bit KV cache: the warp-level kernel,
+// the merge of the key ranges, and the entry points.
+//
+//   s_rj = scale * q_r . k_j,  o_r = sum_j exp(s_rj - lse_r) v_j,  lse_r = ln sum_j exp(s_rj)
+//
+// over the keys j that row r sees (all before prefix_len, and those whose bit
+// is set).  A row that sees nothing answers zeros and lse = -infinity.
+//
+// The floor is one read of the codes (256 bytes a token and KV head at
+// D = 128).  With the query heads of one KV head packed into one 16-row MMA
+// tile (row = head_in_group * Tq + t) a few query rows need 2 MMAs per 8 keys
+// and 16 dims, far below the tensor rate, so what has to be kept small is the
+// work per element: loading, decoding, and the softmax.
+//   * Every warp walks its own 16-key units of the CTA's range with its own
+//     online softmax; the four warps and the splits are joined at the end.
+//     Nothing in the loop waits for another warp.
+//   * Dims of a key are a sum, keys of a value too, so both may be taken in
+//     any order: a thread's 16 consecutive code bytes ARE its MMA fragments
+//     (K: four k-steps of one key; V: one column of 16 output tiles).  Each
+//     thread copies exactly the bytes that it will use (cp.async, 16 bytes)
+//     into its own slots of a ring, so the loop needs no barrier, no
+//     transpose and no bank is hit twice.
+//   * Codes become fp16 (exact) by one conversion per two; Q as fp16 is exact
+//     too once each row is scaled by a power of two (fp16's 11 bits hold
+//     bf16's 8 over 30 binades below the row's largest; what is smaller is
+//     below 2^-30 of it).  K's scale multiplies the fp32 scores.
+//   * V's scale: the accumulators are kept in units of the largest V scale so
+//     far; probabilities are multiplied by (block scale / unit) <= 1, a power
+//     of two, so only values below 2^-37 of the row's largest are rounded
+//     more than fp16's 11 bits (probabilities are kept times 2^12).
+//   * The reference maximum of a row moves only when a score exceeds it by
+//     more than 3 (base 2), so accumulators are rarely rescaled.
+// Tail units (bf16 rows: few) are scaled by a power of two per unit and
+// enter the same fragments.  A value row with a NaN or an infinity makes its
+// key's score NaN, so that rows which do not see it stay what they are.
+#include <math.h>
+
+#include <algorithm>
+
+#include "kv8_attn.h"
+#include "kv8_mma.cuh"
+
+namespace sf {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kRows = 16;      // packed query rows of a CTA
+constexpr int kUnit = 16;      // keys of one step of a warp
+constexpr int kStages = 5;     // units in flight per warp
+constexpr int kStep = kWarps * kUnit;
+constexpr int kMaxSplits = 128;
+constexpr float kPShift = 12.f;  // probabilities are kept times 2^12
+constexpr float kSlack = 3.f;    // a row's reference maximum may lag by this (base 2)
+
+template <int DT>
+struct Layout {
+  static constexpr int kKChunks = DT / 64;             // 16-byte chunks of a key per thread
+  static constexpr int kVBytes = DT / 8;               // bytes of a value row per thread
+  static constexpr int kSteps = DT / 16;               // MMA k-steps of Q K^T
+  static constexpr int kTiles = DT / 8;                // output tiles of P V
+  static constexpr int kKBytes = 2 * kKChunks * 16;    // per thread and unit
+  static constexpr int kUnitBytes = 32 * (kKBytes + 4 * kVBytes);  // 16 keys: K and V codes
+  static constexpr int kRing = kWarps * kStages * kUnitBytes;
+  static constexpr int kJoin = kWarps * kRows * DT * 4;
+  static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+};
+
+// grid: (hkv, row tiles, splits * batch).
+template <int DT>
+__global__ void __launch_bounds__(kWarps * 32)
+kv8_attn_kernel(Kv8Attn p) {
+  using L = Layout<DT>;
+  pdl_wait();
+  pdl_trigger();
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float join_m[kWarps][kRows], join_l[kWarps][kRows];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const int kvh = blockIdx.x;
+  const int req = blockIdx.z / p.splits, split = blockIdx.z % p.splits;
+  const int key_lo = split * p.keys_per_split;
+  const int key_hi = min(p.kv_len, key_lo + p.keys_per_split);
+  const int packed = p.group * p.q_len;
+  const int sealed = (int)p.c.sealed;
+  const int d = p.c.d;
+
+  const uint8_t* kc = p.c.k + req * p.c.c_bs + kvh * p.c.c_hs;
+  const uint8_t* vc = p.c.v + req * p.c.c_bs + kvh * p.c.c_hs;
+  const float* ksc = p.c.ks + req * p.c.s_bs + kvh * p.c.s_hs;
+  const float* vsc = p.c.vs + req * p.c.s_bs + kvh * p.c.s_hs;
+  const __nv_bfloat16* kt = p.c.kt + req * p.c.t_bs + kvh * p.c.t_hs;
+  const __nv_bfloat16* vt = p.c.vt + req * p.c.t_bs + kvh * p.c.t_hs;
+
+  // Slots: [warp][stage][piece][lane], 16 (or 8) bytes each, written and read by one thread.
+  const uint32_t ring = smem_addr(smem) + (uint32_t)warp * kStages * L::kUnitBytes;
+  auto load_unit = [&](int key0, int stage) {
+    if (key0 < key_hi && key0 < sealed) {
+      const uint32_t at = ring + (uint32_t)stage * L::kUnitBytes;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < L::kKChunks; ++j) {
+          const int byte = j * 64 + c * 16;
+          const bool on = byte < d;
+          cp_async<16>(at + (uint32_t)((t * L::kKChunks + j) * 32 + lane) * 16,
+                       kc + (int64_t)(key0 + t * 8 + g) * d + (on ? byte : 0), on);
+        }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int key = key0 + 2 * c + (k & 1) + (k >> 1) * 8;
+        const int byte = g * L::kVBytes;
+        const bool on = byte < d;
+        cp_async<L::kVBytes>(at + 32 * L::kKBytes + (uint32_t)(k * 32 + lane) * L::kVBytes,
+                             vc + (int64_t)key * d + (on ? byte : 0), on);
+      }
+    }
+    cp_commit();
+  };
+
+  const int first = key_lo + warp * kUnit;
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) load_unit(first + s * kStep, s);
+
+  // Q fragments of rows g and g + 8: the dims of k-step (j, w) of this
+  // thread are j * 64 + c * 16 + w * 4 + {0, 1, 2, 3}.
+  uint32_t qf[L::kSteps][4];
+  float qs[2];                 // scale * log2(e) * (power of two taken out of the row)
+  const uint32_t* rbits[2];
+  bool rok[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int pr = blockIdx.y * kRows + g + r * 8;
+    rok[r] = pr < packed;
+    const int t = rok[r] ? pr % p.q_len : 0;
+    const int head = kvh * p.group + (rok[r] ? pr / p.q_len : 0);
+    rbits[r] = p.bits ? p.bits + req * p.bits_bs + (int64_t)t * p.words : nullptr;
+    const __nv_bfloat16* qrow = p.q + req * p.q_bs + head * p.q_hs + t * p.q_rs;
+    qs[r] = p.scale_log2 * q_row_fragments<L::kSteps>(rok[r] ? qrow : nullptr, d, c, qf, r);
+  }
+
+  float o[L::kTiles][4];
+#pragma unroll
+  for (int t = 0; t < L::kTiles; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[t][i] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float unit = 0.f;  // o is in units of this V scale
+
+  int stage = 0;
+  for (int key0 = first; key0 < key_hi; key0 += kStep) {
+    {
+      int ahead = stage + kStages - 1;
+      if (ahead >= kStages) ahead -= kStages;
+      load_unit(key0 + (kStages - 1) * kStep, ahead);
+    }
+    cp_wait<kStages - 1>();  // this thread's pieces of this unit have landed
+    const uint8_t* at = smem + (size_t)warp * kStages * L::kUnitBytes + (size_t)stage * L::kUnitBytes;
+    if (++stage == kStages) stage = 0;
+
+    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    uint32_t vf[4][L::kVBytes / 4];  // codes of four keys, or (tail) fp16 pairs built below
+    float kscale, vscale;
+    const bool coded = key0 < sealed;
+    uint32_t bad = 0;       // tail: bit k set when this thread's key k has a non-finite value
+    const uint2* tail_v[4];
+    bool tail_on[4];
+    float vinv = 1.f;
+    if (coded) {
+      kscale = ksc[key0 >> p.c.block_shift];
+      vscale = vsc[key0 >> p.c.block_shift];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < L::kKChunks; ++j) {
+          const uint4 w = *reinterpret_cast<const uint4*>(at + ((t * L::kKChunks + j) * 32 + lane) * 16);
+          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mma_f16(s[t], qf[j * 4 + i], e4m3x2_to_f16x2(ww[i]), e4m3x2_hi_to_f16x2(ww[i]));
+        }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint8_t* a = at + 32 * L::kKBytes + (k * 32 + lane) * L::kVBytes;
+        if constexpr (L::kVBytes == 16) {
+          const uint4 w = *reinterpret_cast<const uint4*>(a);
+          vf[k][0] = w.x;
+          vf[k][1] = w.y;
+          vf[k][2] = w.z;
+          vf[k][3] = w.w;
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(a);
+          vf[k][0] = w.x;
+          vf[k][1] = w.y;
+        }
+      }
+    } else {
+      // Tail: two looks at the rows, the first for the unit's magnitudes.
+      uint32_t ktop = 0, vtop = 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int key = key0 + t * 8 + g;
+        const __nv_bfloat16* row = kt + (int64_t)(key - sealed) * d;
+#pragma unroll
+        for (int st = 0; st < L::kSteps; ++st) {
+          const int dim = (st >> 2) * 64 + c * 16 + (st & 3) * 4;
+          if (key < key_hi && dim < d) {
+            const uint2 w = *reinterpret_cast<const uint2*>(row + dim);
+            ktop = max(ktop, max(finite_top2(w.x), finite_top2(w.y)));
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int key = key0 + 2 * c + (k & 1) + (k >> 1) * 8;
+        tail_on[k] = key < key_hi;
+        tail_v[k] = reinterpret_cast<const uint2*>(vt + (int64_t)(tail_on[k] ? key - sealed : 0) * d + g * L::kVBytes);
+        tail_on[k] = tail_on[k] && g * L::kVBytes < d;
+#pragma unroll
+        for (int w = 0; w < L::kVBytes / 4; ++w)
+          if (tail_on[k]) {
+            const uint2 x = tail_v[k][w];
+            vtop = max(vtop, max(finite_top2(x.x), finite_top2(x.y)));
+            if (any_nonfinite2(x.x) || any_nonfinite2(x.y)) bad |= 1u << k;
+          }
+      }
+      ktop = __reduce_max_sync(0xffffffffu, ktop);
+      vtop = __reduce_max_sync(0xffffffffu, vtop);
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, off);
+      const int ke = fit_exponent(ktop), ve = fit_exponent(vtop);
+      kscale = pow2f(ke);
+      vscale = pow2f(ve);
+      vinv = pow2f(-ve);
+      const float kinv = pow2f(-ke);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int key = key0 + t * 8 + g;
+        const __nv_bfloat16* row = kt + (int64_t)(key - sealed) * d;
+#pragma unroll
+        for (int st = 0; st < L::kSteps; ++st) {
+          const int dim = (st >> 2) * 64 + c * 16 + (st & 3) * 4;
+          uint2 w = make_uint2(0, 0);
+          if (key < key_hi && dim < d) w = *reinterpret_cast<const uint2*>(row + dim);
+          mma_f16(s[t], qf[st], pack_f16x2(bf_lo(w.x) * kinv, bf_hi(w.x) * kinv),
+                  pack_f16x2(bf_lo(w.y) * kinv, bf_hi(w.y) * kinv));
+        }
+      }
+    }
+
+    // Visibility of keys 2c, 2c + 1 (bits 0, 1) and 8 + 2c, 9 + 2c (bits 2, 3) for both rows.
+    uint32_t vis[2];
+    if (key0 + kUnit <= p.prefix) {  // prefix_len <= kv_len
+      vis[0] = rok[0] ? 15u : 0u;
+      vis[1] = rok[1] ? 15u : 0u;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t w = rok[r] ? (uint32_t)kv8_window(p, rbits[r], key0) : 0u;
+        vis[r] = ((w >> (2 * c)) & 3u) | (((w >> (8 + 2 * c)) & 3u) << 2);
+      }
+    }
+
+    // Scores in base 2; those not seen are never looked at again.
+    float x[2][4];
+    bool grow = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float f = qs[r] * kscale;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float y = s[i >> 1][2 * r + (i & 1)] * f;
+        if ((bad >> i) & 1u) y = __int_as_float(0x7fc00000);
+        x[r][i] = y;
+        if ((vis[r] >> i) & 1u) mx = fmaxf(mx, y);
+      }
+      grow |= mx > m[r] + kSlack || (m[r] == -INFINITY && mx > -INFINITY);
+    }
+    float corr[2] = {1.f, 1.f};
+    bool rescale = false;
+    if (__any_sync(0xffffffffu, grow)) {
+      rescale = true;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float mx = m[r];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((vis[r] >> i) & 1u) mx = fmaxf(mx, x[r][i]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        corr[r] = m[r] == -INFINITY ? 0.f : exp2f(m[r] - mx);
+        m[r] = mx;
+        l[r] *= corr[r];
+      }
+    }
+    float pf = 1.f;  // this block's V scale in the accumulators' units
+    if (vscale != unit) {
+      if (vscale > unit) {  // a larger scale: the accumulators change units
+        const float f = unit / vscale;
+        corr[0] *= f;
+        corr[1] *= f;
+        unit = vscale;
+        rescale = true;
+      } else {
+        pf = vscale / unit;  // < 1, or NaN for a block that holds one
+      }
+    }
+    if (rescale) {
+#pragma unroll
+      for (int t = 0; t < L::kTiles; ++t) {
+        o[t][0] *= corr[0];
+        o[t][1] *= corr[0];
+        o[t][2] *= corr[1];
+        o[t][3] *= corr[1];
+      }
+    }
+    float pv[2][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float base = m[r] == -INFINITY ? 0.f : m[r] - kPShift;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e = (vis[r] >> i) & 1u ? exp2f(x[r][i] - base) : 0.f;
+        l[r] += e;
+        pv[r][i] = (vis[r] >> i) & 1u ? e * pf : 0.f;
+      }
+    }
+    const uint32_t pa[4] = {pack_f16x2(pv[0][0], pv[0][1]), pack_f16x2(pv[1][0], pv[1][1]),
+                            pack_f16x2(pv[0][2], pv[0][3]), pack_f16x2(pv[1][2], pv[1][3])};
+
+    // Output tile t, column g: dim g * kVBytes + t.
+    if (coded) {
+#pragma unroll
+      for (int w = 0; w < L::kVBytes / 4; ++w) {
+        const uint32_t a01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), a23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
+        const uint32_t b01 = __byte_perm(vf[2][w], vf[3][w], 0x5140), b23 = __byte_perm(vf[2][w], vf[3][w], 0x7362);
+        mma_f16(o[4 * w + 0], pa, e4m3x2_to_f16x2(a01), e4m3x2_to_f16x2(b01));
+        mma_f16(o[4 * w + 1], pa, e4m3x2_hi_to_f16x2(a01), e4m3x2_hi_to_f16x2(b01));
+        mma_f16(o[4 * w + 2], pa, e4m3x2_to_f16x2(a23), e4m3x2_to_f16x2(b23));
+        mma_f16(o[4 * w + 3], pa, e4m3x2_hi_to_f16x2(a23), e4m3x2_hi_to_f16x2(b23));
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < L::kVBytes / 4; ++w) {
+        float f[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint2 u = tail_on[k] ? tail_v[k][w] : make_uint2(0, 0);
+          f[k][0] = bf_lo(u.x);
+          f[k][1] = bf_hi(u.x);
+          f[k][2] = bf_lo(u.y);
+          f[k][3] = bf_hi(u.y);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[k][i] = fabsf(f[k][i]) < INFINITY ? f[k][i] * vinv : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mma_f16(o[4 * w + i], pa, pack_f16x2(f[0][i], f[1][i]), pack_f16x2(f[2][i], f[3][i]));
+      }
+    }
+  }
+  cp_wait<0>();
+
+  // Join the four warps: rows' sums over the four threads of a quad, then
+  // partial outputs through shared memory (the ring's space).
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    if (c == 0) {
+      join_m[warp][g + 8 * r] = m[r];
+      join_l[warp][g + 8 * r] = l[r];
+    }
+  }
+  __syncthreads();  // every warp is done with the ring
+  float* po = reinterpret_cast<float*>(smem) + (size_t)warp * kRows * DT;
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int t = 0; t < L::kTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        // column 2c + i of tile t: dim (2c + i) * kVBytes + t
+        const float y = o[t][2 * r + i];
+        po[(g + 8 * r) * DT + (2 * c + i) * L::kVBytes + t] = unit > 0.f ? y * unit : y;
+      }
+  __syncthreads();
+  constexpr int kPerRow = DT / 4;
+  for (int i = threadIdx.x; i < kRows * kPerRow; i += kWarps * 32) {
+    const int row = i / kPerRow, col = (i % kPerRow) * 4;
+    const int pr = blockIdx.y * kRows + row;
+    if (pr >= packed || col >= d) continue;
+    float gm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) gm = fmaxf(gm, join_m[w][row]);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = join_m[w][row];
+      const float f = mw == -INFINITY ? 0.f : exp2f(mw - gm);
+      const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) +
+                                                        ((size_t)w * kRows + row) * DT + col);
+      sum += f * join_l[w][row];  // a NaN passes even where f is 0
+      acc[0] += f * y.x;
+      acc[1] += f * y.y;
+      acc[2] += f * y.z;
+      acc[3] += f * y.w;
+    }
+    const int head = kvh * p.group + pr / p.q_len, t = pr % p.q_len;
+    if (p.splits == 1) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
+      __nv_bfloat162 hi = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+      uint2 w;
+      w.x = *reinterpret_cast<uint32_t*>(&lo);
+      w.y = *reinterpret_cast<uint32_t*>(&hi);
+      *reinterpret_cast<uint2*>(p.out + req * p.out_bs + ((int64_t)t * p.heads + head) * d + col) = w;
+      if (p.lse && col == 0)
+        p.lse[((int64_t)req * p.heads + head) * p.q_len + t] =
+            sum == 0.f ? -INFINITY : (gm == -INFINITY ? sum : (gm - kPShift + log2f(sum)) * 0.69314718055994531f);
+    } else {
+      const int64_t idx = (((int64_t)req * p.splits + split) * p.heads + head) * p.q_len + t;
+      *reinterpret_cast<float4*>(p.part_o + idx * d + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (col == 0) {
+        p.part_ml[idx * 2] = gm == -INFINITY ? gm : gm - kPShift;  // sums carry the 2^12
+        p.part_ml[idx * 2 + 1] = sum;
+      }
+    }
+  }
+}
+
+// Joins the key ranges: one warp per (request, head, row), four dims a lane.
+__global__ void kv8_merge_kernel(Kv8Attn p) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t per_req = (int64_t)p.heads * p.q_len;
+  const int64_t pair = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (pair >= per_req * p.batch) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t req = pair / per_req, at = pair % per_req;
+  const int head = (int)(at / p.q_len), t = (int)(at % p.q_len);
+  const int64_t base = req * p.splits * per_req + at;
+  const int d = p.c.d;
+  float gm = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) gm = fmaxf(gm, p.part_ml[(base + s * per_req) * 2]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  for (int s0 = 0; s0 < p.splits; s0 += 32) {
+    float w = 0.f;
+    if (s0 + lane < p.splits) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (base + (s0 + lane) * per_req) * 2);
+      w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - gm);
+      sum += w * ml.y;
+    }
+    const int n = min(32, p.splits - s0);
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const float f = __shfl_sync(0xffffffffu, w, j);
+      if (lane * 4 < d) {
+        const float4 y = *reinterpret_cast<const float4*>(p.part_o + (base + (int64_t)(s0 + j) * per_req) * d + lane * 4);
+        acc[0] += f * y.x;
+        acc[1] += f * y.y;
+        acc[2] += f * y.z;
+        acc[3] += f * y.w;
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (p.lse && lane == 0)
+    p.lse[pair] = sum == 0.f ? -INFINITY : (gm == -INFINITY ? sum : (gm + log2f(sum)) * 0.69314718055994531f);
+  if (lane * 4 >= d) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
+  __nv_bfloat162 hi = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+  uint2 w;
+  w.x = *reinterpret_cast<uint32_t*>(&lo);
+  w.y = *reinterpret_cast<uint32_t*>(&hi);
+  *reinterpret_cast<uint2*>(p.out + req * p.out_bs + ((int64_t)t * p.heads + head) * d + lane * 4) = w;
+}
+
+template <int DT>
+int launch_mma(const Kv8Attn& p, cudaStream_t stream) {
+  static std::atomic<unsigned long long> configured{0};
+  if (int rc = once_per_device(configured, [] {
+        SF_CHECK_CUDA(cudaFuncSetAttribute(kv8_attn_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           Layout<DT>::kSmem));
+        return SF_OK;
+      }))
+    return rc;
+  const int64_t tiles = ((int64_t)p.group * p.q_len + kRows - 1) / kRows;
+  SF_CHECK_ARG(tiles < 65536 && (int64_t)p.splits * p.batch < 65536, "too many query rows or requests");
+  const dim3 grid((unsigned)p.c.hkv, (unsigned)tiles, (unsigned)(p.splits * p.batch));
+  SF_CHECK_CUDA(launch_pdl(kv8_attn_kernel<DT>, grid, dim3(kWarps * 32), Layout<DT>::kSmem, stream, p));
+  SF_CHECK_LAUNCH();
+  return SF_OK;
+}
+
+}  // namespace
+
+// Two resident CTAs per SM (their rings fill shared memory); a range is at
+// least two steps of the four warps.
+Kv8Split kv8_split_mma(int batch, int hkv, int64_t packed, int64_t kv_len) {
+  const int64_t units = (int64_t)batch * hkv * ((packed + kRows - 1) / kRows);
+  const int64_t steps = (kv_len + kStep - 1) / kStep;
+  int64_t want = std::max<int64_t>(1, 2 * (int64_t)num_sms() / units);
+  want = std::min<int64_t>(want, std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, steps / 2)));
+  const int64_t per = std::max<int64_t>(1, (steps + want - 1) / want);
+  return {(int)std::max<int64_t>(1, (steps + per - 1) / per), (int)(per * kStep)};
+}
+
+}  // namespace sf
+
+extern "C" size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim,
+                                                  int64_t q_len, int64_t kv_len) {
+  using namespace sf;
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
+      head_dim > 128 || q_len <= 0 || kv_len <= 0 || q_len >= (1 << 30) || kv_len >= (1 << 30))
+    return 0;
+  const Kv8Split s = kv8_split_mma(batch, num_kv_heads, (int64_t)(num_heads / num_kv_heads) * q_len, kv_len);
+  if (s.splits == 1) return 0;
+  return (size_t)batch * s.splits * num_heads * q_len * (head_dim + 2) * sizeof(float);
+}
+
+extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride,
+                                     int64_t q_row_stride, int num_heads, int64_t q_len, const sf_kv8_rows* rows,
+                                     const uint32_t* tree_bits, int bit_words, int64_t bits_batch_stride,
+                                     int64_t prefix_len, float scale, void* out, int64_t out_batch_stride, float* lse,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace sf;
+  if (int rc = kv8_check(rows, true)) return rc;
+  const int64_t kv_len = rows->sealed + rows->tail;
+  SF_CHECK_ARG(num_heads > 0 && num_heads % rows->num_kv_heads == 0,
+               "num_heads must be a positive multiple of num_kv_heads");
+  SF_CHECK_ARG(q_len >= 0 && prefix_len >= 0 && prefix_len <= kv_len && kv_len < (1 << 30), "invalid lengths");
+  const int group = num_heads / rows->num_kv_heads;
+  SF_CHECK_ARG((int64_t)group * q_len < (1 << 20), "too many query rows");
+  if (q_len == 0) return SF_OK;
+  SF_CHECK_ARG(q && out, "null pointer argument");
+  SF_CHECK_ARG(kv_len == prefix_len || (tree_bits && (int64_t)bit_words * 32 >= kv_len - prefix_len),
+               "tree_bits must cover the keys from prefix_len on");
+  SF_CHECK_ARG(aligned16(q) && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0 && q_row_stride % 8 == 0,
+               "q rows must be 16-byte aligned");
+  SF_CHECK_ARG(aligned16(out) && out_batch_stride % 8 == 0, "out must be 16-byte aligned");
+  const size_t need = sf_kv8_attention_workspace_bytes(rows->batch, num_heads, rows->num_kv_heads, rows->head_dim,
+                                                       q_len, kv_len);
+  if (workspace_bytes < need || (need && !workspace))
+    return set_error(SF_ERR_WORKSPACE, "8-bit cache attention workspace needs %zu bytes", need);
+  SF_CHECK_ARG(need == 0 || aligned16(workspace), "workspace must be 16-byte aligned");
+  Kv8Attn p;
+  p.c = kv8_view(*rows);
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_bs = q_batch_stride;
+  p.q_hs = q_head_stride;
+  p.q_rs = q_row_stride;
+  p.bits = kv_len == prefix_len ? nullptr : tree_bits;
+  p.words = bit_words;
+  p.bits_bs = bits_batch_stride;
+  p.batch = rows->batch;
+  p.heads = num_heads;
+  p.group = group;
+  p.q_len = (int)q_len;
+  p.kv_len = (int)kv_len;
+  p.prefix = (int)prefix_len;
+  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_bs = out_batch_stride;
+  p.lse = lse;
+  const int64_t packed = (int64_t)group * q_len;
+  const Kv8Split s = kv8_split_mma(rows->batch, rows->num_kv_heads, packed, kv_len);
+  p.splits = s.splits;
+  p.keys_per_split = s.keys_per_split;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + (size_t)rows->batch * s.splits * num_heads * q_len * rows->head_dim;
+  cudaStream_t st = as_stream(stream);
+  const int rc = rows->head_dim <= 64 ? launch_mma<64>(p, st) : launch_mma<128>(p, st);
+  if (rc || s.splits == 1) return rc;
+  const int64_t pairs = (int64_t)rows->batch * num_heads * q_len;
+  SF_CHECK_CUDA(launch_pdl(kv8_merge_kernel, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, st, p));
+  SF_CHECK_LAUNCH();
+  return SF_OK;
+}

@@ -1,0 +1,50 @@
+// Parameters shared by the kernels that attend to the 8-bit KV cache and the
+// merge of their partial results.
+#pragma once
+
+#include "kv8.cuh"
+#include "tree_attn.h"
+
+namespace sf {
+
+struct Kv8Attn {
+  Kv8Rows c;
+  const __nv_bfloat16* q;
+  int64_t q_bs, q_hs, q_rs;
+  const uint32_t* bits;  // [batch, q_len, words] over the keys from prefix_len on; nullable
+  int words;
+  int64_t bits_bs;
+  int batch, heads, group, q_len;
+  int kv_len, prefix;
+  float scale, scale_log2;  // the softmax scale, and times log2(e)
+  int splits, keys_per_split;
+  float* part_o;   // [batch, splits, heads, q_len, D] unnormalised
+  float* part_ml;  // [batch, splits, heads, q_len, 2]: (reference max, sum), base 2
+  __nv_bfloat16* out;  // [batch, q_len, heads, D]
+  int64_t out_bs;
+  float* lse;      // [batch, heads, q_len]; nullable
+};
+
+// Visibility of keys key0 + i, i in [0, 64), for one query row, as bit i.
+__device__ __forceinline__ uint64_t kv8_window(const Kv8Attn& p, const uint32_t* rbits, int key0) {
+  uint64_t w;
+  if (rbits) {
+    w = tree_mask_window(rbits, p.words, key0 - p.prefix);
+  } else {
+    const int n = p.prefix - key0;
+    w = n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1);
+  }
+  const int valid = p.kv_len - key0;
+  if (valid < 64) w &= valid <= 0 ? 0ull : (1ull << valid) - 1;
+  return w;
+}
+
+// Key ranges per (request, KV head, row tile) for `units` such units of work.
+struct Kv8Split {
+  int splits, keys_per_split;
+};
+
+// The warp-level kernel (kv8_attn.cu).
+Kv8Split kv8_split_mma(int batch, int hkv, int64_t packed_rows, int64_t kv_len);
+
+}  // namespace sf

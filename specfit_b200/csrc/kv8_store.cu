@@ -1,0 +1,304 @@
+// Writing the 8-bit KV cache: sealing bf16 rows, reading rows back as bf16,
+// and moving the kept rows of an eviction into a new cache.
+//
+// All three are streams over rows, bound by memory: sealing reads 2 bytes and
+// writes 1 per element, compaction reads a kept row's 1 byte and writes 1.
+// One CTA owns one block of tokens of one head of K or of V: it holds the
+// whole block (at most 128 x 128 values) in registers as bf16 pairs, finds
+// the block's largest magnitude, and writes codes and scale, so each input
+// byte is read once.  The magnitudes are compared as 15-bit integers (bf16
+// orders like its bits), two per instruction, which also finds NaN and
+// infinity (the largest integers).
+#include "kv8.cuh"
+
+namespace sf {
+
+int kv8_check(const sf_kv8_rows* r, bool need_values) {
+  SF_CHECK_ARG(r != nullptr, "null pointer argument");
+  SF_CHECK_ARG(r->batch > 0 && r->num_kv_heads > 0 && (int64_t)r->batch * r->num_kv_heads <= 65535,
+               "batch and num_kv_heads must be positive, their product at most 65535");
+  SF_CHECK_ARG(r->head_dim > 0 && r->head_dim <= 128 && r->head_dim % 16 == 0,
+               "head_dim must be a multiple of 16 in [16, 128]");
+  SF_CHECK_ARG(r->block_tokens == 32 || r->block_tokens == 64 || r->block_tokens == 128,
+               "block_tokens must be 32, 64 or 128");
+  SF_CHECK_ARG(r->sealed >= 0 && r->tail >= 0 && r->sealed % r->block_tokens == 0 &&
+                   r->sealed < (1 << 30) && r->tail < (1 << 30),
+               "sealed must be a whole number of blocks, lengths below 2^30");
+  if (r->sealed > 0) {
+    SF_CHECK_ARG(r->k_codes && r->k_scale && (!need_values || (r->v_codes && r->v_scale)), "null pointer argument");
+    SF_CHECK_ARG(aligned16(r->k_codes) && (!need_values || aligned16(r->v_codes)) &&
+                     r->code_batch_stride % 16 == 0 && r->code_head_stride % 16 == 0,
+                 "codes must be 16-byte aligned");
+  }
+  if (r->tail > 0) {
+    SF_CHECK_ARG(r->k_tail && (!need_values || r->v_tail), "null pointer argument");
+    SF_CHECK_ARG(aligned16(r->k_tail) && (!need_values || aligned16(r->v_tail)) &&
+                     r->tail_batch_stride % 8 == 0 && r->tail_head_stride % 8 == 0,
+                 "tail rows must be 16-byte aligned");
+  }
+  return SF_OK;
+}
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxChunks = 128 * 128 / 8 / kThreads;  // 16-byte bf16 chunks per thread: 8
+
+// Where the rows of a block come from: bf16 rows in order (sealing) ...
+struct SourceRows {
+  const __nv_bfloat16* k;
+  const __nv_bfloat16* v;
+  int64_t bs, hs, rs;
+};
+// ... or kept rows of a cache, by index (compaction).
+struct SourceKept {
+  Kv8Rows c;
+  const int32_t* keep;  // [batch * hkv, n]
+  int64_t n;
+  const float* mass;    // nullable
+  float* mass_out;
+  int64_t m_bs, m_hs, mo_bs, mo_hs;
+};
+
+struct Target {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  __nv_bfloat16* kt;
+  __nv_bfloat16* vt;
+  int64_t c_bs, c_hs, s_bs, s_hs, t_bs, t_hs;
+  int64_t first_block;  // the block that grid x = 0 writes
+  int64_t full_blocks;  // blocks of this launch; the CTA after them writes the tail
+  int hkv, d, block;
+};
+
+// 8 codes of one scale as 8 bf16 values (exact; NaN for a NaN scale).
+__device__ __forceinline__ uint4 codes_to_bf16(uint2 c, float scale) {
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w = i ? c.y : c.x;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t h = j ? e4m3x2_hi_to_f16x2(w) : e4m3x2_to_f16x2(w);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * scale, f.y * scale);
+      o[i * 2 + j] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Eight elements (chunk ch of cache row `row`) of a cache as bf16.
+__device__ __forceinline__ uint4 cache_chunk(const Kv8Rows& c, int b, int h, bool is_v, int64_t row, int ch) {
+  if (row < c.sealed) {
+    const uint8_t* codes = (is_v ? c.v : c.k) + b * c.c_bs + h * c.c_hs + row * c.d + ch * 8;
+    const float* sc = (is_v ? c.vs : c.ks) + b * c.s_bs + h * c.s_hs + (row >> c.block_shift);
+    return codes_to_bf16(*reinterpret_cast<const uint2*>(codes), *sc);
+  }
+  const __nv_bfloat16* t = (is_v ? c.vt : c.kt) + b * c.t_bs + h * c.t_hs + (row - c.sealed) * c.d + ch * 8;
+  return *reinterpret_cast<const uint4*>(t);
+}
+
+__device__ __forceinline__ uint4 load_chunk(const SourceRows& s, int b, int h, bool is_v, int64_t row, int ch) {
+  return *reinterpret_cast<const uint4*>((is_v ? s.v : s.k) + b * s.bs + h * s.hs + row * s.rs + ch * 8);
+}
+
+__device__ __forceinline__ uint4 load_chunk(const SourceKept& s, int b, int h, bool is_v, int64_t row, int ch) {
+  const int32_t at = s.keep[((int64_t)b * s.c.hkv + h) * s.n + row];
+  if (at < 0 || at >= s.c.sealed + s.c.tail) return make_uint4(0, 0, 0, 0);  // not a row of the cache
+  return cache_chunk(s.c, b, h, is_v, at, ch);
+}
+
+__device__ __forceinline__ int64_t source_rows(const SourceRows&, int64_t full) { return full; }
+__device__ __forceinline__ int64_t source_rows(const SourceKept& s, int64_t) { return s.n; }
+
+__device__ __forceinline__ void move_mass(const SourceRows&, int, int, int64_t, int) {}
+__device__ __forceinline__ void move_mass(const SourceKept& s, int b, int h, int64_t row0, int rows) {
+  if (!s.mass) return;
+  for (int i = threadIdx.x; i < rows; i += kThreads) {
+    const int32_t at = s.keep[((int64_t)b * s.c.hkv + h) * s.n + row0 + i];
+    const bool ok = at >= 0 && at < s.c.sealed + s.c.tail;
+    s.mass_out[b * s.mo_bs + h * s.mo_hs + row0 + i] = ok ? s.mass[b * s.m_bs + h * s.m_hs + at] : 0.f;
+  }
+}
+
+// grid: (blocks [+ 1 for the tail], batch * hkv, 2: K and V).
+template <typename Source>
+__global__ void __launch_bounds__(kThreads)
+kv8_write_kernel(Source src, Target t) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ uint32_t tops[kThreads / 32];
+  const int h = blockIdx.y % t.hkv, b = blockIdx.y / t.hkv;
+  const bool is_v = blockIdx.z != 0;
+  const int64_t row0 = (int64_t)blockIdx.x * t.block;
+  const int per_row = t.d >> 3;  // 8-element chunks of a row
+  const int64_t n = source_rows(src, t.full_blocks * t.block);
+  const int rows = (int)min((int64_t)t.block, n - row0);
+  if (!is_v) move_mass(src, b, h, row0, rows);
+  const int chunks = rows * per_row;
+  uint4 x[kMaxChunks];
+#pragma unroll
+  for (int j = 0; j < kMaxChunks; ++j) {
+    const int i = threadIdx.x + j * kThreads;
+    x[j] = i < chunks ? load_chunk(src, b, h, is_v, row0 + i / per_row, i % per_row) : make_uint4(0, 0, 0, 0);
+  }
+  if ((int64_t)blockIdx.x >= t.full_blocks) {  // rows that do not fill a block stay bf16
+    __nv_bfloat16* dst = (is_v ? t.vt : t.kt) + b * t.t_bs + h * t.t_hs;
+#pragma unroll
+    for (int j = 0; j < kMaxChunks; ++j) {
+      const int i = threadIdx.x + j * kThreads;
+      if (i < chunks) *reinterpret_cast<uint4*>(dst + (int64_t)i * 8) = x[j];
+    }
+    return;
+  }
+  uint32_t top2 = 0;  // two 15-bit magnitudes
+#pragma unroll
+  for (int j = 0; j < kMaxChunks; ++j) {
+    top2 = __vmaxu2(top2, x[j].x & 0x7fff7fffu);
+    top2 = __vmaxu2(top2, x[j].y & 0x7fff7fffu);
+    top2 = __vmaxu2(top2, x[j].z & 0x7fff7fffu);
+    top2 = __vmaxu2(top2, x[j].w & 0x7fff7fffu);
+  }
+  uint32_t top = max(top2 & 0xffffu, top2 >> 16);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) top = max(top, tops[w]);
+  const bool bad = top >= 0x7f80u;  // a NaN or an infinity
+  const int e = bad ? 0 : kv8_exponent(top);
+  const float inv = pow2f(-e);
+  const int64_t blk = t.first_block + blockIdx.x;
+  if (threadIdx.x == 0)
+    (is_v ? t.vs : t.ks)[b * t.s_bs + h * t.s_hs + blk] = bad ? __int_as_float(0x7fc00000) : pow2f(e);
+  uint8_t* dst = (is_v ? t.v : t.k) + b * t.c_bs + h * t.c_hs + blk * t.block * t.d;
+#pragma unroll
+  for (int j = 0; j < kMaxChunks; ++j) {
+    const int i = threadIdx.x + j * kThreads;
+    if (i >= chunks) continue;
+    const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+    uint32_t o[2] = {0, 0};
+    if (!bad) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        // Exact products (a power of two), one rounding to nearest-even.
+        const float2 f = make_float2(__uint_as_float(w[p] << 16) * inv, __uint_as_float(w[p] & 0xffff0000u) * inv);
+        o[p >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3) << (16 * (p & 1));
+      }
+    }
+    *reinterpret_cast<uint2*>(dst + (int64_t)i * 8) = make_uint2(o[0], o[1]);
+  }
+}
+
+// Rows [first, first + count) of a cache as bf16; grid (chunk blocks, batch * hkv, 2).
+__global__ void __launch_bounds__(kThreads)
+kv8_read_kernel(Kv8Rows c, int64_t first, int64_t count, __nv_bfloat16* __restrict__ k_out,
+                __nv_bfloat16* __restrict__ v_out, int64_t o_bs, int64_t o_hs) {
+  pdl_wait();
+  pdl_trigger();
+  const int h = blockIdx.y % c.hkv, b = blockIdx.y / c.hkv;
+  const bool is_v = blockIdx.z != 0;
+  const int per_row = c.d >> 3;
+  __nv_bfloat16* dst = (is_v ? v_out : k_out) + b * o_bs + h * o_hs;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count * per_row;
+       i += (int64_t)gridDim.x * kThreads)
+    *reinterpret_cast<uint4*>(dst + i * 8) = cache_chunk(c, b, h, is_v, first + i / per_row, (int)(i % per_row));
+}
+
+Target make_target(const sf_kv8_rows& r, int64_t first_block, int64_t full_blocks) {
+  Target t;
+  t.k = static_cast<uint8_t*>(r.k_codes);
+  t.v = static_cast<uint8_t*>(r.v_codes);
+  t.ks = r.k_scale;
+  t.vs = r.v_scale;
+  t.kt = static_cast<__nv_bfloat16*>(r.k_tail);
+  t.vt = static_cast<__nv_bfloat16*>(r.v_tail);
+  t.c_bs = r.code_batch_stride;
+  t.c_hs = r.code_head_stride;
+  t.s_bs = r.scale_batch_stride;
+  t.s_hs = r.scale_head_stride;
+  t.t_bs = r.tail_batch_stride;
+  t.t_hs = r.tail_head_stride;
+  t.first_block = first_block;
+  t.full_blocks = full_blocks;
+  t.hkv = r.num_kv_heads;
+  t.d = r.head_dim;
+  t.block = r.block_tokens;
+  return t;
+}
+
+}  // namespace
+}  // namespace sf
+
+extern "C" int sf_kv8_seal(const void* k, const void* v, int64_t batch_stride, int64_t head_stride,
+                           int64_t row_stride, const sf_kv8_rows* rows, int64_t first_block, int64_t blocks,
+                           void* stream) {
+  using namespace sf;
+  if (int rc = kv8_check(rows, true)) return rc;
+  SF_CHECK_ARG(blocks >= 0 && first_block >= 0 && blocks < (1 << 24) &&
+                   first_block + blocks <= rows->sealed / rows->block_tokens,
+               "blocks to seal must lie within the cache's sealed rows");
+  if (blocks == 0) return SF_OK;
+  SF_CHECK_ARG(k && v, "null pointer argument");
+  SF_CHECK_ARG(aligned16(k) && aligned16(v) && batch_stride % 8 == 0 && head_stride % 8 == 0 && row_stride % 8 == 0,
+               "k/v rows must be 16-byte aligned");
+  const SourceRows src{static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), batch_stride,
+                       head_stride, row_stride};
+  const dim3 grid((unsigned)blocks, (unsigned)(rows->batch * rows->num_kv_heads), 2);
+  SF_CHECK_CUDA(launch_pdl(kv8_write_kernel<SourceRows>, grid, dim3(kThreads), 0, as_stream(stream), src,
+                           make_target(*rows, first_block, blocks)));
+  SF_CHECK_LAUNCH();
+  return SF_OK;
+}
+
+extern "C" int sf_kv8_read(const sf_kv8_rows* rows, int64_t first, int64_t count, void* k_out, void* v_out,
+                           int64_t out_batch_stride, int64_t out_head_stride, void* stream) {
+  using namespace sf;
+  if (int rc = kv8_check(rows, true)) return rc;
+  SF_CHECK_ARG(first >= 0 && count >= 0 && first + count <= rows->sealed + rows->tail,
+               "rows to read must lie within the cache");
+  if (count == 0) return SF_OK;
+  SF_CHECK_ARG(k_out && v_out, "null pointer argument");
+  SF_CHECK_ARG(aligned16(k_out) && aligned16(v_out) && out_batch_stride % 8 == 0 && out_head_stride % 8 == 0,
+               "output rows must be 16-byte aligned");
+  const int64_t want = (count * (rows->head_dim / 8) + kThreads - 1) / kThreads;
+  const dim3 grid((unsigned)(want < 4096 ? want : 4096), (unsigned)(rows->batch * rows->num_kv_heads), 2);
+  SF_CHECK_CUDA(launch_pdl(kv8_read_kernel, grid, dim3(kThreads), 0, as_stream(stream), kv8_view(*rows), first,
+                           count, static_cast<__nv_bfloat16*>(k_out), static_cast<__nv_bfloat16*>(v_out),
+                           out_batch_stride, out_head_stride));
+  SF_CHECK_LAUNCH();
+  return SF_OK;
+}
+
+extern "C" int sf_kv8_compact(const sf_kv8_rows* rows, const int32_t* keep, int64_t n, const sf_kv8_rows* out,
+                              const float* mass, int64_t mass_batch_stride, int64_t mass_head_stride,
+                              float* mass_out, int64_t mass_out_batch_stride, int64_t mass_out_head_stride,
+                              void* stream) {
+  using namespace sf;
+  if (int rc = kv8_check(rows, true)) return rc;
+  if (int rc = kv8_check(out, true)) return rc;
+  SF_CHECK_ARG(out->batch == rows->batch && out->num_kv_heads == rows->num_kv_heads &&
+                   out->head_dim == rows->head_dim && out->block_tokens == rows->block_tokens,
+               "both caches must share batch, heads, head_dim and block_tokens");
+  SF_CHECK_ARG(n >= 0 && n <= rows->sealed + rows->tail, "more rows kept than the cache holds");
+  SF_CHECK_ARG(out->sealed == n / out->block_tokens * out->block_tokens && out->tail == n - out->sealed,
+               "the new cache must hold the kept rows: whole blocks sealed, the rest as its tail");
+  SF_CHECK_ARG((mass == nullptr) == (mass_out == nullptr), "pass both mass and mass_out or neither");
+  if (n == 0) return SF_OK;
+  SF_CHECK_ARG(keep, "null pointer argument");
+  SF_CHECK_ARG((out->sealed == 0 || (out->k_codes != rows->k_codes && out->v_codes != rows->v_codes)) &&
+                   (out->tail == 0 || (out->k_tail != rows->k_tail && out->v_tail != rows->v_tail)) &&
+                   (mass == nullptr || mass != mass_out),
+               "compaction writes to buffers of its own");
+  SourceKept src{kv8_view(*rows), keep, n, mass, mass_out, mass_batch_stride, mass_head_stride,
+                 mass_out_batch_stride, mass_out_head_stride};
+  const int64_t full = out->sealed / out->block_tokens;
+  const dim3 grid((unsigned)(full + (out->tail > 0 ? 1 : 0)), (unsigned)(rows->batch * rows->num_kv_heads), 2);
+  SF_CHECK_CUDA(launch_pdl(kv8_write_kernel<SourceKept>, grid, dim3(kThreads), 0, as_stream(stream), src,
+                           make_target(*out, 0, full)));
+  SF_CHECK_LAUNCH();
+  return SF_OK;
+}
