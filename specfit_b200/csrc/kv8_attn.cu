@@ -31,8 +31,9 @@
 //   * The reference maximum of a row moves only when a score exceeds it by
 //     more than 3 (base 2), so accumulators are rarely rescaled.
 // Tail units (bf16 rows: few) are scaled by a power of two per unit and
-// enter the same fragments.  A value row with a NaN or an infinity makes its
-// key's score NaN, so that rows which do not see it stay what they are.
+// enter the same fragments.  A value row with a NaN or an infinity (a sealed
+// block of values that holds one) makes its key's score NaN, so that rows
+// which do not see it stay what they are.
 #include <math.h>
 
 #include <algorithm>
@@ -169,6 +170,10 @@ kv8_attn_kernel(Kv8Attn p) {
     if (coded) {
       kscale = ksc[key0 >> p.c.block_shift];
       vscale = vsc[key0 >> p.c.block_shift];
+      if (vscale != vscale) {  // a block with a NaN among its values: its keys' scores are NaN
+        kscale = vscale;
+        vscale = unit;
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -303,7 +308,7 @@ kv8_attn_kernel(Kv8Attn p) {
         unit = vscale;
         rescale = true;
       } else {
-        pf = vscale / unit;  // < 1, or NaN for a block that holds one
+        pf = vscale / unit;  // < 1
       }
     }
     if (rescale) {
@@ -498,6 +503,11 @@ int launch_mma(const Kv8Attn& p, cudaStream_t stream) {
   return SF_OK;
 }
 
+Kv8Split plan(int head_dim, int batch, int hkv, int64_t packed, int64_t kv_len) {
+  return kv8_use_tc(head_dim, packed, kv_len) ? kv8_split_tc(batch, hkv, packed, kv_len)
+                                              : kv8_split_mma(batch, hkv, packed, kv_len);
+}
+
 }  // namespace
 
 // Two resident CTAs per SM (their rings fill shared memory); a range is at
@@ -519,7 +529,7 @@ extern "C" size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int
   if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
       head_dim > 128 || q_len <= 0 || kv_len <= 0 || q_len >= (1 << 30) || kv_len >= (1 << 30))
     return 0;
-  const Kv8Split s = kv8_split_mma(batch, num_kv_heads, (int64_t)(num_heads / num_kv_heads) * q_len, kv_len);
+  const Kv8Split s = plan(head_dim, batch, num_kv_heads, (int64_t)(num_heads / num_kv_heads) * q_len, kv_len);
   if (s.splits == 1) return 0;
   return (size_t)batch * s.splits * num_heads * q_len * (head_dim + 2) * sizeof(float);
 }
@@ -538,6 +548,7 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
   const int group = num_heads / rows->num_kv_heads;
   SF_CHECK_ARG((int64_t)group * q_len < (1 << 20), "too many query rows");
   if (q_len == 0) return SF_OK;
+  SF_CHECK_ARG(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
   SF_CHECK_ARG(q && out, "null pointer argument");
   SF_CHECK_ARG(kv_len == prefix_len || (tree_bits && (int64_t)bit_words * 32 >= kv_len - prefix_len),
                "tree_bits must cover the keys from prefix_len on");
@@ -570,13 +581,17 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
   p.out_bs = out_batch_stride;
   p.lse = lse;
   const int64_t packed = (int64_t)group * q_len;
-  const Kv8Split s = kv8_split_mma(rows->batch, rows->num_kv_heads, packed, kv_len);
+  const Kv8Split s = plan(rows->head_dim, rows->batch, rows->num_kv_heads, packed, kv_len);
   p.splits = s.splits;
   p.keys_per_split = s.keys_per_split;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + (size_t)rows->batch * s.splits * num_heads * q_len * rows->head_dim;
   cudaStream_t st = as_stream(stream);
-  const int rc = rows->head_dim <= 64 ? launch_mma<64>(p, st) : launch_mma<128>(p, st);
+  int rc;
+  if (kv8_use_tc(rows->head_dim, packed, kv_len))
+    rc = kv8_attention_tc(p, st);
+  else
+    rc = rows->head_dim <= 64 ? launch_mma<64>(p, st) : launch_mma<128>(p, st);
   if (rc || s.splits == 1) return rc;
   const int64_t pairs = (int64_t)rows->batch * num_heads * q_len;
   SF_CHECK_CUDA(launch_pdl(kv8_merge_kernel, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, st, p));

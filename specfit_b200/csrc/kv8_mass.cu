@@ -196,6 +196,7 @@ extern "C" int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int6
   const int group = num_heads / rows->num_kv_heads;
   SF_CHECK_ARG((int64_t)group * q_len < (1 << 20), "too many query rows");
   if (q_len == 0 || kv_len == 0) return SF_OK;
+  SF_CHECK_ARG(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
   SF_CHECK_ARG(q && lse && mass, "null pointer argument");
   SF_CHECK_ARG(kv_len == prefix_len || (tree_bits && (int64_t)bit_words * 32 >= kv_len - prefix_len),
                "tree_bits must cover the keys from prefix_len on");
