@@ -503,9 +503,8 @@ int launch_mma(const Kv8Attn& p, cudaStream_t stream) {
   return SF_OK;
 }
 
-Kv8Split plan(int head_dim, int batch, int hkv, int64_t packed, int64_t kv_len) {
-  return kv8_use_tc(head_dim, packed, kv_len) ? kv8_split_tc(batch, hkv, packed, kv_len)
-                                              : kv8_split_mma(batch, hkv, packed, kv_len);
+size_t partial_bytes(const Kv8Split& s, int batch, int heads, int head_dim, int64_t q_len) {
+  return s.splits == 1 ? 0 : (size_t)batch * s.splits * heads * q_len * (head_dim + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -529,9 +528,13 @@ extern "C" size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int
   if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
       head_dim > 128 || q_len <= 0 || kv_len <= 0 || q_len >= (1 << 30) || kv_len >= (1 << 30))
     return 0;
-  const Kv8Split s = plan(head_dim, batch, num_kv_heads, (int64_t)(num_heads / num_kv_heads) * q_len, kv_len);
-  if (s.splits == 1) return 0;
-  return (size_t)batch * s.splits * num_heads * q_len * (head_dim + 2) * sizeof(float);
+  // Enough for either kernel: which one runs depends on the cache's strides too.
+  const int64_t packed = (int64_t)(num_heads / num_kv_heads) * q_len;
+  size_t need = partial_bytes(kv8_split_mma(batch, num_kv_heads, packed, kv_len), batch, num_heads, head_dim, q_len);
+  if (kv8_use_tc(head_dim, packed, kv_len))
+    need = std::max(need, partial_bytes(kv8_split_tc(batch, num_kv_heads, packed, kv_len), batch, num_heads, head_dim,
+                                        q_len));
+  return need;
 }
 
 extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride,
@@ -581,14 +584,16 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
   p.out_bs = out_batch_stride;
   p.lse = lse;
   const int64_t packed = (int64_t)group * q_len;
-  const Kv8Split s = plan(rows->head_dim, rows->batch, rows->num_kv_heads, packed, kv_len);
+  const bool tc = kv8_use_tc(rows->head_dim, packed, kv_len) && kv8_tc_layout(p.c, rows->batch);
+  const Kv8Split s = tc ? kv8_split_tc(rows->batch, rows->num_kv_heads, packed, kv_len)
+                        : kv8_split_mma(rows->batch, rows->num_kv_heads, packed, kv_len);
   p.splits = s.splits;
   p.keys_per_split = s.keys_per_split;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + (size_t)rows->batch * s.splits * num_heads * q_len * rows->head_dim;
   cudaStream_t st = as_stream(stream);
   int rc;
-  if (kv8_use_tc(rows->head_dim, packed, kv_len))
+  if (tc)
     rc = kv8_attention_tc(p, st);
   else
     rc = rows->head_dim <= 64 ? launch_mma<64>(p, st) : launch_mma<128>(p, st);

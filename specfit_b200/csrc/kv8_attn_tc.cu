@@ -12,21 +12,31 @@
 //     softmax.  With more than 128 packed rows the lanes are two row tiles
 //     that share every decoded block; with fewer they are the same rows over
 //     the even and the odd blocks (two partial results).
-//   * Four warps decode: codes are loaded a block ahead into registers,
-//     turned into bf16 and stored in the swizzled operand layout.  An e4m3
-//     code shifted into a bf16's bits is the value times 2^-120; one multiply
-//     by a power of two (times the block's V scale, exact) puts it right, 2.25
-//     instructions an element.  It takes the codes of a 4-byte word as
-//     (0, 2), (1, 3), so the dims of K, V, Q and the output are in that order;
-//     K's scale multiplies the fp32 scores, 32 keys at a time.
-//   * P stays in TMEM: a softmax thread (one per row) reads its scores,
-//     writes bf16 probabilities over them, and the P V MMA takes A from there.
+//   * K is never decoded.  A bf16 query is the sum of two e4m3 numbers (its
+//     upper and its lower 4 significant bits) once its row is scaled by a
+//     power of two, exactly but for bits below 2^-10 of the scaled row (2^-17
+//     of its largest value), so S = Q_hi K^T + Q_lo K^T on the fp8 tensor rate,
+//     twice bf16's: the same time as one bf16 product.  A key's scale
+//     multiplies the fp32 scores.  Tail keys (bf16) are split the same way,
+//     with a power of two per key: four products instead of two.
+//   * V is decoded to fp16 by four warps: one conversion and one multiply per
+//     two codes.  The values are in units of the largest V scale of the CTA's
+//     range (the tail's rows included), found first, so a block's factor is a
+//     power of two at most 1 and only what is below 2^-33 of the largest value
+//     is rounded.
+//   * Codes come by TMA: K straight into the operand layout, V raw.  (Loaded
+//     into registers a block ahead they are waited for at the next proxy fence,
+//     which waits for every load of its warp: 2,200 clocks a block.)
+//   * P stays in TMEM: a softmax thread (one per row) reads its scores 64 at a
+//     time, writes fp16 probabilities over scores that it has read, and the
+//     P V MMA takes A from there.
 //   * O stays in TMEM.  A row's reference maximum moves only when a score
 //     exceeds it by more than 8 (base 2), so O is read, scaled and written
-//     back in the first blocks and hardly ever after (bf16 and fp32 have room
-//     for 2^8).  It is safe then: a lane's scores of block j are issued, hence
-//     complete, after its P V of block j - 1.
-// P is rounded to bf16 (2^-9 relative); sums are fp32 of the unrounded values.
+//     back in the first blocks and hardly ever after (probabilities are kept
+//     times 2^7, which leaves fp16 room for 2^8 and for 2^-31).
+//   * Each lane has its own MMA warp: one that served both spent as long on
+//     waits, commits and descriptors as the tensor core on the products.
+// P is rounded to fp16 (2^-12 relative); sums are fp32 of the unrounded values.
 // TMEM: S / P of lane t in columns [128 t, 128 t + 128), O in [256 + 128 t, ...).
 //
 // Every wait is bounded (sm100_ptx.cuh); one that gives up records its site
@@ -35,6 +45,7 @@
 
 #include "kv8_attn.h"
 #include "sm100_ptx.cuh"
+#include "swiglu.h"
 
 namespace sf {
 namespace {
@@ -44,35 +55,38 @@ __device__ int g_kv8_tc_status;
 constexpr int kD = 128;
 constexpr int kBM = 128;
 constexpr int kKB = 128;
+constexpr int kHalf = 128 * 128;        // a 128-row tile of e4m3 (bytes); hi, then lo
 constexpr int kRegion = 128 * 128;      // one 64-element column region of a 128-row bf16 tile (bytes)
 constexpr int kTileBytes = 2 * kRegion;
 constexpr int kStages = 2;
 constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;
-constexpr int kThreads = (kSoftmaxWarps + kDecodeWarps + 1) * 32;
-constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps;
+constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps;  // and the next: one per lane
+constexpr int kLoadWarp = kMmaWarp + 2;
+constexpr int kThreads = (kLoadWarp + 1) * 32;
 constexpr int kMaxRanges = 64;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
 constexpr float kSlack = 8.f;
+constexpr float kPShift = 7.f;  // probabilities are kept times 2^7
 
 struct __align__(16) Tail {
-  float kf[4][4];  // per block (ring of 4) and 32 keys: scale * log2(e) * K scale; NaN for a block that holds one
+  float qf[2][kBM];  // per row of the Q tiles: the power of two taken out of it; NaN for a row that holds one
+  float unit_top[kDecodeWarps];  // largest V scale seen by each decoder warp
+  float kf[4][kKB];  // per block (ring of 4) and key: scale * log2(e) * K scale; NaN for a key that holds one
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
+  uint64_t raw_full, raw_empty;
   uint64_t s_full[2], p_full[2];
   uint64_t q_ready, mma_done;
   uint32_t tmem_base;
   int abort_flag;
 };
 
-constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + 2 * kStages * kTileBytes + sizeof(Tail);
+constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + 2 * kStages * kTileBytes + kHalf + sizeof(Tail);
 
-// Byte offset of 16-byte chunk c (0..15) of row r: two 64-element regions of
-// 128-byte rows, 128-byte swizzle.
+// Byte offset of 16-byte chunk c of row r of a bf16 tile (c < 16: two
+// 64-element regions) or an e4m3 one (c < 8): 128-byte rows, 128-byte swizzle.
 __device__ __forceinline__ uint32_t sw128(int r, int c) {
   return (uint32_t)((c >> 3) * kRegion + (r >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4));
-}
-__device__ __forceinline__ uint64_t kstep_offset(int k) {
-  return (uint64_t)(((k >> 2) * kRegion + (k & 3) * 32) >> 4);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -80,38 +94,139 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN counts as the least
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
-// Four codes as bf16 pairs (0, 2) and (1, 3), times `mul` (2^120 and more).
-__device__ __forceinline__ void decode4(uint32_t w, uint32_t mul, uint32_t& p02, uint32_t& p13) {
-  const uint32_t x = w << 8;
-  p02 = mul_bf16x2((x & 0x80008000u) | ((x >> 4) & 0x07f007f0u), mul);
-  p13 = mul_bf16x2((w & 0x80008000u) | ((w >> 4) & 0x07f007f0u), mul);
+// Eight codes as fp16, times a power of two.
+__device__ __forceinline__ uint4 decode8(const uint2& c, uint32_t mul) {
+  return make_uint4(mul_f16x2(e4m3x2_to_f16x2(c.x), mul), mul_f16x2(e4m3x2_hi_to_f16x2(c.x), mul),
+                    mul_f16x2(e4m3x2_to_f16x2(c.y), mul), mul_f16x2(e4m3x2_hi_to_f16x2(c.y), mul));
 }
-// bf16 values d0 .. d3 of two words in the same order.
-__device__ __forceinline__ void permute4(uint32_t d01, uint32_t d23, uint32_t& p02, uint32_t& p13) {
-  p02 = __byte_perm(d01, d23, 0x5410);
-  p13 = __byte_perm(d01, d23, 0x7632);
+// Eight bf16 values as fp16, times a power of two; non-finite ones become 0.
+__device__ __forceinline__ uint32_t tail2(uint32_t w, float inv) {
+  const float lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u);
+  return pack_f16x2(fabsf(lo) < INFINITY ? lo * inv : 0.f, fabsf(hi) < INFINITY ? hi * inv : 0.f);
 }
-__device__ __forceinline__ bool nonfinite2(uint32_t w) {
-  return (w & 0x7fffu) >= 0x7f80u || (w & 0x7fff0000u) >= 0x7f800000u;
+__device__ __forceinline__ uint4 tail8(const uint4& x, float inv) {
+  return make_uint4(tail2(x.x, inv), tail2(x.y, inv), tail2(x.z, inv), tail2(x.w, inv));
 }
-__device__ __forceinline__ uint32_t finite2(uint32_t w) {  // non-finite halves become 0
-  if ((w & 0x7fffu) >= 0x7f80u) w &= 0xffff0000u;
-  if ((w & 0x7fff0000u) >= 0x7f800000u) w &= 0xffffu;
-  return w;
+__device__ __forceinline__ uint32_t top2(uint32_t w) { return max(w & 0x7fffu, (w >> 16) & 0x7fffu); }
+// Two bf16 values times `inv` (a power of two that brings them within 448) as
+// e4m3 pairs hi + lo.
+__device__ __forceinline__ void split2(uint32_t w, float inv, uint32_t& hi, uint32_t& lo) {
+  const float2 x = make_float2(__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xffff0000u) * inv);
+  hi = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
+  const uint32_t back = e4m3x2_to_f16x2(hi);
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&back));
+  lo = __nv_cvt_float2_to_fp8x2(make_float2(x.x - h.x, x.y - h.y), __NV_SATFINITE, __NV_E4M3);
+}
+// The largest magnitude (bf16 bits) of a row that eight threads hold, 16 values each.
+__device__ __forceinline__ uint32_t row_top(const uint32_t (&in)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, top2(in[j]));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  return max(top, __shfl_xor_sync(0xffffffffu, top, 4));
+}
+__device__ __forceinline__ void split_store(const uint32_t (&in)[8], float inv, uint8_t* hi_at, uint8_t* lo_at) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t h0, h1, l0, l1;
+    split2(in[2 * j], inv, h0, l0);
+    split2(in[2 * j + 1], inv, h1, l1);
+    h[j] = h0 | (h1 << 16);
+    l[j] = l0 | (l1 << 16);
+  }
+  *reinterpret_cast<uint4*>(hi_at) = make_uint4(h[0], h[1], h[2], h[3]);
+  *reinterpret_cast<uint4*>(lo_at) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+// The largest of 32 scores, scaled.
+__device__ __forceinline__ float scaled_max(const uint32_t (&x)[32], float f) {
+  float a = -INFINITY, d = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    a = max3(a, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+    d = max3(d, __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]));
+  }
+  a = fmaxf(a, d);
+  return a == -INFINITY ? a : a * f;
+}
+// Two fp32 values in one register pair: products and sums of both at once.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t x, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 32 scores to probabilities 2^(f x - base), packed as fp16 pairs into x[0 .. 16).
+__device__ __forceinline__ void probabilities(uint32_t (&x)[32], float f, float base, uint64_t (&ls)[2]) {
+  const uint64_t f2 = pack2(f, f), b2 = pack2(-base, -base);
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    float y0, y1;
+    unpack2(fma2(pack2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), f2, b2), y0, y1);
+    const float p0 = ex2(y0), p1 = ex2(y1);
+    ls[(j >> 1) & 1] = add2(ls[(j >> 1) & 1], pack2(p0, p1));
+    x[j / 2] = pack_f16x2(p0, p1);
+  }
+}
+// 32 scores scaled, key by key, -infinity where the row does not see the key;
+// returns the largest (NaN counts as the least).
+__device__ __forceinline__ float masked_scores(uint32_t (&x)[32], const float* kf, float qf, uint32_t vis) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float y = (vis >> j) & 1u ? __uint_as_float(x[j]) * (kf[j] * qf) : -INFINITY;
+    mx = fmaxf(mx, y);
+    x[j] = __float_as_uint(y);
+  }
+  return mx;
+}
+
+// A warp's wait and arrival, by one lane: 32 lanes at one barrier are served
+// one after another.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int site) {
+  int ok = 0;
+  if ((threadIdx.x & 31) == 0) ok = ptx::mbar_wait(bar, parity, abort_flag, &g_kv8_tc_status, site) ? 1 : 0;
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();  // what the other lanes wrote and fenced is before the arrival
+  if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
-kv8_attn_tc_kernel(Kv8Attn p, int dual, int ranges) {
+kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual, int ranges) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
@@ -119,7 +234,8 @@ kv8_attn_tc_kernel(Kv8Attn p, int dual, int ranges) {
   uint8_t* q_s = smem;
   uint8_t* k_s = q_s + 2 * kTileBytes;
   uint8_t* v_s = k_s + kStages * kTileBytes;
-  Tail* tail = reinterpret_cast<Tail*>(v_s + kStages * kTileBytes);
+  uint8_t* raw_s = v_s + kStages * kTileBytes;  // one block's V codes
+  Tail* tail = reinterpret_cast<Tail*>(raw_s + kHalf);
   volatile int* abort_flag = &tail->abort_flag;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -136,18 +252,21 @@ kv8_attn_tc_kernel(Kv8Attn p, int dual, int ranges) {
   auto block_of = [&](int t, int i) { return dual ? i : 2 * i + t; };
 
   if (threadIdx.x == 0) {
+    const int users = dual ? nlanes : 1;  // lanes that read one block
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(&tail->k_full[s], kDecodeWarps * 32);
-      ptx::mbar_init(&tail->k_empty[s], 1);
-      ptx::mbar_init(&tail->v_full[s], kDecodeWarps * 32);
-      ptx::mbar_init(&tail->v_empty[s], 1);
+      ptx::mbar_init(&tail->k_full[s], kDecodeWarps + 1);  // scales or tail rows, and the copy
+      ptx::mbar_init(&tail->k_empty[s], users);
+      ptx::mbar_init(&tail->v_full[s], kDecodeWarps);
+      ptx::mbar_init(&tail->v_empty[s], users);
     }
+    ptx::mbar_init(&tail->raw_full, 1);
+    ptx::mbar_init(&tail->raw_empty, kDecodeWarps);
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(&tail->s_full[t], 1);
-      ptx::mbar_init(&tail->p_full[t], 128);
+      ptx::mbar_init(&tail->p_full[t], 4);
     }
-    ptx::mbar_init(&tail->q_ready, 256);
-    ptx::mbar_init(&tail->mma_done, 1);
+    ptx::mbar_init(&tail->q_ready, kSoftmaxWarps);
+    ptx::mbar_init(&tail->mma_done, 2);
     tail->abort_flag = 0;
     ptx::fence_mbar_init();
   }
@@ -160,46 +279,80 @@ kv8_attn_tc_kernel(Kv8Attn p, int dual, int ranges) {
   ptx::tc_fence_after();
   const uint32_t tmem = tail->tmem_base;
 
-  if (warp == kMmaWarp) {
-    // ---------------- MMA issuer ----------------
+  if (warp == kLoadWarp) {
+    // ---------------- TMA producer ----------------
     if (lane == 0) {
-      const uint32_t idesc_s = ptx::idesc_bf16_f32(kBM, kKB);
-      const uint32_t idesc_o = ptx::idesc_bf16_f32(kBM, kD) | ptx::kIdescBMajorMN;
-      bool ok = nblocks == 0 || ptx::mbar_wait(&tail->q_ready, 0, abort_flag, &g_kv8_tc_status, 41);
-      auto issue_s = [&](int t, int i) -> bool {
-        const int b = block_of(t, i), s = b % kStages;
-        if (!ptx::mbar_wait(&tail->k_full[s], (b / kStages) & 1, abort_flag, &g_kv8_tc_status, 42)) return false;
-        ptx::tc_fence_after();
-        const uint64_t qdesc = ptx::smem_desc_k_sw128(ptx::smem_u32(q_s + (dual ? t : 0) * kTileBytes));
-        const uint64_t kdesc = ptx::smem_desc_k_sw128(ptx::smem_u32(k_s + s * kTileBytes));
-#pragma unroll
-        for (int k = 0; k < kD / 16; ++k)
-          ptx::umma_f16(tmem + t * kBM, qdesc + kstep_offset(k), kdesc + kstep_offset(k), idesc_s, k != 0);
-        ptx::umma_commit(&tail->s_full[t]);
-        if (!dual || t == nlanes - 1) ptx::umma_commit(&tail->k_empty[s]);
-        return true;
-      };
-      auto issue_o = [&](int t, int i) -> bool {
-        const int b = block_of(t, i), s = b % kStages;
-        if (!ptx::mbar_wait(&tail->v_full[s], (b / kStages) & 1, abort_flag, &g_kv8_tc_status, 43)) return false;
-        if (!ptx::mbar_wait(&tail->p_full[t], i & 1, abort_flag, &g_kv8_tc_status, 44)) return false;
-        ptx::tc_fence_after();
-        const uint64_t vdesc = ptx::smem_desc_mn_sw128(ptx::smem_u32(v_s + s * kTileBytes), kRegion);
-#pragma unroll
-        for (int k = 0; k < kKB / 16; ++k)
-          ptx::umma_f16_ta(tmem + kOCol + t * kD, tmem + t * kBM + k * 8, vdesc + (uint64_t)((k * 16 * 128) >> 4),
-                           idesc_o, i != 0 || k != 0);
-        if (!dual || t == nlanes - 1) ptx::umma_commit(&tail->v_empty[s]);
-        return true;
-      };
-      for (int t = 0; ok && t < nlanes; ++t) ok = lane_blocks(t) == 0 || issue_s(t, 0);
-      for (int i = 0; ok && i < lane_blocks(0); ++i)
-        for (int t = 0; ok && t < nlanes; ++t) {
-          if (i >= lane_blocks(t)) continue;
-          ok = issue_o(t, i);
-          // Over P of block i, which the MMAs just issued read first.
-          if (ok && i + 1 < lane_blocks(t)) ok = issue_s(t, i + 1);
+      const uint8_t* vc = p.c.v + req * p.c.c_bs + kvh * p.c.c_hs;
+      const int coded = max(0, min(nblocks, ((int)p.c.sealed - key_lo) / kKB));  // whole blocks of codes come first
+      int b = 0;
+      bool ok = true;
+      for (; ok && b < nblocks; ++b) {
+        const int s = b % kStages, key0 = key_lo + b * kKB;
+        ok = ptx::mbar_wait(&tail->k_empty[s], ((b / kStages) & 1) ^ 1, abort_flag, &g_kv8_tc_status, 51);
+        if (!ok) break;
+        if (b >= coded) {
+          ptx::mbar_arrive(&tail->k_full[s]);
+          continue;
         }
+        ptx::mbar_arrive_expect_tx(&tail->k_full[s], kHalf);
+        ptx::tma_load_4d(k_s + s * kTileBytes, &tm_k, &tail->k_full[s], 0, key0, kvh, req);
+        ok = ptx::mbar_wait(&tail->raw_empty, (b & 1) ^ 1, abort_flag, &g_kv8_tc_status, 52);
+        if (!ok) break;
+        ptx::mbar_arrive_expect_tx(&tail->raw_full, kHalf);
+        ptx::bulk_load(raw_s, vc + (int64_t)key0 * kD, kHalf, &tail->raw_full);
+      }
+      if (!ok) {  // another role gave up: let the copies in flight land before the CTA ends
+        volatile int never = 0;
+        for (int i = max(0, b - 1); i <= b && i < coded; ++i)
+          ptx::mbar_wait(&tail->k_full[i % kStages], (i / kStages) & 1, &never, &g_kv8_tc_status, 53);
+        if (b > 0 && coded > 0)
+          ptx::mbar_wait(&tail->raw_full, (min(b, coded) - 1) & 1, &never, &g_kv8_tc_status, 54);
+      }
+    }
+  } else if (warp >= kMmaWarp) {
+    // ---------------- MMA issuer of one lane ----------------
+    if (lane == 0) {
+      const int t = warp - kMmaWarp, blocks = t < nlanes ? lane_blocks(t) : 0;
+      const uint32_t idesc_s = ptx::idesc_e4m3_f32(kBM, kKB);
+      const uint32_t idesc_o = ptx::idesc_f16_f32(kBM, kD) | ptx::kIdescBMajorMN;
+      constexpr uint64_t kLo = kHalf >> 4, kStep = 32 >> 4;
+      const uint64_t qdesc = ptx::smem_desc_k_sw128(ptx::smem_u32(q_s + (dual ? t : 0) * kTileBytes));
+      const uint32_t scol = tmem + t * kBM, ocol = tmem + kOCol + t * kD;
+      bool ok = blocks == 0 || ptx::mbar_wait(&tail->q_ready, 0, abort_flag, &g_kv8_tc_status, 41);
+      // O += P V of block i - 1, then S of block i over that block's P, which
+      // the MMAs just issued read first.
+#pragma unroll 1
+      for (int i = 0; ok && i <= blocks && blocks > 0; ++i) {
+        if (i > 0) {
+          const int b = block_of(t, i - 1), s = b % kStages;
+          if (!ptx::mbar_wait(&tail->v_full[s], (b / kStages) & 1, abort_flag, &g_kv8_tc_status, 43) ||
+              !ptx::mbar_wait(&tail->p_full[t], (i - 1) & 1, abort_flag, &g_kv8_tc_status, 44))
+            break;
+          ptx::tc_fence_after();
+          const uint64_t vdesc = ptx::smem_desc_mn_sw128(ptx::smem_u32(v_s + s * kTileBytes), kRegion);
+#pragma unroll
+          for (int k = 0; k < kKB / 16; ++k)
+            ptx::umma_f16_ta(ocol, scol + k * 8, vdesc + (uint64_t)((k * 16 * 128) >> 4), idesc_o, i > 1 || k != 0);
+          ptx::umma_commit(&tail->v_empty[s]);
+        }
+        if (i < blocks) {
+          const int b = block_of(t, i), s = b % kStages;
+          if (!ptx::mbar_wait(&tail->k_full[s], (b / kStages) & 1, abort_flag, &g_kv8_tc_status, 42)) break;
+          ptx::tc_fence_after();
+          const uint64_t kdesc = ptx::smem_desc_k_sw128(ptx::smem_u32(k_s + s * kTileBytes));
+          // hi and lo of Q with K; a block with tail keys has a lower part of K too.
+          const int parts = key_lo + (b + 1) * kKB > (int)p.c.sealed ? 4 : 2;
+#pragma unroll 1
+          for (int x = 0; x < parts; ++x) {
+            const uint64_t qd = qdesc + (x & 1) * kLo, kd = kdesc + (x >> 1) * kLo;
+#pragma unroll
+            for (int k = 0; k < kD / 32; ++k)
+              ptx::umma_f8(scol, qd + k * kStep, kd + k * kStep, idesc_s, x != 0 || k != 0);
+          }
+          ptx::umma_commit(&tail->s_full[t]);
+          ptx::umma_commit(&tail->k_empty[s]);
+        }
+      }
       ptx::umma_commit(&tail->mma_done);
       volatile int never = 0;
       ptx::mbar_wait(&tail->mma_done, 0, &never, &g_kv8_tc_status, 45);
@@ -210,116 +363,180 @@ kv8_attn_tc_kernel(Kv8Attn p, int dual, int ranges) {
     const int row = ct >> 3, part = ct & 7;  // row of 16 in a pass, 16 dims of it
     const int sealed = (int)p.c.sealed;
     const uint8_t* kc = p.c.k + req * p.c.c_bs + kvh * p.c.c_hs + part * 16;
-    const uint8_t* vc = p.c.v + req * p.c.c_bs + kvh * p.c.c_hs + part * 16;
+    const uint8_t* vc = p.c.v + req * p.c.c_bs + kvh * p.c.c_hs + part * 8;  // dims 8 part .. and 64 + 8 part ..
     const float* ksc = p.c.ks + req * p.c.s_bs + kvh * p.c.s_hs;
     const float* vsc = p.c.vs + req * p.c.s_bs + kvh * p.c.s_hs;
     const __nv_bfloat16* kt = p.c.kt + req * p.c.t_bs + kvh * p.c.t_hs + part * 16;
-    const __nv_bfloat16* vt = p.c.vt + req * p.c.t_bs + kvh * p.c.t_hs + part * 16;
-    uint4 kr[8], vr[8];
-    float vs[4], ks = 0.f;
-    auto load = [&](int b) {
+    const __nv_bfloat16* vt = p.c.vt + req * p.c.t_bs + kvh * p.c.t_hs + part * 8;
+    float ks = 0.f, kvs = 0.f, vs[4];  // K and V scale of key ct of the next block; V scales of this one
+    auto load_ks = [&](int b) {
+      const int key = key_lo + b * kKB + ct;
+      if (key < sealed) {
+        ks = ksc[key >> p.c.block_shift];
+        kvs = vsc[key >> p.c.block_shift];
+      }
+    };
+    auto load_vs = [&](int b) {
       const int key0 = key_lo + b * kKB;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int key = key0 + u * 16 + row;
-        if (key < sealed) kr[u] = __ldg(reinterpret_cast<const uint4*>(kc + (int64_t)key * kD));
-      }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int key = key0 + u * 16 + row;
-        if (key < sealed) vr[u] = __ldg(reinterpret_cast<const uint4*>(vc + (int64_t)key * kD));
-      }
-#pragma unroll
-      for (int g = 0; g < 4; ++g) vs[g] = key0 + g * 32 < sealed ? __ldg(vsc + ((key0 + g * 32) >> p.c.block_shift)) : 1.f;
-      if (ct < 4) ks = key0 + ct * 32 < sealed ? __ldg(ksc + ((key0 + ct * 32) >> p.c.block_shift)) : 1.f;
+      for (int g = 0; g < 4; ++g)
+        if (key0 + g * 32 < sealed) vs[g] = vsc[(key0 + g * 32) >> p.c.block_shift];
     };
-    // 16 dims of a row into chunks 2 part and 2 part + 1, the higher dims first
-    // for the upper parts: eight lanes then hit different banks.
-    const int swap = part >> 2;
-    auto store = [&](uint8_t* base, int r, const uint32_t (&w)[8]) {
-      const uint4 lo = make_uint4(w[0], w[1], w[2], w[3]), hi = make_uint4(w[4], w[5], w[6], w[7]);
-      *reinterpret_cast<uint4*>(base + sw128(r, 2 * part + swap)) = swap ? hi : lo;
-      *reinterpret_cast<uint4*>(base + sw128(r, 2 * part + 1 - swap)) = swap ? lo : hi;
-    };
-    if (nblocks > 0) load(0);
-    for (int b = 0; b < nblocks; ++b) {
+    if (nblocks > 0) {
+      load_ks(0);
+      load_vs(0);
+    }
+    // The unit: the largest V scale of the range.
+    float unit = pow2f(kKv8MinExponent);
+    if (key_lo < sealed) {
+      const int last = (min(key_hi, sealed) - 1) >> p.c.block_shift;
+      for (int i = (key_lo >> p.c.block_shift) + ct; i <= last; i += kDecodeWarps * 32) unit = fmaxf(unit, vsc[i]);
+    }
+    {
+      uint32_t top = 0;
+#pragma unroll 4
+      for (int key = max(key_lo, sealed) + row; key < key_hi; key += 16) {
+        const __nv_bfloat16* at = vt + (int64_t)(key - sealed) * kD;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 x = *reinterpret_cast<const uint4*>(at + i * 64);
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = w[j] & 0x7fffu, hi = (w[j] >> 16) & 0x7fffu;
+            top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+          }
+        }
+      }
+      unit = fmaxf(unit, pow2f(kv8_exponent(top)));
+#pragma unroll
+      for (int o = 16; o; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, o));
+      if (lane == 0) tail->unit_top[ct >> 5] = unit;
+      ptx::named_bar_sync(2, kDecodeWarps * 32);
+#pragma unroll
+      for (int i = 0; i < kDecodeWarps; ++i) unit = fmaxf(unit, tail->unit_top[i]);
+    }
+    const float inv = 1.f / unit;  // exact
+    const uint32_t at0 = sw128(row, part);  // 16 rows on: 2,048 bytes
+    // K of block b.  False: a wait gave up.
+    auto store_k = [&](int b) -> bool {
       const int s = b % kStages, key0 = key_lo + b * kKB;
-      const uint32_t ph = (b / kStages) & 1;
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tail->k_empty[s], ph ^ 1, abort_flag, &g_kv8_tc_status, 46))) break;
-      if (ct < 4) {
-        // Ring of four: block b - 4's softmax is over (its K stage was freed twice since).
-        const float v = ct == 0 ? vs[0] : (ct == 1 ? vs[1] : (ct == 2 ? vs[2] : vs[3]));
-        tail->kf[b & 3][ct] = v != v ? v : ks * p.scale_log2;
-      }
-      uint8_t* kst = k_s + s * kTileBytes;
+      if (!warp_wait(&tail->k_empty[s], ((b / kStages) & 1) ^ 1, abort_flag, 46)) return false;
+      // Ring of four: block b - 4's softmax is over.  (The scores that freed this
+      // stage, block b - 2's, were issued after P V of the lane's block before.)
+      float* kf = tail->kf[b & 3];
+      if (key0 + ct < sealed) kf[ct] = kvs != kvs ? kvs : ks * p.scale_log2;
+      uint8_t* kst = k_s + s * kTileBytes + at0;
+      if (key0 + kKB > sealed) {
+        // Tail rows, perhaps behind coded ones (whose lower part is zero); the
+        // next pass's rows are loaded before this one's are split.
+        uint4 x[4], y[4];
+        auto rows = [&](int u, uint4 (&z)[4]) {
+          const int key = key0 + u * 16 + row;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int r = u * 16 + row;
-        uint32_t w[8];
-        if (key0 + u * 16 < sealed) {  // the 16 rows of a pass are all codes or all tail
-          const uint32_t in[4] = {kr[u].x, kr[u].y, kr[u].z, kr[u].w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) decode4(in[j], 0x7b807b80u, w[2 * j], w[2 * j + 1]);
-        } else {
-          uint4 a = make_uint4(0, 0, 0, 0), c = a, x = a, y = a;
-          if (key0 + r < key_hi) {
-            const int64_t at = (int64_t)(key0 + r - sealed) * kD;
-            a = *reinterpret_cast<const uint4*>(kt + at);
-            c = *reinterpret_cast<const uint4*>(kt + at + 8);
-            x = *reinterpret_cast<const uint4*>(vt + at);
-            y = *reinterpret_cast<const uint4*>(vt + at + 8);
+          for (int i = 0; i < 4; ++i) z[i] = make_uint4(0, 0, 0, 0);
+          if (key < sealed) {
+            z[0] = *reinterpret_cast<const uint4*>(kc + (int64_t)key * kD);
+          } else if (key < key_hi) {
+            const int64_t at = (int64_t)(key - sealed) * kD;
+            z[0] = *reinterpret_cast<const uint4*>(kt + at);
+            z[1] = *reinterpret_cast<const uint4*>(kt + at + 8);
+            z[2] = *reinterpret_cast<const uint4*>(vt + at);
+            z[3] = *reinterpret_cast<const uint4*>(vt + at + 64);
           }
-          int bad = nonfinite2(x.x) | nonfinite2(x.y) | nonfinite2(x.z) | nonfinite2(x.w) | nonfinite2(y.x) |
-                    nonfinite2(y.y) | nonfinite2(y.z) | nonfinite2(y.w);
-          bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
-          bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
-          bad |= __shfl_xor_sync(0xffffffffu, bad, 4);
-          permute4(a.x, a.y, w[0], w[1]);
-          permute4(a.z, a.w, w[2], w[3]);
-          permute4(c.x, c.y, w[4], w[5]);
-          permute4(c.z, c.w, w[6], w[7]);
-          if (bad) w[0] = 0x7fc07fc0u;  // a NaN key: rows that see it answer NaN
+        };
+        rows(0, x);
+#pragma unroll 1
+        for (int u = 0; u < 8; ++u) {
+          if (u < 7) rows(u + 1, y);
+          uint8_t* hi_at = kst + u * 2048;
+          if (key0 + u * 16 < sealed) {  // the 16 rows of a pass are all codes or all tail
+            *reinterpret_cast<uint4*>(hi_at) = x[0];
+            *reinterpret_cast<uint4*>(hi_at + kHalf) = x[1];
+          } else {
+            uint32_t in[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+            const uint32_t vals[8] = {x[2].x, x[2].y, x[2].z, x[2].w, x[3].x, x[3].y, x[3].z, x[3].w};
+            const uint32_t top = row_top(in);
+            const bool nan = max(top, row_top(vals)) >= 0x7f80u;  // rows that see the key answer NaN
+            if (nan) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) in[j] = 0;
+            }
+            const int e = nan ? 0 : kv8_exponent(top);
+            split_store(in, pow2f(-e), hi_at, hi_at + kHalf);
+            if (part == 0) kf[u * 16 + row] = nan ? __int_as_float(0x7fc00000) : pow2f(e) * p.scale_log2;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = y[i];
         }
-        store(kst, r, w);
+        ptx::fence_proxy_async_smem();
+      }
+      warp_arrive(&tail->k_full[s]);
+      return true;
+    };
+    auto store_v = [&](int b) -> bool {
+      const int s = b % kStages, key0 = key_lo + b * kKB;
+      const bool coded = key0 + kKB <= sealed;
+      if (coded && !warp_wait(&tail->raw_full, b & 1, abort_flag, 55)) return false;
+      if (!warp_wait(&tail->v_empty[s], ((b / kStages) & 1) ^ 1, abort_flag, 47)) return false;
+      uint8_t* vst = v_s + s * kTileBytes + at0;
+      if (coded) {
+        // The two halves of a row, odd rows the upper one first: four rows of a
+        // warp then cover all banks.
+        const uint8_t* raw = raw_s + row * kD + part * 8;
+        const int h0 = (row & 1) * 64, h1 = 64 - h0;
+        uint8_t *to0 = vst + h0 * (kRegion / 64), *to1 = vst + h1 * (kRegion / 64);
+        uint32_t mul[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float f = vs[g] == vs[g] ? vs[g] * inv : 0.f;  // a block with a NaN counts as zeros
+          mul[g] = pack_f16x2(f, f);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const uint2 a = *reinterpret_cast<const uint2*>(raw + u * 16 * kD + h0);
+          const uint2 c = *reinterpret_cast<const uint2*>(raw + u * 16 * kD + h1);
+          *reinterpret_cast<uint4*>(to0 + u * 2048) = decode8(a, mul[u >> 1]);
+          *reinterpret_cast<uint4*>(to1 + u * 2048) = decode8(c, mul[u >> 1]);
+        }
+        warp_arrive(&tail->raw_empty);
+      } else {
+#pragma unroll 2
+        for (int u = 0; u < 8; ++u) {
+          const int key = key0 + u * 16 + row;
+          uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
+          if (key < sealed) {
+            const float y = vsc[key >> p.c.block_shift];
+            const float f = y == y ? y * inv : 0.f;
+            const uint8_t* at = vc + (int64_t)key * kD;
+            v0 = decode8(*reinterpret_cast<const uint2*>(at), pack_f16x2(f, f));
+            v1 = decode8(*reinterpret_cast<const uint2*>(at + 64), pack_f16x2(f, f));
+          } else if (key < key_hi) {
+            const __nv_bfloat16* at = vt + (int64_t)(key - sealed) * kD;
+            v0 = tail8(*reinterpret_cast<const uint4*>(at), inv);
+            v1 = tail8(*reinterpret_cast<const uint4*>(at + 64), inv);
+          }
+          *reinterpret_cast<uint4*>(vst + u * 2048) = v0;
+          *reinterpret_cast<uint4*>(vst + u * 2048 + kRegion) = v1;
+        }
       }
       ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(&tail->k_full[s]);
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&tail->v_empty[s], ph ^ 1, abort_flag, &g_kv8_tc_status, 47))) break;
-      uint8_t* vst = v_s + s * kTileBytes;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int r = u * 16 + row;
-        uint32_t w[8];
-        if (key0 + u * 16 < sealed) {
-          const uint32_t in[4] = {vr[u].x, vr[u].y, vr[u].z, vr[u].w};
-          const float f = vs[u >> 1];
-          const uint32_t e = f != f ? 0u : (__float_as_uint(f) >> 23) + 120u;  // 2^120 * f, biased
-          // A NaN scale: its codes are zeros and count as zeros here.
-          const uint32_t mul = min(e, 254u) * 0x00800080u;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) decode4(in[j], mul, w[2 * j], w[2 * j + 1]);
-          if (e > 254u) {  // values above 2^16: the rest of the scale in a second product
-            const uint32_t more = (127u + e - 254u) * 0x00800080u;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = mul_bf16x2(w[j], more);
-          }
-        } else {
-          uint4 x = make_uint4(0, 0, 0, 0), y = x;
-          if (key0 + r < key_hi) {
-            const int64_t at = (int64_t)(key0 + r - sealed) * kD;
-            x = *reinterpret_cast<const uint4*>(vt + at);
-            y = *reinterpret_cast<const uint4*>(vt + at + 8);
-          }
-          permute4(finite2(x.x), finite2(x.y), w[0], w[1]);
-          permute4(finite2(x.z), finite2(x.w), w[2], w[3]);
-          permute4(finite2(y.x), finite2(y.y), w[4], w[5]);
-          permute4(finite2(y.z), finite2(y.w), w[6], w[7]);
-        }
-        store(vst, r, w);
+      warp_arrive(&tail->v_full[s]);
+      return true;
+    };
+    // K runs a block ahead of V.  (With one row tile each lane has one stage, and
+    // a V that waited for its lane's last P V in front of the other lane's K
+    // would wait for good.)
+    bool ok = nblocks > 0 && store_k(0);
+    if (ok && nblocks > 1) load_ks(1);
+    for (int b = 0; ok && b < nblocks; ++b) {
+      if (b + 1 < nblocks) {
+        ok = store_k(b + 1);
+        if (!ok) break;
+        if (b + 2 < nblocks) load_ks(b + 2);
       }
-      ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(&tail->v_full[s]);
-      if (b + 1 < nblocks) load(b + 1);
+      ok = store_v(b);
+      if (ok && b + 1 < nblocks) load_vs(b + 1);
     }
   } else {
     // ---------------- softmax / epilogue: one thread per row ----------------
@@ -331,20 +548,38 @@ kv8_attn_tc_kernel(Kv8Attn p, int dual, int ranges) {
     const int row = rok ? pr % p.q_len : 0;
     const int head = kvh * p.group + (rok ? pr / p.q_len : 0);
 
-    if (dual ? t < nlanes : t == 0) {  // Q row -> shared memory
-      const __nv_bfloat16* qrow = p.q + req * p.q_bs + head * p.q_hs + row * p.q_rs;
-      uint8_t* qt = q_s + t * kTileBytes;
-#pragma unroll 4
-      for (int c = 0; c < kD / 8; ++c) {
-        const uint4 x = rok ? *reinterpret_cast<const uint4*>(qrow + c * 8) : make_uint4(0, 0, 0, 0);
-        uint4 y;
-        permute4(x.x, x.y, y.x, y.y);
-        permute4(x.z, x.w, y.z, y.w);
-        *reinterpret_cast<uint4*>(qt + sw128(r, c)) = y;
+    if (dual ? t < nlanes : t == 0) {
+      // Q rows of this tile, eight threads a row, split into their two parts.
+      const int wt = threadIdx.x & 127, qrow = wt >> 3, part = wt & 7;
+      uint8_t* qt = q_s + t * kTileBytes + sw128(qrow, part);
+#pragma unroll 1
+      for (int h = 0; h < 8; h += 4) {  // four rows in flight together
+        uint4 x[4][2];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int at = (tile0 + t) * kBM + (h + u) * 16 + qrow;
+          const bool on = at < packed;
+          const __nv_bfloat16* src = p.q + req * p.q_bs + (int64_t)(kvh * p.group + (on ? at / p.q_len : 0)) * p.q_hs +
+                                     (int64_t)(on ? at % p.q_len : 0) * p.q_rs + part * 16;
+          x[u][0] = on ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+          x[u][1] = on ? *reinterpret_cast<const uint4*>(src + 8) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t in[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
+          const uint32_t top = row_top(in);
+          const bool nan = top >= 0x7f80u;  // the row answers NaN
+          const int e = nan ? 0 : kv8_exponent(top);
+          split_store(in, pow2f(-e), qt + (h + u) * 2048, qt + (h + u) * 2048 + kHalf);
+          if (part == 0) tail->qf[t][(h + u) * 16 + qrow] = nan ? __int_as_float(0x7fc00000) : pow2f(e);
+        }
       }
       ptx::fence_proxy_async_smem();
     }
-    ptx::mbar_arrive(&tail->q_ready);
+    warp_arrive(&tail->q_ready);
+    // The rows' factors come from other warps (the other lane's, with one tile).
+    ptx::named_bar_sync(1, kSoftmaxWarps * 32);
+    const float qf = tail->qf[dual ? t : 0][r];
 
     const uint32_t scol = tmem + ((uint32_t)(quad * 32) << 16) + t * kBM;
     const uint32_t ocol = tmem + ((uint32_t)(quad * 32) << 16) + kOCol + t * kD;
@@ -352,101 +587,95 @@ kv8_attn_tc_kernel(Kv8Attn p, int dual, int ranges) {
     const int n = t < nlanes ? lane_blocks(t) : 0;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int i = 0; i < n; ++i) {
+    for (int i = 0; ok && i < n; ++i) {
       const int b = block_of(t, i), key0 = key_lo + b * kKB;
-      const bool full = key0 + kKB <= p.prefix;
+      const bool full = key0 + kKB <= p.prefix;  // no mask to read
       uint64_t win[2] = {~0ull, ~0ull};
       if (!full) {
         win[0] = rok ? kv8_window(p, rbits, key0) : 0ull;
         win[1] = rok ? kv8_window(p, rbits, key0 + 64) : 0ull;
       }
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&tail->s_full[t], i & 1, abort_flag, &g_kv8_tc_status, 48));
+      ok = warp_wait(&tail->s_full[t], i & 1, abort_flag, 48);
       if (!ok) break;
       ptx::tc_fence_after();
       if (warp_ok) {
-        const float4 f4 = *reinterpret_cast<const float4*>(tail->kf[b & 3]);
-        const float f[4] = {f4.x, f4.y, f4.z, f4.w};
-        float mx = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t sv[32];
-          ptx::tmem_ld_32(scol + c * 32, sv);
-          float a = -INFINITY, d = -INFINITY;
-          if (full) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              a = fmaxf(a, __uint_as_float(sv[j]));
-              d = fmaxf(d, __uint_as_float(sv[j + 1]));
-            }
-          } else {
-            const uint32_t w = (uint32_t)(win[c >> 1] >> ((c & 1) * 32));
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if ((w >> j) & 1u) a = fmaxf(a, __uint_as_float(sv[j]));
-          }
-          a = fmaxf(a, d);
-          mx = fmaxf(mx, a == -INFINITY ? a : a * f[c]);
-        }
-        if (__any_sync(0xffffffffu, mx > m + kSlack || (m == -INFINITY && mx > -INFINITY))) {
-          const float mnew = fmaxf(m, mx);
-          const float alpha = m == -INFINITY ? 1.f : ex2(m - mnew);  // nothing summed yet: O and l are 0
-          m = mnew;
-          l *= alpha;
-          if (i > 0) {
+        // Every key visible and one scale per 32 of them: the rule in a long context.
+        const bool plain = full && key0 + kKB <= (int)p.c.sealed;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t ov[32];
-              ptx::tmem_ld_32(ocol + c * 32, ov);
+        for (int h = 0; h < 2; ++h) {
+          const float* kf = tail->kf[b & 3] + h * 64;
+          uint32_t sa[32], sb[32];
+          ptx::tmem_ld_32_async(scol + h * 64, sa);
+          ptx::tmem_ld_32(scol + h * 64 + 32, sb);
+          float mx, fa = 1.f, fb = 1.f;
+          if (plain) {
+            fa = kf[0] * qf;
+            fb = kf[32] * qf;
+            mx = fmaxf(scaled_max(sa, fa), scaled_max(sb, fb));
+          } else {  // scaled, and -infinity where nothing is seen
+            const uint64_t w = win[h];
+            mx = fmaxf(masked_scores(sa, kf, qf, (uint32_t)w), masked_scores(sb, kf + 32, qf, (uint32_t)(w >> 32)));
+          }
+          if (__any_sync(0xffffffffu, mx > m + kSlack || (m == -INFINITY && mx > -INFINITY))) {
+            const float mnew = fmaxf(m, mx);
+            const float alpha = m == -INFINITY ? 1.f : ex2(m - mnew);  // nothing summed yet: O and l are 0
+            m = mnew;
+            l *= alpha;
+            if (i > 0) {  // P V of the block before is complete, as its successor's scores are
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                uint32_t ov[32];
+                ptx::tmem_ld_32(ocol + c * 32, ov);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
-              ptx::tmem_st_32(ocol + c * 32, ov);
+                for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
+                ptx::tmem_st_32(ocol + c * 32, ov);
+              }
+            }
+            if (h == 1) {  // and the probabilities of this block's first half
+              ptx::tmem_wait_st();
+              const uint32_t a2 = pack_f16x2(alpha, alpha);
+              uint32_t pv[32];
+              ptx::tmem_ld_32(scol, pv);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) pv[j] = mul_f16x2(pv[j], a2);
+              ptx::tmem_st_32(scol, pv);
             }
           }
+          const float base = (m == -INFINITY ? 0.f : m) - kPShift;
+          uint64_t ls[2] = {0, 0};
+          probabilities(sa, fa, base, ls);
+          probabilities(sb, fb, base, ls);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sa[16 + j] = sb[j];
+          ptx::tmem_st_32(scol + h * 32, sa);  // over scores that have been read
+          float l0, l1, l2, l3;
+          unpack2(ls[0], l0, l1);
+          unpack2(ls[1], l2, l3);
+          l += (l0 + l1) + (l2 + l3);
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t sv[32], pk[16];
-          ptx::tmem_ld_32(scol + c * 32, sv);
-          if (full) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float p0 = ex2(fmaf(__uint_as_float(sv[j]), f[c], -base));
-              const float p1 = ex2(fmaf(__uint_as_float(sv[j + 1]), f[c], -base));
-              l0 += p0;
-              l1 += p1;
-              pk[j / 2] = pack_bf16x2(p0, p1);
-            }
-          } else {
-            const uint32_t w = (uint32_t)(win[c >> 1] >> ((c & 1) * 32));
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float p0 = (w >> j) & 1u ? ex2(fmaf(__uint_as_float(sv[j]), f[c], -base)) : 0.f;
-              const float p1 = (w >> (j + 1)) & 1u ? ex2(fmaf(__uint_as_float(sv[j + 1]), f[c], -base)) : 0.f;
-              l0 += p0;
-              l1 += p1;
-              pk[j / 2] = pack_bf16x2(p0, p1);
-            }
-          }
-          ptx::tmem_st_16(scol + c * 16, pk);  // columns whose scores have been read
-        }
-        l += l0 + l1;
         ptx::tmem_wait_st();
       }
       ptx::tc_fence_before();
-      ptx::mbar_arrive(&tail->p_full[t]);
+      warp_arrive(&tail->p_full[t]);
     }
     // The output rows of this lane.
     const bool mine = dual ? t < nlanes : true;  // one row tile: both lanes write a partial result
-    if (ok && mine && n > 0)
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&tail->mma_done, 0, abort_flag, &g_kv8_tc_status, 49));
+    if (ok && mine && nblocks > 0)  // also before shared memory is used again
+      ok = warp_wait(&tail->mma_done, 0, abort_flag, 49);
     if (ok && mine && pr - lane < packed) {
       ptx::tc_fence_after();
       const bool direct = p.splits == 1;
       const int part = dual ? range : 2 * range + t;
       const int64_t idx = (((int64_t)req * p.splits + part) * p.heads + head) * p.q_len + row;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float f = 1.f;  // O is in units of the largest V scale
+#pragma unroll
+      for (int i = 0; i < kDecodeWarps; ++i) f = i == 0 ? tail->unit_top[0] : fmaxf(f, tail->unit_top[i]);
+      if (n == 0) f = 0.f;  // nothing decoded, nothing to scale
+      if (direct) f = l == 0.f ? 0.f : f / l;
+      // Rows leave in whole lines: 32 rows x 32 columns at a time through this
+      // warp's part of the K stages, which no MMA reads any more.
+      const int64_t off = rok ? (direct ? (int64_t)req * p.out_bs + ((int64_t)row * p.heads + head) * kD : idx * kD) : -1;
+      uint8_t* turn = k_s + warp * 32 * 144;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t ov[32];
@@ -456,32 +685,48 @@ kv8_attn_tc_kernel(Kv8Attn p, int dual, int ranges) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) ov[j] = 0;
         }
-        if (!rok) continue;
+        __syncwarp();
         if (direct) {
-          __nv_bfloat16* dst = p.out + req * p.out_bs + ((int64_t)row * p.heads + head) * kD + c * 32;
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            uint4 w;
-            w.x = pack_bf16x2(__uint_as_float(ov[j]) * inv, __uint_as_float(ov[j + 2]) * inv);
-            w.y = pack_bf16x2(__uint_as_float(ov[j + 1]) * inv, __uint_as_float(ov[j + 3]) * inv);
-            w.z = pack_bf16x2(__uint_as_float(ov[j + 4]) * inv, __uint_as_float(ov[j + 6]) * inv);
-            w.w = pack_bf16x2(__uint_as_float(ov[j + 5]) * inv, __uint_as_float(ov[j + 7]) * inv);
-            *reinterpret_cast<uint4*>(dst + j) = w;
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = pack_bf16x2(__uint_as_float(ov[8 * j + 2 * k]) * f, __uint_as_float(ov[8 * j + 2 * k + 1]) * f);
+            *reinterpret_cast<uint4*>(turn + lane * 80 + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          __syncwarp();
+#pragma unroll 1
+          for (int k = 0; k < 4; ++k) {
+            const int rr = k * 8 + (lane >> 2), col = lane & 3;
+            const int64_t o = __shfl_sync(0xffffffffu, off, rr);
+            const uint4 w = *reinterpret_cast<const uint4*>(turn + rr * 80 + col * 16);
+            if (o >= 0) *reinterpret_cast<uint4*>(p.out + o + c * 32 + col * 8) = w;
           }
         } else {
-          float* dst = p.part_o + idx * kD + c * 32;
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<uint4*>(dst + j) = make_uint4(ov[j], ov[j + 2], ov[j + 1], ov[j + 3]);
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(turn + lane * 144 + j * 16) =
+                make_float4(__uint_as_float(ov[4 * j]) * f, __uint_as_float(ov[4 * j + 1]) * f,
+                            __uint_as_float(ov[4 * j + 2]) * f, __uint_as_float(ov[4 * j + 3]) * f);
+          __syncwarp();
+#pragma unroll 2
+          for (int k = 0; k < 8; ++k) {
+            const int rr = k * 4 + (lane >> 3), col = lane & 7;
+            const int64_t o = __shfl_sync(0xffffffffu, off, rr);
+            const float4 w = *reinterpret_cast<const float4*>(turn + rr * 144 + col * 16);
+            if (o >= 0) *reinterpret_cast<float4*>(p.part_o + o + c * 32 + col * 4) = w;
+          }
         }
       }
       if (rok) {
+        const float ref = m == -INFINITY ? m : m - kPShift;  // l carries the 2^7
         if (direct) {
           if (p.lse)
             p.lse[((int64_t)req * p.heads + head) * p.q_len + row] =
-                l == 0.f ? -INFINITY : (m == -INFINITY ? l : (m + log2f(l)) * 0.69314718055994531f);
+                l == 0.f ? -INFINITY : (m == -INFINITY ? l : (ref + log2f(l)) * 0.69314718055994531f);
         } else {
-          p.part_ml[idx * 2] = m;
+          p.part_ml[idx * 2] = ref;
           p.part_ml[idx * 2 + 1] = l;
         }
       }
@@ -509,6 +754,11 @@ Shape shape_of(int64_t packed) {
 }  // namespace
 
 bool kv8_use_tc(int head_dim, int64_t packed, int64_t kv_len) { return head_dim == kD && packed >= 48 && kv_len > 0; }
+
+// Heads and requests of their own rows: what a tensor map can describe.
+bool kv8_tc_layout(const Kv8Rows& c, int batch) {
+  return (c.hkv == 1 || c.c_hs >= c.sealed * kD) && (batch == 1 || c.c_bs >= c.sealed * kD);
+}
 
 // The number of key ranges that minimises (waves of CTAs) x (blocks of a CTA
 // + its fixed cost, about three blocks: set-up, Q, the pipeline's fill and
@@ -543,8 +793,18 @@ int kv8_attention_tc(const Kv8Attn& p, cudaStream_t stream) {
   const Shape sh = shape_of((int64_t)p.group * p.q_len);
   const int ranges = sh.dual ? p.splits : p.splits / 2;
   SF_CHECK_ARG(sh.pairs < 65536 && (int64_t)ranges * p.batch < 65536, "too many query rows or requests");
+  // K's codes, 16 bits at a time (bytes are bytes): [batch][heads][tokens][64].
+  CUtensorMap tm_k = {};
+  if (p.c.sealed >= kKB) {
+    const cuuint64_t dims[4] = {64, (cuuint64_t)p.c.sealed, (cuuint64_t)p.c.hkv, (cuuint64_t)p.batch};
+    const int64_t hs = p.c.hkv > 1 ? p.c.c_hs : p.c.sealed * kD, bs = p.batch > 1 ? p.c.c_bs : p.c.hkv * hs;
+    const cuuint64_t strides[3] = {kD, (cuuint64_t)hs, (cuuint64_t)bs};
+    const cuuint32_t box[4] = {64, kKB, 1, 1};
+    if (int rc = tma_encode_bf16(&tm_k, p.c.k, 4, dims, strides, box)) return rc;
+  }
   const dim3 grid((unsigned)p.c.hkv, (unsigned)sh.pairs, (unsigned)(ranges * p.batch));
-  SF_CHECK_CUDA(launch_pdl(kv8_attn_tc_kernel, grid, dim3(kThreads), kSmemBytes, stream, p, sh.dual ? 1 : 0, ranges));
+  SF_CHECK_CUDA(launch_pdl(kv8_attn_tc_kernel, grid, dim3(kThreads), kSmemBytes, stream, tm_k, p, sh.dual ? 1 : 0,
+                           ranges));
   SF_CHECK_LAUNCH();
   return SF_OK;
 }
