@@ -576,6 +576,7 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
   p.heads = num_heads;
   p.group = group;
   p.q_len = (int)q_len;
+  p.q_magic = ((1ull << 40) + (uint64_t)q_len - 1) / (uint64_t)q_len;
   p.kv_len = (int)kv_len;
   p.prefix = (int)prefix_len;
   p.scale = scale;

@@ -15,6 +15,10 @@ struct Kv8Attn {
   int words;
   int64_t bits_bs;
   int batch, heads, group, q_len;
+  // ceil(2^40 / q_len): n / q_len = (n * q_magic) >> 40 for n, q_len < 2^20.
+  // (q_magic * q_len exceeds 2^40 by less than q_len, so the quotient by less
+  // than n / 2^40 < 1 / q_len.)
+  uint64_t q_magic;
   int kv_len, prefix;
   float scale, scale_log2;  // the softmax scale, and times log2(e)
   int splits, keys_per_split;

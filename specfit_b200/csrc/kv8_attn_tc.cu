@@ -27,15 +27,20 @@
 //   * Codes come by TMA: K straight into the operand layout, V raw.  (Loaded
 //     into registers a block ahead they are waited for at the next proxy fence,
 //     which waits for every load of its warp: 2,200 clocks a block.)
-//   * P stays in TMEM: a softmax thread (one per row) reads its scores 64 at a
-//     time, writes fp16 probabilities over scores that it has read, and the
-//     P V MMA takes A from there.
+//   * P stays in TMEM: two softmax threads a row (sixteen warps: with eight a
+//     scheduler had too little to issue) read 64 scores each, write fp16
+//     probabilities over scores that they have read, and the P V MMA takes A
+//     from there.  The two meet once a block, at a barrier that also says
+//     whether either half's maximum is above the reference.
 //   * O stays in TMEM.  A row's reference maximum moves only when a score
 //     exceeds it by more than 8 (base 2), so O is read, scaled and written
 //     back in the first blocks and hardly ever after (probabilities are kept
 //     times 2^7, which leaves fp16 room for 2^8 and for 2^-31).
 //   * Each lane has its own MMA warp: one that served both spent as long on
-//     waits, commits and descriptors as the tensor core on the products.
+//     waits, commits and descriptors as the tensor core on the products.  A lock
+//     keeps a lane's P V and next S together: interleaved, both lanes get their
+//     scores late and at once, and then fight for the exponentials; one after
+//     the other, a lane's softmax runs under the other's products.
 // P is rounded to fp16 (2^-12 relative); sums are fp32 of the unrounded values.
 // TMEM: S / P of lane t in columns [128 t, 128 t + 128), O in [256 + 128 t, ...).
 //
@@ -59,7 +64,7 @@ constexpr int kHalf = 128 * 128;        // a 128-row tile of e4m3 (bytes); hi, t
 constexpr int kRegion = 128 * 128;      // one 64-element column region of a 128-row bf16 tile (bytes)
 constexpr int kTileBytes = 2 * kRegion;
 constexpr int kStages = 2;
-constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4;
+constexpr int kSoftmaxWarps = 16, kDecodeWarps = 4;
 constexpr int kMmaWarp = kSoftmaxWarps + kDecodeWarps;  // and the next: one per lane
 constexpr int kLoadWarp = kMmaWarp + 2;
 constexpr int kThreads = (kLoadWarp + 1) * 32;
@@ -71,6 +76,8 @@ constexpr float kPShift = 7.f;  // probabilities are kept times 2^7
 
 struct __align__(16) Tail {
   float qf[2][kBM];  // per row of the Q tiles: the power of two taken out of it; NaN for a row that holds one
+  float red[2][2][kBM], sum[2][2][kBM];  // per lane, half and row: maxima and final sums, for the other half
+  int pair_ok[kSoftmaxWarps];
   float unit_top[kDecodeWarps];  // largest V scale seen by each decoder warp
   float kf[4][kKB];  // per block (ring of 4) and key: scale * log2(e) * K scale; NaN for a key that holds one
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
@@ -79,6 +86,7 @@ struct __align__(16) Tail {
   uint64_t q_ready, mma_done;
   uint32_t tmem_base;
   int abort_flag;
+  int tensor_lock;  // held by the lane that is issuing its products
 };
 
 constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + 2 * kStages * kTileBytes + kHalf + sizeof(Tail);
@@ -126,21 +134,24 @@ __device__ __forceinline__ uint32_t tail2(uint32_t w, float inv) {
 __device__ __forceinline__ uint4 tail8(const uint4& x, float inv) {
   return make_uint4(tail2(x.x, inv), tail2(x.y, inv), tail2(x.z, inv), tail2(x.w, inv));
 }
-__device__ __forceinline__ uint32_t top2(uint32_t w) { return max(w & 0x7fffu, (w >> 16) & 0x7fffu); }
 // Two bf16 values times `inv` (a power of two that brings them within 448) as
-// e4m3 pairs hi + lo.
+// e4m3 pairs hi + lo, by way of fp16, which holds them exactly down to 2^-17.
 __device__ __forceinline__ void split2(uint32_t w, float inv, uint32_t& hi, uint32_t& lo) {
-  const float2 x = make_float2(__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xffff0000u) * inv);
-  hi = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
-  const uint32_t back = e4m3x2_to_f16x2(hi);
-  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&back));
-  lo = __nv_cvt_float2_to_fp8x2(make_float2(x.x - h.x, x.y - h.y), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t x = pack_f16x2(__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xffff0000u) * inv);
+  uint16_t h, l;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(x));
+  const uint32_t back = e4m3x2_to_f16x2(h);
+  const __half2 rest = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&back));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
+  hi = h;
+  lo = l;
 }
 // The largest magnitude (bf16 bits) of a row that eight threads hold, 16 values each.
 __device__ __forceinline__ uint32_t row_top(const uint32_t (&in)[8]) {
-  uint32_t top = 0;
+  uint32_t top2 = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, top2(in[j]));
+  for (int j = 0; j < 8; ++j) top2 = __vmaxu2(top2, in[j] & 0x7fff7fffu);
+  uint32_t top = max(top2 & 0xffffu, top2 >> 16);
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
   return max(top, __shfl_xor_sync(0xffffffffu, top, 4));
@@ -152,8 +163,8 @@ __device__ __forceinline__ void split_store(const uint32_t (&in)[8], float inv, 
     uint32_t h0, h1, l0, l1;
     split2(in[2 * j], inv, h0, l0);
     split2(in[2 * j + 1], inv, h1, l1);
-    h[j] = h0 | (h1 << 16);
-    l[j] = l0 | (l1 << 16);
+    h[j] = __byte_perm(h0, h1, 0x5410);
+    l[j] = __byte_perm(l0, l1, 0x5410);
   }
   *reinterpret_cast<uint4*>(hi_at) = make_uint4(h[0], h[1], h[2], h[3]);
   *reinterpret_cast<uint4*>(lo_at) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -188,8 +199,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 32 scores to probabilities 2^(f x - base), packed as fp16 pairs into x[0 .. 16).
-__device__ __forceinline__ void probabilities(uint32_t (&x)[32], float f, float base, uint64_t (&ls)[2]) {
+// 32 scores to probabilities 2^(f x - base), as fp16 pairs, and their sums.
+__device__ __forceinline__ void probabilities(const uint32_t (&x)[32], float f, float base, uint64_t (&ls)[2],
+                                              uint32_t (&pk)[16]) {
   const uint64_t f2 = pack2(f, f), b2 = pack2(-base, -base);
 #pragma unroll
   for (int j = 0; j < 32; j += 2) {
@@ -197,7 +209,7 @@ __device__ __forceinline__ void probabilities(uint32_t (&x)[32], float f, float 
     unpack2(fma2(pack2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), f2, b2), y0, y1);
     const float p0 = ex2(y0), p1 = ex2(y1);
     ls[(j >> 1) & 1] = add2(ls[(j >> 1) & 1], pack2(p0, p1));
-    x[j / 2] = pack_f16x2(p0, p1);
+    pk[j / 2] = pack_f16x2(p0, p1);
   }
 }
 // 32 scores scaled, key by key, -infinity where the row does not see the key;
@@ -213,6 +225,18 @@ __device__ __forceinline__ float masked_scores(uint32_t (&x)[32], const float* k
   return mx;
 }
 
+// Whether any of the 64 threads that meet at barrier `id` says so.
+__device__ __forceinline__ bool pair_any(int id, bool mine) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)mine), "r"(id)
+      : "memory");
+  return r != 0;
+}
+
 // A warp's wait and arrival, by one lane: 32 lanes at one barrier are served
 // one after another.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int site) {
@@ -224,6 +248,28 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   __syncwarp();  // what the other lanes wrote and fenced is before the arrival
   if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar);
 }
+
+// One lane's turn at the tensor core.  False: the wait gave up.
+__device__ __forceinline__ bool take_turn(int* lock, volatile int* abort_flag, int site) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    if (atomicCAS_block(lock, 0, 1) == 0) return true;
+    if ((i & 15u) == 15u) {
+      if (*abort_flag) return false;
+      const uint64_t now = ptx::globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > ptx::kWaitLimitNs) {
+        *abort_flag = 1;
+        atomicCAS(&g_kv8_tc_status, 0, site);
+        return false;
+      }
+    }
+  }
+}
+
+// The query head (within its group) of packed row n: n / q_len.
+__device__ __forceinline__ int row_head(const Kv8Attn& p, int n) { return (int)(((uint64_t)n * p.q_magic) >> 40); }
 
 __global__ void __launch_bounds__(kThreads, 1)
 kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual, int ranges) {
@@ -263,11 +309,12 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
     ptx::mbar_init(&tail->raw_empty, kDecodeWarps);
     for (int t = 0; t < 2; ++t) {
       ptx::mbar_init(&tail->s_full[t], 1);
-      ptx::mbar_init(&tail->p_full[t], 4);
+      ptx::mbar_init(&tail->p_full[t], kSoftmaxWarps / 2);
     }
     ptx::mbar_init(&tail->q_ready, kSoftmaxWarps);
     ptx::mbar_init(&tail->mma_done, 2);
     tail->abort_flag = 0;
+    tail->tensor_lock = 0;
     ptx::fence_mbar_init();
   }
   if (warp == kMmaWarp) {
@@ -323,25 +370,26 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
       // the MMAs just issued read first.
 #pragma unroll 1
       for (int i = 0; ok && i <= blocks && blocks > 0; ++i) {
+        const int bo = block_of(t, i - 1), so = bo & 1, bs = block_of(t, i), ss = bs & 1;
+        if (i < blocks && !ptx::mbar_wait(&tail->k_full[ss], (bs / kStages) & 1, abort_flag, &g_kv8_tc_status, 42)) break;
+        if (i > 0 &&
+            (!ptx::mbar_wait(&tail->v_full[so], (bo / kStages) & 1, abort_flag, &g_kv8_tc_status, 43) ||
+             !ptx::mbar_wait(&tail->p_full[t], (i - 1) & 1, abort_flag, &g_kv8_tc_status, 44)))
+          break;
+        if (!take_turn(&tail->tensor_lock, abort_flag, 56)) break;
+        ptx::tc_fence_after();
         if (i > 0) {
-          const int b = block_of(t, i - 1), s = b % kStages;
-          if (!ptx::mbar_wait(&tail->v_full[s], (b / kStages) & 1, abort_flag, &g_kv8_tc_status, 43) ||
-              !ptx::mbar_wait(&tail->p_full[t], (i - 1) & 1, abort_flag, &g_kv8_tc_status, 44))
-            break;
-          ptx::tc_fence_after();
-          const uint64_t vdesc = ptx::smem_desc_mn_sw128(ptx::smem_u32(v_s + s * kTileBytes), kRegion);
+          const uint64_t vdesc = ptx::smem_desc_mn_sw128(ptx::smem_u32(v_s + so * kTileBytes), kRegion);
 #pragma unroll
           for (int k = 0; k < kKB / 16; ++k)
-            ptx::umma_f16_ta(ocol, scol + k * 8, vdesc + (uint64_t)((k * 16 * 128) >> 4), idesc_o, i > 1 || k != 0);
-          ptx::umma_commit(&tail->v_empty[s]);
+            ptx::umma_f16_ta(ocol, scol + (k >> 2) * 64 + (k & 3) * 8, vdesc + (uint64_t)((k * 16 * 128) >> 4), idesc_o,
+                             i > 1 || k != 0);
+          ptx::umma_commit(&tail->v_empty[so]);
         }
         if (i < blocks) {
-          const int b = block_of(t, i), s = b % kStages;
-          if (!ptx::mbar_wait(&tail->k_full[s], (b / kStages) & 1, abort_flag, &g_kv8_tc_status, 42)) break;
-          ptx::tc_fence_after();
-          const uint64_t kdesc = ptx::smem_desc_k_sw128(ptx::smem_u32(k_s + s * kTileBytes));
+          const uint64_t kdesc = ptx::smem_desc_k_sw128(ptx::smem_u32(k_s + ss * kTileBytes));
           // hi and lo of Q with K; a block with tail keys has a lower part of K too.
-          const int parts = key_lo + (b + 1) * kKB > (int)p.c.sealed ? 4 : 2;
+          const int parts = key_lo + (bs + 1) * kKB > (int)p.c.sealed ? 4 : 2;
 #pragma unroll 1
           for (int x = 0; x < parts; ++x) {
             const uint64_t qd = qdesc + (x & 1) * kLo, kd = kdesc + (x >> 1) * kLo;
@@ -350,8 +398,9 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
               ptx::umma_f8(scol, qd + k * kStep, kd + k * kStep, idesc_s, x != 0 || k != 0);
           }
           ptx::umma_commit(&tail->s_full[t]);
-          ptx::umma_commit(&tail->k_empty[s]);
+          ptx::umma_commit(&tail->k_empty[ss]);
         }
+        atomicExch_block(&tail->tensor_lock, 0);
       }
       ptx::umma_commit(&tail->mma_done);
       volatile int never = 0;
@@ -539,124 +588,137 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
       if (ok && b + 1 < nblocks) load_vs(b + 1);
     }
   } else {
-    // ---------------- softmax / epilogue: one thread per row ----------------
-    const int t = warp >> 2, quad = warp & 3;
+    // ---------------- softmax / epilogue: two threads per row ----------------
+    const int t = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
+    const int pair_bar = 3 + t * 4 + quad;  // the two warps of a lane's quadrant
     const int r = quad * 32 + lane;
     const int pr = (tile0 + (dual ? t : 0)) * kBM + r;
     const bool rok = pr < packed;
-    const bool warp_ok = t < nlanes && pr - lane < packed;  // uniform over the warp
-    const int row = rok ? pr % p.q_len : 0;
-    const int head = kvh * p.group + (rok ? pr / p.q_len : 0);
+    const bool warp_ok = t < nlanes && pr - lane < packed;  // uniform over the pair of warps
+    const int qhead = rok ? row_head(p, pr) : 0, row = rok ? pr - qhead * p.q_len : 0;
+    const int head = kvh * p.group + qhead;
 
-    if (dual ? t < nlanes : t == 0) {
-      // Q rows of this tile, eight threads a row, split into their two parts.
-      const int wt = threadIdx.x & 127, qrow = wt >> 3, part = wt & 7;
-      uint8_t* qt = q_s + t * kTileBytes + sw128(qrow, part);
-#pragma unroll 1
-      for (int h = 0; h < 8; h += 4) {  // four rows in flight together
-        uint4 x[4][2];
+    if (dual ? t < nlanes : true) {
+      // Q rows, eight threads a row, split into their two parts: the lane's own
+      // tile by its eight warps, or the one tile by all sixteen.  Rows past the
+      // last are left as they are: their scores are not looked at.
+      const int per = dual ? 32 : 64, wt = dual ? threadIdx.x & 255 : threadIdx.x;
+      const int qrow = wt >> 3, part = wt & 7, first = (tile0 + (dual ? t : 0)) * kBM;
+      uint8_t* qt = q_s + (dual ? t : 0) * kTileBytes + sw128(qrow, part);
+      uint4 x[4][2];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int at = (tile0 + t) * kBM + (h + u) * 16 + qrow;
-          const bool on = at < packed;
-          const __nv_bfloat16* src = p.q + req * p.q_bs + (int64_t)(kvh * p.group + (on ? at / p.q_len : 0)) * p.q_hs +
-                                     (int64_t)(on ? at % p.q_len : 0) * p.q_rs + part * 16;
-          x[u][0] = on ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-          x[u][1] = on ? *reinterpret_cast<const uint4*>(src + 8) : make_uint4(0, 0, 0, 0);
-        }
+      for (int u = 0; u < 4; ++u) {  // all rows in flight together
+        const int at = first + u * per + qrow;
+        const bool on = u * per < kBM && at < packed;
+        const int h = on ? row_head(p, at) : 0, tt = on ? at - h * p.q_len : 0;
+        const __nv_bfloat16* src = p.q + req * p.q_bs + (int64_t)(kvh * p.group + h) * p.q_hs + (int64_t)tt * p.q_rs +
+                                   part * 16;
+        x[u][0] = on ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+        x[u][1] = on ? *reinterpret_cast<const uint4*>(src + 8) : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t in[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
-          const uint32_t top = row_top(in);
-          const bool nan = top >= 0x7f80u;  // the row answers NaN
-          const int e = nan ? 0 : kv8_exponent(top);
-          split_store(in, pow2f(-e), qt + (h + u) * 2048, qt + (h + u) * 2048 + kHalf);
-          if (part == 0) tail->qf[t][(h + u) * 16 + qrow] = nan ? __int_as_float(0x7fc00000) : pow2f(e);
-        }
+      for (int u = 0; u < 4; ++u) {
+        if (u * per >= kBM || first + u * per + (qrow & ~3) >= packed) continue;  // uniform over the warp
+        const uint32_t in[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
+        const uint32_t top = row_top(in);
+        const bool nan = top >= 0x7f80u;  // the row answers NaN
+        const int e = nan ? 0 : kv8_exponent(top);
+        uint8_t* at = qt + u * per * 128;
+        split_store(in, pow2f(-e), at, at + kHalf);
+        if (part == 0) tail->qf[dual ? t : 0][u * per + qrow] = nan ? __int_as_float(0x7fc00000) : pow2f(e);
       }
       ptx::fence_proxy_async_smem();
     }
     warp_arrive(&tail->q_ready);
-    // The rows' factors come from other warps (the other lane's, with one tile).
-    ptx::named_bar_sync(1, kSoftmaxWarps * 32);
-    const float qf = tail->qf[dual ? t : 0][r];
+    ptx::named_bar_sync(1, kSoftmaxWarps * 32);  // the rows' factors come from other warps
+    const float qf = rok ? tail->qf[dual ? t : 0][r] : 0.f;
 
-    const uint32_t scol = tmem + ((uint32_t)(quad * 32) << 16) + t * kBM;
-    const uint32_t ocol = tmem + ((uint32_t)(quad * 32) << 16) + kOCol + t * kD;
+    const uint32_t scol = tmem + ((uint32_t)(quad * 32) << 16) + t * kBM + half * 64;  // this half's scores
+    const uint32_t ocol = tmem + ((uint32_t)(quad * 32) << 16) + kOCol + t * kD + half * 64;
     const uint32_t* rbits = p.bits ? p.bits + req * p.bits_bs + (int64_t)row * p.words : nullptr;
     const int n = t < nlanes ? lane_blocks(t) : 0;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int i = 0; ok && i < n; ++i) {
-      const int b = block_of(t, i), key0 = key_lo + b * kKB;
-      const bool full = key0 + kKB <= p.prefix;  // no mask to read
-      uint64_t win[2] = {~0ull, ~0ull};
-      if (!full) {
-        win[0] = rok ? kv8_window(p, rbits, key0) : 0ull;
-        win[1] = rok ? kv8_window(p, rbits, key0 + 64) : 0ull;
-      }
+    for (int i = 0; i < n; ++i) {
+      const int b = block_of(t, i), key0 = key_lo + b * kKB + half * 64;
+      const bool full = key0 + 64 <= p.prefix;  // no mask to read
+      uint64_t win = ~0ull;
+      if (!full) win = rok ? kv8_window(p, rbits, key0) : 0ull;
       ok = warp_wait(&tail->s_full[t], i & 1, abort_flag, 48);
-      if (!ok) break;
-      ptx::tc_fence_after();
       if (warp_ok) {
         // Every key visible and one scale per 32 of them: the rule in a long context.
-        const bool plain = full && key0 + kKB <= (int)p.c.sealed;
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          const float* kf = tail->kf[b & 3] + h * 64;
-          uint32_t sa[32], sb[32];
-          ptx::tmem_ld_32_async(scol + h * 64, sa);
-          ptx::tmem_ld_32(scol + h * 64 + 32, sb);
-          float mx, fa = 1.f, fb = 1.f;
+        const bool plain = full && key0 + 64 <= (int)p.c.sealed;
+        const float* kf = tail->kf[b & 3] + half * 64;
+        float mx = -INFINITY, f0 = 1.f, f1 = 1.f;
+        uint32_t s0[32];
+        if (ok) {
+          ptx::tc_fence_after();
           if (plain) {
-            fa = kf[0] * qf;
-            fb = kf[32] * qf;
-            mx = fmaxf(scaled_max(sa, fa), scaled_max(sb, fb));
-          } else {  // scaled, and -infinity where nothing is seen
-            const uint64_t w = win[h];
-            mx = fmaxf(masked_scores(sa, kf, qf, (uint32_t)w), masked_scores(sb, kf + 32, qf, (uint32_t)(w >> 32)));
+            f0 = kf[0] * qf;
+            f1 = kf[32] * qf;
+            ptx::tmem_ld_32(scol, s0);
+            mx = scaled_max(s0, f0);
+            ptx::tmem_ld_32(scol + 32, s0);
+            mx = fmaxf(mx, scaled_max(s0, f1));
+          } else {
+            ptx::tmem_ld_32(scol, s0);
+            mx = masked_scores(s0, kf, qf, (uint32_t)win);
+            ptx::tmem_ld_32(scol + 32, s0);
+            mx = fmaxf(mx, masked_scores(s0, kf + 32, qf, (uint32_t)(win >> 32)));
           }
-          if (__any_sync(0xffffffffu, mx > m + kSlack || (m == -INFINITY && mx > -INFINITY))) {
-            const float mnew = fmaxf(m, mx);
-            const float alpha = m == -INFINITY ? 1.f : ex2(m - mnew);  // nothing summed yet: O and l are 0
-            m = mnew;
-            l *= alpha;
-            if (i > 0) {  // P V of the block before is complete, as its successor's scores are
-#pragma unroll 1
-              for (int c = 0; c < 4; ++c) {
-                uint32_t ov[32];
-                ptx::tmem_ld_32(ocol + c * 32, ov);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * alpha);
-                ptx::tmem_st_32(ocol + c * 32, ov);
-              }
-            }
-            if (h == 1) {  // and the probabilities of this block's first half
-              ptx::tmem_wait_st();
-              const uint32_t a2 = pack_f16x2(alpha, alpha);
-              uint32_t pv[32];
-              ptx::tmem_ld_32(scol, pv);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) pv[j] = mul_f16x2(pv[j], a2);
-              ptx::tmem_st_32(scol, pv);
-            }
-          }
-          const float base = (m == -INFINITY ? 0.f : m) - kPShift;
-          uint64_t ls[2] = {0, 0};
-          probabilities(sa, fa, base, ls);
-          probabilities(sb, fb, base, ls);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) sa[16 + j] = sb[j];
-          ptx::tmem_st_32(scol + h * 32, sa);  // over scores that have been read
-          float l0, l1, l2, l3;
-          unpack2(ls[0], l0, l1);
-          unpack2(ls[1], l2, l3);
-          l += (l0 + l1) + (l2 + l3);
+          ptx::tmem_ld_32_async(scol, s0);  // once more, now for the probabilities
         }
+        if (pair_any(pair_bar, !ok || mx > m + kSlack || (m == -INFINITY && mx > -INFINITY))) {
+          // The other half's maximum, and whether its wait succeeded: both warps
+          // of the pair go on or stop together.
+          tail->red[t][half][r] = mx;
+          if (lane == 0) tail->pair_ok[warp] = ok ? 1 : 0;
+          ptx::named_bar_sync(pair_bar, 64);
+          if (!tail->pair_ok[warp] || !tail->pair_ok[warp ^ 4]) {
+            ok = false;
+            break;
+          }
+          const float mnew = fmaxf(m, fmaxf(mx, tail->red[t][half ^ 1][r]));
+          const float alpha = m == -INFINITY ? 1.f : ex2(m - mnew);  // nothing summed yet: O and l are 0
+          m = mnew;
+          l *= alpha;
+          if (i > 0) {  // P V of the block before is complete, as its successor's scores are
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              float ov[16];
+              ptx::tmem_ld_16(ocol + c * 16, ov);
+              uint32_t w[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(ov[j] * alpha);
+              ptx::tmem_st_16(ocol + c * 16, w);
+            }
+          }
+        }
+        const float base = (m == -INFINITY ? 0.f : m) - kPShift;
+        uint64_t ls[2] = {0, 0};
+        uint32_t pk[16];
+        ptx::tmem_wait_ld();
+        if (!plain) masked_scores(s0, kf, qf, (uint32_t)win);
+        probabilities(s0, f0, base, ls, pk);
+        ptx::tmem_st_16(scol, pk);  // over scores that have been read
+        ptx::tmem_ld_32(scol + 32, s0);
+        if (!plain) masked_scores(s0, kf + 32, qf, (uint32_t)(win >> 32));
+        probabilities(s0, f1, base, ls, pk);
+        ptx::tmem_st_16(scol + 16, pk);
+        float l0, l1, l2, l3;
+        unpack2(ls[0], l0, l1);
+        unpack2(ls[1], l2, l3);
+        l += (l0 + l1) + (l2 + l3);
         ptx::tmem_wait_st();
       }
+      if (!ok) break;
       ptx::tc_fence_before();
       warp_arrive(&tail->p_full[t]);
+    }
+    if (ok && warp_ok) {  // the pair agrees on this: the row's sum is both halves'
+      tail->sum[t][half][r] = l;
+      ptx::named_bar_sync(pair_bar, 64);
+      l = tail->sum[t][0][r] + tail->sum[t][1][r];
     }
     // The output rows of this lane.
     const bool mine = dual ? t < nlanes : true;  // one row tile: both lanes write a partial result
@@ -673,11 +735,11 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
       if (n == 0) f = 0.f;  // nothing decoded, nothing to scale
       if (direct) f = l == 0.f ? 0.f : f / l;
       // Rows leave in whole lines: 32 rows x 32 columns at a time through this
-      // warp's part of the K stages, which no MMA reads any more.
+      // warp's part of the K and V stages, which no MMA reads any more.
       const int64_t off = rok ? (direct ? (int64_t)req * p.out_bs + ((int64_t)row * p.heads + head) * kD : idx * kD) : -1;
       uint8_t* turn = k_s + warp * 32 * 144;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t ov[32];
         if (n > 0) {
           ptx::tmem_ld_32(ocol + c * 32, ov);
@@ -686,6 +748,7 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
           for (int j = 0; j < 32; ++j) ov[j] = 0;
         }
         __syncwarp();
+        const int col0 = half * 64 + c * 32;
         if (direct) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -701,7 +764,7 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
             const int rr = k * 8 + (lane >> 2), col = lane & 3;
             const int64_t o = __shfl_sync(0xffffffffu, off, rr);
             const uint4 w = *reinterpret_cast<const uint4*>(turn + rr * 80 + col * 16);
-            if (o >= 0) *reinterpret_cast<uint4*>(p.out + o + c * 32 + col * 8) = w;
+            if (o >= 0) *reinterpret_cast<uint4*>(p.out + o + col0 + col * 8) = w;
           }
         } else {
 #pragma unroll
@@ -715,11 +778,11 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
             const int rr = k * 4 + (lane >> 3), col = lane & 7;
             const int64_t o = __shfl_sync(0xffffffffu, off, rr);
             const float4 w = *reinterpret_cast<const float4*>(turn + rr * 144 + col * 16);
-            if (o >= 0) *reinterpret_cast<float4*>(p.part_o + o + c * 32 + col * 4) = w;
+            if (o >= 0) *reinterpret_cast<float4*>(p.part_o + o + col0 + col * 4) = w;
           }
         }
       }
-      if (rok) {
+      if (rok && half == 0) {
         const float ref = m == -INFINITY ? m : m - kPShift;  // l carries the 2^7
         if (direct) {
           if (p.lse)

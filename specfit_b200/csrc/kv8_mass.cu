@@ -215,6 +215,7 @@ extern "C" int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int6
   m.a.heads = num_heads;
   m.a.group = group;
   m.a.q_len = (int)q_len;
+  m.a.q_magic = ((1ull << 40) + (uint64_t)q_len - 1) / (uint64_t)q_len;
   m.a.kv_len = (int)kv_len;
   m.a.prefix = (int)prefix_len;
   m.a.scale_log2 = scale * 1.4426950408889634f;
