@@ -808,11 +808,10 @@ SF_API int sf_kv8_read(const sf_kv8_rows* rows, int64_t first, int64_t count, vo
  * log-sum-exp of a row's scaled scores.  A row that sees no key answers zeros
  * and -infinity.  A key with a NaN (or, in its value row, an infinity)
  * answers NaN to the rows that see it and to no other.  workspace (16-byte
- * aligned): sf_kv8_attention_workspace_bytes(...) bytes, 0 where one key range
- * is enough.
+ * aligned): sf_kv8_attention_workspace_bytes(...) bytes, perhaps 0.
  */
 SF_API size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim,
-                                               int64_t q_len, int64_t kv_len);
+                                               int64_t q_len, int64_t sealed, int64_t tail);
 SF_API int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int64_t q_head_stride,
                                  int64_t q_row_stride, int num_heads, int64_t q_len, const sf_kv8_rows* rows,
                                  const uint32_t* tree_bits, int bit_words, int64_t bits_batch_stride,

@@ -212,7 +212,7 @@ SIGNATURES = {
                                _vp, _i64, _i64, _i64, _vp, _vp]),
     "sf_kv8_seal": (_i32, [_vp, _vp, _i64, _i64, _i64, _kv8_p, _i64, _i64, _vp]),
     "sf_kv8_read": (_i32, [_kv8_p, _i64, _i64, _vp, _vp, _i64, _i64, _vp]),
-    "sf_kv8_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64, _i64]),
+    "sf_kv8_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64, _i64, _i64]),
     "sf_kv8_tree_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i64, _kv8_p, _vp, _i32, _i64, _i64, _f32, _vp,
                                      _i64, _vp, _vp, _sz, _vp]),
     "sf_kv8_attention_mass": (_i32, [_vp, _i64, _i64, _i64, _i32, _i64, _vp, _kv8_p, _vp, _i32, _i64, _i64, _f32,

@@ -523,17 +523,20 @@ Kv8Split kv8_split_mma(int batch, int hkv, int64_t packed, int64_t kv_len) {
 }  // namespace sf
 
 extern "C" size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim,
-                                                  int64_t q_len, int64_t kv_len) {
+                                                  int64_t q_len, int64_t sealed, int64_t tail) {
   using namespace sf;
   if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
-      head_dim > 128 || q_len <= 0 || kv_len <= 0 || q_len >= (1 << 30) || kv_len >= (1 << 30))
+      head_dim > 128 || q_len <= 0 || sealed < 0 || tail < 0 || sealed + tail <= 0 || q_len >= (1 << 30) ||
+      sealed >= (1 << 30) || tail >= (1 << 30))
     return 0;
+  const int64_t kv_len = sealed + tail;
   // Enough for either kernel: which one runs depends on the cache's strides too.
   const int64_t packed = (int64_t)(num_heads / num_kv_heads) * q_len;
   size_t need = partial_bytes(kv8_split_mma(batch, num_kv_heads, packed, kv_len), batch, num_heads, head_dim, q_len);
   if (kv8_use_tc(head_dim, packed, kv_len))
     need = std::max(need, partial_bytes(kv8_split_tc(batch, num_kv_heads, packed, kv_len), batch, num_heads, head_dim,
-                                        q_len));
+                                        q_len) +
+                              15 + kv8_tc_prep_bytes(batch, num_kv_heads, packed, tail, kv_len));
   return need;
 }
 
@@ -559,7 +562,7 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
                "q rows must be 16-byte aligned");
   SF_CHECK_ARG(aligned16(out) && out_batch_stride % 8 == 0, "out must be 16-byte aligned");
   const size_t need = sf_kv8_attention_workspace_bytes(rows->batch, num_heads, rows->num_kv_heads, rows->head_dim,
-                                                       q_len, kv_len);
+                                                       q_len, rows->sealed, rows->tail);
   if (workspace_bytes < need || (need && !workspace))
     return set_error(SF_ERR_WORKSPACE, "8-bit cache attention workspace needs %zu bytes", need);
   SF_CHECK_ARG(need == 0 || aligned16(workspace), "workspace must be 16-byte aligned");
@@ -595,7 +598,9 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
   cudaStream_t st = as_stream(stream);
   int rc;
   if (tc)
-    rc = kv8_attention_tc(p, st);
+    rc = kv8_attention_tc(p, static_cast<uint8_t*>(workspace) +
+                                 (partial_bytes(s, rows->batch, num_heads, rows->head_dim, q_len) + 15) / 16 * 16,
+                          st);
   else
     rc = rows->head_dim <= 64 ? launch_mma<64>(p, st) : launch_mma<128>(p, st);
   if (rc || s.splits == 1) return rc;

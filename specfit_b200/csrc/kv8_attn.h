@@ -56,7 +56,9 @@ Kv8Split kv8_split_mma(int batch, int hkv, int64_t packed_rows, int64_t kv_len);
 bool kv8_use_tc(int head_dim, int64_t packed_rows, int64_t kv_len);
 bool kv8_tc_layout(const Kv8Rows& c, int batch);
 Kv8Split kv8_split_tc(int batch, int hkv, int64_t packed_rows, int64_t kv_len);
-int kv8_attention_tc(const Kv8Attn& p, cudaStream_t stream);
+// Workspace behind the partial results (16-byte aligned).
+size_t kv8_tc_prep_bytes(int batch, int hkv, int64_t packed_rows, int64_t tail, int64_t kv_len);
+int kv8_attention_tc(const Kv8Attn& p, void* prep, cudaStream_t stream);
 int kv8_tc_status(int* status, int reset);
 
 }  // namespace sf

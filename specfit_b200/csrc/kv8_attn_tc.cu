@@ -19,10 +19,15 @@
 //     twice bf16's: the same time as one bf16 product.  A key's scale
 //     multiplies the fp32 scores.  Tail keys (bf16) are split the same way,
 //     with a power of two per key: four products instead of two.
+//   * A first kernel (kv8_prep_kernel) lays out what is not codes, once per call:
+//     the query tiles and the blocks that hold tail rows, as images of the
+//     shared-memory tiles, which a CTA copies whole.  Done by every CTA this
+//     took 18,000 clocks of set-up and 17,000 a tail block, and its code made
+//     the main loop's slower.
 //   * V is decoded to fp16 by four warps: one conversion and one multiply per
-//     two codes.  The values are in units of the largest V scale of the CTA's
-//     range (the tail's rows included), found first, so a block's factor is a
-//     power of two at most 1 and only what is below 2^-33 of the largest value
+//     two codes.  The values are in units of the largest V scale of the head's
+//     cache (its tail included), found first, so a block's factor is a power
+//     of two at most 1 and only what is below 2^-33 of the largest value
 //     is rounded.
 //   * Codes come by TMA: K straight into the operand layout, V raw.  (Loaded
 //     into registers a block ahead they are waited for at the next proxy fence,
@@ -75,10 +80,8 @@ constexpr float kSlack = 8.f;
 constexpr float kPShift = 7.f;  // probabilities are kept times 2^7
 
 struct __align__(16) Tail {
-  float qf[2][kBM];  // per row of the Q tiles: the power of two taken out of it; NaN for a row that holds one
   float red[2][2][kBM], sum[2][2][kBM];  // per lane, half and row: maxima and final sums, for the other half
   int pair_ok[kSoftmaxWarps];
-  float unit_top[kDecodeWarps];  // largest V scale seen by each decoder warp
   float kf[4][kKB];  // per block (ring of 4) and key: scale * log2(e) * K scale; NaN for a key that holds one
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t raw_full, raw_empty;
@@ -87,6 +90,17 @@ struct __align__(16) Tail {
   uint32_t tmem_base;
   int abort_flag;
   int tensor_lock;  // held by the lane that is issuing its products
+};
+
+// What the first kernel lays out, for each (request, KV head) bh.
+struct Prep {
+  uint8_t* q;    // [bh][tiles][hi, lo: 128 rows x 128, e4m3, swizzled]
+  uint8_t* k;    // [bh][blocks][hi, lo], the blocks of 128 keys from `first` on, which hold tail rows
+  uint8_t* v;    // [bh][blocks][128 keys x 128, fp16 in units of `unit`, swizzled]
+  float* qf;     // [bh][tiles * 128]: the power of two taken out of a query row; NaN for a row that holds one
+  float* kf;     // [bh][blocks * 128]: a key's scale; NaN for a key that holds one
+  float* unit;   // [bh]: the largest V scale
+  int tiles, blocks, first;
 };
 
 constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + 2 * kStages * kTileBytes + kHalf + sizeof(Tail);
@@ -169,13 +183,13 @@ __device__ __forceinline__ void split_store(const uint32_t (&in)[8], float inv, 
   *reinterpret_cast<uint4*>(hi_at) = make_uint4(h[0], h[1], h[2], h[3]);
   *reinterpret_cast<uint4*>(lo_at) = make_uint4(l[0], l[1], l[2], l[3]);
 }
-// The largest of 32 scores, scaled.
-__device__ __forceinline__ float scaled_max(const uint32_t (&x)[32], float f) {
-  float a = -INFINITY, d = -INFINITY;
+// The largest of 16 scores, scaled.
+__device__ __forceinline__ float scaled_max(const float (&x)[16], float f) {
+  float a = fmaxf(x[0], x[1]), d = fmaxf(x[2], x[3]);
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
-    a = max3(a, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
-    d = max3(d, __uint_as_float(x[j + 2]), __uint_as_float(x[j + 3]));
+  for (int j = 4; j < 16; j += 4) {
+    a = max3(a, x[j], x[j + 1]);
+    d = max3(d, x[j + 2], x[j + 3]);
   }
   a = fmaxf(a, d);
   return a == -INFINITY ? a : a * f;
@@ -199,28 +213,27 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 32 scores to probabilities 2^(f x - base), as fp16 pairs, and their sums.
-__device__ __forceinline__ void probabilities(const uint32_t (&x)[32], float f, float base, uint64_t (&ls)[2],
-                                              uint32_t (&pk)[16]) {
+// 16 scores to probabilities 2^(f x - base), as fp16 pairs, and their sums.
+__device__ __forceinline__ void probabilities(const float (&x)[16], float f, float base, uint64_t (&ls)[2],
+                                              uint32_t* pk) {
   const uint64_t f2 = pack2(f, f), b2 = pack2(-base, -base);
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
+  for (int j = 0; j < 16; j += 2) {
     float y0, y1;
-    unpack2(fma2(pack2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), f2, b2), y0, y1);
+    unpack2(fma2(pack2(x[j], x[j + 1]), f2, b2), y0, y1);
     const float p0 = ex2(y0), p1 = ex2(y1);
     ls[(j >> 1) & 1] = add2(ls[(j >> 1) & 1], pack2(p0, p1));
     pk[j / 2] = pack_f16x2(p0, p1);
   }
 }
-// 32 scores scaled, key by key, -infinity where the row does not see the key;
+// 16 scores scaled, key by key, -infinity where the row does not see the key;
 // returns the largest (NaN counts as the least).
-__device__ __forceinline__ float masked_scores(uint32_t (&x)[32], const float* kf, float qf, uint32_t vis) {
+__device__ __forceinline__ float masked_scores(float (&x)[16], const float* kf, float qf, uint32_t vis) {
   float mx = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    const float y = (vis >> j) & 1u ? __uint_as_float(x[j]) * (kf[j] * qf) : -INFINITY;
-    mx = fmaxf(mx, y);
-    x[j] = __float_as_uint(y);
+  for (int j = 0; j < 16; ++j) {
+    x[j] = (vis >> j) & 1u ? x[j] * (kf[j] * qf) : -INFINITY;
+    mx = fmaxf(mx, x[j]);
   }
   return mx;
 }
@@ -249,6 +262,124 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar);
 }
 
+// The query head (within its group) of packed row n: n / q_len.
+__device__ __forceinline__ int row_head(const Kv8Attn& p, int n) { return (int)(((uint64_t)n * p.q_magic) >> 40); }
+
+// grid: (query tiles, then blocks with tail rows (one CTA for the unit alone if
+// there are none); batch * hkv).
+__global__ void __launch_bounds__(256)
+kv8_prep_kernel(Kv8Attn p, Prep w) {
+  pdl_wait();
+  pdl_trigger();
+  __shared__ float tops[8];
+  const int bh = blockIdx.y, kvh = bh % p.c.hkv, req = bh / p.c.hkv;
+  const int row = threadIdx.x >> 3, part = threadIdx.x & 7;  // row of 32 in a pass, 16 dims of it
+  const uint32_t at0 = sw128(row, part);                     // 32 rows on: 4,096 bytes
+  if ((int)blockIdx.x < w.tiles) {
+    const int tile = blockIdx.x, packed = p.group * p.q_len;
+    uint8_t* img = w.q + ((int64_t)bh * w.tiles + tile) * kTileBytes + at0;
+    uint4 x[4][2];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int at = tile * kBM + u * 32 + row;
+      const bool on = at < packed;
+      const int h = on ? row_head(p, at) : 0, t = on ? at - h * p.q_len : 0;
+      const __nv_bfloat16* src = p.q + req * p.q_bs + (int64_t)(kvh * p.group + h) * p.q_hs + (int64_t)t * p.q_rs +
+                                 part * 16;
+      x[u][0] = on ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+      x[u][1] = on ? *reinterpret_cast<const uint4*>(src + 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t in[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
+      const uint32_t top = row_top(in);
+      const bool nan = top >= 0x7f80u;  // the row answers NaN
+      const int e = nan ? 0 : kv8_exponent(top);
+      split_store(in, pow2f(-e), img + u * 4096, img + u * 4096 + kHalf);
+      if (part == 0)
+        w.qf[((int64_t)bh * w.tiles + tile) * kBM + u * 32 + row] = nan ? __int_as_float(0x7fc00000) : pow2f(e);
+    }
+    return;
+  }
+  // The unit: every CTA that needs it finds it for itself.
+  const int sealed = (int)p.c.sealed, tail_rows = p.kv_len - sealed;
+  const float* vsc = p.c.vs + req * p.c.s_bs + kvh * p.c.s_hs;
+  const float* ksc = p.c.ks + req * p.c.s_bs + kvh * p.c.s_hs;
+  const __nv_bfloat16* kt = p.c.kt + req * p.c.t_bs + kvh * p.c.t_hs;
+  const __nv_bfloat16* vt = p.c.vt + req * p.c.t_bs + kvh * p.c.t_hs;
+  float unit = pow2f(kKv8MinExponent);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < sealed >> p.c.block_shift; i += 256) unit = fmaxf(unit, vsc[i]);  // NaN is passed over
+  uint32_t top = 0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < tail_rows * (kD / 8); i += 256) {
+    const uint4 x = *reinterpret_cast<const uint4*>(vt + (int64_t)i * 8);
+    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = in[j] & 0x7fffu, hi = (in[j] >> 16) & 0x7fffu;
+      top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+    }
+  }
+  unit = fmaxf(unit, pow2f(kv8_exponent(top)));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, o));
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = unit;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) unit = fmaxf(unit, tops[i]);
+  const int blk = blockIdx.x - w.tiles;
+  if (blk == 0 && threadIdx.x == 0) w.unit[bh] = unit;
+  if (blk >= w.blocks) return;
+  const float inv = 1.f / unit;  // exact
+  const uint8_t* kc = p.c.k + req * p.c.c_bs + kvh * p.c.c_hs + part * 16;
+  const uint8_t* vc = p.c.v + req * p.c.c_bs + kvh * p.c.c_hs + part * 8;  // dims 8 part .. and 64 + 8 part ..
+  uint8_t* kimg = w.k + ((int64_t)bh * w.blocks + blk) * kTileBytes + at0;
+  uint8_t* vimg = w.v + ((int64_t)bh * w.blocks + blk) * kTileBytes + at0;
+  float* kf = w.kf + ((int64_t)bh * w.blocks + blk) * kKB;
+  const int key0 = w.first + blk * kKB;
+#pragma unroll 2
+  for (int u = 0; u < 4; ++u) {
+    const int key = key0 + u * 32 + row;
+    uint4 a = make_uint4(0, 0, 0, 0), c = a, x = a, y = a;
+    float f = 1.f;
+    if (key0 + u * 32 < sealed) {  // the 32 rows of a pass are all codes or all tail
+      a = *reinterpret_cast<const uint4*>(kc + (int64_t)key * kD);
+      const float vs = vsc[key >> p.c.block_shift];
+      f = vs == vs ? ksc[key >> p.c.block_shift] : vs;
+      const float r = vs == vs ? vs * inv : 0.f;  // a block with a NaN counts as zeros
+      x = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD), pack_f16x2(r, r));
+      y = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD + 64), pack_f16x2(r, r));
+      *reinterpret_cast<uint4*>(kimg + u * 4096) = a;
+      *reinterpret_cast<uint4*>(kimg + u * 4096 + kHalf) = c;  // codes have no lower part
+    } else {
+      if (key < p.kv_len) {
+        const int64_t at = (int64_t)(key - sealed) * kD;
+        a = *reinterpret_cast<const uint4*>(kt + at + part * 16);
+        c = *reinterpret_cast<const uint4*>(kt + at + part * 16 + 8);
+        x = *reinterpret_cast<const uint4*>(vt + at + part * 8);
+        y = *reinterpret_cast<const uint4*>(vt + at + part * 8 + 64);
+      }
+      uint32_t in[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+      const uint32_t vals[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+      const uint32_t ktop = row_top(in);
+      const bool nan = max(ktop, row_top(vals)) >= 0x7f80u;  // rows that see the key answer NaN
+      if (nan) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) in[j] = 0;
+      }
+      const int e = nan ? 0 : kv8_exponent(ktop);
+      split_store(in, pow2f(-e), kimg + u * 4096, kimg + u * 4096 + kHalf);
+      f = nan ? __int_as_float(0x7fc00000) : pow2f(e);
+      x = tail8(x, inv);
+      y = tail8(y, inv);
+    }
+    *reinterpret_cast<uint4*>(vimg + u * 4096) = x;
+    *reinterpret_cast<uint4*>(vimg + u * 4096 + kRegion) = y;
+    if (part == 0) kf[u * 32 + row] = f;
+  }
+}
+
 // One lane's turn at the tensor core.  False: the wait gave up.
 __device__ __forceinline__ bool take_turn(int* lock, volatile int* abort_flag, int site) {
   uint64_t t0 = 0;
@@ -268,11 +399,8 @@ __device__ __forceinline__ bool take_turn(int* lock, volatile int* abort_flag, i
   }
 }
 
-// The query head (within its group) of packed row n: n / q_len.
-__device__ __forceinline__ int row_head(const Kv8Attn& p, int n) { return (int)(((uint64_t)n * p.q_magic) >> 40); }
-
 __global__ void __launch_bounds__(kThreads, 1)
-kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual, int ranges) {
+kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Prep w, int dual, int ranges) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
@@ -294,6 +422,8 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
   const int nblocks = key_hi > key_lo ? (key_hi - key_lo + kKB - 1) / kKB : 0;
   // Lanes in use, and the blocks of lane t: all of them, or every other one.
   const int nlanes = dual ? ((tile0 + 1) * kBM < packed ? 2 : 1) : min(2, nblocks);
+  // Blocks of codes alone come first; the others are laid out already.
+  const int coded = max(0, min(nblocks, ((int)p.c.sealed - key_lo) / kKB));
   auto lane_blocks = [&](int t) { return dual ? nblocks : (nblocks - t + 1) / 2; };
   auto block_of = [&](int t, int i) { return dual ? i : 2 * i + t; };
 
@@ -311,7 +441,7 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
       ptx::mbar_init(&tail->s_full[t], 1);
       ptx::mbar_init(&tail->p_full[t], kSoftmaxWarps / 2);
     }
-    ptx::mbar_init(&tail->q_ready, kSoftmaxWarps);
+    ptx::mbar_init(&tail->q_ready, 1);
     ptx::mbar_init(&tail->mma_done, 2);
     tail->abort_flag = 0;
     tail->tensor_lock = 0;
@@ -328,9 +458,12 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
 
   if (warp == kLoadWarp) {
     // ---------------- TMA producer ----------------
-    if (lane == 0) {
+    if (lane == 0 && nblocks > 0) {
+      const int bh = req * p.c.hkv + kvh;
+      const uint32_t qbytes = (dual ? nlanes : 1) * kTileBytes;
+      ptx::mbar_arrive_expect_tx(&tail->q_ready, qbytes);
+      ptx::bulk_load(q_s, w.q + ((int64_t)bh * w.tiles + tile0) * kTileBytes, qbytes, &tail->q_ready);
       const uint8_t* vc = p.c.v + req * p.c.c_bs + kvh * p.c.c_hs;
-      const int coded = max(0, min(nblocks, ((int)p.c.sealed - key_lo) / kKB));  // whole blocks of codes come first
       int b = 0;
       bool ok = true;
       for (; ok && b < nblocks; ++b) {
@@ -338,8 +471,10 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
         ok = ptx::mbar_wait(&tail->k_empty[s], ((b / kStages) & 1) ^ 1, abort_flag, &g_kv8_tc_status, 51);
         if (!ok) break;
         if (b >= coded) {
-          ptx::mbar_arrive(&tail->k_full[s]);
-          continue;
+          ptx::mbar_arrive_expect_tx(&tail->k_full[s], kTileBytes);
+          ptx::bulk_load(k_s + s * kTileBytes, w.k + ((int64_t)bh * w.blocks + (key0 - w.first) / kKB) * kTileBytes,
+                         kTileBytes, &tail->k_full[s]);
+          continue;  // V of such a block: the decoders ask for it
         }
         ptx::mbar_arrive_expect_tx(&tail->k_full[s], kHalf);
         ptx::tma_load_4d(k_s + s * kTileBytes, &tm_k, &tail->k_full[s], 0, key0, kvh, req);
@@ -350,7 +485,8 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
       }
       if (!ok) {  // another role gave up: let the copies in flight land before the CTA ends
         volatile int never = 0;
-        for (int i = max(0, b - 1); i <= b && i < coded; ++i)
+        ptx::mbar_wait(&tail->q_ready, 0, &never, &g_kv8_tc_status, 53);
+        for (int i = max(0, b - 1); i <= b && i < nblocks; ++i)
           ptx::mbar_wait(&tail->k_full[i % kStages], (i / kStages) & 1, &never, &g_kv8_tc_status, 53);
         if (b > 0 && coded > 0)
           ptx::mbar_wait(&tail->raw_full, (min(b, coded) - 1) & 1, &never, &g_kv8_tc_status, 54);
@@ -389,7 +525,7 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
         if (i < blocks) {
           const uint64_t kdesc = ptx::smem_desc_k_sw128(ptx::smem_u32(k_s + ss * kTileBytes));
           // hi and lo of Q with K; a block with tail keys has a lower part of K too.
-          const int parts = key_lo + (bs + 1) * kKB > (int)p.c.sealed ? 4 : 2;
+          const int parts = bs >= coded ? 4 : 2;
 #pragma unroll 1
           for (int x = 0; x < parts; ++x) {
             const uint64_t qd = qdesc + (x & 1) * kLo, kd = kdesc + (x >> 1) * kLo;
@@ -408,167 +544,75 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
     }
   } else if (warp >= kSoftmaxWarps) {
     // ---------------- decoders ----------------
-    const int ct = threadIdx.x - kSoftmaxWarps * 32;
-    const int row = ct >> 3, part = ct & 7;  // row of 16 in a pass, 16 dims of it
-    const int sealed = (int)p.c.sealed;
-    const uint8_t* kc = p.c.k + req * p.c.c_bs + kvh * p.c.c_hs + part * 16;
-    const uint8_t* vc = p.c.v + req * p.c.c_bs + kvh * p.c.c_hs + part * 8;  // dims 8 part .. and 64 + 8 part ..
+    const int ct = threadIdx.x - kSoftmaxWarps * 32, bh = req * p.c.hkv + kvh;
+    const int row = ct >> 3, part = ct & 7;  // row of 16 in a pass, 8 + 8 dims of it
     const float* ksc = p.c.ks + req * p.c.s_bs + kvh * p.c.s_hs;
     const float* vsc = p.c.vs + req * p.c.s_bs + kvh * p.c.s_hs;
-    const __nv_bfloat16* kt = p.c.kt + req * p.c.t_bs + kvh * p.c.t_hs + part * 16;
-    const __nv_bfloat16* vt = p.c.vt + req * p.c.t_bs + kvh * p.c.t_hs + part * 8;
-    float ks = 0.f, kvs = 0.f, vs[4];  // K and V scale of key ct of the next block; V scales of this one
+    float ks = 0.f, vs[4];  // scale of key ct of the next block; V scales of this one
     auto load_ks = [&](int b) {
       const int key = key_lo + b * kKB + ct;
-      if (key < sealed) {
-        ks = ksc[key >> p.c.block_shift];
-        kvs = vsc[key >> p.c.block_shift];
+      if (b < coded) {
+        const float y = vsc[key >> p.c.block_shift];
+        ks = y == y ? ksc[key >> p.c.block_shift] : y;  // a block with a NaN among its values: NaN scores
+      } else {
+        ks = w.kf[(int64_t)bh * w.blocks * kKB + (key - w.first)];
       }
     };
     auto load_vs = [&](int b) {
-      const int key0 = key_lo + b * kKB;
+      if (b >= coded) return;
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (key0 + g * 32 < sealed) vs[g] = vsc[(key0 + g * 32) >> p.c.block_shift];
+      for (int g = 0; g < 4; ++g) vs[g] = vsc[(key_lo + b * kKB + g * 32) >> p.c.block_shift];
     };
     if (nblocks > 0) {
       load_ks(0);
       load_vs(0);
     }
-    // The unit: the largest V scale of the range.
-    float unit = pow2f(kKv8MinExponent);
-    if (key_lo < sealed) {
-      const int last = (min(key_hi, sealed) - 1) >> p.c.block_shift;
-      for (int i = (key_lo >> p.c.block_shift) + ct; i <= last; i += kDecodeWarps * 32) unit = fmaxf(unit, vsc[i]);
-    }
-    {
-      uint32_t top = 0;
-#pragma unroll 4
-      for (int key = max(key_lo, sealed) + row; key < key_hi; key += 16) {
-        const __nv_bfloat16* at = vt + (int64_t)(key - sealed) * kD;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 x = *reinterpret_cast<const uint4*>(at + i * 64);
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t lo = w[j] & 0x7fffu, hi = (w[j] >> 16) & 0x7fffu;
-            top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-          }
-        }
-      }
-      unit = fmaxf(unit, pow2f(kv8_exponent(top)));
-#pragma unroll
-      for (int o = 16; o; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, o));
-      if (lane == 0) tail->unit_top[ct >> 5] = unit;
-      ptx::named_bar_sync(2, kDecodeWarps * 32);
-#pragma unroll
-      for (int i = 0; i < kDecodeWarps; ++i) unit = fmaxf(unit, tail->unit_top[i]);
-    }
-    const float inv = 1.f / unit;  // exact
-    const uint32_t at0 = sw128(row, part);  // 16 rows on: 2,048 bytes
-    // K of block b.  False: a wait gave up.
+    const float inv = 1.f / w.unit[bh];  // exact
+    // K of block b is on its way; here its scales.  False: a wait gave up.
     auto store_k = [&](int b) -> bool {
-      const int s = b % kStages, key0 = key_lo + b * kKB;
+      const int s = b % kStages;
       if (!warp_wait(&tail->k_empty[s], ((b / kStages) & 1) ^ 1, abort_flag, 46)) return false;
       // Ring of four: block b - 4's softmax is over.  (The scores that freed this
       // stage, block b - 2's, were issued after P V of the lane's block before.)
-      float* kf = tail->kf[b & 3];
-      if (key0 + ct < sealed) kf[ct] = kvs != kvs ? kvs : ks * p.scale_log2;
-      uint8_t* kst = k_s + s * kTileBytes + at0;
-      if (key0 + kKB > sealed) {
-        // Tail rows, perhaps behind coded ones (whose lower part is zero); the
-        // next pass's rows are loaded before this one's are split.
-        uint4 x[4], y[4];
-        auto rows = [&](int u, uint4 (&z)[4]) {
-          const int key = key0 + u * 16 + row;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) z[i] = make_uint4(0, 0, 0, 0);
-          if (key < sealed) {
-            z[0] = *reinterpret_cast<const uint4*>(kc + (int64_t)key * kD);
-          } else if (key < key_hi) {
-            const int64_t at = (int64_t)(key - sealed) * kD;
-            z[0] = *reinterpret_cast<const uint4*>(kt + at);
-            z[1] = *reinterpret_cast<const uint4*>(kt + at + 8);
-            z[2] = *reinterpret_cast<const uint4*>(vt + at);
-            z[3] = *reinterpret_cast<const uint4*>(vt + at + 64);
-          }
-        };
-        rows(0, x);
-#pragma unroll 1
-        for (int u = 0; u < 8; ++u) {
-          if (u < 7) rows(u + 1, y);
-          uint8_t* hi_at = kst + u * 2048;
-          if (key0 + u * 16 < sealed) {  // the 16 rows of a pass are all codes or all tail
-            *reinterpret_cast<uint4*>(hi_at) = x[0];
-            *reinterpret_cast<uint4*>(hi_at + kHalf) = x[1];
-          } else {
-            uint32_t in[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
-            const uint32_t vals[8] = {x[2].x, x[2].y, x[2].z, x[2].w, x[3].x, x[3].y, x[3].z, x[3].w};
-            const uint32_t top = row_top(in);
-            const bool nan = max(top, row_top(vals)) >= 0x7f80u;  // rows that see the key answer NaN
-            if (nan) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) in[j] = 0;
-            }
-            const int e = nan ? 0 : kv8_exponent(top);
-            split_store(in, pow2f(-e), hi_at, hi_at + kHalf);
-            if (part == 0) kf[u * 16 + row] = nan ? __int_as_float(0x7fc00000) : pow2f(e) * p.scale_log2;
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = y[i];
-        }
-        ptx::fence_proxy_async_smem();
-      }
+      tail->kf[b & 3][ct] = ks * p.scale_log2;
       warp_arrive(&tail->k_full[s]);
       return true;
     };
     auto store_v = [&](int b) -> bool {
-      const int s = b % kStages, key0 = key_lo + b * kKB;
-      const bool coded = key0 + kKB <= sealed;
-      if (coded && !warp_wait(&tail->raw_full, b & 1, abort_flag, 55)) return false;
+      const int s = b % kStages;
+      if (b < coded && !warp_wait(&tail->raw_full, b & 1, abort_flag, 55)) return false;
       if (!warp_wait(&tail->v_empty[s], ((b / kStages) & 1) ^ 1, abort_flag, 47)) return false;
-      uint8_t* vst = v_s + s * kTileBytes + at0;
-      if (coded) {
-        // The two halves of a row, odd rows the upper one first: four rows of a
-        // warp then cover all banks.
-        const uint8_t* raw = raw_s + row * kD + part * 8;
-        const int h0 = (row & 1) * 64, h1 = 64 - h0;
-        uint8_t *to0 = vst + h0 * (kRegion / 64), *to1 = vst + h1 * (kRegion / 64);
-        uint32_t mul[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float f = vs[g] == vs[g] ? vs[g] * inv : 0.f;  // a block with a NaN counts as zeros
-          mul[g] = pack_f16x2(f, f);
+      if (b >= coded) {  // laid out already
+        if (ct == 0) {
+          ptx::mbar_arrive_expect_tx(&tail->v_full[s], kTileBytes);
+          ptx::bulk_load(v_s + s * kTileBytes,
+                         w.v + ((int64_t)bh * w.blocks + (key_lo + b * kKB - w.first) / kKB) * kTileBytes, kTileBytes,
+                         &tail->v_full[s]);
+        } else if (lane == 0) {
+          ptx::mbar_arrive(&tail->v_full[s]);
         }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const uint2 a = *reinterpret_cast<const uint2*>(raw + u * 16 * kD + h0);
-          const uint2 c = *reinterpret_cast<const uint2*>(raw + u * 16 * kD + h1);
-          *reinterpret_cast<uint4*>(to0 + u * 2048) = decode8(a, mul[u >> 1]);
-          *reinterpret_cast<uint4*>(to1 + u * 2048) = decode8(c, mul[u >> 1]);
-        }
-        warp_arrive(&tail->raw_empty);
-      } else {
-#pragma unroll 2
-        for (int u = 0; u < 8; ++u) {
-          const int key = key0 + u * 16 + row;
-          uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
-          if (key < sealed) {
-            const float y = vsc[key >> p.c.block_shift];
-            const float f = y == y ? y * inv : 0.f;
-            const uint8_t* at = vc + (int64_t)key * kD;
-            v0 = decode8(*reinterpret_cast<const uint2*>(at), pack_f16x2(f, f));
-            v1 = decode8(*reinterpret_cast<const uint2*>(at + 64), pack_f16x2(f, f));
-          } else if (key < key_hi) {
-            const __nv_bfloat16* at = vt + (int64_t)(key - sealed) * kD;
-            v0 = tail8(*reinterpret_cast<const uint4*>(at), inv);
-            v1 = tail8(*reinterpret_cast<const uint4*>(at + 64), inv);
-          }
-          *reinterpret_cast<uint4*>(vst + u * 2048) = v0;
-          *reinterpret_cast<uint4*>(vst + u * 2048 + kRegion) = v1;
-        }
+        return true;
       }
+      uint32_t mul[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float f = vs[g] == vs[g] ? vs[g] * inv : 0.f;  // a block with a NaN counts as zeros
+        mul[g] = pack_f16x2(f, f);
+      }
+      // The two halves of a row, odd rows the upper one first: four rows of a
+      // warp then cover all banks.
+      const uint8_t* raw = raw_s + row * kD + part * 8;
+      const int h0 = (row & 1) * 64, h1 = 64 - h0;
+      uint8_t* vst = v_s + s * kTileBytes + sw128(row, part);  // 16 rows on: 2,048 bytes
+      uint8_t *to0 = vst + h0 * (kRegion / 64), *to1 = vst + h1 * (kRegion / 64);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const uint2 a = *reinterpret_cast<const uint2*>(raw + u * 16 * kD + h0);
+        const uint2 c = *reinterpret_cast<const uint2*>(raw + u * 16 * kD + h1);
+        *reinterpret_cast<uint4*>(to0 + u * 2048) = decode8(a, mul[u >> 1]);
+        *reinterpret_cast<uint4*>(to1 + u * 2048) = decode8(c, mul[u >> 1]);
+      }
+      warp_arrive(&tail->raw_empty);
       ptx::fence_proxy_async_smem();
       warp_arrive(&tail->v_full[s]);
       return true;
@@ -578,7 +622,8 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
     // would wait for good.)
     bool ok = nblocks > 0 && store_k(0);
     if (ok && nblocks > 1) load_ks(1);
-    for (int b = 0; ok && b < nblocks; ++b) {
+    int b = 0;
+    for (; ok && b < nblocks; ++b) {
       if (b + 1 < nblocks) {
         ok = store_k(b + 1);
         if (!ok) break;
@@ -586,6 +631,11 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
       }
       ok = store_v(b);
       if (ok && b + 1 < nblocks) load_vs(b + 1);
+    }
+    if (!ok && ct == 0) {  // copies of V that this thread asked for land before the CTA ends
+      volatile int never = 0;
+      for (int i = max(coded, b - 2); i < b; ++i)
+        ptx::mbar_wait(&tail->v_full[i % kStages], (i / kStages) & 1, &never, &g_kv8_tc_status, 57);
     }
   } else {
     // ---------------- softmax / epilogue: two threads per row ----------------
@@ -598,40 +648,9 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
     const int qhead = rok ? row_head(p, pr) : 0, row = rok ? pr - qhead * p.q_len : 0;
     const int head = kvh * p.group + qhead;
 
-    if (dual ? t < nlanes : true) {
-      // Q rows, eight threads a row, split into their two parts: the lane's own
-      // tile by its eight warps, or the one tile by all sixteen.  Rows past the
-      // last are left as they are: their scores are not looked at.
-      const int per = dual ? 32 : 64, wt = dual ? threadIdx.x & 255 : threadIdx.x;
-      const int qrow = wt >> 3, part = wt & 7, first = (tile0 + (dual ? t : 0)) * kBM;
-      uint8_t* qt = q_s + (dual ? t : 0) * kTileBytes + sw128(qrow, part);
-      uint4 x[4][2];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {  // all rows in flight together
-        const int at = first + u * per + qrow;
-        const bool on = u * per < kBM && at < packed;
-        const int h = on ? row_head(p, at) : 0, tt = on ? at - h * p.q_len : 0;
-        const __nv_bfloat16* src = p.q + req * p.q_bs + (int64_t)(kvh * p.group + h) * p.q_hs + (int64_t)tt * p.q_rs +
-                                   part * 16;
-        x[u][0] = on ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-        x[u][1] = on ? *reinterpret_cast<const uint4*>(src + 8) : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (u * per >= kBM || first + u * per + (qrow & ~3) >= packed) continue;  // uniform over the warp
-        const uint32_t in[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
-        const uint32_t top = row_top(in);
-        const bool nan = top >= 0x7f80u;  // the row answers NaN
-        const int e = nan ? 0 : kv8_exponent(top);
-        uint8_t* at = qt + u * per * 128;
-        split_store(in, pow2f(-e), at, at + kHalf);
-        if (part == 0) tail->qf[dual ? t : 0][u * per + qrow] = nan ? __int_as_float(0x7fc00000) : pow2f(e);
-      }
-      ptx::fence_proxy_async_smem();
-    }
-    warp_arrive(&tail->q_ready);
-    ptx::named_bar_sync(1, kSoftmaxWarps * 32);  // the rows' factors come from other warps
-    const float qf = rok ? tail->qf[dual ? t : 0][r] : 0.f;
+    const int64_t bh = (int64_t)req * p.c.hkv + kvh;
+    const float qf = rok ? w.qf[bh * w.tiles * kBM + pr] : 0.f;
+    const float unit = w.unit[bh];
 
     const uint32_t scol = tmem + ((uint32_t)(quad * 32) << 16) + t * kBM + half * 64;  // this half's scores
     const uint32_t ocol = tmem + ((uint32_t)(quad * 32) << 16) + kOCol + t * kD + half * 64;
@@ -649,26 +668,34 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
         // Every key visible and one scale per 32 of them: the rule in a long context.
         const bool plain = full && key0 + 64 <= (int)p.c.sealed;
         const float* kf = tail->kf[b & 3] + half * 64;
-        float mx = -INFINITY, f0 = 1.f, f1 = 1.f;
-        uint32_t s0[32];
-        if (ok) {
-          ptx::tc_fence_after();
-          if (plain) {
-            f0 = kf[0] * qf;
-            f1 = kf[32] * qf;
-            ptx::tmem_ld_32(scol, s0);
-            mx = scaled_max(s0, f0);
-            ptx::tmem_ld_32(scol + 32, s0);
-            mx = fmaxf(mx, scaled_max(s0, f1));
-          } else {
-            ptx::tmem_ld_32(scol, s0);
-            mx = masked_scores(s0, kf, qf, (uint32_t)win);
-            ptx::tmem_ld_32(scol + 32, s0);
-            mx = fmaxf(mx, masked_scores(s0, kf + 32, qf, (uint32_t)(win >> 32)));
+        uint32_t pk[32];  // 64 probabilities
+        uint64_t ls[2];
+        // Once under the reference maximum as it is; if a score of the row (in
+        // either half) is too far above it, once more under a new one.  The
+        // scores are read from TMEM, which the MMAs keep busy, only once in
+        // the first case, and stay there until the probabilities are settled.
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+          const float base = (m == -INFINITY ? 0.f : m) - kPShift;
+          float mx = -INFINITY;
+          ls[0] = ls[1] = 0;
+          if (ok) {
+            if (pass == 0) ptx::tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {  // 16 at a time: nothing is spilled
+              float sc[16];
+              ptx::tmem_ld_16(scol + c * 16, sc);
+              float f = 1.f;
+              if (plain) {
+                f = kf[(c >> 1) * 32] * qf;
+                mx = fmaxf(mx, scaled_max(sc, f));
+              } else {
+                mx = fmaxf(mx, masked_scores(sc, kf + c * 16, qf, (uint32_t)(win >> (c * 16))));
+              }
+              probabilities(sc, f, base, ls, pk + c * 8);
+            }
           }
-          ptx::tmem_ld_32_async(scol, s0);  // once more, now for the probabilities
-        }
-        if (pair_any(pair_bar, !ok || mx > m + kSlack || (m == -INFINITY && mx > -INFINITY))) {
+          if (pass || !pair_any(pair_bar, !ok || mx > m + kSlack || (m == -INFINITY && mx > -INFINITY))) break;
           // The other half's maximum, and whether its wait succeeded: both warps
           // of the pair go on or stop together.
           tail->red[t][half][r] = mx;
@@ -694,22 +721,14 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
             }
           }
         }
-        const float base = (m == -INFINITY ? 0.f : m) - kPShift;
-        uint64_t ls[2] = {0, 0};
-        uint32_t pk[16];
-        ptx::tmem_wait_ld();
-        if (!plain) masked_scores(s0, kf, qf, (uint32_t)win);
-        probabilities(s0, f0, base, ls, pk);
-        ptx::tmem_st_16(scol, pk);  // over scores that have been read
-        ptx::tmem_ld_32(scol + 32, s0);
-        if (!plain) masked_scores(s0, kf + 32, qf, (uint32_t)(win >> 32));
-        probabilities(s0, f1, base, ls, pk);
-        ptx::tmem_st_16(scol + 16, pk);
-        float l0, l1, l2, l3;
-        unpack2(ls[0], l0, l1);
-        unpack2(ls[1], l2, l3);
-        l += (l0 + l1) + (l2 + l3);
-        ptx::tmem_wait_st();
+        if (ok) {
+          ptx::tmem_st_32(scol, pk);  // over scores that have been read
+          float l0, l1, l2, l3;
+          unpack2(ls[0], l0, l1);
+          unpack2(ls[1], l2, l3);
+          l += (l0 + l1) + (l2 + l3);
+          ptx::tmem_wait_st();
+        }
       }
       if (!ok) break;
       ptx::tc_fence_before();
@@ -729,10 +748,7 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
       const bool direct = p.splits == 1;
       const int part = dual ? range : 2 * range + t;
       const int64_t idx = (((int64_t)req * p.splits + part) * p.heads + head) * p.q_len + row;
-      float f = 1.f;  // O is in units of the largest V scale
-#pragma unroll
-      for (int i = 0; i < kDecodeWarps; ++i) f = i == 0 ? tail->unit_top[0] : fmaxf(f, tail->unit_top[i]);
-      if (n == 0) f = 0.f;  // nothing decoded, nothing to scale
+      float f = unit;  // O is in units of the largest V scale
       if (direct) f = l == 0.f ? 0.f : f / l;
       // Rows leave in whole lines: 32 rows x 32 columns at a time through this
       // warp's part of the K and V stages, which no MMA reads any more.
@@ -807,11 +823,23 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, int dual
 
 struct Shape {
   bool dual;
-  int64_t pairs;  // CTAs over the rows
+  int64_t tiles, pairs;  // row tiles, CTAs over them
 };
 Shape shape_of(int64_t packed) {
   const int64_t tiles = (packed + kBM - 1) / kBM;
-  return {tiles > 1, tiles > 1 ? (tiles + 1) / 2 : 1};
+  return {tiles > 1, tiles, tiles > 1 ? (tiles + 1) / 2 : 1};
+}
+
+// Blocks with tail rows: from the one that holds the first, to the end.  (The
+// boundary is a multiple of 32, so one more block than the tail fills can be
+// touched.)
+int64_t tail_blocks(int64_t sealed, int64_t kv_len) {
+  return kv_len > sealed ? (kv_len + kKB - 1) / kKB - sealed / kKB : 0;
+}
+// Bytes of the first kernel's layout, with the given number of such blocks.
+size_t prep_bytes(int64_t heads, int64_t tiles, int64_t blocks) {
+  return (size_t)heads * ((tiles + 2 * blocks) * (size_t)kTileBytes + (tiles + blocks) * kBM * sizeof(float)) +
+         ((size_t)heads * sizeof(float) + 127) / 128 * 128;
 }
 
 }  // namespace
@@ -845,7 +873,11 @@ Kv8Split kv8_split_tc(int batch, int hkv, int64_t packed, int64_t kv_len) {
   return {(int)(sh.dual ? best : 2 * best), (int)(best_per * kKB)};
 }
 
-int kv8_attention_tc(const Kv8Attn& p, cudaStream_t stream) {
+size_t kv8_tc_prep_bytes(int batch, int hkv, int64_t packed, int64_t tail, int64_t kv_len) {
+  return prep_bytes((int64_t)batch * hkv, shape_of(packed).tiles, tail_blocks(kv_len - tail, kv_len));
+}
+
+int kv8_attention_tc(const Kv8Attn& p, void* prep, cudaStream_t stream) {
   static std::atomic<unsigned long long> configured{0};
   if (int rc = once_per_device(configured, [] {
         SF_CHECK_CUDA(cudaFuncSetAttribute(kv8_attn_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -855,7 +887,21 @@ int kv8_attention_tc(const Kv8Attn& p, cudaStream_t stream) {
     return rc;
   const Shape sh = shape_of((int64_t)p.group * p.q_len);
   const int ranges = sh.dual ? p.splits : p.splits / 2;
+  const int64_t heads = (int64_t)p.batch * p.c.hkv;
   SF_CHECK_ARG(sh.pairs < 65536 && (int64_t)ranges * p.batch < 65536, "too many query rows or requests");
+  Prep w;
+  w.tiles = (int)sh.tiles;
+  w.blocks = (int)tail_blocks(p.c.sealed, p.kv_len);
+  w.first = (int)(p.c.sealed / kKB * kKB);
+  w.q = static_cast<uint8_t*>(prep);
+  w.k = w.q + (size_t)heads * w.tiles * kTileBytes;
+  w.v = w.k + (size_t)heads * w.blocks * kTileBytes;
+  w.qf = reinterpret_cast<float*>(w.v + (size_t)heads * w.blocks * kTileBytes);
+  w.kf = w.qf + (size_t)heads * w.tiles * kBM;
+  w.unit = w.kf + (size_t)heads * w.blocks * kKB;
+  const dim3 prep_grid((unsigned)(w.tiles + std::max(w.blocks, 1)), (unsigned)heads);
+  SF_CHECK_CUDA(launch_pdl(kv8_prep_kernel, prep_grid, dim3(256), 0, stream, p, w));
+  SF_CHECK_LAUNCH();
   // K's codes, 16 bits at a time (bytes are bytes): [batch][heads][tokens][64].
   CUtensorMap tm_k = {};
   if (p.c.sealed >= kKB) {
@@ -866,7 +912,7 @@ int kv8_attention_tc(const Kv8Attn& p, cudaStream_t stream) {
     if (int rc = tma_encode_bf16(&tm_k, p.c.k, 4, dims, strides, box)) return rc;
   }
   const dim3 grid((unsigned)p.c.hkv, (unsigned)sh.pairs, (unsigned)(ranges * p.batch));
-  SF_CHECK_CUDA(launch_pdl(kv8_attn_tc_kernel, grid, dim3(kThreads), kSmemBytes, stream, tm_k, p, sh.dual ? 1 : 0,
+  SF_CHECK_CUDA(launch_pdl(kv8_attn_tc_kernel, grid, dim3(kThreads), kSmemBytes, stream, tm_k, p, w, sh.dual ? 1 : 0,
                            ranges));
   SF_CHECK_LAUNCH();
   return SF_OK;

@@ -789,7 +789,8 @@ def kv8_tree_attention(q: torch.Tensor, rows: Kv8Rows, tree_bits: torch.Tensor |
     lse = torch.empty(b, hq, tq, dtype=torch.float32, device=dev) if return_lse else None
     sc = float(d ** -0.5 if scale is None else scale)
     with _on(dev):
-        nbytes = N.lib.sf_kv8_attention_workspace_bytes(b, hq, rows.shape[1], d, tq, rows.length)
+        nbytes = N.lib.sf_kv8_attention_workspace_bytes(b, hq, rows.shape[1], d, tq, rows.sealed,
+                                                        rows.length - rows.sealed)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         N.check(N.lib.sf_kv8_tree_attention(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), hq, tq,
                                             ctypes.byref(rows._c), _ptr(bits), words, bits_bs, int(prefix_len), sc,
