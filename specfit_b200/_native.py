@@ -107,7 +107,7 @@ class Kv8RowsStruct(ctypes.Structure):
                 ("tail_batch_stride", _i64), ("tail_head_stride", _i64)]
 
 
-_kv8_p = ctypes.POINTER(Kv8RowsStruct)
+_kv8_p = _vp  # the structure's address
 
 # name -> (restype, argtypes)
 SIGNATURES = {

@@ -30,6 +30,10 @@
 //     more than fp16's 11 bits (probabilities are kept times 2^12).
 //   * The reference maximum of a row moves only when a score exceeds it by
 //     more than 3 (base 2), so accumulators are rarely rescaled.
+//   * Q's fragments are read from shared memory (one 16-byte load serves two
+//     MMAs) and tail units are converted there, which leaves 128 registers a
+//     thread and four CTAs on an SM: with 200 and two, 131,072 tokens took 47
+//     us where now they take @LONG@.
 // Tail units (bf16 rows: few) are scaled by a power of two per unit and
 // enter the same fragments.  A value row with a NaN or an infinity (a sealed
 // block of values that holds one) makes its key's score NaN, so that rows
@@ -47,9 +51,9 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kRows = 16;      // packed query rows of a CTA
 constexpr int kUnit = 16;      // keys of one step of a warp
-constexpr int kStages = 5;     // units in flight per warp
+constexpr int kStages = 3;     // units of a warp's ring
 constexpr int kStep = kWarps * kUnit;
-constexpr int kMaxSplits = 128;
+constexpr int kMaxSplits = 160;
 constexpr float kPShift = 12.f;  // probabilities are kept times 2^12
 constexpr float kSlack = 3.f;    // a row's reference maximum may lag by this (base 2)
 
@@ -62,19 +66,90 @@ struct Layout {
   static constexpr int kKBytes = 2 * kKChunks * 16;    // per thread and unit
   static constexpr int kUnitBytes = 32 * (kKBytes + 4 * kVBytes);  // 16 keys: K and V codes
   static constexpr int kRing = kWarps * kStages * kUnitBytes;
+  // A tail unit as fp16 takes twice its codes' bytes, in the ring, where no copy is in flight by then.
+  static_assert(kStages >= 2, "a tail unit needs two stages");
   static constexpr int kJoin = kWarps * kRows * DT * 4;
   static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
 };
 
+// A unit of 16 tail rows as fp16 fragments in this thread's slots of `out`
+// ([K: 2 x steps][V: tiles] of 32 lanes), scaled by powers of two that are
+// returned; zeros for keys from key_hi on.  First the rows as they are and
+// their magnitudes, then each slot in place.
+template <int DT>
+__device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bfloat16* vt, int key0, int sealed,
+                                          int key_hi, int d, int g, int c, int lane, uint2* out, float& kscale,
+                                          float& vscale, uint32_t& bad) {
+  using L = Layout<DT>;
+  uint32_t ktop = 0, vtop = 0;
+#pragma unroll 1
+  for (int t = 0; t < 2; ++t) {
+    const int key = key0 + t * 8 + g;
+    const __nv_bfloat16* row = kt + (int64_t)(key < key_hi ? key - sealed : 0) * d;
+#pragma unroll
+    for (int st = 0; st < L::kSteps; ++st) {
+      const int dim = (st >> 2) * 64 + c * 16 + (st & 3) * 4;
+      const uint2 w = key < key_hi && dim < d ? *reinterpret_cast<const uint2*>(row + dim) : make_uint2(0, 0);
+      ktop = max(ktop, max(finite_top2(w.x), finite_top2(w.y)));
+      out[(t * L::kSteps + st) * 32 + lane] = w;
+    }
+  }
+#pragma unroll 1
+  for (int k = 0; k < 4; ++k) {
+    const int key = key0 + 2 * c + (k & 1) + (k >> 1) * 8;
+    const bool on = key < key_hi && g * L::kVBytes < d;
+    const uint2* row = reinterpret_cast<const uint2*>(vt + (int64_t)(on ? key - sealed : 0) * d + g * L::kVBytes);
+#pragma unroll
+    for (int w = 0; w < L::kVBytes / 4; ++w) {
+      const uint2 x = on ? row[w] : make_uint2(0, 0);
+      vtop = max(vtop, max(finite_top2(x.x), finite_top2(x.y)));
+      if (any_nonfinite2(x.x) || any_nonfinite2(x.y)) bad |= 1u << k;
+      out[(2 * L::kSteps + 4 * w + k) * 32 + lane] = x;
+    }
+  }
+  ktop = __reduce_max_sync(0xffffffffu, ktop);
+  vtop = __reduce_max_sync(0xffffffffu, vtop);
+#pragma unroll
+  for (int off = 4; off < 32; off <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, off);
+  const int ke = fit_exponent(ktop), ve = fit_exponent(vtop);
+  kscale = pow2f(ke);
+  vscale = pow2f(ve);
+  const float kinv = pow2f(-ke), vinv = pow2f(-ve);
+#pragma unroll 2
+  for (int i = 0; i < 2 * L::kSteps; ++i) {
+    const uint2 w = out[i * 32 + lane];
+    out[i * 32 + lane] = make_uint2(pack_f16x2(bf_lo(w.x) * kinv, bf_hi(w.x) * kinv),
+                                    pack_f16x2(bf_lo(w.y) * kinv, bf_hi(w.y) * kinv));
+  }
+#pragma unroll 1
+  for (int w = 0; w < L::kVBytes / 4; ++w) {
+    uint2* at = out + (2 * L::kSteps + 4 * w) * 32 + lane;
+    float f[4][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint2 u = at[k * 32];
+      f[k][0] = bf_lo(u.x);
+      f[k][1] = bf_hi(u.x);
+      f[k][2] = bf_lo(u.y);
+      f[k][3] = bf_hi(u.y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[k][i] = fabsf(f[k][i]) < INFINITY ? f[k][i] * vinv : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i * 32] = make_uint2(pack_f16x2(f[0][i], f[1][i]), pack_f16x2(f[2][i], f[3][i]));
+  }
+}
+
 // grid: (hkv, row tiles, splits * batch).
 template <int DT>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, 4)
 kv8_attn_kernel(Kv8Attn p) {
   using L = Layout<DT>;
   pdl_wait();
   pdl_trigger();
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float join_m[kWarps][kRows], join_l[kWarps][kRows];
+  __shared__ __align__(16) uint4 q_frag[L::kSteps][32];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -119,25 +194,32 @@ kv8_attn_kernel(Kv8Attn p) {
     cp_commit();
   };
 
+  uint2* tail_s = reinterpret_cast<uint2*>(smem + (size_t)warp * kStages * L::kUnitBytes);
   const int first = key_lo + warp * kUnit;
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) load_unit(first + s * kStep, s);
 
   // Q fragments of rows g and g + 8: the dims of k-step (j, w) of this
-  // thread are j * 64 + c * 16 + w * 4 + {0, 1, 2, 3}.
-  uint32_t qf[L::kSteps][4];
+  // thread are j * 64 + c * 16 + w * 4 + {0, 1, 2, 3}.  Every warp needs the same
+  // ones: each writes a quarter of them.
   float qs[2];                 // scale * log2(e) * (power of two taken out of the row)
   const uint32_t* rbits[2];
   bool rok[2];
+  {
+    uint32_t qf[L::kSteps][4];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int pr = blockIdx.y * kRows + g + r * 8;
-    rok[r] = pr < packed;
-    const int t = rok[r] ? pr % p.q_len : 0;
-    const int head = kvh * p.group + (rok[r] ? pr / p.q_len : 0);
-    rbits[r] = p.bits ? p.bits + req * p.bits_bs + (int64_t)t * p.words : nullptr;
-    const __nv_bfloat16* qrow = p.q + req * p.q_bs + head * p.q_hs + t * p.q_rs;
-    qs[r] = p.scale_log2 * q_row_fragments<L::kSteps>(rok[r] ? qrow : nullptr, d, c, qf, r);
+    for (int r = 0; r < 2; ++r) {
+      const int pr = blockIdx.y * kRows + g + r * 8;
+      rok[r] = pr < packed;
+      const int qh = rok[r] ? (int)(((uint64_t)pr * p.q_magic) >> 40) : 0, t = rok[r] ? pr - qh * p.q_len : 0;
+      rbits[r] = p.bits ? p.bits + req * p.bits_bs + (int64_t)t * p.words : nullptr;
+      const __nv_bfloat16* qrow = p.q + req * p.q_bs + (int64_t)(kvh * p.group + qh) * p.q_hs + t * p.q_rs;
+      qs[r] = p.scale_log2 * q_row_fragments<L::kSteps>(rok[r] ? qrow : nullptr, d, c, qf, r);
+    }
+#pragma unroll
+    for (int st = 0; st < L::kSteps; ++st)
+      if ((st & (kWarps - 1)) == warp) q_frag[st][lane] = make_uint4(qf[st][0], qf[st][1], qf[st][2], qf[st][3]);
+    __syncthreads();
   }
 
   float o[L::kTiles][4];
@@ -160,13 +242,9 @@ kv8_attn_kernel(Kv8Attn p) {
     if (++stage == kStages) stage = 0;
 
     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    uint32_t vf[4][L::kVBytes / 4];  // codes of four keys, or (tail) fp16 pairs built below
     float kscale, vscale;
     const bool coded = key0 < sealed;
-    uint32_t bad = 0;       // tail: bit k set when this thread's key k has a non-finite value
-    const uint2* tail_v[4];
-    bool tail_on[4];
-    float vinv = 1.f;
+    uint32_t bad = 0;  // tail: bit k set when this thread's key k has a non-finite value
     if (coded) {
       kscale = ksc[key0 >> p.c.block_shift];
       vscale = vsc[key0 >> p.c.block_shift];
@@ -175,81 +253,27 @@ kv8_attn_kernel(Kv8Attn p) {
         vscale = unit;
       }
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int j = 0; j < L::kKChunks; ++j) {
+        const uint4 w0 = *reinterpret_cast<const uint4*>(at + (j * 32 + lane) * 16);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(at + ((L::kKChunks + j) * 32 + lane) * 16);
+        const uint32_t a0[4] = {w0.x, w0.y, w0.z, w0.w}, a1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-        for (int j = 0; j < L::kKChunks; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(at + ((t * L::kKChunks + j) * 32 + lane) * 16);
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mma_f16(s[t], qf[j * 4 + i], e4m3x2_to_f16x2(ww[i]), e4m3x2_hi_to_f16x2(ww[i]));
-        }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint8_t* a = at + 32 * L::kKBytes + (k * 32 + lane) * L::kVBytes;
-        if constexpr (L::kVBytes == 16) {
-          const uint4 w = *reinterpret_cast<const uint4*>(a);
-          vf[k][0] = w.x;
-          vf[k][1] = w.y;
-          vf[k][2] = w.z;
-          vf[k][3] = w.w;
-        } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(a);
-          vf[k][0] = w.x;
-          vf[k][1] = w.y;
+        for (int i = 0; i < 4; ++i) {
+          const uint4 qv = q_frag[j * 4 + i][lane];
+          const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
+          mma_f16(s[0], qa, e4m3x2_to_f16x2(a0[i]), e4m3x2_hi_to_f16x2(a0[i]));
+          mma_f16(s[1], qa, e4m3x2_to_f16x2(a1[i]), e4m3x2_hi_to_f16x2(a1[i]));
         }
       }
     } else {
-      // Tail: two looks at the rows, the first for the unit's magnitudes.
-      uint32_t ktop = 0, vtop = 0;
+      tail_unit<DT>(kt, vt, key0, sealed, key_hi, d, g, c, lane, tail_s, kscale, vscale, bad);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int key = key0 + t * 8 + g;
-        const __nv_bfloat16* row = kt + (int64_t)(key - sealed) * d;
-#pragma unroll
-        for (int st = 0; st < L::kSteps; ++st) {
-          const int dim = (st >> 2) * 64 + c * 16 + (st & 3) * 4;
-          if (key < key_hi && dim < d) {
-            const uint2 w = *reinterpret_cast<const uint2*>(row + dim);
-            ktop = max(ktop, max(finite_top2(w.x), finite_top2(w.y)));
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int key = key0 + 2 * c + (k & 1) + (k >> 1) * 8;
-        tail_on[k] = key < key_hi;
-        tail_v[k] = reinterpret_cast<const uint2*>(vt + (int64_t)(tail_on[k] ? key - sealed : 0) * d + g * L::kVBytes);
-        tail_on[k] = tail_on[k] && g * L::kVBytes < d;
-#pragma unroll
-        for (int w = 0; w < L::kVBytes / 4; ++w)
-          if (tail_on[k]) {
-            const uint2 x = tail_v[k][w];
-            vtop = max(vtop, max(finite_top2(x.x), finite_top2(x.y)));
-            if (any_nonfinite2(x.x) || any_nonfinite2(x.y)) bad |= 1u << k;
-          }
-      }
-      ktop = __reduce_max_sync(0xffffffffu, ktop);
-      vtop = __reduce_max_sync(0xffffffffu, vtop);
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, off);
-      const int ke = fit_exponent(ktop), ve = fit_exponent(vtop);
-      kscale = pow2f(ke);
-      vscale = pow2f(ve);
-      vinv = pow2f(-ve);
-      const float kinv = pow2f(-ke);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int key = key0 + t * 8 + g;
-        const __nv_bfloat16* row = kt + (int64_t)(key - sealed) * d;
-#pragma unroll
-        for (int st = 0; st < L::kSteps; ++st) {
-          const int dim = (st >> 2) * 64 + c * 16 + (st & 3) * 4;
-          uint2 w = make_uint2(0, 0);
-          if (key < key_hi && dim < d) w = *reinterpret_cast<const uint2*>(row + dim);
-          mma_f16(s[t], qf[st], pack_f16x2(bf_lo(w.x) * kinv, bf_hi(w.x) * kinv),
-                  pack_f16x2(bf_lo(w.y) * kinv, bf_hi(w.y) * kinv));
-        }
+      for (int st = 0; st < L::kSteps; ++st) {
+        const uint4 qv = q_frag[st][lane];
+        const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
+        const uint2 b0 = tail_s[st * 32 + lane], b1 = tail_s[(L::kSteps + st) * 32 + lane];
+        mma_f16(s[0], qa, b0.x, b0.y);
+        mma_f16(s[1], qa, b1.x, b1.y);
       }
     }
 
@@ -336,6 +360,22 @@ kv8_attn_kernel(Kv8Attn p) {
 
     // Output tile t, column g: dim g * kVBytes + t.
     if (coded) {
+      uint32_t vf[4][L::kVBytes / 4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint8_t* a = at + 32 * L::kKBytes + (k * 32 + lane) * L::kVBytes;
+        if constexpr (L::kVBytes == 16) {
+          const uint4 w = *reinterpret_cast<const uint4*>(a);
+          vf[k][0] = w.x;
+          vf[k][1] = w.y;
+          vf[k][2] = w.z;
+          vf[k][3] = w.w;
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(a);
+          vf[k][0] = w.x;
+          vf[k][1] = w.y;
+        }
+      }
 #pragma unroll
       for (int w = 0; w < L::kVBytes / 4; ++w) {
         const uint32_t a01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), a23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
@@ -347,21 +387,9 @@ kv8_attn_kernel(Kv8Attn p) {
       }
     } else {
 #pragma unroll
-      for (int w = 0; w < L::kVBytes / 4; ++w) {
-        float f[4][4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint2 u = tail_on[k] ? tail_v[k][w] : make_uint2(0, 0);
-          f[k][0] = bf_lo(u.x);
-          f[k][1] = bf_hi(u.x);
-          f[k][2] = bf_lo(u.y);
-          f[k][3] = bf_hi(u.y);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[k][i] = fabsf(f[k][i]) < INFINITY ? f[k][i] * vinv : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mma_f16(o[4 * w + i], pa, pack_f16x2(f[0][i], f[1][i]), pack_f16x2(f[2][i], f[3][i]));
+      for (int t = 0; t < L::kTiles; ++t) {
+        const uint2 b = tail_s[(2 * L::kSteps + t) * 32 + lane];
+        mma_f16(o[t], pa, b.x, b.y);
       }
     }
   }
@@ -412,7 +440,8 @@ kv8_attn_kernel(Kv8Attn p) {
       acc[2] += f * y.z;
       acc[3] += f * y.w;
     }
-    const int head = kvh * p.group + pr / p.q_len, t = pr % p.q_len;
+    const int qh = (int)(((uint64_t)pr * p.q_magic) >> 40);
+    const int head = kvh * p.group + qh, t = pr - qh * p.q_len;
     if (p.splits == 1) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
@@ -435,33 +464,38 @@ kv8_attn_kernel(Kv8Attn p) {
   }
 }
 
-// Joins the key ranges: one warp per (request, head, row), four dims a lane.
-__global__ void kv8_merge_kernel(Kv8Attn p) {
+// Joins the key ranges: W warps per (request, head, row), four dims a lane.
+// Each warp adds every W-th range, eight loads in flight (one warp that walked
+// 74 ranges of a 131,072-token context took 16 us); the warps' sums are added
+// in warp order, so the same ranges give the same bits.
+template <int W>
+__global__ void __launch_bounds__(256)
+kv8_merge_kernel(Kv8Attn p) {
   pdl_wait();
   pdl_trigger();
+  __shared__ float4 part[8][32];
   const int64_t per_req = (int64_t)p.heads * p.q_len;
-  const int64_t pair = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (pair >= per_req * p.batch) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t req = pair / per_req, at = pair % per_req;
-  const int head = (int)(at / p.q_len), t = (int)(at % p.q_len);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mine = warp % W;
+  const int64_t pair = (int64_t)blockIdx.x * (8 / W) + warp / W;
+  const bool on = pair < per_req * p.batch;
+  const int64_t req = on ? pair / per_req : 0, at = on ? pair % per_req : 0;
   const int64_t base = req * p.splits * per_req + at;
-  const int d = p.c.d;
+  const int d = p.c.d, splits = on ? p.splits : 0;
   float gm = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) gm = fmaxf(gm, p.part_ml[(base + s * per_req) * 2]);
+  for (int s = lane; s < splits; s += 32) gm = fmaxf(gm, p.part_ml[(base + s * per_req) * 2]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  for (int s0 = 0; s0 < p.splits; s0 += 32) {
+  for (int s0 = 0; s0 < splits; s0 += 32) {
     float w = 0.f;
-    if (s0 + lane < p.splits) {
+    if (s0 + lane < splits) {
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (base + (s0 + lane) * per_req) * 2);
       w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - gm);
-      sum += w * ml.y;
+      sum += w * ml.y;  // a NaN passes even where w is 0
     }
-    const int n = min(32, p.splits - s0);
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
+    const int n = min(32, splits - s0);
+#pragma unroll 8
+    for (int j = mine; j < n; j += W) {
       const float f = __shfl_sync(0xffffffffu, w, j);
       if (lane * 4 < d) {
         const float4 y = *reinterpret_cast<const float4*>(p.part_o + (base + (int64_t)(s0 + j) * per_req) * d + lane * 4);
@@ -474,6 +508,21 @@ __global__ void kv8_merge_kernel(Kv8Attn p) {
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if constexpr (W > 1) {
+    part[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    if (mine != 0) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      const float4 y = part[warp + i][lane];
+      acc[0] += y.x;
+      acc[1] += y.y;
+      acc[2] += y.z;
+      acc[3] += y.w;
+    }
+  }
+  if (!on) return;
+  const int head = (int)(at / p.q_len), t = (int)(at % p.q_len);
   if (p.lse && lane == 0)
     p.lse[pair] = sum == 0.f ? -INFINITY : (gm == -INFINITY ? sum : (gm + log2f(sum)) * 0.69314718055994531f);
   if (lane * 4 >= d) return;
@@ -484,6 +533,14 @@ __global__ void kv8_merge_kernel(Kv8Attn p) {
   w.x = *reinterpret_cast<uint32_t*>(&lo);
   w.y = *reinterpret_cast<uint32_t*>(&hi);
   *reinterpret_cast<uint2*>(p.out + req * p.out_bs + ((int64_t)t * p.heads + head) * d + lane * 4) = w;
+}
+
+template <int W>
+int launch_merge(const Kv8Attn& p, cudaStream_t stream) {
+  const int64_t pairs = (int64_t)p.batch * p.heads * p.q_len;
+  SF_CHECK_CUDA(launch_pdl(kv8_merge_kernel<W>, dim3((unsigned)((pairs * W + 7) / 8)), dim3(256), 0, stream, p));
+  SF_CHECK_LAUNCH();
+  return SF_OK;
 }
 
 template <int DT>
@@ -509,12 +566,11 @@ size_t partial_bytes(const Kv8Split& s, int batch, int heads, int head_dim, int6
 
 }  // namespace
 
-// Two resident CTAs per SM (their rings fill shared memory); a range is at
-// least two steps of the four warps.
+// Four resident CTAs per SM; a range is at least two steps of the four warps.
 Kv8Split kv8_split_mma(int batch, int hkv, int64_t packed, int64_t kv_len) {
   const int64_t units = (int64_t)batch * hkv * ((packed + kRows - 1) / kRows);
   const int64_t steps = (kv_len + kStep - 1) / kStep;
-  int64_t want = std::max<int64_t>(1, 2 * (int64_t)num_sms() / units);
+  int64_t want = std::max<int64_t>(1, 4 * (int64_t)num_sms() / units);
   want = std::min<int64_t>(want, std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, steps / 2)));
   const int64_t per = std::max<int64_t>(1, (steps + want - 1) / want);
   return {(int)std::max<int64_t>(1, (steps + per - 1) / per), (int)(per * kStep)};
@@ -604,8 +660,6 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
   else
     rc = rows->head_dim <= 64 ? launch_mma<64>(p, st) : launch_mma<128>(p, st);
   if (rc || s.splits == 1) return rc;
-  const int64_t pairs = (int64_t)rows->batch * num_heads * q_len;
-  SF_CHECK_CUDA(launch_pdl(kv8_merge_kernel, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, st, p));
-  SF_CHECK_LAUNCH();
-  return SF_OK;
+  // Up to about eight ranges a warp.
+  return s.splits <= 8 ? launch_merge<1>(p, st) : (s.splits <= 32 ? launch_merge<4>(p, st) : launch_merge<8>(p, st));
 }

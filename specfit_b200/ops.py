@@ -646,44 +646,47 @@ class Kv8Rows:
     view: it owns nothing and is not changed by the calls that read it."""
 
     __slots__ = ("k_codes", "v_codes", "k_scale", "v_scale", "sealed", "k_tail", "v_tail", "block", "device",
-                 "shape", "_c")
+                 "index", "shape", "_c", "_p")
 
     def __init__(self, k_codes, v_codes, k_scale, v_scale, sealed, k_tail, v_tail, block):
-        self.device = _require_cuda(k_codes, v_codes, k_scale, v_scale, k_tail, v_tail)
-        if k_codes.dtype != torch.float8_e4m3fn or v_codes.dtype != torch.float8_e4m3fn:
+        # The attributes are read once each: this is a good part of a small call's host time.
+        idx = k_codes.get_device()
+        if idx < 0 or not (v_codes.get_device() == k_scale.get_device() == v_scale.get_device()
+                           == k_tail.get_device() == v_tail.get_device() == idx):
+            _require_cuda(k_codes, v_codes, k_scale, v_scale, k_tail, v_tail)
+        if k_codes.dtype is not torch.float8_e4m3fn or v_codes.dtype is not torch.float8_e4m3fn:
             raise TypeError("codes must be float8_e4m3fn")
-        if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        if k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
             raise TypeError("scales must be float32")
-        if k_tail.dtype != torch.bfloat16 or v_tail.dtype != torch.bfloat16:
+        if k_tail.dtype is not torch.bfloat16 or v_tail.dtype is not torch.bfloat16:
             raise TypeError("tail rows must be bfloat16")
-        if k_codes.ndim != 4 or k_tail.ndim != 4 or k_scale.ndim != 3:
+        cs, ss, ts = k_codes.shape, k_scale.shape, k_tail.shape
+        if len(cs) != 4 or len(ts) != 4 or len(ss) != 3:
             raise ValueError("codes and tails are [batch, heads, tokens, head_dim], scales [batch, heads, blocks]")
-        if v_codes.shape != k_codes.shape or v_scale.shape != k_scale.shape or v_tail.shape != k_tail.shape:
+        cst, sst, tst = k_codes.stride(), k_scale.stride(), k_tail.stride()
+        if v_codes.shape != cs or v_scale.shape != ss or v_tail.shape != ts:
             raise ValueError("k and v must have the same shapes")
-        if v_codes.stride() != k_codes.stride() or v_scale.stride() != k_scale.stride() \
-                or v_tail.stride() != k_tail.stride():
+        if v_codes.stride() != cst or v_scale.stride() != sst or v_tail.stride() != tst:
             raise ValueError("k and v must share strides")
-        b, h, cap, d = k_codes.shape
-        n = k_tail.shape[2]
-        block, sealed = int(block), int(sealed)
+        b, h, cap, d = cs
+        n = ts[2]
         if block not in (32, 64, 128):
             raise ValueError("block must be 32, 64 or 128")
-        if (k_scale.shape[0], k_scale.shape[1]) != (b, h) or (k_tail.shape[0], k_tail.shape[1], k_tail.shape[3]) != (b, h, d):
+        if ss[0] != b or ss[1] != h or ts[0] != b or ts[1] != h or ts[3] != d:
             raise ValueError("codes, scales and tails must share batch, heads and head_dim")
-        if sealed < 0 or sealed > cap or sealed % block or k_scale.shape[2] * block < sealed:
+        if sealed < 0 or sealed > cap or sealed % block or ss[2] * block < sealed:
             raise ValueError("sealed must be a whole number of blocks that the codes and scales hold")
-        for t, rows in ((k_codes, cap), (k_tail, n)):
-            if rows and (t.stride(3) != 1 or (rows > 1 and t.stride(2) != d)):
-                raise ValueError("rows must be contiguous, head_dim elements apart")
-        if k_scale.shape[2] > 1 and k_scale.stride(2) != 1:
+        if (cap and (cst[3] != 1 or (cap > 1 and cst[2] != d))) or (n and (tst[3] != 1 or (n > 1 and tst[2] != d))):
+            raise ValueError("rows must be contiguous, head_dim elements apart")
+        if ss[2] > 1 and sst[2] != 1:
             raise ValueError("a head's scales must be contiguous")
         self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
         self.sealed, self.k_tail, self.v_tail, self.block = sealed, k_tail, v_tail, block
-        self.shape = (b, h, sealed + n, d)
-        self._c = N.Kv8RowsStruct(b, h, d, block, sealed, n, k_codes.data_ptr(), v_codes.data_ptr(),
-                                  k_codes.stride(0), k_codes.stride(1), k_scale.data_ptr(), v_scale.data_ptr(),
-                                  k_scale.stride(0), k_scale.stride(1), k_tail.data_ptr(), v_tail.data_ptr(),
-                                  k_tail.stride(0), k_tail.stride(1))
+        self.device, self.index, self.shape = k_codes.device, idx, (b, h, sealed + n, d)
+        self._c = N.Kv8RowsStruct(b, h, d, block, sealed, n, k_codes.data_ptr(), v_codes.data_ptr(), cst[0], cst[1],
+                                  k_scale.data_ptr(), v_scale.data_ptr(), sst[0], sst[1], k_tail.data_ptr(),
+                                  v_tail.data_ptr(), tst[0], tst[1])
+        self._p = ctypes.addressof(self._c)
 
     @property
     def length(self) -> int:
@@ -691,9 +694,28 @@ class Kv8Rows:
         return self.shape[2]
 
 
-def _on(dev: torch.device):
-    """Launches go to ``dev`` whatever the caller's current device is."""
-    return torch.cuda.device(dev)
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _on(index: int):
+    """Launches go to device ``index`` whatever the caller's current device is."""
+    return _HERE if _current_device() == index else torch.cuda.device(index)
+
+
+def _same_device(index: int, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.get_device() != index:
+            raise ValueError("all tensors must be CUDA tensors on the cache's device")
 
 
 def kv8_seal(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor,
@@ -701,28 +723,33 @@ def kv8_seal(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: t
     """Seals bf16 rows ``k, v [B, Hkv, n * block, D]`` into the code and scale
     buffers of a cache (``Kv8Rows``'s layout), starting at ``first_block``.
     ``block`` defaults to the buffers' tokens over their scales."""
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+    if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
         raise TypeError("kv8_seal takes bf16 rows")
-    if k.ndim != 4 or k.shape != v.shape:
+    ks = k.shape
+    if len(ks) != 4 or ks != v.shape:
         raise ValueError("k and v must be [batch, heads, tokens, head_dim]")
-    cap = k_codes.shape[2] if k_codes.ndim == 4 else 0
+    cs, ss = k_codes.shape, k_scale.shape
+    cap = cs[2] if len(cs) == 4 else 0
     if block is None:
-        blocks = k_scale.shape[2] if k_scale.ndim == 3 else 0
-        block = cap // blocks if blocks else 0
+        block = cap // ss[2] if len(ss) == 3 and ss[2] else 0
     none = k[:, :, :0]
     rows = Kv8Rows(k_codes, v_codes, k_scale, v_scale, cap // max(block, 1) * block, none, none, block)
-    dev = _require_cuda(k, k_codes)
-    if (k.shape[0], k.shape[1], k.shape[3]) != (rows.shape[0], rows.shape[1], rows.shape[3]):
+    index = rows.index
+    _same_device(index, k, v)
+    if ks[0] != cs[0] or ks[1] != cs[1] or ks[3] != cs[3]:
         raise ValueError("rows and buffers must share batch, heads and head_dim")
-    if k.shape[2] % block:
+    if ks[2] % block:
         raise ValueError("only whole blocks can be sealed")
-    if k.stride(3) != 1 or k.stride() != v.stride() or any(s % 8 for s in k.stride()[:3]) or k.data_ptr() % 16 \
-            or v.data_ptr() % 16:
+    st = k.stride()
+    kp, vp = k.data_ptr(), v.data_ptr()
+    if st[3] != 1 or (st[0] | st[1] | st[2]) & 7 or (kp | vp) & 15 or v.stride() != st:
         k, v = k.contiguous(), v.contiguous()
-    n = k.shape[2] // block
-    with _on(dev):
-        N.check(N.lib.sf_kv8_seal(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                                  ctypes.byref(rows._c), int(first_block), n, _stream(dev)), "sf_kv8_seal")
+        st, kp, vp = k.stride(), k.data_ptr(), v.data_ptr()
+    n = ks[2] // block
+    with _on(index):
+        rc = N.lib.sf_kv8_seal(kp, vp, st[0], st[1], st[2], rows._p, first_block, n, _raw_stream(index))
+    if rc:
+        N.check(rc, "sf_kv8_seal")
     _launched(1 if n else 0)
 
 
@@ -735,38 +762,44 @@ def kv8_read(rows: Kv8Rows, first: int = 0, count: int | None = None) -> tuple[t
         raise ValueError("rows to read must lie within the cache")
     k = torch.empty(b, h, count, d, dtype=torch.bfloat16, device=rows.device)
     v = torch.empty_like(k)
-    with _on(rows.device):
-        N.check(N.lib.sf_kv8_read(ctypes.byref(rows._c), int(first), count, k.data_ptr(), v.data_ptr(),
-                                  k.stride(0), k.stride(1), _stream(rows.device)), "sf_kv8_read")
+    with _on(rows.index):
+        N.check(N.lib.sf_kv8_read(rows._p, int(first), count, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
+                                  _raw_stream(rows.index)), "sf_kv8_read")
     _launched(1 if count else 0)
     return k, v
 
 
 def _kv8_query(q: torch.Tensor, rows: Kv8Rows, tree_bits: torch.Tensor | None, prefix_len: int):
-    """Checks shared by attention and mass: (q, bits, words, bits' batch stride)."""
-    if q.dtype != torch.bfloat16:
+    """Checks shared by attention and mass: (q, its strides, bits, words, bits'
+    batch stride)."""
+    if q.dtype is not torch.bfloat16:
         raise TypeError("queries must be bf16")
     b, hkv, total, d = rows.shape
-    if q.ndim != 4 or q.shape[0] != b or q.shape[3] != d or q.shape[1] == 0 or q.shape[1] % hkv:
+    qs = q.shape
+    if len(qs) != 4 or qs[0] != b or qs[3] != d or qs[1] == 0 or qs[1] % hkv:
         raise ValueError("q must be [batch, heads, rows, head_dim] with heads a multiple of the KV heads")
     if not 0 <= prefix_len <= total:
         raise ValueError("prefix_len must lie within the cache")
-    if q.stride(3) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.stride(2) % 8 or q.data_ptr() % 16:
+    _same_device(rows.index, q)
+    st = q.stride()
+    if st[3] != 1 or (st[0] | st[1] | st[2]) & 7 or q.data_ptr() & 15:
         q = q.contiguous()
+        st = q.stride()
     if tree_bits is None:
         if prefix_len != total:
             raise ValueError("tree_bits must cover the keys from prefix_len on")
-        _require_cuda(rows.k_codes, q)
-        return q, None, 0, 0
-    _require_cuda(rows.k_codes, q, tree_bits)
-    if tree_bits.dtype != torch.int32 or tree_bits.ndim != 3 or tree_bits.shape[:2] != (b, q.shape[2]):
+        return q, st, None, 0, 0
+    _same_device(rows.index, tree_bits)
+    bs = tree_bits.shape
+    if tree_bits.dtype is not torch.int32 or len(bs) != 3 or bs[0] != b or bs[1] != qs[2]:
         raise ValueError("tree_bits must be int32 [batch, rows, words]")
-    if tree_bits.shape[2] * 32 < total - prefix_len:
+    if bs[2] * 32 < total - prefix_len:
         raise ValueError("tree_bits must cover the keys from prefix_len on")
-    bits = tree_bits
-    if bits.stride(2) != 1 or bits.stride(1) != bits.shape[2]:
-        bits = bits.contiguous()
-    return q, bits, bits.shape[2], bits.stride(0)
+    bst = tree_bits.stride()
+    if bst[2] != 1 or bst[1] != bs[2]:
+        tree_bits = tree_bits.contiguous()
+        bst = tree_bits.stride()
+    return q, st, tree_bits, bs[2], bst[0]
 
 
 def kv8_tree_attention(q: torch.Tensor, rows: Kv8Rows, tree_bits: torch.Tensor | None, prefix_len: int,
@@ -777,25 +810,30 @@ def kv8_tree_attention(q: torch.Tensor, rows: Kv8Rows, tree_bits: torch.Tensor |
     set.  Returns ``[B, Tq, Hq, D]`` bf16 and, with ``return_lse``, the natural
     log-sum-exp of the scaled scores, fp32 ``[B, Hq, Tq]``.  A row that sees
     nothing answers zeros and -infinity."""
-    q, bits, words, bits_bs = _kv8_query(q, rows, tree_bits, prefix_len)
-    dev = rows.device
+    q, st, bits, words, bits_bs = _kv8_query(q, rows, tree_bits, prefix_len)
+    dev, index = rows.device, rows.index
     b, hq, tq, d = q.shape
     if out is None:
-        out = torch.empty(b, tq, hq, d, dtype=torch.bfloat16, device=dev)
+        out = torch.empty((b, tq, hq, d), dtype=torch.bfloat16, device=dev)
+        out_bs = tq * hq * d
     else:
-        _require_cuda(rows.k_codes, out)
-        if out.dtype != torch.bfloat16 or out.shape != (b, tq, hq, d) or (out.numel() and not out[0].is_contiguous()):
-            raise ValueError("out must be bf16 [batch, rows, heads, head_dim], each request contiguous")
-    lse = torch.empty(b, hq, tq, dtype=torch.float32, device=dev) if return_lse else None
-    sc = float(d ** -0.5 if scale is None else scale)
-    with _on(dev):
-        nbytes = N.lib.sf_kv8_attention_workspace_bytes(b, hq, rows.shape[1], d, tq, rows.sealed,
-                                                        rows.length - rows.sealed)
+        _same_device(index, out)
+        if out.dtype is not torch.bfloat16 or out.shape != (b, tq, hq, d) \
+                or (out.numel() and not out[0].is_contiguous()) or out.data_ptr() % 16 or out.stride(0) % 8:
+            raise ValueError("out must be bf16 [batch, rows, heads, head_dim], each request contiguous, 16-byte aligned")
+        out_bs = out.stride(0)
+    lse = torch.empty((b, hq, tq), dtype=torch.float32, device=dev) if return_lse else None
+    total = rows.shape[2]
+    with _on(index):
+        nbytes = N.lib.sf_kv8_attention_workspace_bytes(b, hq, rows.shape[1], d, tq, rows.sealed, total - rows.sealed)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        N.check(N.lib.sf_kv8_tree_attention(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), hq, tq,
-                                            ctypes.byref(rows._c), _ptr(bits), words, bits_bs, int(prefix_len), sc,
-                                            out.data_ptr(), out.stride(0), _ptr(lse), _ptr(ws), nbytes,
-                                            _stream(dev)), "sf_kv8_tree_attention")
+        rc = N.lib.sf_kv8_tree_attention(q.data_ptr(), st[0], st[1], st[2], hq, tq, rows._p,
+                                         None if bits is None else bits.data_ptr(), words, bits_bs, prefix_len,
+                                         d ** -0.5 if scale is None else scale, out.data_ptr(), out_bs,
+                                         None if lse is None else lse.data_ptr(),
+                                         None if ws is None else ws.data_ptr(), nbytes, _raw_stream(index))
+    if rc:
+        N.check(rc, "sf_kv8_tree_attention")
     _launched((2 if nbytes else 1) if tq else 0)
     return (out, lse) if return_lse else out
 
@@ -805,22 +843,25 @@ def kv8_attention_mass(q: torch.Tensor, lse: torch.Tensor, rows: Kv8Rows, tree_b
     """Adds to ``mass`` (fp32 ``[B, Hkv, >= length]``) the attention weight that
     each cached token received from the rows of a ``kv8_tree_attention`` call
     with the same arguments, ``lse`` being what it returned; returns ``mass``."""
-    q, bits, words, bits_bs = _kv8_query(q, rows, tree_bits, prefix_len)
-    dev = _require_cuda(rows.k_codes, lse, mass)
+    q, st, bits, words, bits_bs = _kv8_query(q, rows, tree_bits, prefix_len)
+    index = rows.index
+    _same_device(index, lse, mass)
     b, hq, tq, d = q.shape
-    if lse.dtype != torch.float32 or lse.shape != (b, hq, tq):
+    if lse.dtype is not torch.float32 or lse.shape != (b, hq, tq):
         raise ValueError("lse must be float32 [batch, heads, rows]")
-    if mass.dtype != torch.float32 or mass.ndim != 3 or mass.shape[:2] != rows.shape[:2] \
-            or mass.shape[2] < rows.length or (mass.shape[2] > 1 and mass.stride(2) != 1):
+    ms, mst = mass.shape, mass.stride()
+    if mass.dtype is not torch.float32 or len(ms) != 3 or ms[0] != b or ms[1] != rows.shape[1] \
+            or ms[2] < rows.shape[2] or (ms[2] > 1 and mst[2] != 1):
         raise ValueError("mass must be float32 [batch, KV heads, >= length], contiguous per head")
-    sc = float(d ** -0.5 if scale is None else scale)
     lse = lse.contiguous()
-    with _on(dev):
-        N.check(N.lib.sf_kv8_attention_mass(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), hq, tq,
-                                            lse.data_ptr(), ctypes.byref(rows._c), _ptr(bits), words, bits_bs,
-                                            int(prefix_len), sc, mass.data_ptr(), mass.stride(0), mass.stride(1),
-                                            _stream(dev)), "sf_kv8_attention_mass")
-    _launched(1 if tq and rows.length else 0)
+    with _on(index):
+        rc = N.lib.sf_kv8_attention_mass(q.data_ptr(), st[0], st[1], st[2], hq, tq, lse.data_ptr(), rows._p,
+                                         None if bits is None else bits.data_ptr(), words, bits_bs, prefix_len,
+                                         d ** -0.5 if scale is None else scale, mass.data_ptr(), mst[0], mst[1],
+                                         _raw_stream(index))
+    if rc:
+        N.check(rc, "sf_kv8_attention_mass")
+    _launched(1 if tq and rows.shape[2] else 0)
     return mass
 
 
@@ -829,18 +870,20 @@ def kv_keep_heaviest(mass: torch.Tensor, length: int, budget: int, sinks: int = 
     per request and head of ``mass`` (fp32 ``[B, Hkv, >= length]``): the first
     ``sinks``, the last ``recent``, and the heaviest of the others (ties: the
     earlier token; NaN: the least).  int32 ``[B, Hkv, budget]``, ascending."""
-    dev = _require_cuda(mass)
-    if mass.dtype != torch.float32 or mass.ndim != 3 or mass.shape[2] < length \
-            or (mass.shape[2] > 1 and mass.stride(2) != 1):
+    index = mass.get_device()
+    if index < 0:
+        raise ValueError("specfit_b200 ops need CUDA tensors")
+    ms, mst = mass.shape, mass.stride()
+    if mass.dtype is not torch.float32 or len(ms) != 3 or ms[2] < length or (ms[2] > 1 and mst[2] != 1):
         raise ValueError("mass must be float32 [batch, KV heads, >= length], contiguous per head")
     if sinks < 0 or recent < 0 or sinks + recent > budget or budget > length:
         raise ValueError("sinks + recent <= budget <= length is needed")
-    b, h = mass.shape[:2]
-    keep = torch.empty(b, h, budget, dtype=torch.int32, device=dev)
-    with _on(dev):
-        N.check(N.lib.sf_kv_keep_heaviest(mass.data_ptr(), mass.stride(0), mass.stride(1), b, h, int(length),
-                                          int(budget), int(sinks), int(recent), keep.data_ptr(), _stream(dev)),
-                "sf_kv_keep_heaviest")
+    keep = torch.empty((ms[0], ms[1], budget), dtype=torch.int32, device=mass.device)
+    with _on(index):
+        rc = N.lib.sf_kv_keep_heaviest(mass.data_ptr(), mst[0], mst[1], ms[0], ms[1], length, budget, sinks, recent,
+                                       keep.data_ptr(), _raw_stream(index))
+    if rc:
+        N.check(rc, "sf_kv_keep_heaviest")
     _launched(1 if budget else 0)
     return keep
 
@@ -852,37 +895,42 @@ def kv8_compact(rows: Kv8Rows, keep: torch.Tensor, mass: torch.Tensor | None = N
     the last ``n % block`` rows as its bf16 tail; ``mass`` (optional) moves
     along.  Returns ``(Kv8Rows, mass or None)``, in buffers of its own or in
     ``out`` / ``mass_out`` (other buffers than the source's)."""
-    dev = _require_cuda(rows.k_codes, keep)
+    index, dev = rows.index, rows.device
+    _same_device(index, keep)
     b, h, total, d = rows.shape
-    if keep.dtype != torch.int32 or keep.ndim != 3 or keep.shape[:2] != (b, h) or keep.shape[2] > total:
+    kshape = keep.shape
+    if keep.dtype is not torch.int32 or len(kshape) != 3 or kshape[0] != b or kshape[1] != h or kshape[2] > total:
         raise ValueError("keep must be int32 [batch, KV heads, n], n at most the cache's length")
-    n = keep.shape[2]
-    full = n // rows.block * rows.block
+    n, block = kshape[2], rows.block
+    full = n // block * block
     if out is None:
-        kc = torch.empty(2, b, h, full, d, dtype=torch.float8_e4m3fn, device=dev)
-        sc = torch.empty(2, b, h, full // rows.block, dtype=torch.float32, device=dev)
-        tl = torch.empty(2, b, h, n - full, d, dtype=torch.bfloat16, device=dev)
-        out = Kv8Rows(kc[0], kc[1], sc[0], sc[1], full, tl[0], tl[1], rows.block)
-    elif out.shape != (b, h, n, d) or out.sealed != full or out.block != rows.block or out.device != dev:
+        kc, vc = torch.empty((2, b, h, full, d), dtype=torch.float8_e4m3fn, device=dev).unbind(0)
+        ks, vs = torch.empty((2, b, h, full // block), dtype=torch.float32, device=dev).unbind(0)
+        kt, vt = torch.empty((2, b, h, n - full, d), dtype=torch.bfloat16, device=dev).unbind(0)
+        out = Kv8Rows(kc, vc, ks, vs, full, kt, vt, block)
+    elif out.shape != (b, h, n, d) or out.sealed != full or out.block != block or out.index != index:
         raise ValueError("out must hold the kept rows: whole blocks sealed, the rest as its tail")
+    m = (None, 0, 0, None, 0, 0)
     if mass is not None:
-        _require_cuda(rows.k_codes, mass)
-        if mass.dtype != torch.float32 or mass.ndim != 3 or mass.shape[:2] != (b, h) or mass.shape[2] < total \
-                or (mass.shape[2] > 1 and mass.stride(2) != 1):
+        _same_device(index, mass)
+        ms, mst = mass.shape, mass.stride()
+        if mass.dtype is not torch.float32 or len(ms) != 3 or ms[0] != b or ms[1] != h or ms[2] < total \
+                or (ms[2] > 1 and mst[2] != 1):
             raise ValueError("mass must be float32 [batch, KV heads, >= length], contiguous per head")
         if mass_out is None:
-            mass_out = torch.empty(b, h, n, dtype=torch.float32, device=dev)
-        elif mass_out.dtype != torch.float32 or mass_out.ndim != 3 or mass_out.shape[:2] != (b, h) \
+            mass_out = torch.empty((b, h, n), dtype=torch.float32, device=dev)
+        elif mass_out.dtype is not torch.float32 or mass_out.ndim != 3 or mass_out.shape[:2] != (b, h) \
                 or mass_out.shape[2] < n or (mass_out.shape[2] > 1 and mass_out.stride(2) != 1):
             raise ValueError("mass_out must be float32 [batch, KV heads, >= n], contiguous per head")
-        _require_cuda(mass, mass_out)
+        _same_device(index, mass_out)
+        if n:
+            m = (mass.data_ptr(), mst[0], mst[1], mass_out.data_ptr(), mass_out.stride(0), mass_out.stride(1))
     elif mass_out is not None:
         raise ValueError("mass_out needs mass")
     kp = keep.contiguous()
-    m = (_ptr(mass), mass.stride(0), mass.stride(1), _ptr(mass_out), mass_out.stride(0), mass_out.stride(1)) \
-        if mass is not None and n else (None, 0, 0, None, 0, 0)
-    with _on(dev):
-        N.check(N.lib.sf_kv8_compact(ctypes.byref(rows._c), kp.data_ptr(), n, ctypes.byref(out._c), *m,
-                                     _stream(dev)), "sf_kv8_compact")
+    with _on(index):
+        rc = N.lib.sf_kv8_compact(rows._p, kp.data_ptr(), n, out._p, *m, _raw_stream(index))
+    if rc:
+        N.check(rc, "sf_kv8_compact")
     _launched(1 if n else 0)
     return out, mass_out
