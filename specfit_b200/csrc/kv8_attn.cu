@@ -11,7 +11,7 @@
 // tile (row = head_in_group * Tq + t) a few query rows need 2 MMAs per 8 keys
 // and 16 dims, far below the tensor rate, so what has to be kept small is the
 // work per element: loading, decoding, and the softmax.
-//   * Every warp walks its own 16-key units of the CTA's range with its own
+//   * Every warp walks its own 32-key units of the CTA's range with its own
 //     online softmax; the four warps and the splits are joined at the end.
 //     Nothing in the loop waits for another warp.
 //   * Dims of a key are a sum, keys of a value too, so both may be taken in
@@ -30,10 +30,11 @@
 //     more than fp16's 11 bits (probabilities are kept times 2^12).
 //   * The reference maximum of a row moves only when a score exceeds it by
 //     more than 3 (base 2), so accumulators are rarely rescaled.
-//   * Q's fragments are read from shared memory (one 16-byte load serves two
-//     MMAs) and tail units are converted there, which leaves 128 registers a
-//     thread and four CTAs on an SM: with 200 and two, 131,072 tokens took 47
-//     us where now they take @LONG@.
+//   * What bounds it is instructions: of the 20 or so that 16 codes take, 6 are
+//     conversions (ALU, half rate) and 2 MMAs.  Hence 32 keys a step (645
+//     instructions for 16 keys were 43 us at 131,072 tokens), Q's fragments from
+//     shared memory (one 16-byte load for four MMAs), tail units converted there
+//     too, and addresses that are constants where D is the tile's width.
 // Tail units (bf16 rows: few) are scaled by a power of two per unit and
 // enter the same fragments.  A value row with a NaN or an infinity (a sealed
 // block of values that holds one) makes its key's score NaN, so that rows
@@ -50,10 +51,11 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kRows = 16;      // packed query rows of a CTA
-constexpr int kUnit = 16;      // keys of one step of a warp
-constexpr int kStages = 3;     // units of a warp's ring
+constexpr int kUnit = 32;      // keys of one step of a warp: within one block of codes
+constexpr int kHalves = kUnit / 16;
+constexpr int kStages = 2;     // units of a warp's ring
 constexpr int kStep = kWarps * kUnit;
-constexpr int kMaxSplits = 160;
+constexpr int kMaxSplits = 128;
 constexpr float kPShift = 12.f;  // probabilities are kept times 2^12
 constexpr float kSlack = 3.f;    // a row's reference maximum may lag by this (base 2)
 
@@ -63,8 +65,9 @@ struct Layout {
   static constexpr int kVBytes = DT / 8;               // bytes of a value row per thread
   static constexpr int kSteps = DT / 16;               // MMA k-steps of Q K^T
   static constexpr int kTiles = DT / 8;                // output tiles of P V
-  static constexpr int kKBytes = 2 * kKChunks * 16;    // per thread and unit
-  static constexpr int kUnitBytes = 32 * (kKBytes + 4 * kVBytes);  // 16 keys: K and V codes
+  static constexpr int kKBytes = 2 * kHalves * kKChunks * 16;  // per thread and unit
+  static constexpr int kVKeys = 4 * kHalves;           // keys of a thread in P V
+  static constexpr int kUnitBytes = 32 * (kKBytes + kVKeys * kVBytes);  // K and V codes
   static constexpr int kRing = kWarps * kStages * kUnitBytes;
   // A tail unit as fp16 takes twice its codes' bytes, in the ring, where no copy is in flight by then.
   static_assert(kStages >= 2, "a tail unit needs two stages");
@@ -72,18 +75,21 @@ struct Layout {
   static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
 };
 
-// A unit of 16 tail rows as fp16 fragments in this thread's slots of `out`
-// ([K: 2 x steps][V: tiles] of 32 lanes), scaled by powers of two that are
-// returned; zeros for keys from key_hi on.  First the rows as they are and
-// their magnitudes, then each slot in place.
+// A unit of tail rows as fp16 fragments in this thread's slots of `out`
+// ([K: key tiles x steps][V: halves x output tiles] of 32 lanes), scaled by
+// powers of two that are returned; zeros for keys from key_hi on.  First the
+// rows as they are and their magnitudes, then each slot in place.  Bit k of
+// `bad`: key k of this thread (its two of each key tile) has a value that is
+// not finite.
 template <int DT>
 __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bfloat16* vt, int key0, int sealed,
                                           int key_hi, int d, int g, int c, int lane, uint2* out, float& kscale,
                                           float& vscale, uint32_t& bad) {
   using L = Layout<DT>;
+  constexpr int kKSlots = 2 * kHalves * L::kSteps;
   uint32_t ktop = 0, vtop = 0;
 #pragma unroll 1
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < 2 * kHalves; ++t) {
     const int key = key0 + t * 8 + g;
     const __nv_bfloat16* row = kt + (int64_t)(key < key_hi ? key - sealed : 0) * d;
 #pragma unroll
@@ -95,8 +101,8 @@ __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bf
     }
   }
 #pragma unroll 1
-  for (int k = 0; k < 4; ++k) {
-    const int key = key0 + 2 * c + (k & 1) + (k >> 1) * 8;
+  for (int k = 0; k < L::kVKeys; ++k) {  // half k / 4; keys 2c, 2c + 1, 8 + 2c, 9 + 2c of it
+    const int key = key0 + (k >> 2) * 16 + 2 * c + (k & 1) + ((k >> 1) & 1) * 8;
     const bool on = key < key_hi && g * L::kVBytes < d;
     const uint2* row = reinterpret_cast<const uint2*>(vt + (int64_t)(on ? key - sealed : 0) * d + g * L::kVBytes);
 #pragma unroll
@@ -104,7 +110,7 @@ __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bf
       const uint2 x = on ? row[w] : make_uint2(0, 0);
       vtop = max(vtop, max(finite_top2(x.x), finite_top2(x.y)));
       if (any_nonfinite2(x.x) || any_nonfinite2(x.y)) bad |= 1u << k;
-      out[(2 * L::kSteps + 4 * w + k) * 32 + lane] = x;
+      out[(kKSlots + (k >> 2) * L::kTiles + 4 * w + (k & 3)) * 32 + lane] = x;
     }
   }
   ktop = __reduce_max_sync(0xffffffffu, ktop);
@@ -116,14 +122,14 @@ __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bf
   vscale = pow2f(ve);
   const float kinv = pow2f(-ke), vinv = pow2f(-ve);
 #pragma unroll 2
-  for (int i = 0; i < 2 * L::kSteps; ++i) {
+  for (int i = 0; i < kKSlots; ++i) {
     const uint2 w = out[i * 32 + lane];
     out[i * 32 + lane] = make_uint2(pack_f16x2(bf_lo(w.x) * kinv, bf_hi(w.x) * kinv),
                                     pack_f16x2(bf_lo(w.y) * kinv, bf_hi(w.y) * kinv));
   }
 #pragma unroll 1
-  for (int w = 0; w < L::kVBytes / 4; ++w) {
-    uint2* at = out + (2 * L::kSteps + 4 * w) * 32 + lane;
+  for (int w = 0; w < kHalves * L::kTiles / 4; ++w) {
+    uint2* at = out + (kKSlots + 4 * w) * 32 + lane;
     float f[4][4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -140,9 +146,9 @@ __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bf
   }
 }
 
-// grid: (hkv, row tiles, splits * batch).
-template <int DT>
-__global__ void __launch_bounds__(kWarps * 32, 4)
+// grid: (hkv, row tiles, splits * batch).  Full: D is DT.
+template <int DT, bool Full>
+__global__ void __launch_bounds__(kWarps * 32, 3)
 kv8_attn_kernel(Kv8Attn p) {
   using L = Layout<DT>;
   pdl_wait();
@@ -159,7 +165,7 @@ kv8_attn_kernel(Kv8Attn p) {
   const int key_hi = min(p.kv_len, key_lo + p.keys_per_split);
   const int packed = p.group * p.q_len;
   const int sealed = (int)p.c.sealed;
-  const int d = p.c.d;
+  const int d = Full ? DT : p.c.d;
 
   const uint8_t* kc = p.c.k + req * p.c.c_bs + kvh * p.c.c_hs;
   const uint8_t* vc = p.c.v + req * p.c.c_bs + kvh * p.c.c_hs;
@@ -172,24 +178,22 @@ kv8_attn_kernel(Kv8Attn p) {
   const uint32_t ring = smem_addr(smem) + (uint32_t)warp * kStages * L::kUnitBytes;
   auto load_unit = [&](int key0, int stage) {
     if (key0 < key_hi && key0 < sealed) {
-      const uint32_t at = ring + (uint32_t)stage * L::kUnitBytes;
+      const uint32_t at = ring + (uint32_t)stage * L::kUnitBytes + (uint32_t)lane * 16;
+      const uint8_t* kp = kc + (int64_t)(key0 + g) * d + c * 16;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2 * kHalves; ++t)
 #pragma unroll
         for (int j = 0; j < L::kKChunks; ++j) {
-          const int byte = j * 64 + c * 16;
-          const bool on = byte < d;
-          cp_async<16>(at + (uint32_t)((t * L::kKChunks + j) * 32 + lane) * 16,
-                       kc + (int64_t)(key0 + t * 8 + g) * d + (on ? byte : 0), on);
+          const bool on = Full || j * 64 + c * 16 < d;
+          cp_async<16>(at + (uint32_t)((t * L::kKChunks + j) * 512), on ? kp + t * 8 * d + j * 64 : kc, on);
         }
+      const uint32_t vat = ring + (uint32_t)stage * L::kUnitBytes + 32 * L::kKBytes + (uint32_t)lane * L::kVBytes;
+      const bool on = Full || g * L::kVBytes < d;
+      const uint8_t* vp = vc + (int64_t)(key0 + 2 * c) * d + (on ? g * L::kVBytes : 0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int key = key0 + 2 * c + (k & 1) + (k >> 1) * 8;
-        const int byte = g * L::kVBytes;
-        const bool on = byte < d;
-        cp_async<L::kVBytes>(at + 32 * L::kKBytes + (uint32_t)(k * 32 + lane) * L::kVBytes,
-                             vc + (int64_t)key * d + (on ? byte : 0), on);
-      }
+      for (int k = 0; k < L::kVKeys; ++k)
+        cp_async<L::kVBytes>(vat + (uint32_t)(k * 32 * L::kVBytes),
+                             vp + ((k >> 2) * 16 + (k & 1) + ((k >> 1) & 1) * 8) * d, on);
     }
     cp_commit();
   };
@@ -241,7 +245,12 @@ kv8_attn_kernel(Kv8Attn p) {
     const uint8_t* at = smem + (size_t)warp * kStages * L::kUnitBytes + (size_t)stage * L::kUnitBytes;
     if (++stage == kStages) stage = 0;
 
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    constexpr int kX = 4 * kHalves;  // this thread's keys of a row
+    float s[2 * kHalves][4];
+#pragma unroll
+    for (int t = 0; t < 2 * kHalves; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
     float kscale, vscale;
     const bool coded = key0 < sealed;
     uint32_t bad = 0;  // tail: bit k set when this thread's key k has a non-finite value
@@ -254,15 +263,22 @@ kv8_attn_kernel(Kv8Attn p) {
       }
 #pragma unroll
       for (int j = 0; j < L::kKChunks; ++j) {
-        const uint4 w0 = *reinterpret_cast<const uint4*>(at + (j * 32 + lane) * 16);
-        const uint4 w1 = *reinterpret_cast<const uint4*>(at + ((L::kKChunks + j) * 32 + lane) * 16);
-        const uint32_t a0[4] = {w0.x, w0.y, w0.z, w0.w}, a1[4] = {w1.x, w1.y, w1.z, w1.w};
+        uint32_t w[2 * kHalves][4];
+#pragma unroll
+        for (int t = 0; t < 2 * kHalves; ++t) {
+          const uint4 x = *reinterpret_cast<const uint4*>(at + ((t * L::kKChunks + j) * 32 + lane) * 16);
+          w[t][0] = x.x;
+          w[t][1] = x.y;
+          w[t][2] = x.z;
+          w[t][3] = x.w;
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint4 qv = q_frag[j * 4 + i][lane];
           const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
-          mma_f16(s[0], qa, e4m3x2_to_f16x2(a0[i]), e4m3x2_hi_to_f16x2(a0[i]));
-          mma_f16(s[1], qa, e4m3x2_to_f16x2(a1[i]), e4m3x2_hi_to_f16x2(a1[i]));
+#pragma unroll
+          for (int t = 0; t < 2 * kHalves; ++t)
+            mma_f16(s[t], qa, e4m3x2_to_f16x2(w[t][i]), e4m3x2_hi_to_f16x2(w[t][i]));
         }
       }
     } else {
@@ -271,40 +287,41 @@ kv8_attn_kernel(Kv8Attn p) {
       for (int st = 0; st < L::kSteps; ++st) {
         const uint4 qv = q_frag[st][lane];
         const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
-        const uint2 b0 = tail_s[st * 32 + lane], b1 = tail_s[(L::kSteps + st) * 32 + lane];
-        mma_f16(s[0], qa, b0.x, b0.y);
-        mma_f16(s[1], qa, b1.x, b1.y);
-      }
-    }
-
-    // Visibility of keys 2c, 2c + 1 (bits 0, 1) and 8 + 2c, 9 + 2c (bits 2, 3) for both rows.
-    uint32_t vis[2];
-    if (key0 + kUnit <= p.prefix) {  // prefix_len <= kv_len
-      vis[0] = rok[0] ? 15u : 0u;
-      vis[1] = rok[1] ? 15u : 0u;
-    } else {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t w = rok[r] ? (uint32_t)kv8_window(p, rbits[r], key0) : 0u;
-        vis[r] = ((w >> (2 * c)) & 3u) | (((w >> (8 + 2 * c)) & 3u) << 2);
+        for (int t = 0; t < 2 * kHalves; ++t) {
+          const uint2 b = tail_s[(t * L::kSteps + st) * 32 + lane];
+          mma_f16(s[t], qa, b.x, b.y);
+        }
       }
     }
 
-    // Scores in base 2; those not seen are never looked at again.
-    float x[2][4];
+    // Scores in base 2, those not seen -infinity: keys 2c, 2c + 1 of each key tile.
+    float x[2][kX], mx[2];
+    const bool open = key0 + kUnit <= p.prefix;  // no mask to read (prefix_len <= kv_len)
     bool grow = false;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float f = qs[r] * kscale;
-      float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float y = s[i >> 1][2 * r + (i & 1)] * f;
-        if ((bad >> i) & 1u) y = __int_as_float(0x7fc00000);
-        x[r][i] = y;
-        if ((vis[r] >> i) & 1u) mx = fmaxf(mx, y);
+      for (int i = 0; i < kX; ++i) x[r][i] = s[i >> 1][2 * r + (i & 1)] * f;
+    }
+    if (!open || bad) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t w = open ? ~0u : (rok[r] ? (uint32_t)kv8_window(p, rbits[r], key0) : 0u);
+#pragma unroll
+        for (int i = 0; i < kX; ++i) {
+          if ((bad >> i) & 1u) x[r][i] = __int_as_float(0x7fc00000);
+          if (!((w >> ((i >> 1) * 8 + 2 * c + (i & 1))) & 1u)) x[r][i] = -INFINITY;
+        }
       }
-      grow |= mx > m[r] + kSlack || (m[r] == -INFINITY && mx > -INFINITY);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      mx[r] = x[r][0];
+#pragma unroll
+      for (int i = 1; i < kX; ++i) mx[r] = fmaxf(mx[r], x[r][i]);  // NaN is passed over
+      grow |= mx[r] > m[r] + kSlack;  // m -infinity: any score
     }
     float corr[2] = {1.f, 1.f};
     bool rescale = false;
@@ -312,14 +329,11 @@ kv8_attn_kernel(Kv8Attn p) {
       rescale = true;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float mx = m[r];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if ((vis[r] >> i) & 1u) mx = fmaxf(mx, x[r][i]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        corr[r] = m[r] == -INFINITY ? 0.f : exp2f(m[r] - mx);
-        m[r] = mx;
+        float y = fmaxf(m[r], mx[r]);
+        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+        corr[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - y);
+        m[r] = y;
         l[r] *= corr[r];
       }
     }
@@ -344,52 +358,53 @@ kv8_attn_kernel(Kv8Attn p) {
         o[t][3] *= corr[1];
       }
     }
-    float pv[2][4];
+    uint32_t pa[kHalves][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float base = m[r] == -INFINITY ? 0.f : m[r] - kPShift;
+      const float base = (m[r] == -INFINITY ? 0.f : m[r]) - kPShift;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float e = (vis[r] >> i) & 1u ? exp2f(x[r][i] - base) : 0.f;
-        l[r] += e;
-        pv[r][i] = (vis[r] >> i) & 1u ? e * pf : 0.f;
+      for (int i = 0; i < kX; i += 2) {
+        const float e0 = ex2(x[r][i] - base), e1 = ex2(x[r][i + 1] - base);
+        l[r] += e0 + e1;
+        pa[i >> 2][r + (i & 2)] = pack_f16x2(e0 * pf, e1 * pf);
       }
     }
-    const uint32_t pa[4] = {pack_f16x2(pv[0][0], pv[0][1]), pack_f16x2(pv[1][0], pv[1][1]),
-                            pack_f16x2(pv[0][2], pv[0][3]), pack_f16x2(pv[1][2], pv[1][3])};
 
     // Output tile t, column g: dim g * kVBytes + t.
-    if (coded) {
-      uint32_t vf[4][L::kVBytes / 4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint8_t* a = at + 32 * L::kKBytes + (k * 32 + lane) * L::kVBytes;
-        if constexpr (L::kVBytes == 16) {
-          const uint4 w = *reinterpret_cast<const uint4*>(a);
-          vf[k][0] = w.x;
-          vf[k][1] = w.y;
-          vf[k][2] = w.z;
-          vf[k][3] = w.w;
-        } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(a);
-          vf[k][0] = w.x;
-          vf[k][1] = w.y;
+    for (int h = 0; h < kHalves; ++h) {
+      if (coded) {
+        uint32_t vf[4][L::kVBytes / 4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint8_t* a = at + 32 * L::kKBytes + ((h * 4 + k) * 32 + lane) * L::kVBytes;
+          if constexpr (L::kVBytes == 16) {
+            const uint4 w = *reinterpret_cast<const uint4*>(a);
+            vf[k][0] = w.x;
+            vf[k][1] = w.y;
+            vf[k][2] = w.z;
+            vf[k][3] = w.w;
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(a);
+            vf[k][0] = w.x;
+            vf[k][1] = w.y;
+          }
         }
-      }
 #pragma unroll
-      for (int w = 0; w < L::kVBytes / 4; ++w) {
-        const uint32_t a01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), a23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
-        const uint32_t b01 = __byte_perm(vf[2][w], vf[3][w], 0x5140), b23 = __byte_perm(vf[2][w], vf[3][w], 0x7362);
-        mma_f16(o[4 * w + 0], pa, e4m3x2_to_f16x2(a01), e4m3x2_to_f16x2(b01));
-        mma_f16(o[4 * w + 1], pa, e4m3x2_hi_to_f16x2(a01), e4m3x2_hi_to_f16x2(b01));
-        mma_f16(o[4 * w + 2], pa, e4m3x2_to_f16x2(a23), e4m3x2_to_f16x2(b23));
-        mma_f16(o[4 * w + 3], pa, e4m3x2_hi_to_f16x2(a23), e4m3x2_hi_to_f16x2(b23));
-      }
-    } else {
+        for (int w = 0; w < L::kVBytes / 4; ++w) {
+          const uint32_t a01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), a23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
+          const uint32_t b01 = __byte_perm(vf[2][w], vf[3][w], 0x5140), b23 = __byte_perm(vf[2][w], vf[3][w], 0x7362);
+          mma_f16(o[4 * w + 0], pa[h], e4m3x2_to_f16x2(a01), e4m3x2_to_f16x2(b01));
+          mma_f16(o[4 * w + 1], pa[h], e4m3x2_hi_to_f16x2(a01), e4m3x2_hi_to_f16x2(b01));
+          mma_f16(o[4 * w + 2], pa[h], e4m3x2_to_f16x2(a23), e4m3x2_to_f16x2(b23));
+          mma_f16(o[4 * w + 3], pa[h], e4m3x2_hi_to_f16x2(a23), e4m3x2_hi_to_f16x2(b23));
+        }
+      } else {
 #pragma unroll
-      for (int t = 0; t < L::kTiles; ++t) {
-        const uint2 b = tail_s[(2 * L::kSteps + t) * 32 + lane];
-        mma_f16(o[t], pa, b.x, b.y);
+        for (int t = 0; t < L::kTiles; ++t) {
+          const uint2 b = tail_s[(2 * kHalves * L::kSteps + h * L::kTiles + t) * 32 + lane];
+          mma_f16(o[t], pa[h], b.x, b.y);
+        }
       }
     }
   }
@@ -481,24 +496,30 @@ kv8_merge_kernel(Kv8Attn p) {
   const int64_t req = on ? pair / per_req : 0, at = on ? pair % per_req : 0;
   const int64_t base = req * p.splits * per_req + at;
   const int d = p.c.d, splits = on ? p.splits : 0;
+  constexpr int kPer = kMaxSplits / 32;  // ranges of a lane
+  float2 ml[kPer];
   float gm = -INFINITY;
-  for (int s = lane; s < splits; s += 32) gm = fmaxf(gm, p.part_ml[(base + s * per_req) * 2]);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int s = i * 32 + lane;
+    ml[i] = s < splits ? *reinterpret_cast<const float2*>(p.part_ml + (base + s * per_req) * 2)
+                       : make_float2(-INFINITY, 0.f);
+    gm = fmaxf(gm, ml[i].x);
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  for (int s0 = 0; s0 < splits; s0 += 32) {
-    float w = 0.f;
-    if (s0 + lane < splits) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (base + (s0 + lane) * per_req) * 2);
-      w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - gm);
-      sum += w * ml.y;  // a NaN passes even where w is 0
-    }
-    const int n = min(32, splits - s0);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const float w = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - gm);
+    sum += w * ml[i].y;  // a NaN passes even where w is 0
+    const int n = min(32, splits - i * 32);
 #pragma unroll 8
     for (int j = mine; j < n; j += W) {
       const float f = __shfl_sync(0xffffffffu, w, j);
       if (lane * 4 < d) {
-        const float4 y = *reinterpret_cast<const float4*>(p.part_o + (base + (int64_t)(s0 + j) * per_req) * d + lane * 4);
+        const float4 y =
+            *reinterpret_cast<const float4*>(p.part_o + (base + (int64_t)(i * 32 + j) * per_req) * d + lane * 4);
         acc[0] += f * y.x;
         acc[1] += f * y.y;
         acc[2] += f * y.z;
@@ -543,11 +564,11 @@ int launch_merge(const Kv8Attn& p, cudaStream_t stream) {
   return SF_OK;
 }
 
-template <int DT>
+template <int DT, bool Full>
 int launch_mma(const Kv8Attn& p, cudaStream_t stream) {
   static std::atomic<unsigned long long> configured{0};
   if (int rc = once_per_device(configured, [] {
-        SF_CHECK_CUDA(cudaFuncSetAttribute(kv8_attn_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        SF_CHECK_CUDA(cudaFuncSetAttribute(kv8_attn_kernel<DT, Full>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            Layout<DT>::kSmem));
         return SF_OK;
       }))
@@ -555,7 +576,7 @@ int launch_mma(const Kv8Attn& p, cudaStream_t stream) {
   const int64_t tiles = ((int64_t)p.group * p.q_len + kRows - 1) / kRows;
   SF_CHECK_ARG(tiles < 65536 && (int64_t)p.splits * p.batch < 65536, "too many query rows or requests");
   const dim3 grid((unsigned)p.c.hkv, (unsigned)tiles, (unsigned)(p.splits * p.batch));
-  SF_CHECK_CUDA(launch_pdl(kv8_attn_kernel<DT>, grid, dim3(kWarps * 32), Layout<DT>::kSmem, stream, p));
+  SF_CHECK_CUDA(launch_pdl(kv8_attn_kernel<DT, Full>, grid, dim3(kWarps * 32), Layout<DT>::kSmem, stream, p));
   SF_CHECK_LAUNCH();
   return SF_OK;
 }
@@ -566,12 +587,12 @@ size_t partial_bytes(const Kv8Split& s, int batch, int heads, int head_dim, int6
 
 }  // namespace
 
-// Four resident CTAs per SM; a range is at least two steps of the four warps.
+// Three resident CTAs per SM; a range is at least one step of the four warps.
 Kv8Split kv8_split_mma(int batch, int hkv, int64_t packed, int64_t kv_len) {
   const int64_t units = (int64_t)batch * hkv * ((packed + kRows - 1) / kRows);
   const int64_t steps = (kv_len + kStep - 1) / kStep;
-  int64_t want = std::max<int64_t>(1, 4 * (int64_t)num_sms() / units);
-  want = std::min<int64_t>(want, std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, steps / 2)));
+  int64_t want = std::max<int64_t>(1, 3 * (int64_t)num_sms() / units);
+  want = std::min<int64_t>(want, std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, steps)));
   const int64_t per = std::max<int64_t>(1, (steps + want - 1) / want);
   return {(int)std::max<int64_t>(1, (steps + per - 1) / per), (int)(per * kStep)};
 }
@@ -658,8 +679,11 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
                                  (partial_bytes(s, rows->batch, num_heads, rows->head_dim, q_len) + 15) / 16 * 16,
                           st);
   else
-    rc = rows->head_dim <= 64 ? launch_mma<64>(p, st) : launch_mma<128>(p, st);
+    rc = rows->head_dim == 128  ? launch_mma<128, true>(p, st)
+         : rows->head_dim > 64  ? launch_mma<128, false>(p, st)
+         : rows->head_dim == 64 ? launch_mma<64, true>(p, st)
+                                : launch_mma<64, false>(p, st);
   if (rc || s.splits == 1) return rc;
-  // Up to about eight ranges a warp.
-  return s.splits <= 8 ? launch_merge<1>(p, st) : (s.splits <= 32 ? launch_merge<4>(p, st) : launch_merge<8>(p, st));
+  // One warp a row walks 16 ranges as fast as four join them (65 rows, 12 ranges: 5.7 and 9.1 us).
+  return s.splits <= 16 ? launch_merge<1>(p, st) : (s.splits <= 32 ? launch_merge<4>(p, st) : launch_merge<8>(p, st));
 }
