@@ -2,6 +2,7 @@
 from .cache_observer import CacheTransition, CacheTransitionObserver, RecordingCacheTransitionObserver
 from .cache_snapshot import CacheSlotSnapshot, GpuExpertCacheSnapshot, PendingTransferSnapshot
 from .gpu_expert_cache import GpuExpertCache
+from .kv8_cache import Kv8Cache
 from .lease import ExpertCacheStats, ExpertLease, NoEvictableSlotError
 from .moe_block import Qwen3B200SparseMoeBlock, Qwen3B200TopKRouter
 from .qwen3_expert_prefetch import Qwen3ExpertPrefetch
@@ -11,7 +12,7 @@ from .state import ExpertKey, RuntimeEventKind
 
 __all__ = [
     "CacheSlotSnapshot", "CacheTransition", "CacheTransitionObserver", "ExpertCacheStats",
-    "ExpertExecutionPolicy", "ExpertKey", "ExpertLease", "GpuExpertCache", "GpuExpertCacheSnapshot",
+    "ExpertExecutionPolicy", "ExpertKey", "ExpertLease", "GpuExpertCache", "GpuExpertCacheSnapshot", "Kv8Cache",
     "NoEvictableSlotError", "PendingTransferSnapshot", "Qwen3B200SparseMoeBlock",
     "Qwen3B200TopKRouter", "Qwen3ExpertPrefetch", "Qwen3OffloadedExperts",
     "RecordingCacheTransitionObserver",

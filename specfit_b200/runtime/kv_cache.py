@@ -27,6 +27,8 @@ from transformers.cache_utils import DynamicCache, DynamicLayer
 
 
 class ReservedLayer(DynamicLayer):
+    in_place = True  # rolling back is ``crop``
+
     def __init__(self, capacity: int) -> None:
         super().__init__()
         if capacity <= 0:
@@ -151,6 +153,12 @@ def compact_tree_cache_(cache, *, base_kv_length: int, verification_positions: t
     expected = base_kv_length + verification_node_count
     n = len(verification_positions)
     layers = cache.layers
+    if layers and all(hasattr(l, "keep_tail_rows") and l.is_initialized for l in layers):  # the 8-bit cache
+        if any(l.get_seq_length() != expected for l in layers):
+            raise RuntimeError("target cache layer has an unexpected length")
+        for l in layers:
+            l.keep_tail_rows(base_kv_length, verification_positions)
+        return
     if (layers and all(isinstance(l, ReservedLayer) and l.is_initialized for l in layers)
             and layers[0]._kbuf.is_cuda and layers[0]._kbuf.shape[0] == 1
             and layers[0]._kbuf.dtype == torch.bfloat16):

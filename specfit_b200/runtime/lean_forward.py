@@ -27,7 +27,10 @@ Hooks that the runtime relies on are honoured by hand: forward pre-hooks of
 ``self_attn`` (the prefetch scheduler's attention hook) run before each
 layer's attention, and forward hooks of each decoder layer receive the
 layer's output.  The model object stays the weight container; only
-``ReservedCache`` caches are supported.
+``ReservedCache`` and ``Kv8Cache`` caches are supported.  With the latter, k
+and v rows go to the cache's bf16 tail, attention reads codes and tail
+(``sf_kv8_tree_attention``), a cache with a budget adds up the weights its
+tokens received, and a causal pass seals its blocks layer by layer.
 """
 from __future__ import annotations
 
@@ -38,6 +41,7 @@ import torch.nn.functional as F
 
 from .. import _native as N
 from .. import ops
+from .kv8_cache import Kv8Layer
 from .kv_cache import ReservedLayer
 from .moe_block import Qwen3B200SparseMoeBlock
 from .qwen3_offloaded_experts import Qwen3OffloadedExperts
@@ -100,6 +104,60 @@ class LeanQwen3Forward:
         out = experts.forward_sorted(hn, idx, weights)
         return None if out is None else (out[0], out[1], idx)
 
+    def _after_attention(self, li, L, attn, res, hn, B, T, stream):
+        """The rest of layer ``li``: o projection, norms, MoE block, hooks."""
+        Nt, layer = B * T, L.layer
+        o = ops.linear(attn.view(Nt, self.hq * self.D), L.wo)
+        self._norm(o, res, res, L.ln_post, hn, stream)
+        nxt = self.layers[li + 1].ln_in if li + 1 < len(self.layers) else self.final
+        sorted_out = self._moe_sorted(layer.mlp, hn)
+        if sorted_out is not None:  # combine + residual add + next norm in one launch
+            ys, d, idx = sorted_out
+            ops.moe_combine_add_rmsnorm(ys, d, idx, res, nxt, self.eps, out=hn)
+        else:
+            moe = layer.mlp(hn.view(B, T, self.H)).reshape(Nt, self.H)
+            self._norm(moe, res, res, nxt, hn, stream)
+        if layer._forward_hooks:
+            out = res.view(B, T, self.H).clone()
+            for hook in tuple(layer._forward_hooks.values()):
+                hook(layer, (), out)
+
+    def _kv8_attention(self, cl, L, hn, cos, sin, B, T, attention_mask, attention_words, bits, stream):
+        """One layer's attention over an 8-bit cache layer: (rows' outputs,
+        (visibility words, first masked column))."""
+        if (cl._b, cl._h, cl._d) != (B, self.hkv, self.D):
+            raise ValueError("batch or head count differs from the 8-bit cache")
+        dev = hn.device
+        cl.begin(T)
+        room = cl._kt.shape[2]
+        qkv = ops.linear(hn, L.wqkv)
+        q = torch.empty(B, self.hq, T, self.D, dtype=hn.dtype, device=dev)
+        N.check(N.lib.sf_qk_norm_rope(qkv.data_ptr(), B, T, self.hq, self.hkv, self.D, L.qn.data_ptr(),
+                                      L.kn.data_ptr(), cos.data_ptr(), sin.data_ptr(), self.eps, q.data_ptr(),
+                                      cl._kt.data_ptr(), cl._vt.data_ptr(), self.hkv * room * self.D, room * self.D,
+                                      cl.tail, None, stream), "sf_qk_norm_rope")
+        ops._launched(1)
+        cl.end(T)
+        total = cl.length
+        causal = attention_mask is None and attention_words is None
+        if bits is None:  # every layer holds the same number of rows
+            if attention_words is not None:
+                bits = (attention_words, 0)
+            elif causal:
+                bits = (_causal_bits(T, dev).unsqueeze(0).expand(B, -1, -1), total - T)
+            else:
+                bits = (torch.stack([m.reshape(T, -1) for m in _packed_bits(attention_mask, T, total, B)]), 0)
+        attn = torch.empty(B, T, self.hq, self.D, dtype=hn.dtype, device=dev)
+        rows = cl.rows()
+        if cl.scored:
+            _, lse = ops.kv8_tree_attention(q, rows, bits[0], bits[1], out=attn, return_lse=True)
+            ops.kv8_attention_mass(q, lse, rows, bits[0], bits[1], cl.mass)
+        else:
+            ops.kv8_tree_attention(q, rows, bits[0], bits[1], out=attn)
+        if causal and T > 1:
+            cl.seal()  # a prompt's rows stay: no layer keeps them in bf16 through the pass
+        return attn, bits
+
     @torch.no_grad()
     def __call__(self, input_ids, attention_mask=None, position_ids=None, past_key_values=None,
                  logits_to_keep: int = 0, use_cache: bool = True, attention_words=None):
@@ -107,15 +165,16 @@ class LeanQwen3Forward:
         ``ops.tree_mask_words``) replaces ``attention_mask``: visibility bits
         over every cache row (prefix 0)."""
         cache = past_key_values
-        if cache is None or not all(isinstance(l, ReservedLayer) for l in cache.layers):
-            raise ValueError("the lean forward needs a ReservedCache")
+        kv8 = cache is not None and len(cache.layers) > 0 and all(isinstance(l, Kv8Layer) for l in cache.layers)
+        if not kv8 and (cache is None or not all(isinstance(l, ReservedLayer) for l in cache.layers)):
+            raise ValueError("the lean forward needs a ReservedCache or a Kv8Cache")
         m = self.model.model
         B, T = input_ids.shape
         Nt = B * T
         dev = input_ids.device
         stream = torch.cuda.current_stream(dev).cuda_stream
         x = m.embed_tokens(input_ids).reshape(Nt, self.H)
-        base = cache.get_seq_length()
+        base = cache.next_position if kv8 else cache.get_seq_length()
         if position_ids is None:
             position_ids = torch.arange(base, base + T, device=dev).unsqueeze(0).expand(B, -1)
         cos, sin = m.rotary_emb(x.view(B, T, self.H), position_ids)
@@ -124,7 +183,8 @@ class LeanQwen3Forward:
         res = torch.empty_like(x)
         hn = torch.empty_like(x)
         self._norm(x, None, res, self.layers[0].ln_in, hn, stream)
-        static = cache.layers[0].static_offset is not None
+        static = not kv8 and cache.layers[0].static_offset is not None
+        kv8_bits = None  # [B, T, words] and the prefix, one for all layers
         stacked_bits = None  # (kv_len, [B, T, words]) built once per pass for the batched attention
         for li, L in enumerate(self.layers):
             layer = L.layer
@@ -134,6 +194,11 @@ class LeanQwen3Forward:
             if not cl.is_initialized:  # allocate the reserved buffers (shapes only matter)
                 probe = torch.empty(B, self.hkv, T, self.D, dtype=x.dtype, device=dev)
                 cl.lazy_initialization(probe, probe)
+            if kv8:
+                attn, kv8_bits = self._kv8_attention(cl, L, hn, cos, sin, B, T, attention_mask, attention_words,
+                                                     kv8_bits, stream)
+                self._after_attention(li, L, attn, res, hn, B, T, stream)
+                continue
             if cl._kbuf.shape[0] != B or cl._kbuf.shape[1] != self.hkv:
                 raise ValueError("batch or head count differs from the reserved cache")
             if static:
@@ -179,20 +244,7 @@ class LeanQwen3Forward:
                 for b in range(B):
                     ops.tree_attention(q[b], cl._kbuf[b, :, :kv_len], cl._vbuf[b, :, :kv_len], bits[b],
                                        prefix, scale=self.D ** -0.5, out=attn[b])
-            o = ops.linear(attn.view(Nt, self.hq * self.D), L.wo)
-            self._norm(o, res, res, L.ln_post, hn, stream)
-            nxt = self.layers[li + 1].ln_in if li + 1 < len(self.layers) else self.final
-            sorted_out = self._moe_sorted(layer.mlp, hn)
-            if sorted_out is not None:  # combine + residual add + next norm in one launch
-                ys, d, idx = sorted_out
-                ops.moe_combine_add_rmsnorm(ys, d, idx, res, nxt, self.eps, out=hn)
-            else:
-                moe = layer.mlp(hn.view(B, T, self.H)).reshape(Nt, self.H)
-                self._norm(moe, res, res, nxt, hn, stream)
-            if layer._forward_hooks:
-                out = res.view(B, T, self.H).clone()
-                for hook in tuple(layer._forward_hooks.values()):
-                    hook(layer, (), out)
+            self._after_attention(li, L, attn, res, hn, B, T, stream)
         keep = T if not logits_to_keep else min(int(logits_to_keep), T)
         rows = hn.view(B, T, self.H)[:, T - keep:, :].contiguous()
         head = self.model.lm_head.weight

@@ -46,6 +46,7 @@ from .. import ops
 from .. import selection as sel
 from .. import synthetic
 from .eagle3_types import tree_from_arrays
+from .kv8_cache import Kv8Cache
 from .kv_cache import ReservedCache, compact_tree_cache_
 from .tree_attention import clear_mask_cache
 
@@ -136,7 +137,16 @@ class B200TreeSpeculator:
     def __init__(self, loaded, drafter, *, cost_model, acceptance: BernoulliAcceptance,
                  route_seed: int = 0, top_k: int = 4, max_depth: int = 8, first_width: int = 4,
                  level_width: int = 8, max_nodes: int = sel.MAX_DRAFT_NODES,
-                 graphs: bool = False, reserve_tokens: int = 0, lean: bool = False) -> None:
+                 graphs: bool = False, reserve_tokens: int = 0, lean: bool = False, kv8: bool = False,
+                 kv8_budget: int | None = None) -> None:
+        """``kv8``: the target's keys and values in 8 bits (``Kv8Cache``; needs
+        ``lean``, and no ``graphs``); ``kv8_budget``: cut the cache to that many
+        tokens per head after every cycle, by the attention they received."""
+        if kv8 and (not lean or graphs):
+            raise ValueError("an 8-bit cache needs the lean forward and eager verify passes")
+        if kv8_budget is not None and not kv8:
+            raise ValueError("kv8_budget needs kv8")
+        self.kv8, self.kv8_budget = kv8, kv8_budget
         self.loaded = loaded
         self.model = loaded.model
         if lean:
@@ -400,6 +410,11 @@ class B200TreeSpeculator:
                 cache.set_length(0)
             if self._offset is None:
                 self._offset = torch.zeros((), dtype=torch.long, device=dev)
+        elif self.kv8:
+            recent = {} if self.kv8_budget is None else {"recent": min(64, self.kv8_budget // 2),
+                                                         "sinks": min(4, self.kv8_budget // 4)}
+            cache = Kv8Cache(config=self.model.config, capacity=need, tail_room=q_max, budget=self.kv8_budget,
+                             **recent)
         else:
             cache = ReservedCache(config=self.model.config, capacity=need)
         self.drafter.begin_generation(ctx + max_new_tokens + 2 + self.first_width
@@ -487,7 +502,8 @@ class B200TreeSpeculator:
                 else:
                     verify_ids = tree.verification_token_ids(pending)
                     mask = tree.verification_attention_mask(base_kv_length=base, device=dev)
-                    pos = tree.verification_position_ids(base_kv_length=base, device=dev)
+                    pos = tree.verification_position_ids(base_kv_length=cache.next_position if self.kv8 else base,
+                                                         device=dev)
                     self._override = routes[[0] + list(tree.source_raw_ids)].transpose(0, 1).contiguous()
                     try:
                         with torch.no_grad():
@@ -504,6 +520,8 @@ class B200TreeSpeculator:
                 n = len(positions)
                 compact_tree_cache_(cache, base_kv_length=base, verification_positions=positions,
                                     verification_node_count=verify_ids.shape[1])
+                if self.kv8_budget is not None:
+                    cache.evict()
                 ph = self._pos_host[:n]
                 ph.numpy()[:] = positions
                 ptens = ph.to(dev, non_blocking=True)

@@ -10,9 +10,9 @@ committed length and replays it, removing the per-op host launch cost of the
 eager Hugging Face forward.
 
 The KV cache's committed prefix is not modified by a replay.  With a
-``ReservedCache`` the captured forward writes the tree's keys/values into
-the reserved rows after the prefix (the same rows on every replay) and the
-rollback is ``crop``.  With a plain ``DynamicCache`` the captured forward
+``ReservedCache`` (or a ``Kv8Cache`` without a budget) the captured forward
+writes the tree's keys/values into the reserved rows after the prefix (the
+same rows on every replay) and the rollback is ``crop``.  With a plain ``DynamicCache`` the captured forward
 concatenates the prefix with the tree's keys/values into graph-owned
 buffers, exactly as an eager ``update`` followed by a rollback would; the
 prefix tensors are then kept alive for the graph's lifetime, and the cache
@@ -22,7 +22,6 @@ from __future__ import annotations
 
 import torch
 
-from .kv_cache import ReservedLayer
 from .tree_attention import clear_mask_cache
 
 
@@ -43,6 +42,8 @@ class VerifyGraph:
         self.mask = torch.zeros(batch, 1, q_len, self.prefix_len + q_len, dtype=torch.bool,
                                 device=self.device)
         self.pos = torch.zeros(batch, q_len, dtype=torch.long, device=self.device)
+        if any(getattr(layer, "scored", False) for layer in kv_cache.layers):
+            raise RuntimeError("VerifyGraph replays a pass at will: a cache that scores its passes cannot be captured")
         self._prefix = [(layer.keys, layer.values) for layer in kv_cache.layers]
         self.graph = None
         self.logits = None
@@ -50,7 +51,7 @@ class VerifyGraph:
 
     def _restore_prefix(self) -> None:
         for layer, (k, v) in zip(self.cache.layers, self._prefix):
-            if isinstance(layer, ReservedLayer):
+            if getattr(layer, "in_place", False):
                 layer.crop(self.prefix_len)
             else:
                 layer.keys, layer.values = k, v
@@ -89,8 +90,10 @@ class VerifyGraph:
     def capture(self, ids, mask, pos, warmup: int = 2) -> None:
         self._require_resident()
         for layer in self.cache.layers:
-            if isinstance(layer, ReservedLayer) and layer.capacity < self.prefix_len + self.q_len:
+            if getattr(layer, "in_place", False) and layer.capacity < self.prefix_len + self.q_len:
                 raise RuntimeError("the reserved KV cache must hold the prefix plus the tree")
+            if getattr(layer, "tail_room", self.q_len) < self.q_len:
+                raise RuntimeError("the 8-bit cache must have tail_room for the tree's rows")
         self.load(ids, mask, pos)
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
