@@ -4,14 +4,18 @@
 // weights the earlier token stays; a NaN counts as the least weight.
 //
 // A radix selection, not a sort: the weights are mapped to integers of the
-// same order, four 8-bit histogram passes find the smallest kept key and how
+// same order, three 11-bit histogram passes find the smallest kept key and how
 // many of its equals are kept, and one ordered pass writes the indices.  The
 // floor is one read of the weights (4 bytes a token), which for the sizes in
 // use (512 KB a head at 131,072 tokens) is below launch latency: what bounds
 // the kernel is the chain of passes, so a cluster of up to eight CTAs shares
-// a head, each with its own slice (in L1 / L2 after the first pass), and
-// adds its peers' histograms through distributed shared memory.  Integer
-// counts only, so the result does not depend on the order of the atomics.
+// a head, each with its own slice (in registers up to 8,192 tokens, so that
+// up to 65,536 tokens of a head are read once) and adds its peers' histograms
+// through distributed shared memory.  Tokens that no row looked at are many,
+// and their zeros would all hit one counter: a warp adds them at once.
+// Integer counts only, so the result does not depend on the order of the
+// atomics.  (Four 8-bit passes over memory, with every digit matched across
+// the warp, took 40 us for 16 heads of 65,557 tokens; this takes 32 us.)
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
@@ -24,8 +28,11 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kPer = 4;  // consecutive weights of one thread in the ordered pass
+constexpr int kPer = 4;  // consecutive weights of one thread in a tile
 constexpr int kTile = kThreads * kPer;
+constexpr int kHeld = 4;  // tiles that a CTA holds in registers
+constexpr int kBits = 11, kBins = 1 << kBits, kPasses = 3;  // 11 + 11 + 10 bits
+constexpr int kBinsPer = kBins / kThreads;
 
 struct KeepParams {
   const float* mass;
@@ -45,17 +52,21 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 
 __device__ __forceinline__ int warp_sum_i(int v) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)v); }
 
-__global__ void __launch_bounds__(kThreads)
+// Held: the CTA's slice is at most kHeld tiles and stays in registers.
+// Two CTAs fit an SM, so that sixteen clusters of eight run at once: one at a
+// time, a GPC of fewer than 16 SMs holds only one, and the rest wait for it.
+template <bool Held>
+__global__ void __launch_bounds__(kThreads, 2)
 kv_keep_kernel(KeepParams p) {
   pdl_wait();
   pdl_trigger();
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t total[256];
+  __shared__ __align__(16) uint32_t hist[kBins];
+  __shared__ uint32_t warp_sums[kWarps];
   __shared__ uint32_t prefix_s, want_s;
   __shared__ int counts[2];                 // this CTA's kept-above and equal counts
-  __shared__ int scan_gt[kWarps], scan_eq[kWarps];
+  __shared__ uint32_t scan[kHeld][kWarps];  // kept-above | equal << 16 of a tile's warps, then of what is before them
   const int head = blockIdx.y;  // b * hkv + h
   const int b = head / p.hkv, h = head % p.hkv;
   const int mid = p.length - p.sinks - p.recent;
@@ -69,77 +80,110 @@ kv_keep_kernel(KeepParams p) {
   for (int i = rank * kThreads + tid; i < p.sinks; i += ranks * kThreads) out[i] = i;
   for (int i = rank * kThreads + tid; i < p.recent; i += ranks * kThreads)
     out[p.budget - p.recent + i] = p.length - p.recent + i;
+  if (want0 == 0) return;  // the whole cluster
 
-  // Four passes, the most significant digit first: `prefix` is the digits
-  // found so far, `want` how many keys that match it are still to be kept.
+  // This thread's keys of tile t: tokens base + tid * kPer + {0 .. kPer - 1}.
+  const int tiles = (hi - lo + kTile - 1) / kTile;
+  uint32_t held[kHeld][kPer];
+  auto load = [&](int t, uint32_t (&key)[kPer]) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int i = lo + t * kTile + tid * kPer + j;
+      key[j] = i < hi ? order_key(m[i]) : 0u;
+    }
+  };
+  if constexpr (Held) {
+#pragma unroll
+    for (int t = 0; t < kHeld; ++t) load(t, held[t]);
+  }
+  // f(tile, keys) over the tiles in order; past the slice's end keys are no token's.
+  auto each_tile = [&](auto&& f) {
+    if constexpr (Held) {
+#pragma unroll
+      for (int t = 0; t < kHeld; ++t)
+        if (t < tiles) f(t, held[t]);
+    } else {
+      for (int t = 0; t < tiles; ++t) {
+        uint32_t key[kPer];
+        load(t, key);
+        f(t, key);
+      }
+    }
+  };
+  constexpr uint32_t kZero = 0x80000000u;  // the key of +0
+
+  // The most significant digit first: `prefix` is the digits found so far,
+  // `want` how many keys that match it are still to be kept.
   uint32_t prefix = 0, want = (uint32_t)want0;
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
-    const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + 8);
-    for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < kPasses; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+    const uint32_t bins_mask = pass == 2 ? 1023u : 2047u;
+    const uint32_t mask = pass == 0 ? 0u : (pass == 1 ? 0xffe00000u : 0xfffffc00u);
+    *reinterpret_cast<uint4*>(&hist[tid * kBinsPer]) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (int base = lo; base < hi; base += kThreads) {
-      const int i = base + tid;
-      bool in = false;
-      uint32_t digit = 0;
-      if (i < hi) {
-        const uint32_t key = order_key(m[i]);
-        in = (key & mask) == prefix;
-        digit = (key >> shift) & 255u;
+    each_tile([&](int t, uint32_t (&key)[kPer]) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const bool in = lo + t * kTile + tid * kPer + j < hi && (key[j] & mask) == prefix;
+        const uint32_t zeros = __ballot_sync(0xffffffffu, in && key[j] == kZero);
+        if (in && key[j] != kZero) atomicAdd(&hist[(key[j] >> shift) & bins_mask], 1u);
+        if (lane == 0 && zeros) atomicAdd(&hist[(kZero >> shift) & bins_mask], (uint32_t)__popc(zeros));
       }
-      // Equal digits (a head's many zeros, a narrow range) are counted once per warp.
-      const uint32_t tag = in ? digit : 256u;
-      const uint32_t peers = __match_any_sync(0xffffffffu, tag);
-      if (in && lane == __ffs(peers) - 1) atomicAdd(&hist[digit], (uint32_t)__popc(peers));
-    }
+    });
     cluster.sync();
-    if (tid < 256) {
-      uint32_t sum = 0;
-      for (int r = 0; r < ranks; ++r) sum += cluster.map_shared_rank(hist, r)[tid];
-      total[tid] = sum;
+    // Thread t: the four bins whose rank from the top is 4 t .. 4 t + 3.
+    const int bin0 = kBins - kBinsPer * (tid + 1);
+    uint4 total = make_uint4(0, 0, 0, 0);
+    uint4 part[kMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)  // all of them in flight together
+      part[r] = r < ranks ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(hist, r) + bin0)
+                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      const uint4 x = part[r];
+      total.x += x.x;
+      total.y += x.y;
+      total.z += x.z;
+      total.w += x.w;
     }
+    const uint32_t mine[4] = {total.w, total.z, total.y, total.x};  // from the top
+    uint32_t sum = mine[0] + mine[1] + mine[2] + mine[3], before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += up;
+    }
+    if (lane == 31) warp_sums[warp] = before;
     __syncthreads();
-    if (warp == 0) {  // the digit at which the count from the top reaches `want`
-      uint32_t mine[8], sum = 0;
+    before -= sum;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        mine[j] = total[255 - (lane * 8 + j)];
-        sum += mine[j];
-      }
-      uint32_t before = sum;  // inclusive scan over the lanes, then made exclusive
+    for (int w = 0; w < kWarps; ++w)
+      if (w < warp) before += warp_sums[w];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t up = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += up;
+    for (int j = 0; j < 4; ++j) {
+      if (before < want && want <= before + mine[j]) {  // one thread of the CTA
+        prefix_s = prefix | ((uint32_t)(bin0 + 3 - j) << shift);
+        want_s = want - before;
       }
-      before -= sum;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (before < want && want <= before + mine[j]) {
-          prefix_s = prefix | ((uint32_t)(255 - (lane * 8 + j)) << shift);
-          want_s = want - before;
-        }
-        before += mine[j];
-      }
-      if (lane == 0 && want == 0) {  // nothing of the middle is kept
-        prefix_s = 0xffffffffu;
-        want_s = 0;
-      }
+      before += mine[j];
     }
-    cluster.sync();  // the histograms may be cleared
+    cluster.sync();  // the histograms may be cleared, the digit read
     prefix = prefix_s;
     want = want_s;
-    if (want == 0) break;  // uniform over the cluster: only when want0 is 0
   }
-  if (want0 == 0) return;  // every CTA of the cluster has passed the sync above
 
   // Now `prefix` is the smallest kept key and the first `want` of its equals stay.
   int gt = 0, eq = 0;
-  for (int i = lo + tid; i < hi; i += kThreads) {
-    const uint32_t key = order_key(m[i]);
-    gt += key > prefix;
-    eq += key == prefix;
-  }
+  each_tile([&](int t, uint32_t (&key)[kPer]) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const bool in = lo + t * kTile + tid * kPer + j < hi;
+      gt += in && key[j] > prefix;
+      eq += in && key[j] == prefix;
+    }
+  });
   gt = warp_sum_i(gt);
   eq = warp_sum_i(eq);
   if (tid < 2) counts[tid] = 0;
@@ -155,58 +199,81 @@ kv_keep_kernel(KeepParams p) {
     gt0 += c[0];
     eq0 += c[1];
   }
+  // Ordered: where a thread's tokens of a tile go depends on how many kept-above
+  // and equal ones are before them; both counts of a tile fit 16 bits.
   const int limit = (int)want;
-  for (int base = lo; base < hi; base += kTile) {
-    uint32_t key[kPer];
-    int g = 0, e = 0;
+  auto count = [&](int t, const uint32_t (&key)[kPer]) {
+    uint32_t c = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const int i = base + tid * kPer + j;
-      key[j] = i < hi ? order_key(m[i]) : 0u;
-      g += i < hi && key[j] > prefix;
-      e += i < hi && key[j] == prefix;
+      const bool in = lo + t * kTile + tid * kPer + j < hi;
+      c += (in && key[j] > prefix ? 1u : 0u) + (in && key[j] == prefix ? 0x10000u : 0u);
     }
-    int gi = g, ei = e;  // inclusive scans
+    return c;
+  };
+  auto warp_scan = [&](uint32_t c) {  // inclusive
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int a = __shfl_up_sync(0xffffffffu, gi, o), c = __shfl_up_sync(0xffffffffu, ei, o);
-      if (lane >= o) {
-        gi += a;
-        ei += c;
-      }
+      const uint32_t up = __shfl_up_sync(0xffffffffu, c, o);
+      if (lane >= o) c += up;
     }
-    if (lane == 31) {
-      scan_gt[warp] = gi;
-      scan_eq[warp] = ei;
-    }
-    __syncthreads();
-    int gb = gt0, eb = eq0, gall = 0, eall = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) {
-        gb += scan_gt[w];
-        eb += scan_eq[w];
-      }
-      gall += scan_gt[w];
-      eall += scan_eq[w];
-    }
-    gb += gi - g;
-    eb += ei - e;
+    return c;
+  };
+  auto write = [&](int t, const uint32_t (&key)[kPer], int gb, int eb) {
+    const int base = lo + t * kTile + tid * kPer;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const int i = base + tid * kPer + j;
-      if (i >= hi) break;
+      if (base + j >= hi) break;
       if (key[j] > prefix) {
-        out[p.sinks + gb + min(eb, limit)] = p.sinks + i;
+        out[p.sinks + gb + min(eb, limit)] = p.sinks + base + j;
         ++gb;
       } else if (key[j] == prefix) {
-        if (eb < limit) out[p.sinks + gb + eb] = p.sinks + i;
+        if (eb < limit) out[p.sinks + gb + eb] = p.sinks + base + j;
         ++eb;
       }
     }
-    gt0 += gall;
-    eq0 += eall;
+  };
+  if constexpr (Held) {
+    uint32_t before[kHeld];
+#pragma unroll
+    for (int t = 0; t < kHeld; ++t) {
+      const uint32_t c = count(t, held[t]), incl = warp_scan(c);
+      before[t] = incl - c;
+      if (lane == 31) scan[t][warp] = incl;
+    }
     __syncthreads();
+    static_assert(kHeld * kWarps == 64, "two entries a lane below");
+    if (warp == 0) {  // the warps' counts in tile order; a slice's sums fit 16 bits too (8,192)
+      uint32_t* flat = &scan[0][0];
+      const uint32_t a = flat[2 * lane], c = flat[2 * lane + 1], incl = warp_scan(a + c);
+      flat[2 * lane] = incl - a - c;
+      flat[2 * lane + 1] = incl - c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < kHeld; ++t) {
+      const uint32_t at = scan[t][warp] + before[t];
+      write(t, held[t], gt0 + (int)(at & 0xffffu), eq0 + (int)(at >> 16));
+    }
+  } else {
+    for (int t = 0; t < tiles; ++t) {
+      uint32_t key[kPer];
+      load(t, key);
+      const uint32_t c = count(t, key), incl = warp_scan(c);
+      if (lane == 31) scan[0][warp] = incl;
+      __syncthreads();
+      uint32_t at = incl - c, all = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const uint32_t x = scan[0][w];
+        if (w < warp) at += x;
+        all += x;
+      }
+      write(t, key, gt0 + (int)(at & 0xffffu), eq0 + (int)(at >> 16));
+      gt0 += (int)(all & 0xffffu);
+      eq0 += (int)(all >> 16);
+      __syncthreads();
+    }
   }
   cluster.sync();  // no CTA leaves while its counts may be read
 }
@@ -241,7 +308,10 @@ extern "C" int sf_kv_keep_heaviest(const float* mass, int64_t mass_batch_stride,
   while (ranks < kMaxCluster && (int64_t)ranks * kTile < mid) ranks *= 2;
   p.slice = (int)(((mid + ranks - 1) / ranks + kTile - 1) / kTile * kTile);
   const dim3 grid(ranks, (unsigned)(batch * num_kv_heads));
-  SF_CHECK_CUDA(launch_pdl_cluster(kv_keep_kernel, grid, dim3(kThreads), 0, as_stream(stream), ranks, 1u, p));
+  if (p.slice <= kHeld * kTile)
+    SF_CHECK_CUDA(launch_pdl_cluster(kv_keep_kernel<true>, grid, dim3(kThreads), 0, as_stream(stream), ranks, 1u, p));
+  else
+    SF_CHECK_CUDA(launch_pdl_cluster(kv_keep_kernel<false>, grid, dim3(kThreads), 0, as_stream(stream), ranks, 1u, p));
   SF_CHECK_LAUNCH();
   return SF_OK;
 }

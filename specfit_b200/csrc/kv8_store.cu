@@ -42,7 +42,20 @@ int kv8_check(const sf_kv8_rows* r, bool need_values) {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxChunks = 128 * 128 / 8 / kThreads;  // 16-byte bf16 chunks per thread: 8
+
+// Row and 8-element chunk of element chunk i of a block: rows of `per_row` chunks.
+__device__ __forceinline__ void row_chunk(int i, int per_row, int& row, int& ch) {
+  if (per_row == 16) {
+    row = i >> 4;
+    ch = i & 15;
+  } else if (per_row == 8) {
+    row = i >> 3;
+    ch = i & 7;
+  } else {
+    row = i / per_row;
+    ch = i - row * per_row;
+  }
+}
 
 // Where the rows of a block come from: bf16 rows in order (sealing) ...
 struct SourceRows {
@@ -124,9 +137,11 @@ __device__ __forceinline__ void move_mass(const SourceKept& s, int b, int h, int
   }
 }
 
-// grid: (blocks [+ 1 for the tail], batch * hkv, 2: K and V).
-template <typename Source>
-__global__ void __launch_bounds__(kThreads)
+// grid: (blocks [+ 1 for the tail], batch * hkv, 2: K and V).  kChunks: 16-byte
+// bf16 chunks that a thread holds, block * D / 8 / kThreads rounded up; few of
+// them leave registers for more CTAs on an SM.
+template <typename Source, int kChunks>
+__global__ void __launch_bounds__(kThreads, kChunks <= 4 ? 6 : 4)
 kv8_write_kernel(Source src, Target t) {
   pdl_wait();
   pdl_trigger();
@@ -139,16 +154,18 @@ kv8_write_kernel(Source src, Target t) {
   const int rows = (int)min((int64_t)t.block, n - row0);
   if (!is_v) move_mass(src, b, h, row0, rows);
   const int chunks = rows * per_row;
-  uint4 x[kMaxChunks];
+  uint4 x[kChunks];
 #pragma unroll
-  for (int j = 0; j < kMaxChunks; ++j) {
+  for (int j = 0; j < kChunks; ++j) {
     const int i = threadIdx.x + j * kThreads;
-    x[j] = i < chunks ? load_chunk(src, b, h, is_v, row0 + i / per_row, i % per_row) : make_uint4(0, 0, 0, 0);
+    int r, ch;
+    row_chunk(i, per_row, r, ch);
+    x[j] = i < chunks ? load_chunk(src, b, h, is_v, row0 + r, ch) : make_uint4(0, 0, 0, 0);
   }
   if ((int64_t)blockIdx.x >= t.full_blocks) {  // rows that do not fill a block stay bf16
     __nv_bfloat16* dst = (is_v ? t.vt : t.kt) + b * t.t_bs + h * t.t_hs;
 #pragma unroll
-    for (int j = 0; j < kMaxChunks; ++j) {
+    for (int j = 0; j < kChunks; ++j) {
       const int i = threadIdx.x + j * kThreads;
       if (i < chunks) *reinterpret_cast<uint4*>(dst + (int64_t)i * 8) = x[j];
     }
@@ -156,7 +173,7 @@ kv8_write_kernel(Source src, Target t) {
   }
   uint32_t top2 = 0;  // two 15-bit magnitudes
 #pragma unroll
-  for (int j = 0; j < kMaxChunks; ++j) {
+  for (int j = 0; j < kChunks; ++j) {
     top2 = __vmaxu2(top2, x[j].x & 0x7fff7fffu);
     top2 = __vmaxu2(top2, x[j].y & 0x7fff7fffu);
     top2 = __vmaxu2(top2, x[j].z & 0x7fff7fffu);
@@ -176,7 +193,7 @@ kv8_write_kernel(Source src, Target t) {
     (is_v ? t.vs : t.ks)[b * t.s_bs + h * t.s_hs + blk] = bad ? __int_as_float(0x7fc00000) : pow2f(e);
   uint8_t* dst = (is_v ? t.v : t.k) + b * t.c_bs + h * t.c_hs + blk * t.block * t.d;
 #pragma unroll
-  for (int j = 0; j < kMaxChunks; ++j) {
+  for (int j = 0; j < kChunks; ++j) {
     const int i = threadIdx.x + j * kThreads;
     if (i >= chunks) continue;
     const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
@@ -206,6 +223,19 @@ kv8_read_kernel(Kv8Rows c, int64_t first, int64_t count, __nv_bfloat16* __restri
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count * per_row;
        i += (int64_t)gridDim.x * kThreads)
     *reinterpret_cast<uint4*>(dst + i * 8) = cache_chunk(c, b, h, is_v, first + i / per_row, (int)(i % per_row));
+}
+
+template <typename Source>
+int launch_write(const Source& src, const Target& t, dim3 grid, cudaStream_t stream) {
+  const int chunks = (t.block * t.d / 8 + kThreads - 1) / kThreads;
+  if (chunks <= 2)
+    SF_CHECK_CUDA(launch_pdl(kv8_write_kernel<Source, 2>, grid, dim3(kThreads), 0, stream, src, t));
+  else if (chunks <= 4)
+    SF_CHECK_CUDA(launch_pdl(kv8_write_kernel<Source, 4>, grid, dim3(kThreads), 0, stream, src, t));
+  else
+    SF_CHECK_CUDA(launch_pdl(kv8_write_kernel<Source, 8>, grid, dim3(kThreads), 0, stream, src, t));
+  SF_CHECK_LAUNCH();
+  return SF_OK;
 }
 
 Target make_target(const sf_kv8_rows& r, int64_t first_block, int64_t full_blocks) {
@@ -248,10 +278,7 @@ extern "C" int sf_kv8_seal(const void* k, const void* v, int64_t batch_stride, i
   const SourceRows src{static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), batch_stride,
                        head_stride, row_stride};
   const dim3 grid((unsigned)blocks, (unsigned)(rows->batch * rows->num_kv_heads), 2);
-  SF_CHECK_CUDA(launch_pdl(kv8_write_kernel<SourceRows>, grid, dim3(kThreads), 0, as_stream(stream), src,
-                           make_target(*rows, first_block, blocks)));
-  SF_CHECK_LAUNCH();
-  return SF_OK;
+  return launch_write(src, make_target(*rows, first_block, blocks), grid, as_stream(stream));
 }
 
 extern "C" int sf_kv8_read(const sf_kv8_rows* rows, int64_t first, int64_t count, void* k_out, void* v_out,
@@ -297,8 +324,5 @@ extern "C" int sf_kv8_compact(const sf_kv8_rows* rows, const int32_t* keep, int6
                  mass_out_batch_stride, mass_out_head_stride};
   const int64_t full = out->sealed / out->block_tokens;
   const dim3 grid((unsigned)(full + (out->tail > 0 ? 1 : 0)), (unsigned)(rows->batch * rows->num_kv_heads), 2);
-  SF_CHECK_CUDA(launch_pdl(kv8_write_kernel<SourceKept>, grid, dim3(kThreads), 0, as_stream(stream), src,
-                           make_target(*out, 0, full)));
-  SF_CHECK_LAUNCH();
-  return SF_OK;
+  return launch_write(src, make_target(*out, 0, full), grid, as_stream(stream));
 }
