@@ -830,12 +830,10 @@ Shape shape_of(int64_t packed) {
   return {tiles > 1, tiles, tiles > 1 ? (tiles + 1) / 2 : 1};
 }
 
-// Blocks with tail rows: from the one that holds the first, to the end.  (The
-// boundary is a multiple of 32, so one more block than the tail fills can be
-// touched.)
-int64_t tail_blocks(int64_t sealed, int64_t kv_len) {
-  return kv_len > sealed ? (kv_len + kKB - 1) / kKB - sealed / kKB : 0;
-}
+// Blocks that are not codes alone: from the one that holds the first tail row
+// to the end.  (The boundary is a multiple of 32: without a tail that can be a
+// last block that the codes do not fill.)
+int64_t tail_blocks(int64_t sealed, int64_t kv_len) { return (kv_len + kKB - 1) / kKB - sealed / kKB; }
 // Bytes of the first kernel's layout, with the given number of such blocks.
 size_t prep_bytes(int64_t heads, int64_t tiles, int64_t blocks) {
   return (size_t)heads * ((tiles + 2 * blocks) * (size_t)kTileBytes + (tiles + blocks) * kBM * sizeof(float)) +

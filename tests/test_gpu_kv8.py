@@ -189,6 +189,9 @@ ATTENTION = [
     (1, 8, 2, 128, 64, 192, 200, 150, "causal"),
     (1, 8, 1, 128, 64, 0, 300, 257, "causal"),
     (1, 16, 1, 128, 32, 2080, 17, 16, "any"),
+    # No tail, and codes that end inside a block of 128 keys.
+    (2, 16, 2, 128, 32, 96, 0, 65, "any"),
+    (1, 8, 1, 128, 64, 704, 0, 130, "any"),
 ]
 
 
