@@ -823,12 +823,16 @@ SF_API int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int64_t 
  * heads of its KV head and the rows that see it of exp(scale * q . k - lse),
  * lse [batch, num_heads, q_len] as sf_kv8_tree_attention returned it.  Rows
  * with lse -infinity add nothing.  Only the key side of `rows` is read.
+ * workspace (16-byte aligned): sf_kv8_mass_workspace_bytes(...) bytes, perhaps 0.
  */
+SF_API size_t sf_kv8_mass_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim,
+                                          int64_t q_len, int64_t sealed, int64_t tail);
 SF_API int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int64_t q_head_stride,
                                  int64_t q_row_stride, int num_heads, int64_t q_len, const float* lse,
                                  const sf_kv8_rows* rows, const uint32_t* tree_bits, int bit_words,
                                  int64_t bits_batch_stride, int64_t prefix_len, float scale, float* mass,
-                                 int64_t mass_batch_stride, int64_t mass_head_stride, void* stream);
+                                 int64_t mass_batch_stride, int64_t mass_head_stride, void* workspace,
+                                 size_t workspace_bytes, void* stream);
 /*
  * The tokens an eviction keeps: keep [batch, num_kv_heads, budget] int32,
  * ascending: the first `sinks`, the last `recent`, and the heaviest of the

@@ -45,11 +45,12 @@ extern "C" int sf_abi_version(void) { return 1; }
 extern "C" int sf_device_status(int* status, int reset) {
   using namespace sf;
   SF_CHECK_ARG(status, "null pointer argument");
-  int a = 0, b = 0, c = 0, d = 0;
+  int a = 0, b = 0, c = 0, d = 0, e = 0;
   if (int rc = swiglu_status(&a, reset)) return rc;
   if (int rc = dense_status(&b, reset)) return rc;
   if (int rc = tree_attention_tc_status(&c, reset)) return rc;
   if (int rc = kv8_tc_status(&d, reset)) return rc;
-  *status = a ? a : (b ? b : (c ? c : d));
+  if (int rc = kv8_mass_tc_status(&e, reset)) return rc;
+  *status = a ? a : (b ? b : (c ? c : (d ? d : e)));
   return SF_OK;
 }

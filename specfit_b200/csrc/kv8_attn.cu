@@ -613,7 +613,7 @@ extern "C" size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int
   if (kv8_use_tc(head_dim, packed, kv_len))
     need = std::max(need, partial_bytes(kv8_split_tc(batch, num_kv_heads, packed, kv_len), batch, num_heads, head_dim,
                                         q_len) +
-                              15 + kv8_tc_prep_bytes(batch, num_kv_heads, packed, tail, kv_len));
+                              15 + kv8_prep_layout(nullptr, nullptr, false, (int64_t)batch * num_kv_heads, packed, sealed, kv_len));
   return need;
 }
 

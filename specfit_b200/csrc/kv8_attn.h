@@ -2,6 +2,8 @@
 // merge of their partial results.
 #pragma once
 
+#include <cuda.h>
+
 #include "kv8.cuh"
 #include "tree_attn.h"
 
@@ -56,9 +58,34 @@ Kv8Split kv8_split_mma(int batch, int hkv, int64_t packed_rows, int64_t kv_len);
 bool kv8_use_tc(int head_dim, int64_t packed_rows, int64_t kv_len);
 bool kv8_tc_layout(const Kv8Rows& c, int batch);
 Kv8Split kv8_split_tc(int batch, int hkv, int64_t packed_rows, int64_t kv_len);
-// Workspace behind the partial results (16-byte aligned).
-size_t kv8_tc_prep_bytes(int batch, int hkv, int64_t packed_rows, int64_t tail, int64_t kv_len);
 int kv8_attention_tc(const Kv8Attn& p, void* prep, cudaStream_t stream);
+
+// What a first kernel lays out for the tcgen05 kernels, for each (request, KV
+// head) bh: the query tiles and the blocks of 128 keys that hold tail rows, as
+// images of the kernels' shared-memory tiles.
+struct Kv8Prep {
+  uint8_t* q;    // [bh][tiles][hi, lo: 128 rows x 128, e4m3, swizzled]
+  uint8_t* k;    // [bh][blocks][hi, lo], the blocks from key `first` on
+  float* kf;     // [bh][blocks * 128]: a key's scale; NaN for a key that holds one
+  // For attention (null otherwise):
+  uint8_t* v;    // [bh][blocks][128 keys x 128, fp16 in units of `unit`, swizzled]
+  float* qf;     // [bh][tiles * 128]: the power of two taken out of a query row; NaN for a row that holds one
+  float* unit;   // [bh]: the largest V scale
+  // For the mass (null otherwise):
+  float2* rowc;  // [bh][tiles * 128]: (that power times scale * log2(e), lse * log2(e))
+  int tiles, blocks, first;
+};
+// Fills `w` (nullable) with places from `base` (16-byte aligned) on; returns the bytes.
+size_t kv8_prep_layout(Kv8Prep* w, void* base, bool for_mass, int64_t heads, int64_t packed_rows, int64_t sealed,
+                       int64_t kv_len);
+int kv8_prep(const Kv8Attn& p, const Kv8Prep& w, cudaStream_t stream);
+// Tensor map of K's codes: boxes of 128 keys.
+int kv8_key_map(CUtensorMap* map, const Kv8Rows& c, int batch);
+
+// The mass on tcgen05 (kv8_mass_tc.cu).
+bool kv8_mass_use_tc(int head_dim, int64_t packed_rows);
+int kv8_mass_tc(const Kv8Attn& p, float* mass, int64_t m_bs, int64_t m_hs, void* prep, cudaStream_t stream);
+int kv8_mass_tc_status(int* status, int reset);
 int kv8_tc_status(int* status, int reset);
 
 }  // namespace sf

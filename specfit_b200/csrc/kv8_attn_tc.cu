@@ -92,17 +92,6 @@ struct __align__(16) Tail {
   int tensor_lock;  // held by the lane that is issuing its products
 };
 
-// What the first kernel lays out, for each (request, KV head) bh.
-struct Prep {
-  uint8_t* q;    // [bh][tiles][hi, lo: 128 rows x 128, e4m3, swizzled]
-  uint8_t* k;    // [bh][blocks][hi, lo], the blocks of 128 keys from `first` on, which hold tail rows
-  uint8_t* v;    // [bh][blocks][128 keys x 128, fp16 in units of `unit`, swizzled]
-  float* qf;     // [bh][tiles * 128]: the power of two taken out of a query row; NaN for a row that holds one
-  float* kf;     // [bh][blocks * 128]: a key's scale; NaN for a key that holds one
-  float* unit;   // [bh]: the largest V scale
-  int tiles, blocks, first;
-};
-
 constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + 2 * kStages * kTileBytes + kHalf + sizeof(Tail);
 
 // Byte offset of 16-byte chunk c of row r of a bf16 tile (c < 16: two
@@ -268,7 +257,7 @@ __device__ __forceinline__ int row_head(const Kv8Attn& p, int n) { return (int)(
 // grid: (query tiles, then blocks with tail rows (one CTA for the unit alone if
 // there are none); batch * hkv).
 __global__ void __launch_bounds__(256)
-kv8_prep_kernel(Kv8Attn p, Prep w) {
+kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
   pdl_wait();
   pdl_trigger();
   __shared__ float tops[8];
@@ -296,11 +285,26 @@ kv8_prep_kernel(Kv8Attn p, Prep w) {
       const bool nan = top >= 0x7f80u;  // the row answers NaN
       const int e = nan ? 0 : kv8_exponent(top);
       split_store(in, pow2f(-e), img + u * 4096, img + u * 4096 + kHalf);
-      if (part == 0)
-        w.qf[((int64_t)bh * w.tiles + tile) * kBM + u * 32 + row] = nan ? __int_as_float(0x7fc00000) : pow2f(e);
+      if (part == 0) {
+        const int64_t at = ((int64_t)bh * w.tiles + tile) * kBM + u * 32 + row;
+        const float f = nan ? __int_as_float(0x7fc00000) : pow2f(e);
+        if (w.qf) w.qf[at] = f;
+        if (w.rowc) {
+          const int pr = tile * kBM + u * 32 + row;
+          float lse = -INFINITY;
+          if (pr < packed) {
+            const int h = row_head(p, pr);
+            lse = p.lse[((int64_t)req * p.heads + kvh * p.group + h) * p.q_len + (pr - h * p.q_len)];
+          }
+          // Rows that see nothing, and those past the last, add 2^-infinity.
+          w.rowc[at] = make_float2(f * p.scale_log2, lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f);
+        }
+      }
     }
     return;
   }
+  const bool values = w.v != nullptr;
+  if (!values && (int)blockIdx.x - w.tiles >= w.blocks) return;
   // The unit: every CTA that needs it finds it for itself.
   const int sealed = (int)p.c.sealed, tail_rows = p.kv_len - sealed;
   const float* vsc = p.c.vs + req * p.c.s_bs + kvh * p.c.s_hs;
@@ -309,10 +313,11 @@ kv8_prep_kernel(Kv8Attn p, Prep w) {
   const __nv_bfloat16* vt = p.c.vt + req * p.c.t_bs + kvh * p.c.t_hs;
   float unit = pow2f(kKv8MinExponent);
 #pragma unroll 4
-  for (int i = threadIdx.x; i < sealed >> p.c.block_shift; i += 256) unit = fmaxf(unit, vsc[i]);  // NaN is passed over
+  for (int i = threadIdx.x; values && i < sealed >> p.c.block_shift; i += 256)
+    unit = fmaxf(unit, vsc[i]);  // NaN is passed over
   uint32_t top = 0;
 #pragma unroll 8
-  for (int i = threadIdx.x; i < tail_rows * (kD / 8); i += 256) {
+  for (int i = threadIdx.x; values && i < tail_rows * (kD / 8); i += 256) {
     const uint4 x = *reinterpret_cast<const uint4*>(vt + (int64_t)i * 8);
     const uint32_t in[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -329,7 +334,7 @@ kv8_prep_kernel(Kv8Attn p, Prep w) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) unit = fmaxf(unit, tops[i]);
   const int blk = blockIdx.x - w.tiles;
-  if (blk == 0 && threadIdx.x == 0) w.unit[bh] = unit;
+  if (values && blk == 0 && threadIdx.x == 0) w.unit[bh] = unit;
   if (blk >= w.blocks) return;
   const float inv = 1.f / unit;  // exact
   const uint8_t* kc = p.c.k + req * p.c.c_bs + kvh * p.c.c_hs + part * 16;
@@ -345,11 +350,14 @@ kv8_prep_kernel(Kv8Attn p, Prep w) {
     float f = 1.f;
     if (key0 + u * 32 < sealed) {  // the 32 rows of a pass are all codes or all tail
       a = *reinterpret_cast<const uint4*>(kc + (int64_t)key * kD);
-      const float vs = vsc[key >> p.c.block_shift];
-      f = vs == vs ? ksc[key >> p.c.block_shift] : vs;
-      const float r = vs == vs ? vs * inv : 0.f;  // a block with a NaN counts as zeros
-      x = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD), pack_f16x2(r, r));
-      y = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD + 64), pack_f16x2(r, r));
+      f = ksc[key >> p.c.block_shift];
+      if (values) {
+        const float vs = vsc[key >> p.c.block_shift];
+        if (vs != vs) f = vs;
+        const float r = vs == vs ? vs * inv : 0.f;  // a block with a NaN counts as zeros
+        x = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD), pack_f16x2(r, r));
+        y = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD + 64), pack_f16x2(r, r));
+      }
       *reinterpret_cast<uint4*>(kimg + u * 4096) = a;
       *reinterpret_cast<uint4*>(kimg + u * 4096 + kHalf) = c;  // codes have no lower part
     } else {
@@ -357,8 +365,10 @@ kv8_prep_kernel(Kv8Attn p, Prep w) {
         const int64_t at = (int64_t)(key - sealed) * kD;
         a = *reinterpret_cast<const uint4*>(kt + at + part * 16);
         c = *reinterpret_cast<const uint4*>(kt + at + part * 16 + 8);
-        x = *reinterpret_cast<const uint4*>(vt + at + part * 8);
-        y = *reinterpret_cast<const uint4*>(vt + at + part * 8 + 64);
+        if (values) {
+          x = *reinterpret_cast<const uint4*>(vt + at + part * 8);
+          y = *reinterpret_cast<const uint4*>(vt + at + part * 8 + 64);
+        }
       }
       uint32_t in[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
       const uint32_t vals[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
@@ -374,8 +384,10 @@ kv8_prep_kernel(Kv8Attn p, Prep w) {
       x = tail8(x, inv);
       y = tail8(y, inv);
     }
-    *reinterpret_cast<uint4*>(vimg + u * 4096) = x;
-    *reinterpret_cast<uint4*>(vimg + u * 4096 + kRegion) = y;
+    if (values) {
+      *reinterpret_cast<uint4*>(vimg + u * 4096) = x;
+      *reinterpret_cast<uint4*>(vimg + u * 4096 + kRegion) = y;
+    }
     if (part == 0) kf[u * 32 + row] = f;
   }
 }
@@ -400,7 +412,7 @@ __device__ __forceinline__ bool take_turn(int* lock, volatile int* abort_flag, i
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
-kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Prep w, int dual, int ranges) {
+kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep w, int dual, int ranges) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
@@ -830,16 +842,6 @@ Shape shape_of(int64_t packed) {
   return {tiles > 1, tiles, tiles > 1 ? (tiles + 1) / 2 : 1};
 }
 
-// Blocks that are not codes alone: from the one that holds the first tail row
-// to the end.  (The boundary is a multiple of 32: without a tail that can be a
-// last block that the codes do not fill.)
-int64_t tail_blocks(int64_t sealed, int64_t kv_len) { return (kv_len + kKB - 1) / kKB - sealed / kKB; }
-// Bytes of the first kernel's layout, with the given number of such blocks.
-size_t prep_bytes(int64_t heads, int64_t tiles, int64_t blocks) {
-  return (size_t)heads * ((tiles + 2 * blocks) * (size_t)kTileBytes + (tiles + blocks) * kBM * sizeof(float)) +
-         ((size_t)heads * sizeof(float) + 127) / 128 * 128;
-}
-
 }  // namespace
 
 bool kv8_use_tc(int head_dim, int64_t packed, int64_t kv_len) { return head_dim == kD && packed >= 48 && kv_len > 0; }
@@ -871,8 +873,56 @@ Kv8Split kv8_split_tc(int batch, int hkv, int64_t packed, int64_t kv_len) {
   return {(int)(sh.dual ? best : 2 * best), (int)(best_per * kKB)};
 }
 
-size_t kv8_tc_prep_bytes(int batch, int hkv, int64_t packed, int64_t tail, int64_t kv_len) {
-  return prep_bytes((int64_t)batch * hkv, shape_of(packed).tiles, tail_blocks(kv_len - tail, kv_len));
+// Blocks that are not codes alone: from the one that holds the first tail row
+// to the end.  (The boundary is a multiple of 32: without a tail that can be a
+// last block that the codes do not fill.)
+static int64_t tail_blocks(int64_t sealed, int64_t kv_len) { return (kv_len + kKB - 1) / kKB - sealed / kKB; }
+
+size_t kv8_prep_layout(Kv8Prep* w, void* base, bool for_mass, int64_t heads, int64_t packed, int64_t sealed,
+                       int64_t kv_len) {
+  const int64_t tiles = shape_of(packed).tiles, blocks = tail_blocks(sealed, kv_len);
+  uint8_t* at = static_cast<uint8_t*>(base);
+  size_t used = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* p = at + used;
+    used += (bytes + 127) / 128 * 128;
+    return p;
+  };
+  Kv8Prep r = {};
+  r.tiles = (int)tiles;
+  r.blocks = (int)blocks;
+  r.first = (int)(sealed / kKB * kKB);
+  r.q = take((size_t)heads * tiles * kTileBytes);
+  r.k = take((size_t)heads * blocks * kTileBytes);
+  r.kf = reinterpret_cast<float*>(take((size_t)heads * blocks * kKB * sizeof(float)));
+  if (for_mass) {
+    r.rowc = reinterpret_cast<float2*>(take((size_t)heads * tiles * kBM * sizeof(float2)));
+  } else {
+    r.v = take((size_t)heads * std::max<int64_t>(blocks, 1) * kTileBytes);  // not null: values are laid out
+    r.qf = reinterpret_cast<float*>(take((size_t)heads * tiles * kBM * sizeof(float)));
+    r.unit = reinterpret_cast<float*>(take((size_t)heads * sizeof(float)));
+  }
+  if (w) *w = r;
+  return used;
+}
+
+int kv8_prep(const Kv8Attn& p, const Kv8Prep& w, cudaStream_t stream) {
+  const int extra = w.v ? std::max(w.blocks, 1) : w.blocks;
+  const dim3 grid((unsigned)(w.tiles + extra), (unsigned)(p.batch * p.c.hkv));
+  SF_CHECK_CUDA(launch_pdl(kv8_prep_kernel, grid, dim3(256), 0, stream, p, w));
+  SF_CHECK_LAUNCH();
+  return SF_OK;
+}
+
+int kv8_key_map(CUtensorMap* map, const Kv8Rows& c, int batch) {
+  // K's codes, 16 bits at a time (bytes are bytes): [batch][heads][tokens][64].
+  *map = {};
+  if (c.sealed < kKB) return SF_OK;  // no block of codes alone, no load by this map
+  const cuuint64_t dims[4] = {64, (cuuint64_t)c.sealed, (cuuint64_t)c.hkv, (cuuint64_t)batch};
+  const int64_t hs = c.hkv > 1 ? c.c_hs : c.sealed * kD, bs = batch > 1 ? c.c_bs : c.hkv * hs;
+  const cuuint64_t strides[3] = {kD, (cuuint64_t)hs, (cuuint64_t)bs};
+  const cuuint32_t box[4] = {64, kKB, 1, 1};
+  return tma_encode_bf16(map, c.k, 4, dims, strides, box);
 }
 
 int kv8_attention_tc(const Kv8Attn& p, void* prep, cudaStream_t stream) {
@@ -887,28 +937,11 @@ int kv8_attention_tc(const Kv8Attn& p, void* prep, cudaStream_t stream) {
   const int ranges = sh.dual ? p.splits : p.splits / 2;
   const int64_t heads = (int64_t)p.batch * p.c.hkv;
   SF_CHECK_ARG(sh.pairs < 65536 && (int64_t)ranges * p.batch < 65536, "too many query rows or requests");
-  Prep w;
-  w.tiles = (int)sh.tiles;
-  w.blocks = (int)tail_blocks(p.c.sealed, p.kv_len);
-  w.first = (int)(p.c.sealed / kKB * kKB);
-  w.q = static_cast<uint8_t*>(prep);
-  w.k = w.q + (size_t)heads * w.tiles * kTileBytes;
-  w.v = w.k + (size_t)heads * w.blocks * kTileBytes;
-  w.qf = reinterpret_cast<float*>(w.v + (size_t)heads * w.blocks * kTileBytes);
-  w.kf = w.qf + (size_t)heads * w.tiles * kBM;
-  w.unit = w.kf + (size_t)heads * w.blocks * kKB;
-  const dim3 prep_grid((unsigned)(w.tiles + std::max(w.blocks, 1)), (unsigned)heads);
-  SF_CHECK_CUDA(launch_pdl(kv8_prep_kernel, prep_grid, dim3(256), 0, stream, p, w));
-  SF_CHECK_LAUNCH();
-  // K's codes, 16 bits at a time (bytes are bytes): [batch][heads][tokens][64].
-  CUtensorMap tm_k = {};
-  if (p.c.sealed >= kKB) {
-    const cuuint64_t dims[4] = {64, (cuuint64_t)p.c.sealed, (cuuint64_t)p.c.hkv, (cuuint64_t)p.batch};
-    const int64_t hs = p.c.hkv > 1 ? p.c.c_hs : p.c.sealed * kD, bs = p.batch > 1 ? p.c.c_bs : p.c.hkv * hs;
-    const cuuint64_t strides[3] = {kD, (cuuint64_t)hs, (cuuint64_t)bs};
-    const cuuint32_t box[4] = {64, kKB, 1, 1};
-    if (int rc = tma_encode_bf16(&tm_k, p.c.k, 4, dims, strides, box)) return rc;
-  }
+  Kv8Prep w;
+  kv8_prep_layout(&w, prep, false, heads, (int64_t)p.group * p.q_len, p.c.sealed, p.kv_len);
+  if (int rc = kv8_prep(p, w, stream)) return rc;
+  CUtensorMap tm_k;
+  if (int rc = kv8_key_map(&tm_k, p.c, p.batch)) return rc;
   const dim3 grid((unsigned)p.c.hkv, (unsigned)sh.pairs, (unsigned)(ranges * p.batch));
   SF_CHECK_CUDA(launch_pdl(kv8_attn_tc_kernel, grid, dim3(kThreads), kSmemBytes, stream, tm_k, p, w, sh.dual ? 1 : 0,
                            ranges));

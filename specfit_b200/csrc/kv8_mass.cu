@@ -182,11 +182,24 @@ int launch_mass(const MassParams& p, cudaStream_t stream) {
 }  // namespace
 }  // namespace sf
 
+extern "C" size_t sf_kv8_mass_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim, int64_t q_len,
+                                             int64_t sealed, int64_t tail) {
+  using namespace sf;
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
+      head_dim > 128 || q_len <= 0 || sealed < 0 || tail < 0 || sealed + tail <= 0 || q_len >= (1 << 30) ||
+      sealed >= (1 << 30) || tail >= (1 << 30))
+    return 0;
+  const int64_t packed = (int64_t)(num_heads / num_kv_heads) * q_len;
+  if (!kv8_mass_use_tc(head_dim, packed)) return 0;
+  return kv8_prep_layout(nullptr, nullptr, true, (int64_t)batch * num_kv_heads, packed, sealed, sealed + tail);
+}
+
 extern "C" int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int64_t q_head_stride,
                                      int64_t q_row_stride, int num_heads, int64_t q_len, const float* lse,
                                      const sf_kv8_rows* rows, const uint32_t* tree_bits, int bit_words,
                                      int64_t bits_batch_stride, int64_t prefix_len, float scale, float* mass,
-                                     int64_t mass_batch_stride, int64_t mass_head_stride, void* stream) {
+                                     int64_t mass_batch_stride, int64_t mass_head_stride, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
   using namespace sf;
   if (int rc = kv8_check(rows, false)) return rc;
   const int64_t kv_len = rows->sealed + rows->tail;
@@ -202,6 +215,11 @@ extern "C" int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int6
                "tree_bits must cover the keys from prefix_len on");
   SF_CHECK_ARG(aligned16(q) && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0 && q_row_stride % 8 == 0,
                "q rows must be 16-byte aligned");
+  const size_t need = sf_kv8_mass_workspace_bytes(rows->batch, num_heads, rows->num_kv_heads, rows->head_dim, q_len,
+                                                  rows->sealed, rows->tail);
+  if (workspace_bytes < need || (need && !workspace))
+    return set_error(SF_ERR_WORKSPACE, "8-bit cache mass workspace needs %zu bytes", need);
+  SF_CHECK_ARG(need == 0 || aligned16(workspace), "workspace must be 16-byte aligned");
   MassParams m = {};
   m.a.c = kv8_view(*rows);
   m.a.q = static_cast<const __nv_bfloat16*>(q);
@@ -224,5 +242,7 @@ extern "C" int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int6
   m.m_bs = mass_batch_stride;
   m.m_hs = mass_head_stride;
   m.tiles = (int)((kv_len + kTileKeys - 1) / kTileKeys);
+  if (need && kv8_tc_layout(m.a.c, rows->batch))
+    return kv8_mass_tc(m.a, mass, mass_batch_stride, mass_head_stride, workspace, as_stream(stream));
   return rows->head_dim <= 64 ? launch_mass<64>(m, as_stream(stream)) : launch_mass<128>(m, as_stream(stream));
 }

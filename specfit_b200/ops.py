@@ -855,13 +855,15 @@ def kv8_attention_mass(q: torch.Tensor, lse: torch.Tensor, rows: Kv8Rows, tree_b
         raise ValueError("mass must be float32 [batch, KV heads, >= length], contiguous per head")
     lse = lse.contiguous()
     with _on(index):
+        nbytes = N.lib.sf_kv8_mass_workspace_bytes(b, hq, ms[1], d, tq, rows.sealed, rows.shape[2] - rows.sealed)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=rows.device) if nbytes else None
         rc = N.lib.sf_kv8_attention_mass(q.data_ptr(), st[0], st[1], st[2], hq, tq, lse.data_ptr(), rows._p,
                                          None if bits is None else bits.data_ptr(), words, bits_bs, prefix_len,
                                          d ** -0.5 if scale is None else scale, mass.data_ptr(), mst[0], mst[1],
-                                         _raw_stream(index))
+                                         None if ws is None else ws.data_ptr(), nbytes, _raw_stream(index))
     if rc:
         N.check(rc, "sf_kv8_attention_mass")
-    _launched(1 if tq and rows.shape[2] else 0)
+    _launched((2 if nbytes else 1) if tq and rows.shape[2] else 0)
     return mass
 
 

@@ -230,7 +230,9 @@ def _long(ops, b, hkv, d, block, sealed, tail, seed):
 
 @pytest.mark.parametrize("b,hq,hkv,d,rows,sealed,tail", [(1, 32, 4, 128, 1, 65536, 33), (1, 16, 2, 128, 65, 8192, 65),
                                                          (1, 16, 2, 128, 40, 4096, 40), (2, 16, 2, 64, 20, 8192, 20),
-                                                         (1, 8, 1, 128, 300, 4096, 300)])
+                                                         (1, 8, 1, 128, 300, 4096, 300),
+                                                         (2, 16, 4, 128, 65, 8192, 97),
+                                                         (2, 8, 2, 128, 180, 12288, 200)])
 def test_attention_over_long_caches(ops, b, hq, hkv, d, rows, sealed, tail):
     cache = _long(ops, b, hkv, d, 64, sealed, tail, rows)
     q = queries(b, hq, rows, d, rows)

@@ -77,7 +77,7 @@ def test_malformed_calls_are_refused():
     # Mass and selection.
     mass = lambda **k: N.lib.sf_kv8_attention_mass(k.get("q", 256), 0, 0, 128, k.get("heads", 8), 3, k.get("lse", 256),
                                                    addr(s), 256, 1, 0, k.get("prefix", 133), k.get("scale", 0.1),
-                                                   k.get("mass", 256), 0, 0, None)
+                                                   k.get("mass", 256), 0, 0, None, 0, None)
     for kw in (dict(heads=3), dict(prefix=200), dict(scale=0.0), dict(lse=None), dict(mass=None), dict(q=None)):
         assert mass(**kw) == N.SF_ERR_INVALID_ARGUMENT, kw
     keep = lambda length, budget, sinks, recent, m=256: N.lib.sf_kv_keep_heaviest(m, 0, 0, 1, 1, length, budget, sinks,
