@@ -72,7 +72,7 @@ struct Kv8Prep {
   float* qf;     // [bh][tiles * 128]: the power of two taken out of a query row; NaN for a row that holds one
   float* unit;   // [bh]: the largest V scale
   // For the mass (null otherwise):
-  float2* rowc;  // [bh][tiles * 128]: (that power times scale * log2(e), lse * log2(e))
+  float* rowc;   // [bh][tiles][2][128]: that power times scale * log2(e); -lse * log2(e)
   int tiles, blocks, first;
 };
 // Fills `w` (nullable) with places from `base` (16-byte aligned) on; returns the bytes.

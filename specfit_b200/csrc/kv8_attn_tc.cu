@@ -183,35 +183,16 @@ __device__ __forceinline__ float scaled_max(const float (&x)[16], float f) {
   a = fmaxf(a, d);
   return a == -INFINITY ? a : a * f;
 }
-// Two fp32 values in one register pair: products and sums of both at once.
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t x, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // 16 scores to probabilities 2^(f x - base), as fp16 pairs, and their sums.
 __device__ __forceinline__ void probabilities(const float (&x)[16], float f, float base, uint64_t (&ls)[2],
                                               uint32_t* pk) {
-  const uint64_t f2 = pack2(f, f), b2 = pack2(-base, -base);
+  const uint64_t f2 = ptx::pack2(f, f), b2 = ptx::pack2(-base, -base);
 #pragma unroll
   for (int j = 0; j < 16; j += 2) {
     float y0, y1;
-    unpack2(fma2(pack2(x[j], x[j + 1]), f2, b2), y0, y1);
+    ptx::unpack2(ptx::fma2(ptx::pack2(x[j], x[j + 1]), f2, b2), y0, y1);
     const float p0 = ex2(y0), p1 = ex2(y1);
-    ls[(j >> 1) & 1] = add2(ls[(j >> 1) & 1], pack2(p0, p1));
+    ls[(j >> 1) & 1] = ptx::add2(ls[(j >> 1) & 1], ptx::pack2(p0, p1));
     pk[j / 2] = pack_f16x2(p0, p1);
   }
 }
@@ -297,7 +278,9 @@ kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
             lse = p.lse[((int64_t)req * p.heads + kvh * p.group + h) * p.q_len + (pr - h * p.q_len)];
           }
           // Rows that see nothing, and those past the last, add 2^-infinity.
-          w.rowc[at] = make_float2(f * p.scale_log2, lse == -INFINITY ? INFINITY : lse * 1.4426950408889634f);
+          float* c = w.rowc + 2 * (at - u * 32 - row) + u * 32 + row;
+          c[0] = f * p.scale_log2;
+          c[kBM] = lse == -INFINITY ? lse : -lse * 1.4426950408889634f;
         }
       }
     }
@@ -736,8 +719,8 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
         if (ok) {
           ptx::tmem_st_32(scol, pk);  // over scores that have been read
           float l0, l1, l2, l3;
-          unpack2(ls[0], l0, l1);
-          unpack2(ls[1], l2, l3);
+          ptx::unpack2(ls[0], l0, l1);
+          ptx::unpack2(ls[1], l2, l3);
           l += (l0 + l1) + (l2 + l3);
           ptx::tmem_wait_st();
         }
@@ -896,7 +879,7 @@ size_t kv8_prep_layout(Kv8Prep* w, void* base, bool for_mass, int64_t heads, int
   r.k = take((size_t)heads * blocks * kTileBytes);
   r.kf = reinterpret_cast<float*>(take((size_t)heads * blocks * kKB * sizeof(float)));
   if (for_mass) {
-    r.rowc = reinterpret_cast<float2*>(take((size_t)heads * tiles * kBM * sizeof(float2)));
+    r.rowc = reinterpret_cast<float*>(take((size_t)heads * tiles * 2 * kBM * sizeof(float)));
   } else {
     r.v = take((size_t)heads * std::max<int64_t>(blocks, 1) * kTileBytes);  // not null: values are laid out
     r.qf = reinterpret_cast<float*>(take((size_t)heads * tiles * kBM * sizeof(float)));

@@ -11,10 +11,10 @@
 //     order; for each it takes the head's query tiles (images laid out by
 //     kv8_prep_kernel) one after the other.  Up to five tiles stay in shared
 //     memory while the head stays the same (a 65-row tree has five).
-//   * D[128 keys x 128 rows] goes to one of four TMEM buffers; two lanes of
-//     eight warps take them in turn, two threads a key, 64 rows each.
-//   * At a block's end the four partial sums of a key are added in one order,
-//     so the same inputs give the same bits.
+//   * D[128 keys x 128 rows] goes to one of four TMEM buffers; sixteen warps
+//     read it, four threads a key, 32 rows each.
+//   * At a block's end one warp adds the four partial sums of a key, in one
+//     order, so the same inputs give the same bits.
 // Every wait is bounded; a warp whose wait gave up skips the work but still
 // meets the others at the barriers.
 #include <cuda.h>
@@ -39,15 +39,16 @@ constexpr int kQStages = 5;
 constexpr int kKStages = 2;
 constexpr int kBufs = 4;              // of D
 constexpr int kSumWarps = 16;
-constexpr int kThreads = (kSumWarps + 2) * 32;
-constexpr int kMmaWarp = kSumWarps, kLoadWarp = kSumWarps + 1;
+constexpr int kThreads = (kSumWarps + 3) * 32;
+constexpr int kMmaWarp = kSumWarps, kLoadWarp = kSumWarps + 1, kAddWarp = kSumWarps + 2;
 
 struct __align__(16) Tail {
-  float2 rowc[kQStages][kBM];
-  float part[2][4][kKB];  // by block parity: lane and half's sums of a key
+  float rowc[kQStages][2][kBM];
+  float part[2][4][kKB];  // by block parity: a key's sums by quarters of the rows
   uint64_t q_full[kQStages], q_empty[kQStages];
   uint64_t k_full[kKStages], k_empty[kKStages], lo_full, lo_empty;
   uint64_t d_full[kBufs], d_empty[kBufs];
+  uint64_t part_full[2], part_empty[2];
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort_flag;
@@ -60,12 +61,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int site) {
-  int ok = 0;
-  if ((threadIdx.x & 31) == 0) ok = ptx::mbar_wait(bar, parity, abort_flag, &g_kv8_mass_status, site) ? 1 : 0;
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
-}
-
 __global__ void __launch_bounds__(kThreads, 1)
 kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep w, float* __restrict__ mass,
                    int64_t m_bs, int64_t m_hs, int nblocks, int per_cta) {
@@ -87,7 +82,7 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kQStages; ++s) {
       ptx::mbar_init(&tail->q_full[s], 1);
-      ptx::mbar_init(&tail->q_empty[s], 1 + kSumWarps / 2);  // the products, and the readers of the row constants
+      ptx::mbar_init(&tail->q_empty[s], 1 + kSumWarps);  // the products, and the readers of the row constants
     }
     for (int s = 0; s < kKStages; ++s) {
       ptx::mbar_init(&tail->k_full[s], 1);
@@ -97,7 +92,11 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
     ptx::mbar_init(&tail->lo_empty, 1);
     for (int s = 0; s < kBufs; ++s) {
       ptx::mbar_init(&tail->d_full[s], 1);
-      ptx::mbar_init(&tail->d_empty[s], kSumWarps / 2);
+      ptx::mbar_init(&tail->d_empty[s], kSumWarps);
+    }
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(&tail->part_full[s], kSumWarps);
+      ptx::mbar_init(&tail->part_empty[s], 1);
     }
     ptx::mbar_init(&tail->mma_done, 1);
     tail->abort_flag = 0;
@@ -146,7 +145,7 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
           ptx::mbar_arrive_expect_tx(&tail->q_full[s], kTileBytes + (uint32_t)sizeof(tail->rowc[0]));
           ptx::bulk_load(q_s + s * kTileBytes, w.q + ((int64_t)bh * w.tiles + i) * kTileBytes, kTileBytes,
                          &tail->q_full[s]);
-          ptx::bulk_load(tail->rowc[s], w.rowc + ((int64_t)bh * w.tiles + i) * kBM, sizeof(tail->rowc[0]),
+          ptx::bulk_load(tail->rowc[s], w.rowc + ((int64_t)bh * w.tiles + i) * 2 * kBM, sizeof(tail->rowc[0]),
                          &tail->q_full[s]);
         }
       }
@@ -204,78 +203,128 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       volatile int never = 0;
       ptx::mbar_wait(&tail->mma_done, 0, &never, &g_kv8_mass_status, 69);
     }
+  } else if (warp == kAddWarp) {
+    // ---------------- adds a block's sums to the mass, four keys a lane ----------------
+    bool ok = true;
+    for (int u = u0; u < u1; ++u) {
+      const int bh = u / nblocks, key = (u - bh * nblocks) * kKB + lane, nu = u - u0;
+      const int kvh = bh % p.c.hkv, req = bh / p.c.hkv;
+      float* const to = mass + req * m_bs + kvh * m_hs + key;
+      float before[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) before[j] = key + j * 32 < p.kv_len ? to[j * 32] : 0.f;
+      ok = ok && ptx::mbar_wait(&tail->part_full[nu & 1], (nu >> 1) & 1, abort_flag, &g_kv8_mass_status, 73);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const float(*x)[kKB] = tail->part[nu & 1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = lane + j * 32;
+        if (key + j * 32 < p.kv_len) to[j * 32] = before[j] + ((x[0][at] + x[1][at]) + (x[2][at] + x[3][at]));
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&tail->part_empty[nu & 1]);
+    }
   } else {
-    // ---------------- sums: a key's two threads of lane t ----------------
-    const int t = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
+    // ---------------- sums: a key's four threads, 32 rows of a tile each ----------------
+    const int part = warp >> 2, quad = warp & 3;
     const int key_in = quad * 32 + lane;
-    const uint32_t col = tmem + ((uint32_t)(quad * 32) << 16) + half * 64;
+    const uint32_t col = tmem + ((uint32_t)(quad * 32) << 16) + part * 32;
     const int packed = p.group * p.q_len;
     bool ok = true;
-    int n0 = 0, m = 0, parity = 0;
-    for (int u = u0; u < u1; ++u, parity ^= 1) {
-      const int bh = u / nblocks, blk = u - bh * nblocks, key0 = blk * kKB, key = key0 + key_in;
+    int m = 0, s0 = 0, qphase = 0;  // stage and phase of this block's first tile
+    // The key's scale is loaded a block ahead.
+    auto key_scale = [&](int u) {
+      const int bh = u / nblocks, key = (u - bh * nblocks) * kKB + key_in;
       const int kvh = bh % p.c.hkv, req = bh / p.c.hkv;
-      if (u != u0 && (blk == 0 || !resident)) n0 += w.tiles;
+      return (key - key_in) + kKB <= sealed ? p.c.ks[req * p.c.s_bs + kvh * p.c.s_hs + (key >> p.c.block_shift)]
+                                            : w.kf[(int64_t)bh * w.blocks * kKB + (key - w.first)];
+    };
+    float next_kf = u0 < u1 ? key_scale(u0) : 0.f;
+    for (int u = u0; u < u1; ++u) {
+      const int bh = u / nblocks, blk = u - bh * nblocks, key0 = blk * kKB;
+      const bool fresh = u == u0 || blk == 0 || !resident;  // tiles not seen yet
       const bool last = !resident || u + 1 == u1 || blk + 1 == nblocks;
       const bool full = key0 + kKB <= p.prefix;  // no mask to read
-      const float kf = key0 + kKB <= sealed
-                           ? p.c.ks[req * p.c.s_bs + kvh * p.c.s_hs + (key >> p.c.block_shift)]
-                           : w.kf[(int64_t)bh * w.blocks * kKB + (key - w.first)];
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      const float kf = next_kf;
+      if (u + 1 < u1) next_kf = key_scale(u + 1);
+      const uint64_t kf2 = ptx::pack2(kf, kf);
+      uint64_t acc[2] = {0, 0};
+      int s = s0, phase = qphase;
       for (int i = 0; i < w.tiles; ++i, ++m) {
-        if ((m & 1) != t) continue;
-        const int n = n0 + i, s = n % kQStages, buf = m % kBufs;
-        ok = ok && warp_wait(&tail->q_full[s], (n / kQStages) & 1, abort_flag, 70);
-        ok = ok && warp_wait(&tail->d_full[buf], (m / kBufs) & 1, abort_flag, 71);
-        if (ok) {
+        const int buf = m % kBufs;
+        const int row0 = i * kBM + part * 32;
+        uint32_t seen = 0;  // row row0 + lane: which of the warp's keys it sees
+        if (!full && row0 + lane < packed) {
+          const int h = (int)(((uint64_t)(row0 + lane) * p.q_magic) >> 40), row = row0 + lane - h * p.q_len;
+          const int req = bh / p.c.hkv;
+          seen = (uint32_t)kv8_window(p, p.bits ? p.bits + req * p.bits_bs + (int64_t)row * p.words : nullptr,
+                                      key0 + quad * 32);
+        }
+        if (fresh) ok = ok && ptx::mbar_wait(&tail->q_full[s], phase, abort_flag, &g_kv8_mass_status, 70);
+        ok = ok && ptx::mbar_wait(&tail->d_full[buf], (m / kBufs) & 1, abort_flag, &g_kv8_mass_status, 71);
+        ok = __all_sync(0xffffffffu, ok);
+        if (ok && row0 < packed) {
           ptx::tc_fence_after();
-          const float4* rc = reinterpret_cast<const float4*>(tail->rowc[s] + half * 64);  // two rows each
-          const int row0 = i * kBM + half * 64;
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float d[16];
-            ptx::tmem_ld_16(col + buf * kBM + c * 16, d);
+          uint32_t d[2][16];
+          ptx::tmem_ld_16_async(col + buf * kBM, d[0]);
+          ptx::tmem_wait_ld_16(d[0]);
+          ptx::tmem_ld_16_async(col + buf * kBM + 16, d[1]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float* f = tail->rowc[s][0] + part * 32 + c * 16;
+            const float* l = tail->rowc[s][1] + part * 32 + c * 16;
+            if (c == 1) {
+              ptx::tmem_wait_ld_16(d[1]);
+              ptx::tc_fence_before();
+              if (lane == 0) ptx::mbar_arrive(&tail->d_empty[buf]);
+            }
             if (full) {
 #pragma unroll
-              for (int j = 0; j < 16; j += 2) {
-                const float4 r = rc[c * 8 + j / 2];
-                acc[j & 2] += ex2(fmaf(d[j], r.x * kf, -r.y));
-                acc[(j & 2) + 1] += ex2(fmaf(d[j + 1], r.z * kf, -r.w));
+              for (int j = 0; j < 16; j += 4) {
+                const ulonglong2 ff = *reinterpret_cast<const ulonglong2*>(f + j);
+                const ulonglong2 ll = *reinterpret_cast<const ulonglong2*>(l + j);
+                const uint64_t y[2] = {ptx::fma2(ptx::pack2(__uint_as_float(d[c][j]), __uint_as_float(d[c][j + 1])),
+                                                 ptx::mul2(ff.x, kf2), ll.x),
+                                       ptx::fma2(ptx::pack2(__uint_as_float(d[c][j + 2]), __uint_as_float(d[c][j + 3])),
+                                                 ptx::mul2(ff.y, kf2), ll.y)};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                  float y0, y1;
+                  ptx::unpack2(y[x], y0, y1);
+                  acc[x] = ptx::add2(acc[x], ptx::pack2(ex2(y0), ex2(y1)));
+                }
               }
             } else {
-              // Visibility of this key for 16 rows, their words loaded together.
-              uint32_t word[16];
-              const int at = key - p.prefix;
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const int pr = row0 + c * 16 + j;
-                const int h = (int)(((uint64_t)pr * p.q_magic) >> 40), row = pr - h * p.q_len;
-                word[j] = 0;
-                if (pr < packed && key < p.kv_len)
-                  word[j] = at < 0 ? ~0u : (p.bits ? p.bits[req * p.bits_bs + (int64_t)row * p.words + (at >> 5)] : 0u);
-              }
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float2 r = tail->rowc[s][half * 64 + c * 16 + j];
-                if ((word[j] >> (at & 31)) & 1u) acc[j & 3] += ex2(fmaf(d[j], r.x * kf, -r.y));
+              for (int j = 0; j < 16; j += 2) {
+                const float2 ff = *reinterpret_cast<const float2*>(f + j), ll = *reinterpret_cast<const float2*>(l + j);
+                const uint32_t w0 = __shfl_sync(0xffffffffu, seen, c * 16 + j);
+                const uint32_t w1 = __shfl_sync(0xffffffffu, seen, c * 16 + j + 1);
+                const float y0 = fmaf(__uint_as_float(d[c][j]), ff.x * kf, ll.x);
+                const float y1 = fmaf(__uint_as_float(d[c][j + 1]), ff.y * kf, ll.y);
+                acc[(j >> 1) & 1] = ptx::add2(acc[(j >> 1) & 1], ptx::pack2((w0 >> lane) & 1u ? ex2(y0) : 0.f,
+                                                                           (w1 >> lane) & 1u ? ex2(y1) : 0.f));
               }
             }
           }
-          ptx::tc_fence_before();
-        }
-        __syncwarp();
-        if (lane == 0) {
+          __syncwarp();
+        } else if (lane == 0) {
           ptx::mbar_arrive(&tail->d_empty[buf]);
-          // The lane that summed a tile's last block is the last reader of its constants.
-          if (last) ptx::mbar_arrive(&tail->q_empty[s]);
         }
+        if (last && lane == 0) ptx::mbar_arrive(&tail->q_empty[s]);
+        if (++s == kQStages) s = 0, phase ^= 1;
       }
-      tail->part[parity][t * 2 + half][key_in] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-      ptx::named_bar_sync(1, kSumWarps * 32);
-      if (warp < 4 && ok && key < p.kv_len) {  // t = 0, half = 0: this thread's key
-        const float* x = tail->part[parity][0];
-        mass[req * m_bs + kvh * m_hs + key] += (x[key_in] + x[kKB + key_in]) + (x[2 * kKB + key_in] + x[3 * kKB + key_in]);
-      }
+      if (last) s0 = s, qphase = phase;
+      float a[4];
+      ptx::unpack2(acc[0], a[0], a[1]);
+      ptx::unpack2(acc[1], a[2], a[3]);
+      const int nu = u - u0;
+      ok = ok && ptx::mbar_wait(&tail->part_empty[nu & 1], ((nu >> 1) & 1) ^ 1, abort_flag, &g_kv8_mass_status, 72);
+      tail->part[nu & 1][part][key_in] = (a[0] + a[1]) + (a[2] + a[3]);
+      __syncwarp();
+      ok = __all_sync(0xffffffffu, ok);
+      if (lane == 0) ptx::mbar_arrive(&tail->part_full[nu & 1]);
     }
   }
 
