@@ -34,7 +34,7 @@ struct MassParams {
 
 // grid: (CTAs over the key tiles, batch * hkv).
 template <int DT>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, 4)
 kv8_mass_kernel(MassParams mp) {
   pdl_wait();
   pdl_trigger();
@@ -54,20 +54,41 @@ kv8_mass_kernel(MassParams mp) {
   float* mass = mp.mass + req * mp.m_bs + kvh * mp.m_hs;
   int staged = -1;
 
+  // What a tile reads, a tile ahead: the codes, their scale and the mass so far.
+  uint4 next[2][kChunks];
+  float next_scale = 1.f, next_mass[4];
+  auto load = [&](int tile) {
+    const int key0 = tile * kTileKeys + warp * kKeys;
+    if (key0 < sealed) {
+      next_scale = ksc[key0 >> p.c.block_shift];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+          const int byte = j * 64 + c * 16;
+          next[t][j] = make_uint4(0, 0, 0, 0);
+          if (byte < d) next[t][j] = *reinterpret_cast<const uint4*>(kc + (int64_t)(key0 + t * 8 + g) * d + byte);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int key = key0 + 2 * c + (k & 1) + (k >> 1) * 8;
+      next_mass[k] = g == 0 && key < p.kv_len ? mass[key] : 0.f;
+    }
+  };
+  if ((int)blockIdx.x < mp.tiles) load(blockIdx.x);
   for (int tile = blockIdx.x; tile < mp.tiles; tile += gridDim.x) {
     const int key0 = tile * kTileKeys + warp * kKeys;
     // This warp's keys as fp16 B fragments.
     uint32_t kf[2][kSteps][2];
     float kscale = 1.f;
     if (key0 < sealed) {
-      kscale = ksc[key0 >> p.c.block_shift];
+      kscale = next_scale;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
-          const int byte = j * 64 + c * 16;
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (byte < d) w = *reinterpret_cast<const uint4*>(kc + (int64_t)(key0 + t * 8 + g) * d + byte);
+          const uint4 w = next[t][j];
           const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -101,6 +122,11 @@ kv8_mass_kernel(MassParams mp) {
           kf[t][s][1] = pack_f16x2(bf_lo(x[t][s].y) * inv, bf_hi(x[t][s].y) * inv);
         }
     }
+
+    float before[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) before[k] = next_mass[k];
+    if (tile + (int)gridDim.x < mp.tiles) load(tile + gridDim.x);
 
     float acc[4] = {0.f, 0.f, 0.f, 0.f};  // keys 2c, 2c + 1, 8 + 2c, 9 + 2c
     for (int chunk = 0; chunk < chunks; ++chunk) {
@@ -139,6 +165,7 @@ kv8_mass_kernel(MassParams mp) {
         }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
+          if (chunk * kChunkRows + i * 16 + 8 * r >= packed) break;  // a lone token's group of 8 heads or fewer
           const int at = i * 16 + g + 8 * r, pr = chunk * kChunkRows + at;
           uint32_t vis = 15u;
           if (key0 + kKeys > p.prefix) {
@@ -150,7 +177,7 @@ kv8_mass_kernel(MassParams mp) {
           const float f = row_f[at] * kscale, lse = row_lse[at];  // rows past the last: lse +infinity
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if ((vis >> k) & 1u) acc[k] += exp2f(s[k >> 1][2 * r + (k & 1)] * f - lse);
+            if ((vis >> k) & 1u) acc[k] += ex2(s[k >> 1][2 * r + (k & 1)] * f - lse);
         }
       }
     }
@@ -162,7 +189,7 @@ kv8_mass_kernel(MassParams mp) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int key = key0 + 2 * c + (k & 1) + (k >> 1) * 8;
-        if (key < p.kv_len) mass[key] += acc[k];
+        if (key < p.kv_len) mass[key] = before[k] + acc[k];
       }
     }
   }
