@@ -146,8 +146,9 @@ __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bf
   }
 }
 
-// grid: (hkv, row tiles, splits * batch).  Full: D is DT.
-template <int DT, bool Full>
+// grid: (hkv, row tiles, splits * batch).  Full: D is DT.  Narrow: at most
+// eight query rows.
+template <int DT, bool Full, bool Narrow>
 __global__ void __launch_bounds__(kWarps * 32, 3)
 kv8_attn_kernel(Kv8Attn p) {
   using L = Layout<DT>;
@@ -206,29 +207,45 @@ kv8_attn_kernel(Kv8Attn p) {
   // Q fragments of rows g and g + 8: the dims of k-step (j, w) of this
   // thread are j * 64 + c * 16 + w * 4 + {0, 1, 2, 3}.  Every warp needs the same
   // ones: each writes a quarter of them.
+  // The rows whose scores this thread gets: g and g + 8, or 2c and 2c + 1.
+  auto row_of = [&](int r) { return Narrow ? 2 * c + r : g + 8 * r; };
   float qs[2];                 // scale * log2(e) * (power of two taken out of the row)
   const uint32_t* rbits[2];
   bool rok[2];
   {
     uint32_t qf[L::kSteps][4];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < (Narrow ? 1 : 2); ++r) {
       const int pr = blockIdx.y * kRows + g + r * 8;
+      const bool on = pr < packed;
+      const int qh = on ? (int)(((uint64_t)pr * p.q_magic) >> 40) : 0, t = on ? pr - qh * p.q_len : 0;
+      const __nv_bfloat16* qrow = p.q + req * p.q_bs + (int64_t)(kvh * p.group + qh) * p.q_hs + t * p.q_rs;
+      qs[r] = p.scale_log2 * q_row_fragments<L::kSteps>(on ? qrow : nullptr, d, c, qf, r);
+    }
+    if constexpr (Narrow) {
+      const float f = qs[0];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) qs[r] = __shfl_sync(0xffffffffu, f, (2 * c + r) * 4);
+#pragma unroll
+      for (int st = 0; st < L::kSteps; ++st) qf[st][1] = qf[st][3] = 0;
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int pr = blockIdx.y * kRows + row_of(r);
       rok[r] = pr < packed;
       const int qh = rok[r] ? (int)(((uint64_t)pr * p.q_magic) >> 40) : 0, t = rok[r] ? pr - qh * p.q_len : 0;
       rbits[r] = p.bits ? p.bits + req * p.bits_bs + (int64_t)t * p.words : nullptr;
-      const __nv_bfloat16* qrow = p.q + req * p.q_bs + (int64_t)(kvh * p.group + qh) * p.q_hs + t * p.q_rs;
-      qs[r] = p.scale_log2 * q_row_fragments<L::kSteps>(rok[r] ? qrow : nullptr, d, c, qf, r);
     }
 #pragma unroll
     for (int st = 0; st < L::kSteps; ++st)
-      if ((st & (kWarps - 1)) == warp) q_frag[st][lane] = make_uint4(qf[st][0], qf[st][1], qf[st][2], qf[st][3]);
+      if ((st & (kWarps - 1)) == warp) q_frag[st][lane] = make_uint4(qf[st][0], qf[st][2], qf[st][1], qf[st][3]);
     __syncthreads();
   }
 
-  float o[L::kTiles][4];
+  constexpr int kOTiles = Narrow ? L::kTiles / 2 : L::kTiles;
+  float o[kOTiles][4];
 #pragma unroll
-  for (int t = 0; t < L::kTiles; ++t)
+  for (int t = 0; t < kOTiles; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[t][i] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -245,10 +262,11 @@ kv8_attn_kernel(Kv8Attn p) {
     const uint8_t* at = smem + (size_t)warp * kStages * L::kUnitBytes + (size_t)stage * L::kUnitBytes;
     if (++stage == kStages) stage = 0;
 
-    constexpr int kX = 4 * kHalves;  // this thread's keys of a row
-    float s[2 * kHalves][4];
+    constexpr int kX = (Narrow ? 2 : 4) * kHalves;  // this thread's keys of a row
+    constexpr int kSTiles = (Narrow ? 1 : 2) * kHalves;
+    float s[kSTiles][4];
 #pragma unroll
-    for (int t = 0; t < 2 * kHalves; ++t)
+    for (int t = 0; t < kSTiles; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
     float kscale, vscale;
@@ -274,11 +292,21 @@ kv8_attn_kernel(Kv8Attn p) {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint4 qv = q_frag[j * 4 + i][lane];
-          const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
+          if constexpr (Narrow) {
+            const uint2 qv = *reinterpret_cast<const uint2*>(&q_frag[j * 4 + i][lane]);
 #pragma unroll
-          for (int t = 0; t < 2 * kHalves; ++t)
-            mma_f16(s[t], qa, e4m3x2_to_f16x2(w[t][i]), e4m3x2_hi_to_f16x2(w[t][i]));
+            for (int h = 0; h < kHalves; ++h) {
+              const uint32_t ka[4] = {e4m3x2_to_f16x2(w[2 * h][i]), e4m3x2_to_f16x2(w[2 * h + 1][i]),
+                                      e4m3x2_hi_to_f16x2(w[2 * h][i]), e4m3x2_hi_to_f16x2(w[2 * h + 1][i])};
+              mma_f16(s[h], ka, qv.x, qv.y);
+            }
+          } else {
+            const uint4 qv = q_frag[j * 4 + i][lane];
+            const uint32_t qa[4] = {qv.x, qv.z, qv.y, qv.w};
+#pragma unroll
+            for (int t = 0; t < 2 * kHalves; ++t)
+              mma_f16(s[t], qa, e4m3x2_to_f16x2(w[t][i]), e4m3x2_hi_to_f16x2(w[t][i]));
+          }
         }
       }
     } else {
@@ -286,16 +314,31 @@ kv8_attn_kernel(Kv8Attn p) {
 #pragma unroll
       for (int st = 0; st < L::kSteps; ++st) {
         const uint4 qv = q_frag[st][lane];
-        const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
+        uint2 b[2 * kHalves];
 #pragma unroll
-        for (int t = 0; t < 2 * kHalves; ++t) {
-          const uint2 b = tail_s[(t * L::kSteps + st) * 32 + lane];
-          mma_f16(s[t], qa, b.x, b.y);
+        for (int t = 0; t < 2 * kHalves; ++t) b[t] = tail_s[(t * L::kSteps + st) * 32 + lane];
+        if constexpr (Narrow) {
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            const uint32_t ka[4] = {b[2 * h].x, b[2 * h + 1].x, b[2 * h].y, b[2 * h + 1].y};
+            mma_f16(s[h], ka, qv.x, qv.y);
+          }
+        } else {
+          const uint32_t qa[4] = {qv.x, qv.z, qv.y, qv.w};
+#pragma unroll
+          for (int t = 0; t < 2 * kHalves; ++t) mma_f16(s[t], qa, b[t].x, b[t].y);
         }
+      }
+      // Bit i: this thread's key i (narrow: key g of key tile i, found by the quad's lane g / 2).
+      if constexpr (Narrow) {
+        const uint32_t w = __shfl_sync(0xffffffffu, bad, (lane & 28) | (g >> 1)) >> (g & 1);
+        bad = 0;
+#pragma unroll
+        for (int i = 0; i < kX; ++i) bad |= ((w >> (2 * i)) & 1u) << i;
       }
     }
 
-    // Scores in base 2, those not seen -infinity: keys 2c, 2c + 1 of each key tile.
+    // Scores in base 2, those not seen -infinity: keys 2c, 2c + 1 (narrow: g) of each key tile.
     float x[2][kX], mx[2];
     const bool open = key0 + kUnit <= p.prefix;  // no mask to read (prefix_len <= kv_len)
     bool grow = false;
@@ -303,7 +346,7 @@ kv8_attn_kernel(Kv8Attn p) {
     for (int r = 0; r < 2; ++r) {
       const float f = qs[r] * kscale;
 #pragma unroll
-      for (int i = 0; i < kX; ++i) x[r][i] = s[i >> 1][2 * r + (i & 1)] * f;
+      for (int i = 0; i < kX; ++i) x[r][i] = s[i >> 1][Narrow ? 2 * (i & 1) + r : 2 * r + (i & 1)] * f;
     }
     if (!open || bad) {
 #pragma unroll
@@ -312,7 +355,7 @@ kv8_attn_kernel(Kv8Attn p) {
 #pragma unroll
         for (int i = 0; i < kX; ++i) {
           if ((bad >> i) & 1u) x[r][i] = __int_as_float(0x7fc00000);
-          if (!((w >> ((i >> 1) * 8 + 2 * c + (i & 1))) & 1u)) x[r][i] = -INFINITY;
+          if (!((w >> (Narrow ? i * 8 + g : (i >> 1) * 8 + 2 * c + (i & 1))) & 1u)) x[r][i] = -INFINITY;
         }
       }
     }
@@ -330,8 +373,9 @@ kv8_attn_kernel(Kv8Attn p) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float y = fmaxf(m[r], mx[r]);
-        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
-        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+#pragma unroll
+        for (int off = Narrow ? 4 : 1; off < (Narrow ? 32 : 4); off <<= 1)  // the threads of a row
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, off));
         corr[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - y);
         m[r] = y;
         l[r] *= corr[r];
@@ -351,14 +395,25 @@ kv8_attn_kernel(Kv8Attn p) {
     }
     if (rescale) {
 #pragma unroll
-      for (int t = 0; t < L::kTiles; ++t) {
+      for (int t = 0; t < kOTiles; ++t) {
         o[t][0] *= corr[0];
-        o[t][1] *= corr[0];
-        o[t][2] *= corr[1];
+        o[t][1] *= corr[Narrow ? 1 : 0];
+        o[t][2] *= corr[Narrow ? 0 : 1];
         o[t][3] *= corr[1];
       }
     }
     uint32_t pa[kHalves][4];
+    if constexpr (Narrow) {
+      const float base0 = (m[0] == -INFINITY ? 0.f : m[0]) - kPShift, base1 = (m[1] == -INFINITY ? 0.f : m[1]) - kPShift;
+#pragma unroll
+      for (int i = 0; i < kX; ++i) {
+        const float e0 = ex2(x[0][i] - base0), e1 = ex2(x[1][i] - base1);
+        l[0] += e0;
+        l[1] += e1;
+        // Key g, rows 2c and 2c + 1; turned: keys 2c and 2c + 1, row g.
+        pa[i >> 1][i & 1] = transpose_8x8(pack_f16x2(e0 * pf, e1 * pf));
+      }
+    } else {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float base = (m[r] == -INFINITY ? 0.f : m[r]) - kPShift;
@@ -368,6 +423,7 @@ kv8_attn_kernel(Kv8Attn p) {
         l[r] += e0 + e1;
         pa[i >> 2][r + (i & 2)] = pack_f16x2(e0 * pf, e1 * pf);
       }
+    }
     }
 
     // Output tile t, column g: dim g * kVBytes + t.
@@ -394,16 +450,32 @@ kv8_attn_kernel(Kv8Attn p) {
         for (int w = 0; w < L::kVBytes / 4; ++w) {
           const uint32_t a01 = __byte_perm(vf[0][w], vf[1][w], 0x5140), a23 = __byte_perm(vf[0][w], vf[1][w], 0x7362);
           const uint32_t b01 = __byte_perm(vf[2][w], vf[3][w], 0x5140), b23 = __byte_perm(vf[2][w], vf[3][w], 0x7362);
-          mma_f16(o[4 * w + 0], pa[h], e4m3x2_to_f16x2(a01), e4m3x2_to_f16x2(b01));
-          mma_f16(o[4 * w + 1], pa[h], e4m3x2_hi_to_f16x2(a01), e4m3x2_hi_to_f16x2(b01));
-          mma_f16(o[4 * w + 2], pa[h], e4m3x2_to_f16x2(a23), e4m3x2_to_f16x2(b23));
-          mma_f16(o[4 * w + 3], pa[h], e4m3x2_hi_to_f16x2(a23), e4m3x2_hi_to_f16x2(b23));
+          if constexpr (Narrow) {  // two output tiles are the 16 rows of an MMA
+            const uint32_t v0[4] = {e4m3x2_to_f16x2(a01), e4m3x2_hi_to_f16x2(a01), e4m3x2_to_f16x2(b01),
+                                    e4m3x2_hi_to_f16x2(b01)};
+            const uint32_t v1[4] = {e4m3x2_to_f16x2(a23), e4m3x2_hi_to_f16x2(a23), e4m3x2_to_f16x2(b23),
+                                    e4m3x2_hi_to_f16x2(b23)};
+            mma_f16(o[2 * w + 0], v0, pa[h][0], pa[h][1]);
+            mma_f16(o[2 * w + 1], v1, pa[h][0], pa[h][1]);
+          } else {
+            mma_f16(o[4 * w + 0], pa[h], e4m3x2_to_f16x2(a01), e4m3x2_to_f16x2(b01));
+            mma_f16(o[4 * w + 1], pa[h], e4m3x2_hi_to_f16x2(a01), e4m3x2_hi_to_f16x2(b01));
+            mma_f16(o[4 * w + 2], pa[h], e4m3x2_to_f16x2(a23), e4m3x2_to_f16x2(b23));
+            mma_f16(o[4 * w + 3], pa[h], e4m3x2_hi_to_f16x2(a23), e4m3x2_hi_to_f16x2(b23));
+          }
         }
       } else {
 #pragma unroll
-        for (int t = 0; t < L::kTiles; ++t) {
-          const uint2 b = tail_s[(2 * kHalves * L::kSteps + h * L::kTiles + t) * 32 + lane];
-          mma_f16(o[t], pa[h], b.x, b.y);
+        for (int t = 0; t < L::kTiles; t += 2) {
+          const uint2* at_t = tail_s + (2 * kHalves * L::kSteps + h * L::kTiles + t) * 32 + lane;
+          const uint2 b = at_t[0], e = at_t[32];
+          if constexpr (Narrow) {
+            const uint32_t v[4] = {b.x, e.x, b.y, e.y};
+            mma_f16(o[t / 2], v, pa[h][0], pa[h][1]);
+          } else {
+            mma_f16(o[t], pa[h], b.x, b.y);
+            mma_f16(o[t + 1], pa[h], e.x, e.y);
+          }
         }
       }
     }
@@ -414,11 +486,11 @@ kv8_attn_kernel(Kv8Attn p) {
   // partial outputs through shared memory (the ring's space).
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    if (c == 0) {
-      join_m[warp][g + 8 * r] = m[r];
-      join_l[warp][g + 8 * r] = l[r];
+#pragma unroll
+    for (int off = Narrow ? 4 : 1; off < (Narrow ? 32 : 4); off <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], off);
+    if (Narrow ? g == 0 : c == 0) {
+      join_m[warp][row_of(r)] = m[r];
+      join_l[warp][row_of(r)] = l[r];
     }
   }
   __syncthreads();  // every warp is done with the ring
@@ -426,16 +498,18 @@ kv8_attn_kernel(Kv8Attn p) {
 #pragma unroll
   for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int t = 0; t < L::kTiles; ++t)
+    for (int t = 0; t < kOTiles; ++t)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        // column 2c + i of tile t: dim (2c + i) * kVBytes + t
-        const float y = o[t][2 * r + i];
-        po[(g + 8 * r) * DT + (2 * c + i) * L::kVBytes + t] = unit > 0.f ? y * unit : y;
+        // Column 2c + i of tile t: dim (2c + i) * kVBytes + t.  Narrow: row g + 8i of
+        // tile t: dim g * kVBytes + 2t + i.
+        const float y = o[t][Narrow ? 2 * i + r : 2 * r + i];
+        po[row_of(r) * DT + (Narrow ? g * L::kVBytes + 2 * t + i : (2 * c + i) * L::kVBytes + t)] =
+            unit > 0.f ? y * unit : y;
       }
   __syncthreads();
   constexpr int kPerRow = DT / 4;
-  for (int i = threadIdx.x; i < kRows * kPerRow; i += kWarps * 32) {
+  for (int i = threadIdx.x; i < (Narrow ? 8 : kRows) * kPerRow; i += kWarps * 32) {
     const int row = i / kPerRow, col = (i % kPerRow) * 4;
     const int pr = blockIdx.y * kRows + row;
     if (pr >= packed || col >= d) continue;
@@ -564,11 +638,11 @@ int launch_merge(const Kv8Attn& p, cudaStream_t stream) {
   return SF_OK;
 }
 
-template <int DT, bool Full>
+template <int DT, bool Full, bool Narrow>
 int launch_mma(const Kv8Attn& p, cudaStream_t stream) {
   static std::atomic<unsigned long long> configured{0};
   if (int rc = once_per_device(configured, [] {
-        SF_CHECK_CUDA(cudaFuncSetAttribute(kv8_attn_kernel<DT, Full>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        SF_CHECK_CUDA(cudaFuncSetAttribute(kv8_attn_kernel<DT, Full, Narrow>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            Layout<DT>::kSmem));
         return SF_OK;
       }))
@@ -576,9 +650,15 @@ int launch_mma(const Kv8Attn& p, cudaStream_t stream) {
   const int64_t tiles = ((int64_t)p.group * p.q_len + kRows - 1) / kRows;
   SF_CHECK_ARG(tiles < 65536 && (int64_t)p.splits * p.batch < 65536, "too many query rows or requests");
   const dim3 grid((unsigned)p.c.hkv, (unsigned)tiles, (unsigned)(p.splits * p.batch));
-  SF_CHECK_CUDA(launch_pdl(kv8_attn_kernel<DT, Full>, grid, dim3(kWarps * 32), Layout<DT>::kSmem, stream, p));
+  SF_CHECK_CUDA(launch_pdl(kv8_attn_kernel<DT, Full, Narrow>, grid, dim3(kWarps * 32), Layout<DT>::kSmem, stream, p));
   SF_CHECK_LAUNCH();
   return SF_OK;
+}
+
+template <int DT, bool Full>
+int launch_rows(const Kv8Attn& p, cudaStream_t stream) {
+  return (int64_t)p.group * p.q_len <= 8 ? launch_mma<DT, Full, true>(p, stream)
+                                         : launch_mma<DT, Full, false>(p, stream);
 }
 
 size_t partial_bytes(const Kv8Split& s, int batch, int heads, int head_dim, int64_t q_len) {
@@ -679,10 +759,10 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
                                  (partial_bytes(s, rows->batch, num_heads, rows->head_dim, q_len) + 15) / 16 * 16,
                           st);
   else
-    rc = rows->head_dim == 128  ? launch_mma<128, true>(p, st)
-         : rows->head_dim > 64  ? launch_mma<128, false>(p, st)
-         : rows->head_dim == 64 ? launch_mma<64, true>(p, st)
-                                : launch_mma<64, false>(p, st);
+    rc = rows->head_dim == 128  ? launch_rows<128, true>(p, st)
+         : rows->head_dim > 64  ? launch_rows<128, false>(p, st)
+         : rows->head_dim == 64 ? launch_rows<64, true>(p, st)
+                                : launch_rows<64, false>(p, st);
   if (rc || s.splits == 1) return rc;
   // One warp a row walks 16 ranges as fast as four join them (65 rows, 12 ranges: 5.7 and 9.1 us).
   return s.splits <= 16 ? launch_merge<1>(p, st) : (s.splits <= 32 ? launch_merge<4>(p, st) : launch_merge<8>(p, st));

@@ -299,7 +299,7 @@ kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
   for (int i = threadIdx.x; values && i < sealed >> p.c.block_shift; i += 256)
     unit = fmaxf(unit, vsc[i]);  // NaN is passed over
   uint32_t top = 0;
-#pragma unroll 8
+#pragma unroll 16
   for (int i = threadIdx.x; values && i < tail_rows * (kD / 8); i += 256) {
     const uint4 x = *reinterpret_cast<const uint4*>(vt + (int64_t)i * 8);
     const uint32_t in[4] = {x.x, x.y, x.z, x.w};

@@ -189,6 +189,10 @@ ATTENTION = [
     (1, 8, 2, 128, 64, 192, 200, 150, "causal"),
     (1, 8, 1, 128, 64, 0, 300, 257, "causal"),
     (1, 16, 1, 128, 32, 2080, 17, 16, "any"),
+    # At most eight query rows for a KV head.
+    (2, 4, 2, 112, 32, 288, 45, 4, "any"),
+    (1, 3, 1, 64, 64, 640, 70, 2, "tree"),
+    (2, 7, 7, 128, 128, 512, 33, 7, "causal"),
     # No tail, and codes that end inside a block of 128 keys.
     (2, 16, 2, 128, 32, 96, 0, 65, "any"),
     (1, 8, 1, 128, 64, 704, 0, 130, "any"),
@@ -254,11 +258,11 @@ def test_attention_over_long_caches(ops, b, hq, hkv, d, rows, sealed, tail):
     assert abs(float(mass.double().sum()) / (b * hq * rows) - 1) < 1e-4
 
 
-@pytest.mark.parametrize("rows", [2, 70])
-def test_masked_garbage_stays_out(ops, rows):
+@pytest.mark.parametrize("rows,hq", [(2, 8), (70, 8), (8, 1)])
+def test_masked_garbage_stays_out(ops, rows, hq):
     """NaN and infinities in keys and values that a row does not see change
     nothing for it; rows that see them answer NaN."""
-    b, hq, hkv, d, block, sealed, tail = 1, 8, 1, 128, 64, 256, 96
+    b, hkv, d, block, sealed, tail = 1, 1, 128, 64, 256, 96
     cache = make_rows(ops, b, hkv, d, block, sealed, tail, 5)
     k, v = opened(cache)
     cache.k_scale[0, 0, 1] = math.nan       # a sealed block that held a NaN key
