@@ -76,7 +76,7 @@ constexpr int kThreads = (kLoadWarp + 1) * 32;
 constexpr int kMaxRanges = 64;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
-constexpr float kSlack = 8.f;
+constexpr float kMaxSum = 0x1p15f; // of a row's 64 probabilities of a block, before the reference moves
 constexpr float kPShift = 7.f;  // probabilities are kept times 2^7
 
 struct __align__(16) Tail {
@@ -664,64 +664,77 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
         const bool plain = full && key0 + 64 <= (int)p.c.sealed;
         const float* kf = tail->kf[b & 3] + half * 64;
         uint32_t pk[32];  // 64 probabilities
-        uint64_t ls[2];
-        // Once under the reference maximum as it is; if a score of the row (in
-        // either half) is too far above it, once more under a new one.  The
-        // scores are read from TMEM, which the MMAs keep busy, only once in
-        // the first case, and stay there until the probabilities are settled.
+        // Once under the reference maximum as it is.  If the sum of a row's 64
+        // probabilities (in either half) passes 2^15, one of them may be too
+        // large for fp16: then (and for the first block) the maximum is found, and
+        // they are taken under it.  (A maximum in every pass was 36 of 230
+        // instructions.)  The scores stay in TMEM until the probabilities are
+        // settled.
+        if (ok) ptx::tc_fence_after();
 #pragma unroll 1
-        for (int pass = 0; pass < 2; ++pass) {
+        for (int pass = i == 0 ? 1 : 0;; ++pass) {
+          if (pass) {
+            float mx = -INFINITY;
+            if (ok) {
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                float sc[16];
+                ptx::tmem_ld_16(scol + c * 16, sc);
+                mx = fmaxf(mx, plain ? scaled_max(sc, kf[(c >> 1) * 32] * qf)
+                                     : masked_scores(sc, kf + c * 16, qf, (uint32_t)(win >> (c * 16))));
+              }
+            }
+            // The other half's maximum, and whether its wait succeeded: both warps
+            // of the pair go on or stop together.
+            tail->red[t][half][r] = mx;
+            if (lane == 0) tail->pair_ok[warp] = ok ? 1 : 0;
+            ptx::named_bar_sync(pair_bar, 64);
+            if (!tail->pair_ok[warp] || !tail->pair_ok[warp ^ 4]) {
+              ok = false;
+              break;
+            }
+            const float mnew = fmaxf(m, fmaxf(mx, tail->red[t][half ^ 1][r]));
+            const float alpha = m == -INFINITY ? 1.f : ex2(m - mnew);  // nothing summed yet: O and l are 0
+            m = mnew;
+            l *= alpha;
+            if (i > 0) {  // P V of the block before is complete, as its successor's scores are
+#pragma unroll 1
+              for (int c = 0; c < 4; ++c) {
+                float ov[16];
+                ptx::tmem_ld_16(ocol + c * 16, ov);
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(ov[j] * alpha);
+                ptx::tmem_st_16(ocol + c * 16, w);
+              }
+            }
+          }
           const float base = (m == -INFINITY ? 0.f : m) - kPShift;
-          float mx = -INFINITY;
-          ls[0] = ls[1] = 0;
+          float sum = 0.f;
           if (ok) {
-            if (pass == 0) ptx::tc_fence_after();
+            uint64_t ls[2] = {0, 0};
 #pragma unroll
             for (int c = 0; c < 4; ++c) {  // 16 at a time: nothing is spilled
               float sc[16];
               ptx::tmem_ld_16(scol + c * 16, sc);
               float f = 1.f;
-              if (plain) {
+              if (plain)
                 f = kf[(c >> 1) * 32] * qf;
-                mx = fmaxf(mx, scaled_max(sc, f));
-              } else {
-                mx = fmaxf(mx, masked_scores(sc, kf + c * 16, qf, (uint32_t)(win >> (c * 16))));
-              }
+              else
+                masked_scores(sc, kf + c * 16, qf, (uint32_t)(win >> (c * 16)));
               probabilities(sc, f, base, ls, pk + c * 8);
             }
+            float s0, s1;
+            ptx::unpack2(ptx::add2(ls[0], ls[1]), s0, s1);
+            sum = s0 + s1;
           }
-          if (pass || !pair_any(pair_bar, !ok || mx > m + kSlack || (m == -INFINITY && mx > -INFINITY))) break;
-          // The other half's maximum, and whether its wait succeeded: both warps
-          // of the pair go on or stop together.
-          tail->red[t][half][r] = mx;
-          if (lane == 0) tail->pair_ok[warp] = ok ? 1 : 0;
-          ptx::named_bar_sync(pair_bar, 64);
-          if (!tail->pair_ok[warp] || !tail->pair_ok[warp ^ 4]) {
-            ok = false;
+          if (pass || !pair_any(pair_bar, !ok || !(sum <= kMaxSum) || (m == -INFINITY && rok))) {
+            l += sum;
             break;
-          }
-          const float mnew = fmaxf(m, fmaxf(mx, tail->red[t][half ^ 1][r]));
-          const float alpha = m == -INFINITY ? 1.f : ex2(m - mnew);  // nothing summed yet: O and l are 0
-          m = mnew;
-          l *= alpha;
-          if (i > 0) {  // P V of the block before is complete, as its successor's scores are
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              float ov[16];
-              ptx::tmem_ld_16(ocol + c * 16, ov);
-              uint32_t w[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(ov[j] * alpha);
-              ptx::tmem_st_16(ocol + c * 16, w);
-            }
           }
         }
         if (ok) {
           ptx::tmem_st_32(scol, pk);  // over scores that have been read
-          float l0, l1, l2, l3;
-          ptx::unpack2(ls[0], l0, l1);
-          ptx::unpack2(ls[1], l2, l3);
-          l += (l0 + l1) + (l2 + l3);
           ptx::tmem_wait_st();
         }
       }
