@@ -16,10 +16,15 @@
 //     Nothing in the loop waits for another warp.
 //   * Dims of a key are a sum, keys of a value too, so both may be taken in
 //     any order: a thread's 16 consecutive code bytes ARE its MMA fragments
-//     (K: four k-steps of one key; V: one column of 16 output tiles).  Each
-//     thread copies exactly the bytes that it will use (cp.async, 16 bytes)
-//     into its own slots of a ring, so the loop needs no barrier, no
-//     transpose and no bank is hit twice.
+//     (K: four k-steps of one key; V: one column of 16 output tiles), so the
+//     loop needs no transpose.  A warp copies its units into its own ring
+//     (cp.async), 512 consecutive bytes an instruction: with each thread copying
+//     the bytes that it uses itself, eight rows of 64 bytes an instruction, 131,072
+//     tokens took 33 us instead of 30.
+//   * At most eight query rows (a token of a group of eight heads): keys, then
+//     dims, are the MMA's 16 rows and the query rows its 8 columns, half the MMAs
+//     and exponentials of the other way round (38 to 33 us).  Probabilities turn
+//     from key rows to query-row columns by 8 x 8 transposes in registers.
 //   * Codes become fp16 (exact) by one conversion per two; Q as fp16 is exact
 //     too once each row is scaled by a power of two (fp16's 11 bits hold
 //     bf16's 8 over 30 binades below the row's largest; what is smaller is
@@ -175,26 +180,31 @@ kv8_attn_kernel(Kv8Attn p) {
   const __nv_bfloat16* kt = p.c.kt + req * p.c.t_bs + kvh * p.c.t_hs;
   const __nv_bfloat16* vt = p.c.vt + req * p.c.t_bs + kvh * p.c.t_hs;
 
-  // Slots: [warp][stage][piece][lane], 16 (or 8) bytes each, written and read by one thread.
+  // A warp's ring: [stage][K: 32 keys x DT bytes][V]; a row's 16-byte chunks in
+  // an order of its own (k_chunk, v_chunk) that spreads what 8 lanes read at once
+  // over the banks.
   const uint32_t ring = smem_addr(smem) + (uint32_t)warp * kStages * L::kUnitBytes;
+  auto k_chunk = [](int row, int chunk) { return DT == 128 ? chunk ^ ((row & 1) << 2) : chunk; };
+  auto v_chunk = [](int row, int chunk) {
+    return DT == 128 ? chunk ^ (((row >> 1) & 3) << 1) : chunk ^ (((row >> 1) & 1) << 1);
+  };
   auto load_unit = [&](int key0, int stage) {
     if (key0 < key_hi && key0 < sealed) {
-      const uint32_t at = ring + (uint32_t)stage * L::kUnitBytes + (uint32_t)lane * 16;
-      const uint8_t* kp = kc + (int64_t)(key0 + g) * d + c * 16;
+      constexpr int kChunksRow = DT / 16, kRowsAt = 32 / kChunksRow;  // a copy's rows: consecutive bytes
+      const int row = lane / kChunksRow, chunk = lane % kChunksRow;
+      const bool on = Full || chunk * 16 < d;
+      const uint32_t at = ring + (uint32_t)stage * L::kUnitBytes;
+      const int64_t from = (int64_t)(key0 + row) * d + (on ? chunk * 16 : 0);
 #pragma unroll
-      for (int t = 0; t < 2 * kHalves; ++t)
+      for (int i = 0; i < kUnit / kRowsAt; ++i) {
+        const int r = i * kRowsAt + row;
+        cp_async<16>(at + (uint32_t)(r * DT + k_chunk(r, chunk) * 16), kc + from + i * kRowsAt * d, on);
+      }
 #pragma unroll
-        for (int j = 0; j < L::kKChunks; ++j) {
-          const bool on = Full || j * 64 + c * 16 < d;
-          cp_async<16>(at + (uint32_t)((t * L::kKChunks + j) * 512), on ? kp + t * 8 * d + j * 64 : kc, on);
-        }
-      const uint32_t vat = ring + (uint32_t)stage * L::kUnitBytes + 32 * L::kKBytes + (uint32_t)lane * L::kVBytes;
-      const bool on = Full || g * L::kVBytes < d;
-      const uint8_t* vp = vc + (int64_t)(key0 + 2 * c) * d + (on ? g * L::kVBytes : 0);
-#pragma unroll
-      for (int k = 0; k < L::kVKeys; ++k)
-        cp_async<L::kVBytes>(vat + (uint32_t)(k * 32 * L::kVBytes),
-                             vp + ((k >> 2) * 16 + (k & 1) + ((k >> 1) & 1) * 8) * d, on);
+      for (int i = 0; i < kUnit / kRowsAt; ++i) {
+        const int r = i * kRowsAt + row;
+        cp_async<16>(at + (uint32_t)(kUnit * DT + r * DT + v_chunk(r, chunk) * 16), vc + from + i * kRowsAt * d, on);
+      }
     }
     cp_commit();
   };
@@ -256,9 +266,11 @@ kv8_attn_kernel(Kv8Attn p) {
     {
       int ahead = stage + kStages - 1;
       if (ahead >= kStages) ahead -= kStages;
+      __syncwarp();  // every lane has read the unit before
       load_unit(key0 + (kStages - 1) * kStep, ahead);
     }
-    cp_wait<kStages - 1>();  // this thread's pieces of this unit have landed
+    cp_wait<kStages - 1>();  // this lane's pieces of this unit have landed,
+    __syncwarp();            // and the other lanes'
     const uint8_t* at = smem + (size_t)warp * kStages * L::kUnitBytes + (size_t)stage * L::kUnitBytes;
     if (++stage == kStages) stage = 0;
 
@@ -284,7 +296,7 @@ kv8_attn_kernel(Kv8Attn p) {
         uint32_t w[2 * kHalves][4];
 #pragma unroll
         for (int t = 0; t < 2 * kHalves; ++t) {
-          const uint4 x = *reinterpret_cast<const uint4*>(at + ((t * L::kKChunks + j) * 32 + lane) * 16);
+          const uint4 x = *reinterpret_cast<const uint4*>(at + (t * 8 + g) * DT + k_chunk(g, j * 4 + c) * 16);
           w[t][0] = x.x;
           w[t][1] = x.y;
           w[t][2] = x.z;
@@ -433,7 +445,8 @@ kv8_attn_kernel(Kv8Attn p) {
         uint32_t vf[4][L::kVBytes / 4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint8_t* a = at + 32 * L::kKBytes + ((h * 4 + k) * 32 + lane) * L::kVBytes;
+          const int row = h * 16 + 2 * c + (k & 1) + (k >> 1) * 8, byte = g * L::kVBytes;
+          const uint8_t* a = at + kUnit * DT + row * DT + v_chunk(row, byte >> 4) * 16 + (byte & 15);
           if constexpr (L::kVBytes == 16) {
             const uint4 w = *reinterpret_cast<const uint4*>(a);
             vf[k][0] = w.x;
