@@ -11,8 +11,8 @@
 //     order; for each it takes the head's query tiles (images laid out by
 //     kv8_prep_kernel) one after the other.  Up to five tiles stay in shared
 //     memory while the head stays the same (a 65-row tree has five).
-//   * D[128 keys x 128 rows] goes to one of four TMEM buffers; sixteen warps
-//     read it, four threads a key, 32 rows each.
+//   * D[128 keys x 128 rows] goes to one of four TMEM buffers; two lanes of
+//     eight warps take them in turn, two threads a key, 64 rows each.
 //   * At a block's end one warp adds the four partial sums of a key, in one
 //     order, so the same inputs give the same bits.
 // Every wait is bounded; a warp whose wait gave up skips the work but still
@@ -44,7 +44,7 @@ constexpr int kMmaWarp = kSumWarps, kLoadWarp = kSumWarps + 1, kAddWarp = kSumWa
 
 struct __align__(16) Tail {
   float rowc[kQStages][2][kBM];
-  float part[2][4][kKB];  // by block parity: a key's sums by quarters of the rows
+  float part[2][4][kKB];  // by block parity: a key's sums, by lane and half of a tile's rows
   uint64_t q_full[kQStages], q_empty[kQStages];
   uint64_t k_full[kKStages], k_empty[kKStages], lo_full, lo_empty;
   uint64_t d_full[kBufs], d_empty[kBufs];
@@ -92,7 +92,7 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
     ptx::mbar_init(&tail->lo_empty, 1);
     for (int s = 0; s < kBufs; ++s) {
       ptx::mbar_init(&tail->d_full[s], 1);
-      ptx::mbar_init(&tail->d_empty[s], kSumWarps);
+      ptx::mbar_init(&tail->d_empty[s], kSumWarps / 2);
     }
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&tail->part_full[s], kSumWarps);
@@ -226,10 +226,10 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       if (lane == 0) ptx::mbar_arrive(&tail->part_empty[nu & 1]);
     }
   } else {
-    // ---------------- sums: a key's four threads, 32 rows of a tile each ----------------
-    const int part = warp >> 2, quad = warp & 3;
+    // ---------------- sums: lane t takes every other tile, two threads a key, 64 rows each ----------------
+    const int t = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
     const int key_in = quad * 32 + lane;
-    const uint32_t col = tmem + ((uint32_t)(quad * 32) << 16) + part * 32;
+    const uint32_t col = tmem + ((uint32_t)(quad * 32) << 16) + half * 64;
     const int packed = p.group * p.q_len;
     bool ok = true;
     int m = 0, s0 = 0, qphase = 0;  // stage and phase of this block's first tile
@@ -252,66 +252,71 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       uint64_t acc[2] = {0, 0};
       int s = s0, phase = qphase;
       for (int i = 0; i < w.tiles; ++i, ++m) {
-        const int buf = m % kBufs;
-        const int row0 = i * kBM + part * 32;
-        uint32_t seen = 0;  // row row0 + lane: which of the warp's keys it sees
-        if (!full && row0 + lane < packed) {
-          const int h = (int)(((uint64_t)(row0 + lane) * p.q_magic) >> 40), row = row0 + lane - h * p.q_len;
-          const int req = bh / p.c.hkv;
-          seen = (uint32_t)kv8_window(p, p.bits ? p.bits + req * p.bits_bs + (int64_t)row * p.words : nullptr,
-                                      key0 + quad * 32);
-        }
-        if (fresh) ok = ok && ptx::mbar_wait(&tail->q_full[s], phase, abort_flag, &g_kv8_mass_status, 70);
-        ok = ok && ptx::mbar_wait(&tail->d_full[buf], (m / kBufs) & 1, abort_flag, &g_kv8_mass_status, 71);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok && row0 < packed) {
-          ptx::tc_fence_after();
-          uint32_t d[2][16];
-          ptx::tmem_ld_16_async(col + buf * kBM, d[0]);
-          ptx::tmem_wait_ld_16(d[0]);
-          ptx::tmem_ld_16_async(col + buf * kBM + 16, d[1]);
+        if ((m & 1) == t) {
+          const int buf = m % kBufs, row0 = i * kBM + half * 64;
+          uint32_t seen[2] = {0, 0};  // rows row0 + lane and 32 on: which of the warp's keys they see
+          if (!full) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float* f = tail->rowc[s][0] + part * 32 + c * 16;
-            const float* l = tail->rowc[s][1] + part * 32 + c * 16;
-            if (c == 1) {
-              ptx::tmem_wait_ld_16(d[1]);
-              ptx::tc_fence_before();
-              if (lane == 0) ptx::mbar_arrive(&tail->d_empty[buf]);
-            }
-            if (full) {
-#pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const ulonglong2 ff = *reinterpret_cast<const ulonglong2*>(f + j);
-                const ulonglong2 ll = *reinterpret_cast<const ulonglong2*>(l + j);
-                const uint64_t y[2] = {ptx::fma2(ptx::pack2(__uint_as_float(d[c][j]), __uint_as_float(d[c][j + 1])),
-                                                 ptx::mul2(ff.x, kf2), ll.x),
-                                       ptx::fma2(ptx::pack2(__uint_as_float(d[c][j + 2]), __uint_as_float(d[c][j + 3])),
-                                                 ptx::mul2(ff.y, kf2), ll.y)};
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                  float y0, y1;
-                  ptx::unpack2(y[x], y0, y1);
-                  acc[x] = ptx::add2(acc[x], ptx::pack2(ex2(y0), ex2(y1)));
-                }
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; j += 2) {
-                const float2 ff = *reinterpret_cast<const float2*>(f + j), ll = *reinterpret_cast<const float2*>(l + j);
-                const uint32_t w0 = __shfl_sync(0xffffffffu, seen, c * 16 + j);
-                const uint32_t w1 = __shfl_sync(0xffffffffu, seen, c * 16 + j + 1);
-                const float y0 = fmaf(__uint_as_float(d[c][j]), ff.x * kf, ll.x);
-                const float y1 = fmaf(__uint_as_float(d[c][j + 1]), ff.y * kf, ll.y);
-                acc[(j >> 1) & 1] = ptx::add2(acc[(j >> 1) & 1], ptx::pack2((w0 >> lane) & 1u ? ex2(y0) : 0.f,
-                                                                           (w1 >> lane) & 1u ? ex2(y1) : 0.f));
-              }
+            for (int x = 0; x < 2; ++x) {
+              const int pr = row0 + x * 32 + lane;
+              const int h = (int)(((uint64_t)pr * p.q_magic) >> 40), row = pr - h * p.q_len, req = bh / p.c.hkv;
+              if (pr < packed)
+                seen[x] = (uint32_t)kv8_window(
+                    p, p.bits ? p.bits + req * p.bits_bs + (int64_t)row * p.words : nullptr, key0 + quad * 32);
             }
           }
-          __syncwarp();
-        } else if (lane == 0) {
-          ptx::mbar_arrive(&tail->d_empty[buf]);
+          if (fresh) ok = ok && ptx::mbar_wait(&tail->q_full[s], phase, abort_flag, &g_kv8_mass_status, 70);
+          ok = ok && ptx::mbar_wait(&tail->d_full[buf], (m / kBufs) & 1, abort_flag, &g_kv8_mass_status, 71);
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) {
+            ptx::tc_fence_after();
+            uint32_t d[2][16];
+            const int rows = packed - row0;  // the last tile's are fewer
+            ptx::tmem_ld_16_async(col + buf * kBM, d[0]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t(&dc)[16] = d[c & 1];
+              ptx::tmem_wait_ld_16(dc);
+              if (c * 16 >= rows) break;
+              if (c < 3) ptx::tmem_ld_16_async(col + buf * kBM + (c + 1) * 16, d[(c + 1) & 1]);
+              const float* f = tail->rowc[s][0] + half * 64 + c * 16;
+              const float* l = tail->rowc[s][1] + half * 64 + c * 16;
+              if (full) {
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  const ulonglong2 ff = *reinterpret_cast<const ulonglong2*>(f + j);
+                  const ulonglong2 ll = *reinterpret_cast<const ulonglong2*>(l + j);
+                  const uint64_t y[2] = {ptx::fma2(ptx::pack2(__uint_as_float(dc[j]), __uint_as_float(dc[j + 1])),
+                                                   ptx::mul2(ff.x, kf2), ll.x),
+                                         ptx::fma2(ptx::pack2(__uint_as_float(dc[j + 2]), __uint_as_float(dc[j + 3])),
+                                                   ptx::mul2(ff.y, kf2), ll.y)};
+#pragma unroll
+                  for (int x = 0; x < 2; ++x) {
+                    float y0, y1;
+                    ptx::unpack2(y[x], y0, y1);
+                    acc[x] = ptx::add2(acc[x], ptx::pack2(ex2(y0), ex2(y1)));
+                  }
+                }
+              } else {
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                  const float2 ff = *reinterpret_cast<const float2*>(f + j);
+                  const float2 ll = *reinterpret_cast<const float2*>(l + j);
+                  const uint32_t w0 = __shfl_sync(0xffffffffu, seen[c >> 1], (c & 1) * 16 + j);
+                  const uint32_t w1 = __shfl_sync(0xffffffffu, seen[c >> 1], (c & 1) * 16 + j + 1);
+                  const float y0 = fmaf(__uint_as_float(dc[j]), ff.x * kf, ll.x);
+                  const float y1 = fmaf(__uint_as_float(dc[j + 1]), ff.y * kf, ll.y);
+                  acc[(j >> 1) & 1] = ptx::add2(acc[(j >> 1) & 1], ptx::pack2((w0 >> lane) & 1u ? ex2(y0) : 0.f,
+                                                                             (w1 >> lane) & 1u ? ex2(y1) : 0.f));
+                }
+              }
+            }
+            ptx::tc_fence_before();
+            __syncwarp();
+          }
+          if (lane == 0) ptx::mbar_arrive(&tail->d_empty[buf]);
         }
+        // Both lanes have then read this tile's row constants for the last time.
         if (last && lane == 0) ptx::mbar_arrive(&tail->q_empty[s]);
         if (++s == kQStages) s = 0, phase ^= 1;
       }
@@ -321,7 +326,7 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       ptx::unpack2(acc[1], a[2], a[3]);
       const int nu = u - u0;
       ok = ok && ptx::mbar_wait(&tail->part_empty[nu & 1], ((nu >> 1) & 1) ^ 1, abort_flag, &g_kv8_mass_status, 72);
-      tail->part[nu & 1][part][key_in] = (a[0] + a[1]) + (a[2] + a[3]);
+      tail->part[nu & 1][t * 2 + half][key_in] = (a[0] + a[1]) + (a[2] + a[3]);
       __syncwarp();
       ok = __all_sync(0xffffffffu, ok);
       if (lane == 0) ptx::mbar_arrive(&tail->part_full[nu & 1]);
