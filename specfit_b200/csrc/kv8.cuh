@@ -27,6 +27,16 @@ constexpr int kKv8MinExponent = -100;
 // Checks shared by every entry point that reads a sf_kv8_rows.
 int kv8_check(const sf_kv8_rows* r, bool need_values);
 
+// Whether the requests and heads of something to be written lie apart: each
+// is `extent` elements, `b` of them bs apart, `h` hs apart.
+inline bool kv8_apart(int64_t b, int64_t bs, int64_t h, int64_t hs, int64_t extent) {
+  if (extent <= 0) return true;
+  if (b > 1 && bs < extent) return false;
+  if (h > 1 && hs < extent) return false;
+  if (b <= 1 || h <= 1) return true;
+  return bs >= hs ? (bs - extent) / hs >= h - 1 : (hs - extent) / bs >= b - 1;
+}
+
 struct Kv8Rows {
   const uint8_t* k;
   const uint8_t* v;

@@ -731,6 +731,8 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
   SF_CHECK_ARG(aligned16(q) && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0 && q_row_stride % 8 == 0,
                "q rows must be 16-byte aligned");
   SF_CHECK_ARG(aligned16(out) && out_batch_stride % 8 == 0, "out must be 16-byte aligned");
+  SF_CHECK_ARG(kv8_apart(rows->batch, out_batch_stride, 1, 0, q_len * num_heads * rows->head_dim),
+               "requests of out must not overlap");
   const size_t need = sf_kv8_attention_workspace_bytes(rows->batch, num_heads, rows->num_kv_heads, rows->head_dim,
                                                        q_len, rows->sealed, rows->tail);
   if (workspace_bytes < need || (need && !workspace))

@@ -242,6 +242,8 @@ extern "C" int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int6
                "tree_bits must cover the keys from prefix_len on");
   SF_CHECK_ARG(aligned16(q) && q_batch_stride % 8 == 0 && q_head_stride % 8 == 0 && q_row_stride % 8 == 0,
                "q rows must be 16-byte aligned");
+  SF_CHECK_ARG(kv8_apart(rows->batch, mass_batch_stride, rows->num_kv_heads, mass_head_stride, kv_len),
+               "requests and heads of mass must not overlap");
   const size_t need = sf_kv8_mass_workspace_bytes(rows->batch, num_heads, rows->num_kv_heads, rows->head_dim, q_len,
                                                   rows->sealed, rows->tail);
   if (workspace_bytes < need || (need && !workspace))

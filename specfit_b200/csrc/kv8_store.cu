@@ -260,6 +260,15 @@ Target make_target(const sf_kv8_rows& r, int64_t first_block, int64_t full_block
   return t;
 }
 
+bool target_apart(const sf_kv8_rows& r) {
+  auto apart = [&](int64_t bs, int64_t hs, int64_t extent) {
+    return kv8_apart(r.batch, bs, r.num_kv_heads, hs, extent);
+  };
+  return apart(r.code_batch_stride, r.code_head_stride, r.sealed * r.head_dim) &&
+         apart(r.scale_batch_stride, r.scale_head_stride, r.sealed / r.block_tokens) &&
+         apart(r.tail_batch_stride, r.tail_head_stride, r.tail * r.head_dim);
+}
+
 }  // namespace
 }  // namespace sf
 
@@ -269,10 +278,11 @@ extern "C" int sf_kv8_seal(const void* k, const void* v, int64_t batch_stride, i
   using namespace sf;
   if (int rc = kv8_check(rows, true)) return rc;
   SF_CHECK_ARG(blocks >= 0 && first_block >= 0 && blocks < (1 << 24) &&
-                   first_block + blocks <= rows->sealed / rows->block_tokens,
+                   first_block <= rows->sealed / rows->block_tokens - blocks,
                "blocks to seal must lie within the cache's sealed rows");
   if (blocks == 0) return SF_OK;
   SF_CHECK_ARG(k && v, "null pointer argument");
+  SF_CHECK_ARG(target_apart(*rows), "requests and heads of the target must not overlap");
   SF_CHECK_ARG(aligned16(k) && aligned16(v) && batch_stride % 8 == 0 && head_stride % 8 == 0 && row_stride % 8 == 0,
                "k/v rows must be 16-byte aligned");
   const SourceRows src{static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), batch_stride,
@@ -285,7 +295,8 @@ extern "C" int sf_kv8_read(const sf_kv8_rows* rows, int64_t first, int64_t count
                            int64_t out_batch_stride, int64_t out_head_stride, void* stream) {
   using namespace sf;
   if (int rc = kv8_check(rows, true)) return rc;
-  SF_CHECK_ARG(first >= 0 && count >= 0 && first + count <= rows->sealed + rows->tail,
+  SF_CHECK_ARG(first >= 0 && count >= 0 && count <= rows->sealed + rows->tail &&
+                   first <= rows->sealed + rows->tail - count,
                "rows to read must lie within the cache");
   if (count == 0) return SF_OK;
   SF_CHECK_ARG(k_out && v_out, "null pointer argument");
@@ -320,6 +331,9 @@ extern "C" int sf_kv8_compact(const sf_kv8_rows* rows, const int32_t* keep, int6
                    (out->tail == 0 || (out->k_tail != rows->k_tail && out->v_tail != rows->v_tail)) &&
                    (mass == nullptr || mass != mass_out),
                "compaction writes to buffers of its own");
+  SF_CHECK_ARG(target_apart(*out) && (mass == nullptr || kv8_apart(out->batch, mass_out_batch_stride, out->num_kv_heads,
+                                                                   mass_out_head_stride, n)),
+               "requests and heads of the target must not overlap");
   SourceKept src{kv8_view(*rows), keep, n, mass, mass_out, mass_batch_stride, mass_head_stride,
                  mass_out_batch_stride, mass_out_head_stride};
   const int64_t full = out->sealed / out->block_tokens;

@@ -253,6 +253,10 @@ class Kv8Cache(DynamicCache):
         self.budget, self.sinks, self.recent = budget, sinks, recent
         self.dropped = 0  # tokens that evictions took out of each head
 
+    def reset(self) -> None:
+        super().reset()
+        self.dropped = 0
+
     @property
     def next_position(self) -> int:
         """Position of the next token: rows held and rows evicted."""

@@ -486,3 +486,24 @@ def test_offsets_past_32_bits(ops):
     assert float(new.k_codes[-1, -1, -1, 0].float()) * float(new.k_scale[-1, -1, 0]) == 1.0
     k, _ = ops.kv8_read(rows, sealed - 2, 2)
     assert k[-1, -1, :, 5].tolist() == [0.0, 1.0]
+
+
+@pytest.mark.parametrize("rows", [1, 65])
+def test_heads_and_requests_that_share_memory(ops, rows):
+    """A cache whose heads (or requests) are one tensor expanded is read like
+    its copy, whichever kernel its strides allow."""
+    one = make_rows(ops, 1, 1, 128, 64, 320, 70, 31)
+    k, v = opened(one)
+    for b, h in ((1, 2), (3, 1), (2, 2)):
+        parts = [t.expand(b, h, *t.shape[2:]) for t in (one.k_codes, one.v_codes, one.k_scale, one.v_scale)]
+        tails = [t.expand(b, h, *t.shape[2:]) for t in (one.k_tail, one.v_tail)]
+        cache = ops.Kv8Rows(*parts, 320, *tails, 64)
+        q = queries(b, 4 * h, rows, 128, 31)
+        bits, prefix, vis = masks("any", b, rows, 390, 31)
+        out, lse = ops.kv8_tree_attention(q, cache, bits, prefix, return_lse=True)
+        kk, vv = k.expand(b, h, *k.shape[2:]), v.expand(b, h, *v.shape[2:])
+        want, wlse = ref.attention(q, kk, vv, vis, 128 ** -0.5)
+        check_attention(out, lse, want, wlse, float(v.abs().max()))
+        mass = ops.kv8_attention_mass(q, lse, cache, bits, prefix, torch.zeros(b, h, 390, device=DEV))
+        wmass = ref.mass(q, wlse, kk, vis, 128 ** -0.5)
+        assert bool(((mass.double().cpu() - wmass).abs() <= 4e-4 * wmass + 2.0 ** -22 * (1 + wmass)).all())

@@ -71,8 +71,11 @@ def test_malformed_calls_are_refused():
     seal = lambda first, n, k=256, rs=128: N.lib.sf_kv8_seal(k, 256, 0, 0, rs, addr(s), first, n, None)
     for args in ((0, 3), (2, 1), (-1, 1), (0, -1), (0, 1, 264), (0, 1, 256, 12), (0, 1, None)):
         assert seal(*args) == N.SF_ERR_INVALID_ARGUMENT, args
+    for args in (((1 << 63) - 1, 1), ((1 << 63) - 1, 2)):  # their sum has no 64 bits
+        assert seal(*args) == N.SF_ERR_INVALID_ARGUMENT, args
     assert seal(2, 0) == N.SF_OK
     assert N.lib.sf_kv8_read(addr(s), 100, 37, 256, 256, 0, 0, None) == N.SF_ERR_INVALID_ARGUMENT
+    assert N.lib.sf_kv8_read(addr(s), (1 << 63) - 1, 2, 256, 256, 0, 0, None) == N.SF_ERR_INVALID_ARGUMENT
     assert N.lib.sf_kv8_read(addr(s), 136, 0, None, None, 0, 0, None) == N.SF_OK
     # Mass and selection.
     mass = lambda **k: N.lib.sf_kv8_attention_mass(k.get("q", 256), 0, 0, 128, k.get("heads", 8), 3, k.get("lse", 256),
@@ -94,6 +97,33 @@ def test_malformed_calls_are_refused():
         assert comp(out, n) == N.SF_ERR_INVALID_ARGUMENT
     assert comp(struct(sealed=64, tail=6, **other), 70, 256, 256) == N.SF_ERR_INVALID_ARGUMENT
     assert comp(struct(sealed=64, tail=6, **other), 70, 256, None) == N.SF_ERR_INVALID_ARGUMENT
+
+
+def test_expanded_targets_are_refused():
+    """Requests or heads that share memory may be read, not written."""
+    other = dict(k_codes=512, v_codes=512, k_tail=512, v_tail=512)
+    for kw in (dict(code_head_stride=0), dict(scale_head_stride=1), dict(code_head_stride=127 * 128),
+               dict(batch=2, code_batch_stride=128 * 128, scale_batch_stride=4, tail_batch_stride=2048),
+               dict(batch=2, code_batch_stride=256 * 128, scale_batch_stride=2, tail_batch_stride=2048)):
+        s = struct(**kw)
+        assert N.lib.sf_kv8_seal(256, 256, 0, 0, 128, addr(s), 0, 1, None) == N.SF_ERR_INVALID_ARGUMENT, kw
+        assert "overlap" in N.last_error(), kw
+    src = struct()
+    for kw in (dict(code_head_stride=0), dict(tail_head_stride=0), dict(tail_head_stride=5 * 128)):
+        out = struct(**{**other, "sealed": 64, "tail": 6, **kw})
+        assert N.lib.sf_kv8_compact(addr(src), 256, 70, addr(out), None, 0, 0, None, 0, 0,
+                                    None) == N.SF_ERR_INVALID_ARGUMENT, kw
+        assert "overlap" in N.last_error(), kw
+    out = struct(sealed=64, tail=6, **other)
+    assert N.lib.sf_kv8_compact(addr(src), 256, 70, addr(out), 256, 0, 136, 512, 0, 69,
+                                None) == N.SF_ERR_INVALID_ARGUMENT
+    assert "overlap" in N.last_error()
+    for hs in (0, 135):
+        assert N.lib.sf_kv8_attention_mass(256, 0, 0, 128, 8, 3, 256, addr(src), 256, 1, 0, 133, 0.1, 256, 0, hs, None,
+                                           0, None) == N.SF_ERR_INVALID_ARGUMENT
+        assert "overlap" in N.last_error()
+    two = struct(batch=2)  # read twice: allowed; written to one place: not
+    assert attention(two) == N.SF_ERR_INVALID_ARGUMENT and "overlap" in N.last_error()
 
 
 def test_python_entries_refuse_cpu_tensors_and_wrong_types():
@@ -266,6 +296,8 @@ def test_eviction(plain):
     assert c.get_seq_length() == 43 and c.next_position == 93
     assert float(c.layers[0].mass[:, :, 40:43].abs().max()) == 0
     assert c.evict() == 3 and c.next_position == 93
+    c.reset()
+    assert c.get_seq_length() == 0 and c.next_position == 0
 
 
 def test_refusals(plain):
