@@ -35,11 +35,16 @@
 //     more than fp16's 11 bits (probabilities are kept times 2^12).
 //   * The reference maximum of a row moves only when a score exceeds it by
 //     more than 3 (base 2), so accumulators are rarely rescaled.
-//   * What bounds it is instructions: of the 20 or so that 16 codes take, 6 are
+//   * What bounds it is a warp's chain of instructions (three warps a scheduler
+//     issue in one clock of four): of the 20 or so that 16 codes take, 6 are
 //     conversions (ALU, half rate) and 2 MMAs.  Hence 32 keys a step (645
 //     instructions for 16 keys were 43 us at 131,072 tokens), Q's fragments from
 //     shared memory (one 16-byte load for four MMAs), tail units converted there
 //     too, and addresses that are constants where D is the tile's width.
+// What it measured: one token, 32 heads over 131,113 tokens, 30 us, 4.5 TB/s, of
+// which about five are the launch, Q, the join and the partial results, and 7
+// more the merge.  Four CTAs an SM, with a ring of 12 KB a warp, took 37: each
+// has that cost, and a shorter range.
 // Tail units (bf16 rows: few) are scaled by a power of two per unit and
 // enter the same fragments.  A value row with a NaN or an infinity (a sealed
 // block of values that holds one) makes its key's score NaN, so that rows
