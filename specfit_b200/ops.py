@@ -631,7 +631,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = Non
 
 
 # ---------------------------------------------------------------------------
-# K10 the 8-bit KV cache: sealing, attention, attention mass, eviction
+# K13 the 8-bit KV cache: sealing, attention, attention mass, eviction
 
 
 class Kv8Rows:
