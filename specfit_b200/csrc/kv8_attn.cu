@@ -49,6 +49,7 @@
 // enter the same fragments.  A value row with a NaN or an infinity (a sealed
 // block of values that holds one) makes its key's score NaN, so that rows
 // which do not see it stay what they are.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <algorithm>
@@ -66,6 +67,12 @@ constexpr int kHalves = kUnit / 16;
 constexpr int kStages = 2;     // units of a warp's ring
 constexpr int kStep = kWarps * kUnit;
 constexpr int kMaxSplits = 128;
+constexpr int kMaxCluster = 8; // key ranges that a cluster joins itself
+// Up to so many steps of a CTA the ranges are at most a cluster's: a token
+// over 545 / 1,569 tokens 10.9 / 11.5 us against 12.5 / 14.3 with a range a step
+// and the merge kernel (8 rows: 13.1 / 15.2 against 14.7 / 18.9), and one launch
+// less; at 2,593 tokens they are equal, at 4,129 the merge is faster.
+constexpr int kClusterSteps = 24;
 constexpr float kPShift = 12.f;  // probabilities are kept times 2^12
 constexpr float kSlack = 3.f;    // a row's reference maximum may lag by this (base 2)
 
@@ -82,7 +89,9 @@ struct Layout {
   // A tail unit as fp16 takes twice its codes' bytes, in the ring, where no copy is in flight by then.
   static_assert(kStages >= 2, "a tail unit needs two stages");
   static constexpr int kJoin = kWarps * kRows * DT * 4;
-  static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  // The CTA's own rows, where its cluster reads them: behind the warps'.
+  static constexpr int kRows0 = kJoin, kNeed = kJoin + kRows * DT * 4;
+  static constexpr int kSmem = kRing > kNeed ? kRing : kNeed;
 };
 
 // A unit of tail rows as fp16 fragments in this thread's slots of `out`
@@ -166,6 +175,7 @@ kv8_attn_kernel(Kv8Attn p) {
   pdl_trigger();
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float join_m[kWarps][kRows], join_l[kWarps][kRows];
+  __shared__ float2 row_ml[kRows];  // of the CTA, for its cluster
   __shared__ __align__(16) uint4 q_frag[L::kSteps][32];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -526,8 +536,22 @@ kv8_attn_kernel(Kv8Attn p) {
             unit > 0.f ? y * unit : y;
       }
   __syncthreads();
-  constexpr int kPerRow = DT / 4;
-  for (int i = threadIdx.x; i < (Narrow ? 8 : kRows) * kPerRow; i += kWarps * 32) {
+  constexpr int kPerRow = DT / 4, kJoinRows = Narrow ? 8 : kRows;
+  auto store_row = [&](int pr, int col, const float(&acc)[4], float sum, float gm) {
+    const int qh = (int)(((uint64_t)pr * p.q_magic) >> 40);
+    const int head = kvh * p.group + qh, t = pr - qh * p.q_len;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
+    __nv_bfloat162 hi = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+    uint2 w;
+    w.x = *reinterpret_cast<uint32_t*>(&lo);
+    w.y = *reinterpret_cast<uint32_t*>(&hi);
+    *reinterpret_cast<uint2*>(p.out + req * p.out_bs + ((int64_t)t * p.heads + head) * d + col) = w;
+    if (p.lse && col == 0)
+      p.lse[((int64_t)req * p.heads + head) * p.q_len + t] =
+          sum == 0.f ? -INFINITY : (gm == -INFINITY ? sum : (gm - kPShift + log2f(sum)) * 0.69314718055994531f);
+  };
+  for (int i = threadIdx.x; i < kJoinRows * kPerRow; i += kWarps * 32) {
     const int row = i / kPerRow, col = (i % kPerRow) * 4;
     const int pr = blockIdx.y * kRows + row;
     if (pr >= packed || col >= d) continue;
@@ -550,16 +574,10 @@ kv8_attn_kernel(Kv8Attn p) {
     const int qh = (int)(((uint64_t)pr * p.q_magic) >> 40);
     const int head = kvh * p.group + qh, t = pr - qh * p.q_len;
     if (p.splits == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
-      __nv_bfloat162 hi = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
-      uint2 w;
-      w.x = *reinterpret_cast<uint32_t*>(&lo);
-      w.y = *reinterpret_cast<uint32_t*>(&hi);
-      *reinterpret_cast<uint2*>(p.out + req * p.out_bs + ((int64_t)t * p.heads + head) * d + col) = w;
-      if (p.lse && col == 0)
-        p.lse[((int64_t)req * p.heads + head) * p.q_len + t] =
-            sum == 0.f ? -INFINITY : (gm == -INFINITY ? sum : (gm - kPShift + log2f(sum)) * 0.69314718055994531f);
+      store_row(pr, col, acc, sum, gm);
+    } else if (p.splits <= kMaxCluster) {
+      *reinterpret_cast<float4*>(smem + L::kRows0 + (row * DT + col) * 4) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (col == 0) row_ml[row] = make_float2(gm, sum);
     } else {
       const int64_t idx = (((int64_t)req * p.splits + split) * p.heads + head) * p.q_len + t;
       *reinterpret_cast<float4*>(p.part_o + idx * d + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -569,6 +587,97 @@ kv8_attn_kernel(Kv8Attn p) {
       }
     }
   }
+  if (p.splits > 1 && p.splits <= kMaxCluster) {
+    // The cluster is the row tile's key ranges: each CTA joins a part of the
+    // rows from all of them, in range order.
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int i = (int)cluster.block_rank() * kWarps * 32 + threadIdx.x; i < kJoinRows * kPerRow;
+         i += p.splits * kWarps * 32) {
+      const int row = i / kPerRow, col = (i % kPerRow) * 4;
+      const int pr = blockIdx.y * kRows + row;
+      if (pr >= packed || col >= d) continue;
+      float2 ml[kMaxCluster];
+      float4 y[kMaxCluster];
+      float gm = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        if (r >= p.splits) break;
+        ml[r] = *cluster.map_shared_rank(row_ml + row, r);
+        y[r] = *cluster.map_shared_rank(reinterpret_cast<const float4*>(smem + L::kRows0 + (row * DT + col) * 4), r);
+        gm = fmaxf(gm, ml[r].x);
+      }
+      float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        if (r >= p.splits) break;
+        const float f = ml[r].x == -INFINITY ? 0.f : exp2f(ml[r].x - gm);
+        sum += f * ml[r].y;  // a NaN passes even where f is 0
+        acc[0] += f * y[r].x;
+        acc[1] += f * y[r].y;
+        acc[2] += f * y[r].z;
+        acc[3] += f * y[r].w;
+      }
+      store_row(pr, col, acc, sum, gm);
+    }
+    cluster.sync();  // no CTA leaves while its rows may be read
+  }
+}
+
+// A joined row's output, four dims a lane, and its log-sum-exp.
+__device__ __forceinline__ void store_joined(const Kv8Attn& p, int64_t pair, int64_t req, int64_t at, int lane,
+                                             const float (&acc)[4], float sum, float gm) {
+  const int head = (int)(at / p.q_len), t = (int)(at % p.q_len), d = p.c.d;
+  if (p.lse && lane == 0)
+    p.lse[pair] = sum == 0.f ? -INFINITY : (gm == -INFINITY ? sum : (gm + log2f(sum)) * 0.69314718055994531f);
+  if (lane * 4 >= d) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
+  __nv_bfloat162 hi = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+  uint2 w;
+  w.x = *reinterpret_cast<uint32_t*>(&lo);
+  w.y = *reinterpret_cast<uint32_t*>(&hi);
+  *reinterpret_cast<uint2*>(p.out + req * p.out_bs + ((int64_t)t * p.heads + head) * d + lane * 4) = w;
+}
+
+// Joins up to N key ranges, a warp per (request, head, row): everything is
+// loaded at once.
+template <int N>
+__global__ void __launch_bounds__(256)
+kv8_merge_few_kernel(Kv8Attn p) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t per_req = (int64_t)p.heads * p.q_len;
+  const int lane = threadIdx.x & 31, d = p.c.d;
+  const int64_t pair = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (pair >= per_req * p.batch) return;
+  const int64_t req = pair / per_req, at = pair - req * per_req;
+  const int64_t base = req * p.splits * per_req + at;
+  float2 ml[N];
+  float4 y[N];
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    ml[s] = s < p.splits ? *reinterpret_cast<const float2*>(p.part_ml + (base + s * per_req) * 2)
+                         : make_float2(-INFINITY, 0.f);
+    y[s] = s < p.splits && lane * 4 < d
+               ? *reinterpret_cast<const float4*>(p.part_o + (base + s * per_req) * d + lane * 4)
+               : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  float gm = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < N; ++s) gm = fmaxf(gm, ml[s].x);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    const float f = ml[s].x == -INFINITY ? 0.f : exp2f(ml[s].x - gm);
+    sum += f * ml[s].y;  // a NaN passes even where f is 0
+    acc[0] += f * y[s].x;
+    acc[1] += f * y[s].y;
+    acc[2] += f * y[s].z;
+    acc[3] += f * y[s].w;
+  }
+  store_joined(p, pair, req, at, lane, acc, sum, gm);
 }
 
 // Joins the key ranges: W warps per (request, head, row), four dims a lane.
@@ -621,31 +730,26 @@ kv8_merge_kernel(Kv8Attn p) {
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if constexpr (W > 1) {
-    part[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    __syncthreads();
-    if (mine != 0) return;
+  part[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+  __syncthreads();
+  if (mine != 0) return;
 #pragma unroll
-    for (int i = 1; i < W; ++i) {
-      const float4 y = part[warp + i][lane];
-      acc[0] += y.x;
-      acc[1] += y.y;
-      acc[2] += y.z;
-      acc[3] += y.w;
-    }
+  for (int i = 1; i < W; ++i) {
+    const float4 y = part[warp + i][lane];
+    acc[0] += y.x;
+    acc[1] += y.y;
+    acc[2] += y.z;
+    acc[3] += y.w;
   }
-  if (!on) return;
-  const int head = (int)(at / p.q_len), t = (int)(at % p.q_len);
-  if (p.lse && lane == 0)
-    p.lse[pair] = sum == 0.f ? -INFINITY : (gm == -INFINITY ? sum : (gm + log2f(sum)) * 0.69314718055994531f);
-  if (lane * 4 >= d) return;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
-  __nv_bfloat162 hi = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
-  uint2 w;
-  w.x = *reinterpret_cast<uint32_t*>(&lo);
-  w.y = *reinterpret_cast<uint32_t*>(&hi);
-  *reinterpret_cast<uint2*>(p.out + req * p.out_bs + ((int64_t)t * p.heads + head) * d + lane * 4) = w;
+  if (on) store_joined(p, pair, req, at, lane, acc, sum, gm);
+}
+
+template <int N>
+int launch_merge_few(const Kv8Attn& p, cudaStream_t stream) {
+  const int64_t pairs = (int64_t)p.batch * p.heads * p.q_len;
+  SF_CHECK_CUDA(launch_pdl(kv8_merge_few_kernel<N>, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, stream, p));
+  SF_CHECK_LAUNCH();
+  return SF_OK;
 }
 
 template <int W>
@@ -668,7 +772,11 @@ int launch_mma(const Kv8Attn& p, cudaStream_t stream) {
   const int64_t tiles = ((int64_t)p.group * p.q_len + kRows - 1) / kRows;
   SF_CHECK_ARG(tiles < 65536 && (int64_t)p.splits * p.batch < 65536, "too many query rows or requests");
   const dim3 grid((unsigned)p.c.hkv, (unsigned)tiles, (unsigned)(p.splits * p.batch));
-  SF_CHECK_CUDA(launch_pdl(kv8_attn_kernel<DT, Full, Narrow>, grid, dim3(kWarps * 32), Layout<DT>::kSmem, stream, p));
+  if (p.splits > 1 && p.splits <= kMaxCluster)
+    SF_CHECK_CUDA(launch_pdl_cluster3(kv8_attn_kernel<DT, Full, Narrow>, grid, dim3(kWarps * 32), Layout<DT>::kSmem,
+                                      stream, dim3(1, 1, (unsigned)p.splits), p));
+  else
+    SF_CHECK_CUDA(launch_pdl(kv8_attn_kernel<DT, Full, Narrow>, grid, dim3(kWarps * 32), Layout<DT>::kSmem, stream, p));
   SF_CHECK_LAUNCH();
   return SF_OK;
 }
@@ -685,11 +793,12 @@ size_t partial_bytes(const Kv8Split& s, int batch, int heads, int head_dim, int6
 
 }  // namespace
 
-// Three resident CTAs per SM; a range is at least one step of the four warps.
+// Three resident CTAs per SM, in short contexts one cluster a row tile; a range is at least one step of the four warps.
 Kv8Split kv8_split_mma(int batch, int hkv, int64_t packed, int64_t kv_len) {
   const int64_t units = (int64_t)batch * hkv * ((packed + kRows - 1) / kRows);
   const int64_t steps = (kv_len + kStep - 1) / kStep;
   int64_t want = std::max<int64_t>(1, 3 * (int64_t)num_sms() / units);
+  if (steps <= kClusterSteps) want = std::min<int64_t>(want, kMaxCluster);
   want = std::min<int64_t>(want, std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, steps)));
   const int64_t per = std::max<int64_t>(1, (steps + want - 1) / want);
   return {(int)std::max<int64_t>(1, (steps + per - 1) / per), (int)(per * kStep)};
@@ -707,7 +816,8 @@ extern "C" size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int
   const int64_t kv_len = sealed + tail;
   // Enough for either kernel: which one runs depends on the cache's strides too.
   const int64_t packed = (int64_t)(num_heads / num_kv_heads) * q_len;
-  size_t need = partial_bytes(kv8_split_mma(batch, num_kv_heads, packed, kv_len), batch, num_heads, head_dim, q_len);
+  const Kv8Split mma = kv8_split_mma(batch, num_kv_heads, packed, kv_len);
+  size_t need = mma.splits <= kMaxCluster ? 0 : partial_bytes(mma, batch, num_heads, head_dim, q_len);
   if (kv8_use_tc(head_dim, packed, kv_len))
     need = std::max(need, partial_bytes(kv8_split_tc(batch, num_kv_heads, packed, kv_len), batch, num_heads, head_dim,
                                         q_len) +
@@ -783,7 +893,8 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
          : rows->head_dim > 64  ? launch_rows<128, false>(p, st)
          : rows->head_dim == 64 ? launch_rows<64, true>(p, st)
                                 : launch_rows<64, false>(p, st);
-  if (rc || s.splits == 1) return rc;
-  // One warp a row walks 16 ranges as fast as four join them (65 rows, 12 ranges: 5.7 and 9.1 us).
-  return s.splits <= 16 ? launch_merge<1>(p, st) : (s.splits <= 32 ? launch_merge<4>(p, st) : launch_merge<8>(p, st));
+  if (rc || s.splits == 1 || (!tc && s.splits <= kMaxCluster)) return rc;
+  if (s.splits <= 4) return launch_merge_few<4>(p, st);
+  if (s.splits <= 16) return launch_merge_few<16>(p, st);
+  return s.splits <= 32 ? launch_merge<4>(p, st) : launch_merge<8>(p, st);
 }

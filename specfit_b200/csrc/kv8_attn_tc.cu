@@ -242,9 +242,11 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 // The query head (within its group) of packed row n: n / q_len.
 __device__ __forceinline__ int row_head(const Kv8Attn& p, int n) { return (int)(((uint64_t)n * p.q_magic) >> 40); }
 
-// grid: (query tiles, then blocks with tail rows (one CTA for the unit alone if
-// there are none); batch * hkv).
-__global__ void __launch_bounds__(256)
+constexpr int kScan = 16;  // loads of a thread under way while it looks for the unit
+
+// grid: (blocks that are not codes alone (one CTA for the unit alone if there
+// are none), which take longest, then query tiles; batch * hkv).
+__global__ void __launch_bounds__(256, 2)
 kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
   pdl_wait();
   pdl_trigger();
@@ -252,8 +254,9 @@ kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
   const int bh = blockIdx.y, kvh = bh % p.c.hkv, req = bh / p.c.hkv;
   const int row = threadIdx.x >> 3, part = threadIdx.x & 7;  // row of 32 in a pass, 16 dims of it
   const uint32_t at0 = sw128(row, part);                     // 32 rows on: 4,096 bytes
-  if ((int)blockIdx.x < w.tiles) {
-    const int tile = blockIdx.x, packed = p.group * p.q_len;
+  const int others = (int)gridDim.x - w.tiles;
+  if ((int)blockIdx.x >= others) {
+    const int tile = blockIdx.x - others, packed = p.group * p.q_len;
     uint8_t* img = w.q + ((int64_t)bh * w.tiles + tile) * kTileBytes + at0;
     uint4 x[4][2];
 #pragma unroll
@@ -294,7 +297,6 @@ kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
     return;
   }
   const bool values = w.v != nullptr;
-  if (!values && (int)blockIdx.x - w.tiles >= w.blocks) return;
   // The unit: every CTA that needs it finds it for itself.
   const int sealed = (int)p.c.sealed, tail_rows = p.kv_len - sealed;
   const float* vsc = p.c.vs + req * p.c.s_bs + kvh * p.c.s_hs;
@@ -306,14 +308,22 @@ kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
   for (int i = threadIdx.x; values && i < sealed >> p.c.block_shift; i += 256)
     unit = fmaxf(unit, vsc[i]);  // NaN is passed over
   uint32_t top = 0;
-#pragma unroll 16
-  for (int i = threadIdx.x; values && i < tail_rows * (kD / 8); i += 256) {
-    const uint4 x = *reinterpret_cast<const uint4*>(vt + (int64_t)i * 8);
-    const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+  const int pieces = values ? tail_rows * (kD / 8) : 0;
+  for (int i0 = threadIdx.x; i0 < pieces; i0 += kScan * 256) {
+    uint4 x[kScan];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = in[j] & 0x7fffu, hi = (in[j] >> 16) & 0x7fffu;
-      top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+    for (int j = 0; j < kScan; ++j) {
+      const int i = i0 + j * 256;
+      x[j] = i < pieces ? *reinterpret_cast<const uint4*>(vt + (int64_t)i * 8) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) {
+      const uint32_t in[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = in[k] & 0x7fffu, hi = (in[k] >> 16) & 0x7fffu;
+        top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+      }
     }
   }
   unit = fmaxf(unit, pow2f(kv8_exponent(top)));
@@ -323,7 +333,7 @@ kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) unit = fmaxf(unit, tops[i]);
-  const int blk = blockIdx.x - w.tiles;
+  const int blk = blockIdx.x;
   if (values && blk == 0 && threadIdx.x == 0) w.unit[bh] = unit;
   if (blk >= w.blocks) return;
   const float inv = 1.f / unit;  // exact
@@ -333,7 +343,7 @@ kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
   uint8_t* vimg = w.v + ((int64_t)bh * w.blocks + blk) * kTileBytes + at0;
   float* kf = w.kf + ((int64_t)bh * w.blocks + blk) * kKB;
   const int key0 = w.first + blk * kKB;
-#pragma unroll 2
+#pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int key = key0 + u * 32 + row;
     uint4 a = make_uint4(0, 0, 0, 0), c = a, x = a, y = a;
