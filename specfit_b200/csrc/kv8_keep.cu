@@ -288,7 +288,7 @@ extern "C" int sf_kv_keep_heaviest(const float* mass, int64_t mass_batch_stride,
   SF_CHECK_ARG(batch > 0 && num_kv_heads > 0 && (int64_t)batch * num_kv_heads <= 65535,
                "batch and num_kv_heads must be positive, their product at most 65535");
   SF_CHECK_ARG(length >= 0 && length < (1 << 30), "length must be in [0, 2^30)");
-  SF_CHECK_ARG(sinks >= 0 && recent >= 0 && sinks + recent <= budget && budget <= length,
+  SF_CHECK_ARG(sinks >= 0 && recent >= 0 && sinks <= budget && recent <= budget - sinks && budget <= length,
                "sinks + recent <= budget <= length is needed");
   if (budget == 0) return SF_OK;
   SF_CHECK_ARG(mass && keep, "null pointer argument");

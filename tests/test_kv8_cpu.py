@@ -85,7 +85,8 @@ def test_malformed_calls_are_refused():
         assert mass(**kw) == N.SF_ERR_INVALID_ARGUMENT, kw
     keep = lambda length, budget, sinks, recent, m=256: N.lib.sf_kv_keep_heaviest(m, 0, 0, 1, 1, length, budget, sinks,
                                                                                  recent, 256, None)
-    for args in ((10, 11, 0, 0), (10, 5, 3, 3), (10, 5, -1, 0), (10, -1, 0, 0), (1 << 30, 5, 0, 0), (10, 5, 0, 0, None)):
+    for args in ((10, 11, 0, 0), (10, 5, 3, 3), (10, 5, -1, 0), (10, -1, 0, 0), (1 << 30, 5, 0, 0), (10, 5, 0, 0, None),
+                 (10, 5, 1 << 62, 1 << 62)):
         assert keep(*args) == N.SF_ERR_INVALID_ARGUMENT, args
     assert keep(10, 0, 0, 0) == N.SF_OK
     # Compaction: the target holds the kept rows, in buffers of its own.
