@@ -41,9 +41,10 @@
 //     instructions for 16 keys were 43 us at 131,072 tokens), Q's fragments from
 //     shared memory (one 16-byte load for four MMAs), tail units converted there
 //     too, and addresses that are constants where D is the tile's width.
-// What it measured: one token, 32 heads over 131,113 tokens, 30 us, 4.5 TB/s, of
+// What it measured: one token, 32 heads over 131,113 tokens, 26 us, 5.1 TB/s, of
 // which about five are the launch, Q, the join and the partial results, and 7
-// more the merge.  Four CTAs an SM, with a ring of 12 KB a warp, took 37: each
+// more the merge.  (30 us while a tail unit's loads came a key after the other:
+// the last range's CTA ended late.)  Four CTAs an SM, with a ring of 12 KB a warp, took 37: each
 // has that cost, and a shorter range.
 // Tail units (bf16 rows: few) are scaled by a power of two per unit and
 // enter the same fragments.  A value row with a NaN or an infinity (a sealed
@@ -97,7 +98,8 @@ struct Layout {
 // A unit of tail rows as fp16 fragments in this thread's slots of `out`
 // ([K: key tiles x steps][V: halves x output tiles] of 32 lanes), scaled by
 // powers of two that are returned; zeros for keys from key_hi on.  First the
-// rows as they are and their magnitudes, then each slot in place.  Bit k of
+// rows as they are, all on their way at once, then their magnitudes, then each
+// slot in place.  Bit k of
 // `bad`: key k of this thread (its two of each key tile) has a value that is
 // not finite.
 template <int DT>
@@ -106,7 +108,7 @@ __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bf
                                           float& vscale, uint32_t& bad) {
   using L = Layout<DT>;
   constexpr int kKSlots = 2 * kHalves * L::kSteps;
-  uint32_t ktop = 0, vtop = 0;
+  const uint32_t slots = smem_addr(out) + (uint32_t)lane * 8;
 #pragma unroll 1
   for (int t = 0; t < 2 * kHalves; ++t) {
     const int key = key0 + t * 8 + g;
@@ -114,23 +116,33 @@ __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bf
 #pragma unroll
     for (int st = 0; st < L::kSteps; ++st) {
       const int dim = (st >> 2) * 64 + c * 16 + (st & 3) * 4;
-      const uint2 w = key < key_hi && dim < d ? *reinterpret_cast<const uint2*>(row + dim) : make_uint2(0, 0);
-      ktop = max(ktop, max(finite_top2(w.x), finite_top2(w.y)));
-      out[(t * L::kSteps + st) * 32 + lane] = w;
+      const bool on = key < key_hi && dim < d;
+      cp_async<8>(slots + (uint32_t)((t * L::kSteps + st) * 256), on ? row + dim : kt, on);
     }
   }
 #pragma unroll 1
   for (int k = 0; k < L::kVKeys; ++k) {  // half k / 4; keys 2c, 2c + 1, 8 + 2c, 9 + 2c of it
     const int key = key0 + (k >> 2) * 16 + 2 * c + (k & 1) + ((k >> 1) & 1) * 8;
     const bool on = key < key_hi && g * L::kVBytes < d;
-    const uint2* row = reinterpret_cast<const uint2*>(vt + (int64_t)(on ? key - sealed : 0) * d + g * L::kVBytes);
+    const __nv_bfloat16* row = on ? vt + (int64_t)(key - sealed) * d + g * L::kVBytes : vt;
 #pragma unroll
-    for (int w = 0; w < L::kVBytes / 4; ++w) {
-      const uint2 x = on ? row[w] : make_uint2(0, 0);
-      vtop = max(vtop, max(finite_top2(x.x), finite_top2(x.y)));
-      if (any_nonfinite2(x.x) || any_nonfinite2(x.y)) bad |= 1u << k;
-      out[(kKSlots + (k >> 2) * L::kTiles + 4 * w + (k & 3)) * 32 + lane] = x;
-    }
+    for (int w = 0; w < L::kVBytes / 4; ++w)
+      cp_async<8>(slots + (uint32_t)((kKSlots + (k >> 2) * L::kTiles + 4 * w + (k & 3)) * 256), row + (on ? w * 4 : 0),
+                  on);
+  }
+  cp_commit();
+  cp_wait<0>();
+  uint32_t ktop = 0, vtop = 0;
+#pragma unroll 8
+  for (int i = 0; i < kKSlots; ++i) {
+    const uint2 w = out[i * 32 + lane];
+    ktop = max(ktop, max(finite_top2(w.x), finite_top2(w.y)));
+  }
+#pragma unroll 8
+  for (int i = 0; i < kHalves * L::kTiles; ++i) {  // slot i: key (i / kTiles) * 4 + i % 4 of this thread
+    const uint2 x = out[(kKSlots + i) * 32 + lane];
+    vtop = max(vtop, max(finite_top2(x.x), finite_top2(x.y)));
+    if (any_nonfinite2(x.x) || any_nonfinite2(x.y)) bad |= 1u << (i / L::kTiles * 4 + (i & 3));
   }
   ktop = __reduce_max_sync(0xffffffffu, ktop);
   vtop = __reduce_max_sync(0xffffffffu, vtop);
