@@ -507,3 +507,32 @@ def test_heads_and_requests_that_share_memory(ops, rows):
         mass = ops.kv8_attention_mass(q, lse, cache, bits, prefix, torch.zeros(b, h, 390, device=DEV))
         wmass = ref.mass(q, wlse, kk, vis, 128 ** -0.5)
         assert bool(((mass.double().cpu() - wmass).abs() <= 4e-4 * wmass + 2.0 ** -22 * (1 + wmass)).all())
+
+
+@pytest.mark.parametrize("rows", [1, 9, 70, 130])
+def test_scores_that_rise_and_fall_along_the_cache(ops, rows):
+    """Each block's scores lie far above (or below) the ones before, for every
+    second row the other way round: the reference maximum moves all the time.
+    Scores reach 30 here, so their partial sums stay below the 64 that the
+    log-sum-exp's tolerance was derived for."""
+    b, hq, hkv, d, sealed, tail = 1, 2, 1, 128, 1408, 70
+    g = torch.Generator().manual_seed(rows)
+    u = torch.where(torch.rand(d, generator=g) < 0.5, -1.0, 1.0)
+    size = torch.linspace(-2.5, 2.5, sealed + tail)
+    size[::7] *= 0.5
+    k = (size[:, None] * u + 0.05 * torch.randn(sealed + tail, d, generator=g)).to(torch.bfloat16)[None, None]
+    v = torch.randn(1, 1, sealed + tail, d, generator=g).to(torch.bfloat16)
+    codes, scale = zip(*(ref.seal(x[:, :, :sealed], 64) for x in (k, v)))
+    cache = ops.Kv8Rows(*(c.float().to(ref.E4M3).to(DEV) for c in codes), *(s.float().to(DEV) for s in scale), sealed,
+                        *(x[:, :, sealed:].contiguous().to(DEV) for x in (k, v)), 64)
+    k, v = opened(cache)
+    sign = torch.where(torch.arange(rows) % 2 == 0, 1.0, -1.0) * torch.linspace(1.0, 0.3, rows)
+    q = (sign[None, None, :, None] * u).expand(b, hq, rows, d).to(torch.bfloat16).contiguous().to(DEV)
+    bits, prefix, vis = masks("any", b, rows, sealed + tail, 3)
+    for use, pre, seen in ((bits, prefix, vis), (None, sealed + tail, torch.ones_like(vis))):
+        out, lse = ops.kv8_tree_attention(q, cache, use, pre, return_lse=True)
+        want, wlse = ref.attention(q, k, v, seen, d ** -0.5)
+        check_attention(out, lse, want, wlse, float(v.abs().max()))
+        mass = ops.kv8_attention_mass(q, lse, cache, use, pre, torch.zeros(b, hkv, sealed + tail, device=DEV))
+        wmass = ref.mass(q, wlse, k, seen, d ** -0.5)
+        assert bool(((mass.double().cpu() - wmass).abs() <= 4e-4 * wmass + 2.0 ** -22 * (1 + wmass)).all())
