@@ -822,7 +822,8 @@ SF_API int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int64_t 
  * weight that each cached token received in a pass: the sum over the query
  * heads of its KV head and the rows that see it of exp(scale * q . k - lse),
  * lse [batch, num_heads, q_len] as sf_kv8_tree_attention returned it.  Rows
- * with lse -infinity add nothing.  Only the key side of `rows` is read.
+ * with lse -infinity add nothing (but NaN to a visible key that holds one).
+ * Only the key side of `rows` is read; requests and heads of mass lie apart.
  * workspace (16-byte aligned): sf_kv8_mass_workspace_bytes(...) bytes, perhaps 0.
  */
 SF_API size_t sf_kv8_mass_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim,
