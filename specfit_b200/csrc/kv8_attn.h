@@ -84,6 +84,7 @@ int kv8_key_map(CUtensorMap* map, const Kv8Rows& c, int batch);
 
 // The mass on tcgen05 (kv8_mass_tc.cu).
 bool kv8_mass_use_tc(int head_dim, int64_t packed_rows);
+size_t kv8_mass_tc_bytes(int64_t heads, int64_t packed_rows, int64_t sealed, int64_t kv_len);
 int kv8_mass_tc(const Kv8Attn& p, float* mass, int64_t m_bs, int64_t m_hs, void* prep, cudaStream_t stream);
 int kv8_mass_tc_status(int* status, int reset);
 int kv8_tc_status(int* status, int reset);

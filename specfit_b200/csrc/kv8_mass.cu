@@ -221,7 +221,7 @@ extern "C" size_t sf_kv8_mass_workspace_bytes(int batch, int num_heads, int num_
     return 0;
   const int64_t packed = (int64_t)(num_heads / num_kv_heads) * q_len;
   if (!kv8_mass_use_tc(head_dim, packed)) return 0;
-  return kv8_prep_layout(nullptr, nullptr, true, (int64_t)batch * num_kv_heads, packed, sealed, sealed + tail);
+  return kv8_mass_tc_bytes((int64_t)batch * num_kv_heads, packed, sealed, sealed + tail);
 }
 
 extern "C" int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int64_t q_head_stride,

@@ -13,6 +13,8 @@
 //     memory while the head stays the same (a 65-row tree has five).
 //   * D[128 keys x 128 rows] goes to one of four TMEM buffers; two lanes of
 //     eight warps take them in turn, two threads a key, 64 rows each.
+//   * A cache too short for all SMs: the query tiles are dealt out in parts, whose
+//     sums a second kernel adds to the mass, again in one order.
 //   * At a block's end one warp adds the four partial sums of a key, in one
 //     order, so the same inputs give the same bits.
 // What it measured: 8 requests of 65 rows, 32 heads, over 4,161 tokens 47 us (the
@@ -66,7 +68,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __global__ void __launch_bounds__(kThreads, 1)
 kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep w, float* __restrict__ mass,
-                   int64_t m_bs, int64_t m_hs, int nblocks, int per_cta) {
+                   int64_t m_bs, int64_t m_hs, int nblocks, int per_cta, int tiles_part, float* __restrict__ parts) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ uint8_t smem_raw[];
@@ -79,7 +81,9 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = p.batch * p.c.hkv * nblocks;  // (head, block), the head first
   const int u0 = min(units, (int)blockIdx.x * per_cta), u1 = min(units, u0 + per_cta);
-  const bool resident = w.tiles <= kQStages;
+  // This CTA's query tiles: all of them, or one part (then its sums go to `parts`).
+  const int t0 = blockIdx.y * tiles_part, tiles = min(tiles_part, w.tiles - t0);
+  const bool resident = tiles <= kQStages;
   const int sealed = (int)p.c.sealed;
 
   if (threadIdx.x == 0) {
@@ -141,14 +145,15 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
           ++nlo;
         }
         if (resident && u != u0 && blk != 0) continue;  // the head's tiles are here
-        for (int i = 0; ok && i < w.tiles; ++i, ++n) {
+        for (int i = 0; ok && i < tiles; ++i, ++n) {
           const int s = n % kQStages;
+          const int64_t at = (int64_t)bh * w.tiles + t0 + i;
           ok = ptx::mbar_wait(&tail->q_empty[s], ((n / kQStages) & 1) ^ 1, abort_flag, &g_kv8_mass_status, 63);
           if (!ok) break;
           ptx::mbar_arrive_expect_tx(&tail->q_full[s], kTileBytes + (uint32_t)sizeof(tail->rowc[0]));
-          ptx::bulk_load(q_s + s * kTileBytes, w.q + ((int64_t)bh * w.tiles + i) * kTileBytes, kTileBytes,
+          ptx::bulk_load(q_s + s * kTileBytes, w.q + at * kTileBytes, kTileBytes,
                          &tail->q_full[s]);
-          ptx::bulk_load(tail->rowc[s], w.rowc + ((int64_t)bh * w.tiles + i) * 2 * kBM, sizeof(tail->rowc[0]),
+          ptx::bulk_load(tail->rowc[s], w.rowc + at * 2 * kBM, sizeof(tail->rowc[0]),
                          &tail->q_full[s]);
         }
       }
@@ -169,7 +174,7 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       int n0 = 0, nk = 0, nlo = 0, m = 0;  // n0: the load number of this block's first tile
       for (int u = u0; ok && u < u1; ++u, ++nk) {
         const int blk = u % nblocks, key0 = blk * kKB;
-        if (u != u0 && (blk == 0 || !resident)) n0 += w.tiles;
+        if (u != u0 && (blk == 0 || !resident)) n0 += tiles;
         const bool last = !resident || u + 1 == u1 || blk + 1 == nblocks;  // of these tiles
         const bool mixed = key0 + kKB > sealed;
         const int ks = nk % kKStages;
@@ -178,7 +183,7 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
         if (!ok) break;
         const uint64_t khi = ptx::smem_desc_k_sw128(ptx::smem_u32(k_s + ks * kHalf));
         const uint64_t klo = ptx::smem_desc_k_sw128(ptx::smem_u32(lo_s));
-        for (int i = 0; ok && i < w.tiles; ++i, ++m) {
+        for (int i = 0; ok && i < tiles; ++i, ++m) {
           const int n = n0 + i, s = n % kQStages, buf = m % kBufs;
           ok = ptx::mbar_wait(&tail->q_full[s], (n / kQStages) & 1, abort_flag, &g_kv8_mass_status, 67) &&
                ptx::mbar_wait(&tail->d_empty[buf], ((m / kBufs) & 1) ^ 1, abort_flag, &g_kv8_mass_status, 68);
@@ -212,10 +217,11 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
     for (int u = u0; u < u1; ++u) {
       const int bh = u / nblocks, key = (u - bh * nblocks) * kKB + lane, nu = u - u0;
       const int kvh = bh % p.c.hkv, req = bh / p.c.hkv;
-      float* const to = mass + req * m_bs + kvh * m_hs + key;
+      float* const to = parts ? parts + ((int64_t)blockIdx.y * p.batch * p.c.hkv + bh) * p.kv_len + key
+                              : mass + req * m_bs + kvh * m_hs + key;
       float before[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) before[j] = key + j * 32 < p.kv_len ? to[j * 32] : 0.f;
+      for (int j = 0; j < 4; ++j) before[j] = !parts && key + j * 32 < p.kv_len ? to[j * 32] : 0.f;
       ok = ok && ptx::mbar_wait(&tail->part_full[nu & 1], (nu >> 1) & 1, abort_flag, &g_kv8_mass_status, 73);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -254,9 +260,9 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       const uint64_t kf2 = ptx::pack2(kf, kf);
       uint64_t acc[2] = {0, 0};
       int s = s0, phase = qphase;
-      for (int i = 0; i < w.tiles; ++i, ++m) {
+      for (int i = 0; i < tiles; ++i, ++m) {
         if ((m & 1) == t) {
-          const int buf = m % kBufs, row0 = i * kBM + half * 64;
+          const int buf = m % kBufs, row0 = (t0 + i) * kBM + half * 64;
           uint32_t seen[2] = {0, 0};  // rows row0 + lane and 32 on: which of the warp's keys they see
           if (!full) {
 #pragma unroll
@@ -345,6 +351,33 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
   }
 }
 
+// mass += the parts' sums, in order.  grid: (keys, batch * hkv).
+__global__ void __launch_bounds__(256)
+kv8_mass_add_kernel(const float* __restrict__ parts, int count, float* __restrict__ mass, int64_t m_bs, int64_t m_hs,
+                    int hkv, int kv_len) {
+  pdl_wait();
+  pdl_trigger();
+  const int bh = blockIdx.y, key = blockIdx.x * 256 + threadIdx.x;
+  if (key >= kv_len) return;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < count; ++i) sum += parts[((int64_t)i * gridDim.y + bh) * kv_len + key];
+  mass[(bh / hkv) * m_bs + (bh % hkv) * m_hs + key] += sum;
+}
+
+// A short cache has few blocks: its query tiles are then dealt out too, in
+// parts of at least two, so that no SM is idle (four heads, 641 tokens, 321 rows:
+// 19 us instead of 44; one part where the blocks fill the SMs).
+struct Parts {
+  int tiles, count;  // of a part; parts
+};
+Parts parts_of(int64_t units, int64_t tiles) {
+  const int64_t want = std::min<int64_t>(std::max<int64_t>(1, num_sms() / units), std::max<int64_t>(1, tiles / 2));
+  const int64_t per = (tiles + want - 1) / want;
+  return {(int)per, (int)((tiles + per - 1) / per)};
+}
+int64_t blocks_of(int64_t kv_len) { return (kv_len + kKB - 1) / kKB; }
+
 }  // namespace
 
 // Microseconds a call, this kernel's against the warp-level one's, four KV heads
@@ -354,6 +387,13 @@ kv8_mass_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
 //   96:             11 / 19 / 21 against 14 / 46 / 55
 bool kv8_mass_use_tc(int head_dim, int64_t packed) { return head_dim == kD && packed >= 64; }
 
+size_t kv8_mass_tc_bytes(int64_t heads, int64_t packed, int64_t sealed, int64_t kv_len) {
+  Kv8Prep w;
+  const size_t prep = kv8_prep_layout(&w, nullptr, true, heads, packed, sealed, kv_len);
+  const Parts parts = parts_of(heads * blocks_of(kv_len), w.tiles);
+  return prep + (parts.count > 1 ? (size_t)parts.count * heads * kv_len * sizeof(float) : 0);
+}
+
 int kv8_mass_tc(const Kv8Attn& p, float* mass, int64_t m_bs, int64_t m_hs, void* prep, cudaStream_t stream) {
   static std::atomic<unsigned long long> configured{0};
   if (int rc = once_per_device(configured, [] {
@@ -362,17 +402,26 @@ int kv8_mass_tc(const Kv8Attn& p, float* mass, int64_t m_bs, int64_t m_hs, void*
         return SF_OK;
       }))
     return rc;
-  const int64_t heads = (int64_t)p.batch * p.c.hkv, nblocks = ((int64_t)p.kv_len + kKB - 1) / kKB;
+  const int64_t heads = (int64_t)p.batch * p.c.hkv, nblocks = blocks_of(p.kv_len);
   SF_CHECK_ARG(heads * nblocks < (1 << 30), "too many keys for one call");
   Kv8Prep w;
-  kv8_prep_layout(&w, prep, true, heads, (int64_t)p.group * p.q_len, p.c.sealed, p.kv_len);
+  const size_t used = kv8_prep_layout(&w, prep, true, heads, (int64_t)p.group * p.q_len, p.c.sealed, p.kv_len);
+  const Parts parts = parts_of(heads * nblocks, w.tiles);
+  float* sums = parts.count > 1 ? reinterpret_cast<float*>(static_cast<uint8_t*>(prep) + used) : nullptr;
   if (int rc = kv8_prep(p, w, stream)) return rc;
   CUtensorMap tm_k;
   if (int rc = kv8_key_map(&tm_k, p.c, p.batch)) return rc;
   const int64_t units = heads * nblocks, per = (units + num_sms() - 1) / num_sms();
-  SF_CHECK_CUDA(launch_pdl(kv8_mass_tc_kernel, dim3((unsigned)((units + per - 1) / per)), dim3(kThreads), kSmemBytes,
-                           stream, tm_k, p, w, mass, m_bs, m_hs, (int)nblocks, (int)per));
+  SF_CHECK_CUDA(launch_pdl(kv8_mass_tc_kernel, dim3((unsigned)((units + per - 1) / per), (unsigned)parts.count),
+                           dim3(kThreads), kSmemBytes, stream, tm_k, p, w, mass, m_bs, m_hs, (int)nblocks, (int)per,
+                           parts.tiles, sums));
   SF_CHECK_LAUNCH();
+  if (sums) {
+    SF_CHECK_CUDA(launch_pdl(kv8_mass_add_kernel, dim3((unsigned)((p.kv_len + 255) / 256), (unsigned)heads), dim3(256),
+                             0, stream, static_cast<const float*>(sums), parts.count, mass, m_bs, m_hs, p.c.hkv,
+                             p.kv_len));
+    SF_CHECK_LAUNCH();
+  }
   return SF_OK;
 }
 
