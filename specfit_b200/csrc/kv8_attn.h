@@ -68,9 +68,9 @@ struct Kv8Prep {
   uint8_t* k;    // [bh][blocks][hi, lo], the blocks from key `first` on
   float* kf;     // [bh][blocks * 128]: a key's scale; NaN for a key that holds one
   // For attention (null otherwise):
-  uint8_t* v;    // [bh][blocks][128 keys x 128, fp16 in units of `unit`, swizzled]
+  uint8_t* v;    // [bh][blocks][128 keys x 128, fp16 in units of `vf`, swizzled]
+  float* vf;     // [bh][blocks * 128]: a value row's scale
   float* qf;     // [bh][tiles * 128]: the power of two taken out of a query row; NaN for a row that holds one
-  float* unit;   // [bh]: the largest V scale
   // For the mass (null otherwise):
   float* rowc;   // [bh][tiles][2][128]: that power times scale * log2(e); -lse * log2(e)
   int tiles, blocks, first;

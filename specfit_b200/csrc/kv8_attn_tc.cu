@@ -24,11 +24,13 @@
 //     shared-memory tiles, which a CTA copies whole.  Done by every CTA this
 //     took 18,000 clocks of set-up and 17,000 a tail block, and its code made
 //     the main loop's slower.
-//   * V is decoded to fp16 by four warps: one conversion and one multiply per
-//     two codes.  The values are in units of the largest V scale of the head's
-//     cache (its tail included), found first, so a block's factor is a power
-//     of two at most 1 and only what is below 2^-33 of the largest value
-//     is rounded.
+//   * V is decoded to fp16 by four warps, one conversion per two codes, exactly;
+//     a tail value's row has a power of two of its own.  These scales enter the
+//     exponent: P = 2^(s + log2 scale - reference), the reference a row's own
+//     maximum of s + log2 scale over the keys that it sees, and the sum of the
+//     probabilities is that of P times the inverse, a factor for 32 keys of one
+//     scale.  (A unit for the whole head, applied to V, made every block 0 that
+//     was 2^25 below the largest, a key that no row sees included.)
 //   * Codes come by TMA: K straight into the operand layout, V raw.  (Loaded
 //     into registers a block ahead they are waited for at the next proxy fence,
 //     which waits for every load of its warp: 2,200 clocks a block.)
@@ -37,10 +39,10 @@
 //     probabilities over scores that they have read, and the P V MMA takes A
 //     from there.  The two meet once a block, at a barrier that also says
 //     whether either half wants a larger reference.
-//   * O stays in TMEM.  A row's reference maximum moves only when the sum of
-//     64 probabilities, kept times 2^7, passes 2^15 (so none is too large for
-//     fp16), and O is read, scaled and written back in the first blocks and
-//     hardly ever after.  The maximum is not looked for otherwise.
+//   * O stays in TMEM.  A row's reference moves only when the sum of 64 P,
+//     kept times 2^7, passes 2^15 (so none is too large for fp16), and O is
+//     read, scaled and written back in the first blocks and hardly ever after.
+//     The maximum is not looked for otherwise.
 //   * Each lane has its own MMA warp: one that served both spent as long on
 //     waits, commits and descriptors as the tensor core on the products.  A lock
 //     keeps a lane's P V and next S together: interleaved, both lanes get their
@@ -85,11 +87,18 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kOCol = 256;
 constexpr float kMaxSum = 0x1p15f; // of a row's 64 probabilities of a block, before the reference moves
 constexpr float kPShift = 7.f;  // probabilities are kept times 2^7
+// Where neither |v| nor what a row's reference lies above its largest score
+// passes these, P 2^-v stands for the probability: the largest one's P is at least
+// 2^-80, so fp32 holds what is down to 2^-46 of it.
+constexpr float kMaxV = 40.f, kMaxAbove = 40.f;
 
 struct __align__(16) Tail {
   float red[2][2][kBM], sum[2][2][kBM];  // per lane, half and row: maxima and final sums, for the other half
   int pair_ok[kSoftmaxWarps];
-  float kf[4][kKB];  // per block (ring of 4) and key: scale * log2(e) * K scale; NaN for a key that holds one
+  // Per block (ring of 4) and key: scale * log2(e) * K scale (NaN for a key that
+  // holds one), v = log2 of the V scale times 2^7, 2^min(v, 0), 2^-max(v, 0); per 32
+  // keys, of the first: the first two, and 2^-v.
+  float4 key[4][kKB], group[4][kKB / 32];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t raw_full, raw_empty;
   uint64_t s_full[2], p_full[2];
@@ -125,21 +134,15 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
+// Eight codes as fp16.
+__device__ __forceinline__ uint4 decode8(const uint2& c) {
+  return make_uint4(e4m3x2_to_f16x2(c.x), e4m3x2_hi_to_f16x2(c.x), e4m3x2_to_f16x2(c.y), e4m3x2_hi_to_f16x2(c.y));
 }
-
-// Eight codes as fp16, times a power of two.
-__device__ __forceinline__ uint4 decode8(const uint2& c, uint32_t mul) {
-  return make_uint4(mul_f16x2(e4m3x2_to_f16x2(c.x), mul), mul_f16x2(e4m3x2_hi_to_f16x2(c.x), mul),
-                    mul_f16x2(e4m3x2_to_f16x2(c.y), mul), mul_f16x2(e4m3x2_hi_to_f16x2(c.y), mul));
-}
-// Eight bf16 values as fp16, times a power of two; non-finite ones become 0.
+// log2 of a power of two.
+__device__ __forceinline__ int log2_scale(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }
+// Eight bf16 values as fp16, times a power of two.
 __device__ __forceinline__ uint32_t tail2(uint32_t w, float inv) {
-  const float lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u);
-  return pack_f16x2(fabsf(lo) < INFINITY ? lo * inv : 0.f, fabsf(hi) < INFINITY ? hi * inv : 0.f);
+  return pack_f16x2(__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xffff0000u) * inv);
 }
 __device__ __forceinline__ uint4 tail8(const uint4& x, float inv) {
   return make_uint4(tail2(x.x, inv), tail2(x.y, inv), tail2(x.z, inv), tail2(x.w, inv));
@@ -190,7 +193,7 @@ __device__ __forceinline__ float scaled_max(const float (&x)[16], float f) {
   a = fmaxf(a, d);
   return a == -INFINITY ? a : a * f;
 }
-// 16 scores to probabilities 2^(f x - base), as fp16 pairs, and their sums.
+// 16 scores to 2^(f x - base), as fp16 pairs, and their sums.
 __device__ __forceinline__ void probabilities(const float (&x)[16], float f, float base, uint64_t (&ls)[2],
                                               uint32_t* pk) {
   const uint64_t f2 = ptx::pack2(f, f), b2 = ptx::pack2(-base, -base);
@@ -203,16 +206,44 @@ __device__ __forceinline__ void probabilities(const float (&x)[16], float f, flo
     pk[j / 2] = pack_f16x2(p0, p1);
   }
 }
-// 16 scores scaled, key by key, -infinity where the row does not see the key;
-// returns the largest (NaN counts as the least).
-__device__ __forceinline__ float masked_scores(float (&x)[16], const float* kf, float qf, uint32_t vis) {
-  float mx = -INFINITY;
+// A key's constants, loaded where they are used: sixteen at once cost 64 registers.
+__device__ __forceinline__ float4 load_key(const float4* key) {
+  float4 k;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(k.x), "=f"(k.y), "=f"(k.z), "=f"(k.w)
+               : "r"(ptx::smem_u32(key)));
+  return k;
+}
+// The same key by key, 0 where the row does not see the key; `ls` sums the
+// probabilities, `ps` P.  One exponential for both, of the larger of the two, so
+// that it is not lost where the other is far below.
+__device__ __forceinline__ void weighed(const float (&x)[16], const float4* key, float qf, uint32_t vis, float base,
+                                        float& ls, float& ps, uint32_t* pk) {
+#pragma unroll
+  for (int j = 0; j < 16; j += 2) {
+    float p[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 k = load_key(key + j + i);
+      const float y = (vis >> (j + i)) & 1u ? ex2(x[j + i] * (k.x * qf) - (base - fmaxf(k.y, 0.f))) : 0.f;
+      ls = fmaf(y, k.w, ls);
+      p[i] = y * k.z;
+      ps += p[i];
+    }
+    pk[j / 2] = pack_f16x2(p[0], p[1]);
+  }
+}
+// The largest of 16 scores (mx) and of their sums with v (mv), of the keys that
+// the row sees (NaN counts as the least).
+__device__ __forceinline__ void masked_max(const float (&x)[16], const float4* key, float qf, uint32_t vis, float& mx,
+                                           float& mv) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    x[j] = (vis >> j) & 1u ? x[j] * (kf[j] * qf) : -INFINITY;
-    mx = fmaxf(mx, x[j]);
+    const float4 k = load_key(key + j);
+    const float y = (vis >> j) & 1u ? x[j] * (k.x * qf) : -INFINITY;
+    mx = fmaxf(mx, y);
+    mv = fmaxf(mv, y + k.y);
   }
-  return mx;
 }
 
 // Whether any of the 64 threads that meet at barrier `id` says so.
@@ -242,15 +273,12 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 // The query head (within its group) of packed row n: n / q_len.
 __device__ __forceinline__ int row_head(const Kv8Attn& p, int n) { return (int)(((uint64_t)n * p.q_magic) >> 40); }
 
-constexpr int kScan = 16;  // loads of a thread under way while it looks for the unit
-
-// grid: (blocks that are not codes alone (one CTA for the unit alone if there
-// are none), which take longest, then query tiles; batch * hkv).
+// grid: (blocks that are not codes alone, which take longest, then query tiles;
+// batch * hkv).
 __global__ void __launch_bounds__(256, 2)
 kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float tops[8];
   const int bh = blockIdx.y, kvh = bh % p.c.hkv, req = bh / p.c.hkv;
   const int row = threadIdx.x >> 3, part = threadIdx.x & 7;  // row of 32 in a pass, 16 dims of it
   const uint32_t at0 = sw128(row, part);                     // 32 rows on: 4,096 bytes
@@ -297,66 +325,35 @@ kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
     return;
   }
   const bool values = w.v != nullptr;
-  // The unit: every CTA that needs it finds it for itself.
-  const int sealed = (int)p.c.sealed, tail_rows = p.kv_len - sealed;
+  const int sealed = (int)p.c.sealed;
   const float* vsc = p.c.vs + req * p.c.s_bs + kvh * p.c.s_hs;
   const float* ksc = p.c.ks + req * p.c.s_bs + kvh * p.c.s_hs;
   const __nv_bfloat16* kt = p.c.kt + req * p.c.t_bs + kvh * p.c.t_hs;
   const __nv_bfloat16* vt = p.c.vt + req * p.c.t_bs + kvh * p.c.t_hs;
-  float unit = pow2f(kKv8MinExponent);
-#pragma unroll 4
-  for (int i = threadIdx.x; values && i < sealed >> p.c.block_shift; i += 256)
-    unit = fmaxf(unit, vsc[i]);  // NaN is passed over
-  uint32_t top = 0;
-  const int pieces = values ? tail_rows * (kD / 8) : 0;
-  for (int i0 = threadIdx.x; i0 < pieces; i0 += kScan * 256) {
-    uint4 x[kScan];
-#pragma unroll
-    for (int j = 0; j < kScan; ++j) {
-      const int i = i0 + j * 256;
-      x[j] = i < pieces ? *reinterpret_cast<const uint4*>(vt + (int64_t)i * 8) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int j = 0; j < kScan; ++j) {
-      const uint32_t in[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t lo = in[k] & 0x7fffu, hi = (in[k] >> 16) & 0x7fffu;
-        top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-      }
-    }
-  }
-  unit = fmaxf(unit, pow2f(kv8_exponent(top)));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) unit = fmaxf(unit, __shfl_xor_sync(0xffffffffu, unit, o));
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = unit;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) unit = fmaxf(unit, tops[i]);
   const int blk = blockIdx.x;
-  if (values && blk == 0 && threadIdx.x == 0) w.unit[bh] = unit;
-  if (blk >= w.blocks) return;
-  const float inv = 1.f / unit;  // exact
   const uint8_t* kc = p.c.k + req * p.c.c_bs + kvh * p.c.c_hs + part * 16;
   const uint8_t* vc = p.c.v + req * p.c.c_bs + kvh * p.c.c_hs + part * 8;  // dims 8 part .. and 64 + 8 part ..
   uint8_t* kimg = w.k + ((int64_t)bh * w.blocks + blk) * kTileBytes + at0;
   uint8_t* vimg = w.v + ((int64_t)bh * w.blocks + blk) * kTileBytes + at0;
   float* kf = w.kf + ((int64_t)bh * w.blocks + blk) * kKB;
+  float* vf = w.vf + ((int64_t)bh * w.blocks + blk) * kKB;
   const int key0 = w.first + blk * kKB;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int key = key0 + u * 32 + row;
     uint4 a = make_uint4(0, 0, 0, 0), c = a, x = a, y = a;
-    float f = 1.f;
+    float f = 1.f, fv = 1.f;
     if (key0 + u * 32 < sealed) {  // the 32 rows of a pass are all codes or all tail
       a = *reinterpret_cast<const uint4*>(kc + (int64_t)key * kD);
       f = ksc[key >> p.c.block_shift];
       if (values) {
-        const float vs = vsc[key >> p.c.block_shift];
-        if (vs != vs) f = vs;
-        const float r = vs == vs ? vs * inv : 0.f;  // a block with a NaN counts as zeros
-        x = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD), pack_f16x2(r, r));
-        y = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD + 64), pack_f16x2(r, r));
+        fv = vsc[key >> p.c.block_shift];
+        if (fv != fv) {  // rows that see the key answer NaN; its codes are zeros
+          f = fv;
+          fv = 1.f;
+        }
+        x = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD));
+        y = decode8(*reinterpret_cast<const uint2*>(vc + (int64_t)key * kD + 64));
       }
       *reinterpret_cast<uint4*>(kimg + u * 4096) = a;
       *reinterpret_cast<uint4*>(kimg + u * 4096 + kHalf) = c;  // codes have no lower part
@@ -372,23 +369,29 @@ kv8_prep_kernel(Kv8Attn p, Kv8Prep w) {
       }
       uint32_t in[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
       const uint32_t vals[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-      const uint32_t ktop = row_top(in);
-      const bool nan = max(ktop, row_top(vals)) >= 0x7f80u;  // rows that see the key answer NaN
+      const uint32_t ktop = row_top(in), vtop = row_top(vals);
+      const bool nan = max(ktop, vtop) >= 0x7f80u;  // rows that see the key answer NaN
       if (nan) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) in[j] = 0;
+        x = y = make_uint4(0, 0, 0, 0);
       }
       const int e = nan ? 0 : kv8_exponent(ktop);
       split_store(in, pow2f(-e), kimg + u * 4096, kimg + u * 4096 + kHalf);
       f = nan ? __int_as_float(0x7fc00000) : pow2f(e);
-      x = tail8(x, inv);
-      y = tail8(y, inv);
+      const int ev = nan ? 0 : kv8_exponent(vtop);
+      fv = pow2f(ev);
+      x = tail8(x, pow2f(-ev));
+      y = tail8(y, pow2f(-ev));
     }
     if (values) {
       *reinterpret_cast<uint4*>(vimg + u * 4096) = x;
       *reinterpret_cast<uint4*>(vimg + u * 4096 + kRegion) = y;
     }
-    if (part == 0) kf[u * 32 + row] = f;
+    if (part == 0) {
+      kf[u * 32 + row] = f;
+      if (values) vf[u * 32 + row] = fv;
+    }
   }
 }
 
@@ -560,33 +563,32 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
     const int row = ct >> 3, part = ct & 7;  // row of 16 in a pass, 8 + 8 dims of it
     const float* ksc = p.c.ks + req * p.c.s_bs + kvh * p.c.s_hs;
     const float* vsc = p.c.vs + req * p.c.s_bs + kvh * p.c.s_hs;
-    float ks = 0.f, vs[4];  // scale of key ct of the next block; V scales of this one
+    float ks = 0.f, vs = 1.f;  // scales of key ct of the next block
     auto load_ks = [&](int b) {
       const int key = key_lo + b * kKB + ct;
       if (b < coded) {
-        const float y = vsc[key >> p.c.block_shift];
-        ks = y == y ? ksc[key >> p.c.block_shift] : y;  // a block with a NaN among its values: NaN scores
+        vs = vsc[key >> p.c.block_shift];
+        ks = ksc[key >> p.c.block_shift];
+        if (vs != vs) {  // a block with a NaN among its values: NaN scores, zero codes
+          ks = vs;
+          vs = 1.f;
+        }
       } else {
         ks = w.kf[(int64_t)bh * w.blocks * kKB + (key - w.first)];
+        vs = w.vf[(int64_t)bh * w.blocks * kKB + (key - w.first)];
       }
     };
-    auto load_vs = [&](int b) {
-      if (b >= coded) return;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) vs[g] = vsc[(key_lo + b * kKB + g * 32) >> p.c.block_shift];
-    };
-    if (nblocks > 0) {
-      load_ks(0);
-      load_vs(0);
-    }
-    const float inv = 1.f / w.unit[bh];  // exact
+    if (nblocks > 0) load_ks(0);
     // K of block b is on its way; here its scales.  False: a wait gave up.
     auto store_k = [&](int b) -> bool {
       const int s = b % kStages;
       if (!warp_wait(&tail->k_empty[s], ((b / kStages) & 1) ^ 1, abort_flag, 46)) return false;
       // Ring of four: block b - 4's softmax is over.  (The scores that freed this
       // stage, block b - 2's, were issued after P V of the lane's block before.)
-      tail->kf[b & 3][ct] = ks * p.scale_log2;
+      const float kf = ks * p.scale_log2;
+      const int v = log2_scale(vs) + (int)kPShift;
+      tail->key[b & 3][ct] = make_float4(kf, (float)v, pow2f(min(v, 0)), pow2f(-max(v, 0)));
+      if (lane == 0) tail->group[b & 3][ct >> 5] = make_float4(kf, (float)v, pow2f(-v), 0.f);
       warp_arrive(&tail->k_full[s]);
       return true;
     };
@@ -605,12 +607,6 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
         }
         return true;
       }
-      uint32_t mul[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float f = vs[g] == vs[g] ? vs[g] * inv : 0.f;  // a block with a NaN counts as zeros
-        mul[g] = pack_f16x2(f, f);
-      }
       // The two halves of a row, odd rows the upper one first: four rows of a
       // warp then cover all banks.
       const uint8_t* raw = raw_s + row * kD + part * 8;
@@ -621,8 +617,8 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       for (int u = 0; u < 8; ++u) {
         const uint2 a = *reinterpret_cast<const uint2*>(raw + u * 16 * kD + h0);
         const uint2 c = *reinterpret_cast<const uint2*>(raw + u * 16 * kD + h1);
-        *reinterpret_cast<uint4*>(to0 + u * 2048) = decode8(a, mul[u >> 1]);
-        *reinterpret_cast<uint4*>(to1 + u * 2048) = decode8(c, mul[u >> 1]);
+        *reinterpret_cast<uint4*>(to0 + u * 2048) = decode8(a);
+        *reinterpret_cast<uint4*>(to1 + u * 2048) = decode8(c);
       }
       warp_arrive(&tail->raw_empty);
       ptx::fence_proxy_async_smem();
@@ -642,7 +638,6 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
         if (b + 2 < nblocks) load_ks(b + 2);
       }
       ok = store_v(b);
-      if (ok && b + 1 < nblocks) load_vs(b + 1);
     }
     if (!ok && ct == 0) {  // copies of V that this thread asked for land before the CTA ends
       volatile int never = 0;
@@ -657,19 +652,16 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
     const int pr = (tile0 + (dual ? t : 0)) * kBM + r;
     const bool rok = pr < packed;
     const bool warp_ok = t < nlanes && pr - lane < packed;  // uniform over the pair of warps
-    const int qhead = rok ? row_head(p, pr) : 0, row = rok ? pr - qhead * p.q_len : 0;
-    const int head = kvh * p.group + qhead;
 
-    const int64_t bh = (int64_t)req * p.c.hkv + kvh;
-    const float qf = rok ? w.qf[bh * w.tiles * kBM + pr] : 0.f;
-    const float unit = w.unit[bh];
+    const float qf = rok ? w.qf[((int64_t)req * p.c.hkv + kvh) * w.tiles * kBM + pr] : 0.f;
 
     const uint32_t scol = tmem + ((uint32_t)(quad * 32) << 16) + t * kBM + half * 64;  // this half's scores
-    const uint32_t ocol = tmem + ((uint32_t)(quad * 32) << 16) + kOCol + t * kD + half * 64;
-    const uint32_t* rbits = p.bits ? p.bits + req * p.bits_bs + (int64_t)row * p.words : nullptr;
+    const uint32_t ocol = scol + kOCol;
+    const int row0 = rok ? pr - row_head(p, pr) * p.q_len : 0;
+    const uint32_t* rbits = p.bits ? p.bits + req * p.bits_bs + (int64_t)row0 * p.words : nullptr;
     const int n = t < nlanes ? lane_blocks(t) : 0;
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
+    float m = -INFINITY, l = 0.f;  // the reference (base 2) of O and of the sum of the probabilities
+    bool ok = true, close = true;  // close: the reference is not far above the row's scores (uniform over the warp)
     for (int i = 0; i < n; ++i) {
       const int b = block_of(t, i), key0 = key_lo + b * kKB + half * 64;
       const bool full = key0 + 64 <= p.prefix;  // no mask to read
@@ -679,38 +671,45 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       if (warp_ok) {
         // Every key visible and one scale per 32 of them: the rule in a long context.
         const bool plain = full && key0 + 64 <= (int)p.c.sealed;
-        const float* kf = tail->kf[b & 3] + half * 64;
+        const float4 *key = tail->key[b & 3] + half * 64, *group = tail->group[b & 3] + half * 2;
         uint32_t pk[32];  // 64 probabilities
-        // Once under the reference maximum as it is.  If the sum of a row's 64
-        // probabilities (in either half) passes 2^15, one of them may be too
-        // large for fp16: then (and for the first block) the maximum is found, and
-        // they are taken under it.  (A maximum in every pass was 36 of 230
-        // instructions.)  The scores stay in TMEM until the probabilities are
-        // settled.
+        // Once under the reference as it is.  If the sum of a row's 64 P (in
+        // either half) passes 2^15, one of them may be too large for fp16: then
+        // (and for the first block) the maximum is found, and they are taken
+        // under it.  (A maximum in every pass was 36 of 230 instructions.)  The
+        // scores stay in TMEM until the probabilities are settled.
         if (ok) ptx::tc_fence_after();
 #pragma unroll 1
         for (int pass = i == 0 ? 1 : 0;; ++pass) {
           if (pass) {
-            float mx = -INFINITY;
+            float mx = -INFINITY, mv = -INFINITY;
             if (ok) {
 #pragma unroll 1
               for (int c = 0; c < 4; ++c) {
                 float sc[16];
                 ptx::tmem_ld_16(scol + c * 16, sc);
-                mx = fmaxf(mx, plain ? scaled_max(sc, kf[(c >> 1) * 32] * qf)
-                                     : masked_scores(sc, kf + c * 16, qf, (uint32_t)(win >> (c * 16))));
+                if (plain) {
+                  const float y = scaled_max(sc, group[c >> 1].x * qf);
+                  mx = fmaxf(mx, y);
+                  mv = fmaxf(mv, y + group[c >> 1].y);
+                } else {
+                  masked_max(sc, key + c * 16, qf, (uint32_t)(win >> (c * 16)), mx, mv);
+                }
               }
             }
+            close = close && !__any_sync(0xffffffffu, mv > m && mv - mx > kMaxAbove);
             // The other half's maximum, and whether its wait succeeded: both warps
             // of the pair go on or stop together.
-            tail->red[t][half][r] = mx;
-            if (lane == 0) tail->pair_ok[warp] = ok ? 1 : 0;
+            tail->red[t][half][r] = mv;
+            if (lane == 0) tail->pair_ok[warp] = (ok ? 1 : 0) | (close ? 2 : 0);
             ptx::named_bar_sync(pair_bar, 64);
-            if (!tail->pair_ok[warp] || !tail->pair_ok[warp ^ 4]) {
+            const int both = tail->pair_ok[warp] & tail->pair_ok[warp ^ 4];
+            if (!(both & 1)) {
               ok = false;
               break;
             }
-            const float mnew = fmaxf(m, fmaxf(mx, tail->red[t][half ^ 1][r]));
+            close = both & 2;
+            const float mnew = fmaxf(m, fmaxf(mv, tail->red[t][half ^ 1][r]) - kPShift);
             const float alpha = m == -INFINITY ? 1.f : ex2(m - mnew);  // nothing summed yet: O and l are 0
             m = mnew;
             l *= alpha;
@@ -726,26 +725,43 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
               }
             }
           }
-          const float base = (m == -INFINITY ? 0.f : m) - kPShift;
-          float sum = 0.f;
+          const float base = m == -INFINITY ? 0.f : m;
+          float sum = 0.f, psum = 0.f;  // of the probabilities, and of P
           if (ok) {
-            uint64_t ls[2] = {0, 0};
+            if (plain && close && fmaxf(fabsf(group[0].y), fabsf(group[1].y)) <= kMaxV) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {  // 16 at a time: nothing is spilled
-              float sc[16];
-              ptx::tmem_ld_16(scol + c * 16, sc);
-              float f = 1.f;
-              if (plain)
-                f = kf[(c >> 1) * 32] * qf;
-              else
-                masked_scores(sc, kf + c * 16, qf, (uint32_t)(win >> (c * 16)));
-              probabilities(sc, f, base, ls, pk + c * 8);
+              for (int g = 0; g < 2; ++g) {
+                const float4 gr = group[g];
+                uint64_t ls[2] = {0, 0};
+#pragma unroll
+                for (int c = 2 * g; c < 2 * g + 2; ++c) {  // 16 at a time: nothing is spilled
+                  float sc[16];
+                  ptx::tmem_ld_16(scol + c * 16, sc);
+                  probabilities(sc, gr.x * qf, base - gr.y, ls, pk + c * 8);
+                }
+                float s0, s1;
+                ptx::unpack2(ptx::add2(ls[0], ls[1]), s0, s1);
+                psum += s0 + s1;
+                sum = fmaf(s0 + s1, gr.z, sum);
+              }
+            } else {
+              // Key by key: masked blocks, tail rows, scales far apart.  Not unrolled
+              // (the registers move down instead): four copies of this body made the path
+              // above it a quarter slower, by what was spilled.
+#pragma unroll
+              for (int j = 0; j < 32; ++j) pk[j] = 0;
+              const int chunks = __any_sync(0xffffffffu, win != 0) ? 4 : 0;  // 0: no row of the warp sees any of them
+#pragma unroll 1
+              for (int c = 0; c < chunks; ++c) {
+                float sc[16];
+                ptx::tmem_ld_16(scol + c * 16, sc);
+#pragma unroll
+                for (int j = 0; j < 24; ++j) pk[j] = pk[j + 8];
+                weighed(sc, key + c * 16, qf, (uint32_t)(win >> (c * 16)), base, sum, psum, pk + 24);
+              }
             }
-            float s0, s1;
-            ptx::unpack2(ptx::add2(ls[0], ls[1]), s0, s1);
-            sum = s0 + s1;
           }
-          if (pass || !pair_any(pair_bar, !ok || !(sum <= kMaxSum) || (m == -INFINITY && rok))) {
+          if (pass || !pair_any(pair_bar, !ok || !(psum <= kMaxSum) || (m == -INFINITY && rok))) {
             l += sum;
             break;
           }
@@ -769,12 +785,16 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
     if (ok && mine && nblocks > 0)  // also before shared memory is used again
       ok = warp_wait(&tail->mma_done, 0, abort_flag, 49);
     if (ok && mine && pr - lane < packed) {
+      const int qhead = rok ? row_head(p, pr) : 0, row = rok ? pr - qhead * p.q_len : 0;
+      const int head = kvh * p.group + qhead;
       ptx::tc_fence_after();
       const bool direct = p.splits == 1;
       const int part = dual ? range : 2 * range + t;
       const int64_t idx = (((int64_t)req * p.splits + part) * p.heads + head) * p.q_len + row;
-      float f = unit;  // O is in units of the largest V scale
-      if (direct) f = l == 0.f ? 0.f : f / l;
+      // P carries 2^7.  Partial results are in units in which the row's sum is about
+      // 1, wherever the scale of its values put the reference.
+      const int lx = !direct && l > 0.f && l < INFINITY ? max(-100, min(100, log2_scale(l))) : 0;
+      const float f = direct ? (l == 0.f ? 0.f : 0x1p-7f / l) : pow2f(-7 - lx);
       // Rows leave in whole lines: 32 rows x 32 columns at a time through this
       // warp's part of the K and V stages, which no MMA reads any more.
       const int64_t off = rok ? (direct ? (int64_t)req * p.out_bs + ((int64_t)row * p.heads + head) * kD : idx * kD) : -1;
@@ -824,14 +844,13 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
         }
       }
       if (rok && half == 0) {
-        const float ref = m == -INFINITY ? m : m - kPShift;  // l carries the 2^7
         if (direct) {
           if (p.lse)
             p.lse[((int64_t)req * p.heads + head) * p.q_len + row] =
-                l == 0.f ? -INFINITY : (m == -INFINITY ? l : (ref + log2f(l)) * 0.69314718055994531f);
+                l == 0.f ? -INFINITY : (m == -INFINITY ? l : (m + log2f(l)) * 0.69314718055994531f);
         } else {
-          p.part_ml[idx * 2] = ref;
-          p.part_ml[idx * 2 + 1] = l;
+          p.part_ml[idx * 2] = m + (float)lx;
+          p.part_ml[idx * 2 + 1] = l * pow2f(-lx);
         }
       }
     }
@@ -917,17 +936,16 @@ size_t kv8_prep_layout(Kv8Prep* w, void* base, bool for_mass, int64_t heads, int
   if (for_mass) {
     r.rowc = reinterpret_cast<float*>(take((size_t)heads * tiles * 2 * kBM * sizeof(float)));
   } else {
-    r.v = take((size_t)heads * std::max<int64_t>(blocks, 1) * kTileBytes);  // not null: values are laid out
+    r.v = take((size_t)heads * blocks * kTileBytes);  // not null even so: values are laid out
     r.qf = reinterpret_cast<float*>(take((size_t)heads * tiles * kBM * sizeof(float)));
-    r.unit = reinterpret_cast<float*>(take((size_t)heads * sizeof(float)));
+    r.vf = reinterpret_cast<float*>(take((size_t)heads * blocks * kKB * sizeof(float)));
   }
   if (w) *w = r;
   return used;
 }
 
 int kv8_prep(const Kv8Attn& p, const Kv8Prep& w, cudaStream_t stream) {
-  const int extra = w.v ? std::max(w.blocks, 1) : w.blocks;
-  const dim3 grid((unsigned)(w.tiles + extra), (unsigned)(p.batch * p.c.hkv));
+  const dim3 grid((unsigned)(w.tiles + w.blocks), (unsigned)(p.batch * p.c.hkv));
   SF_CHECK_CUDA(launch_pdl(kv8_prep_kernel, grid, dim3(256), 0, stream, p, w));
   SF_CHECK_LAUNCH();
   return SF_OK;

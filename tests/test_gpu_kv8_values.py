@@ -1,0 +1,152 @@
+"""The 8-bit KV cache's operators where magnitudes lie far apart: keys that a row
+does not see hold large finite values, and rows see values that are small beside
+others of the same cache.  Held to the bounds that ``kv8_bounds`` derives; the
+weight of a token to the relative error of its exponentials, 4e-4."""
+import math
+
+import pytest
+import torch
+
+import kv8_bounds as kb
+import kv8_reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from specfit_b200 import ops as _ops
+
+    return _ops
+
+
+def sealed_cache(ops, k, v, sealed, block):
+    """bf16 rows ``[B, Hkv, T, D]`` as a cache whose first ``sealed`` are codes."""
+    parts = []
+    for x in (k, v):
+        codes, scale = ref.seal(x[:, :, :sealed], block)
+        parts.append((codes.float().to(ref.E4M3).to(DEV), scale.float().to(DEV), x[:, :, sealed:].contiguous().to(DEV)))
+    (kc, ks, kt), (vc, vs, vt) = parts
+    return ops.Kv8Rows(kc, vc, ks, vs, sealed, kt, vt, block)
+
+
+def opened(rows):
+    return (ref.open_rows(rows.k_codes, rows.k_scale, rows.sealed, rows.k_tail, rows.block).to(DEV),
+            ref.open_rows(rows.v_codes, rows.v_scale, rows.sealed, rows.v_tail, rows.block).to(DEV))
+
+
+def pack(vis):
+    b, r, n = vis.shape
+    words = max(1, (n + 31) // 32)
+    w = torch.zeros(b, r, words * 32, dtype=torch.int64)
+    w[..., :n] = vis.long()
+    x = (w.view(b, r, words, 32) << torch.arange(32)).sum(-1)
+    return torch.where(x >= 1 << 31, x - (1 << 32), x).to(torch.int32).to(DEV)
+
+
+def draw(b, hq, hkv, rows, total, d, seed, k_size=1.0):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(b, hq, rows, d, generator=g).to(torch.bfloat16)
+    k = (k_size * torch.randn(b, hkv, total, d, generator=g)).to(torch.bfloat16)
+    v = torch.randn(b, hkv, total, d, generator=g).to(torch.bfloat16)
+    return q.to(DEV), k, v
+
+
+def compare(ops, q, cache, vis):
+    """Attention of one call against the definition."""
+    d = q.shape[-1]
+    k, v = opened(cache)
+    bits = pack(vis)
+    out, lse = ops.kv8_tree_attention(q, cache, bits, 0, return_lse=True)
+    want = kb.attention(q, k, v, vis.to(DEV), d ** -0.5)
+    assert kb.off(out, want) is None, kb.off(out, want)
+    assert kb.lse_off(lse, want) is None, kb.lse_off(lse, want)
+
+
+# Query heads of one KV head, rows, head_dim: what the form for many query rows takes.
+MANY = [(8, 9, 128), (8, 33, 128)]
+
+
+@pytest.mark.parametrize("hq,rows,d", MANY)
+@pytest.mark.parametrize("where", ["tail", "codes"])
+@pytest.mark.parametrize("size", [1e3, 1e9, 1e30])
+def test_large_values_of_an_unseen_key_stay_out_many_rows(ops, hq, rows, d, where, size):
+    unseen_large(ops, hq, rows, d, where, size, keys=False)
+
+
+def unseen_large(ops, hq, rows, d, where, size, keys):
+    sealed, tail, block = 448, 41, 64
+    total = sealed + tail
+    q, k, v = draw(1, hq, 1, rows, total, d, 11)
+    hidden = [sealed + 3, sealed + 20, total - 1] if where == "tail" else list(range(64, 128)) + [300]
+    vis = torch.ones(1, rows, total, dtype=torch.bool)
+    v[:, :, hidden] = size
+    if keys:
+        k[:, :, hidden] = size
+    if where == "codes":
+        hidden = list(range(64, 128)) + list(range(256, 320))  # whole blocks: a scale is a block's
+    vis[:, :, hidden] = False
+    compare(ops, q, sealed_cache(ops, k, v, sealed, block), vis)
+
+
+def test_rows_that_see_small_values_only_many_rows(ops):
+    small_beside_large(ops, 8, 16, 128)
+
+
+def small_beside_large(ops, hq, rows, d):
+    """Every second row sees the large values, the others only the small ones,
+    2^40 below."""
+    sealed, tail, block = 512, 70, 64
+    total = sealed + tail
+    q, k, v = draw(1, hq, 1, rows, total, d, 12)
+    large = torch.zeros(total, dtype=torch.bool)
+    large[128:256] = True
+    large[sealed + 10:sealed + 13] = True
+    v[:, :, large] = (v[:, :, large].float() * 2.0 ** 40).to(torch.bfloat16)
+    vis = torch.ones(1, rows, total, dtype=torch.bool)
+    vis[:, ::2, large] = False
+    compare(ops, q, sealed_cache(ops, k, v, sealed, block), vis)
+
+
+def test_values_that_shrink_while_scores_grow_many_rows(ops):
+    shrinking(ops, 8, 16, 128)
+
+
+def shrinking(ops, hq, rows, d):
+    """Blocks of values 2^6 smaller each, scores 3 higher each: the last blocks
+    decide the softmax, the first were the largest values."""
+    sealed, tail, block = 640, 30, 64
+    total = sealed + tail
+    q, k, v = draw(1, hq, 1, rows, total, d, 13, k_size=0.05)
+    u = torch.ones(d)
+    step = torch.arange(total) // block
+    k = (k.float() + step[None, None, :, None] * (3.0 / math.sqrt(d)) * u).to(torch.bfloat16)
+    q = (torch.ones_like(q.float()) + 0.05 * q.float()).to(torch.bfloat16)
+    v = (v.float() * torch.pow(2.0, -6.0 * step)[None, None, :, None]).to(torch.bfloat16)
+    cache = sealed_cache(ops, k, v, sealed, block)
+    vis = torch.ones(1, rows, total, dtype=torch.bool)
+    vis[:, 1::2, 320:] = False
+    compare(ops, q, cache, vis)
+
+
+@pytest.mark.parametrize("hq,hkv,rows,sealed,tail", [(32, 4, 65, 8192, 65), (8, 1, 300, 4096, 300),
+                                                     (16, 2, 100, 16384, 0)])
+def test_long_caches_many_rows(ops, hq, hkv, rows, sealed, tail):
+    long_cache(ops, hq, hkv, rows, sealed, tail, 128)
+
+
+def long_cache(ops, hq, hkv, rows, sealed, tail, d):
+    """Averages over thousands of keys are far smaller than the values."""
+    total = sealed + tail
+    g = torch.Generator(device=DEV).manual_seed(rows + sealed)
+    codes = [(torch.randn(1, hkv, sealed, d, generator=g, device=DEV) * 60).to(ref.E4M3) for _ in range(2)]
+    scale = [torch.full((1, hkv, sealed // 64), 2.0 ** -6, device=DEV) for _ in range(2)]
+    scale[1][:, :, ::3] = 2.0 ** -4
+    tails = [torch.randn(1, hkv, tail, d, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2)]
+    cache = ops.Kv8Rows(codes[0], codes[1], scale[0], scale[1], sealed, tails[0], tails[1], 64)
+    q = torch.randn(1, hq, rows, d, generator=g, device=DEV).to(torch.bfloat16)
+    vis = torch.ones(1, rows, total, dtype=torch.bool)
+    if tail >= rows:
+        vis[:, :, total - rows:] = torch.ones(rows, rows, dtype=torch.bool).tril()
+    compare(ops, q, cache, vis)
