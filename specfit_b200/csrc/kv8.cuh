@@ -75,6 +75,9 @@ inline Kv8Rows kv8_view(const sf_kv8_rows& r) {
 // 2^e as fp32, e in [-126, 127].
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// log2 of a power of two, rounded down for others.
+__device__ __forceinline__ int scale_log2(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }
+
 // The exponent of the power-of-two scale of a block whose largest magnitude
 // has the bf16 bits `top` (finite, sign cleared): 448 = 1.75 * 2^8.
 __device__ __forceinline__ int kv8_exponent(uint32_t top) {

@@ -29,12 +29,15 @@
 //     too once each row is scaled by a power of two (fp16's 11 bits hold
 //     bf16's 8 over 30 binades below the row's largest; what is smaller is
 //     below 2^-30 of it).  K's scale multiplies the fp32 scores.
-//   * V's scale: the accumulators are kept in units of the largest V scale so
-//     far; probabilities are multiplied by (block scale / unit) <= 1, a power
-//     of two, so only values below 2^-37 of the row's largest are rounded
-//     more than fp16's 11 bits (probabilities are kept times 2^12).
-//   * The reference maximum of a row moves only when a score exceeds it by
-//     more than 3 (base 2), so accumulators are rarely rescaled.
+//   * V's scale enters the exponent: P = 2^(s + log2 scale - m), so m, a row's own
+//     reference, is the largest of s + log2 scale among the keys that it sees,
+//     and only what is below 2^-26 of the row's largest probability times scale
+//     is rounded more than fp16's 11 bits (P is kept times 2^12).  One exponential
+//     gives P and the probability, the larger of the two, and the other by a
+//     power of two.  (A unit for a warp's accumulators, the largest scale that it
+//     had met, lost a row's small values beside large ones that the row did not see.)
+//   * m moves only when a score exceeds it by more than 3 (base 2), so
+//     accumulators are rarely rescaled.
 //   * What bounds it is a warp's chain of instructions (three warps a scheduler
 //     issue in one clock of four): of the 20 or so that 16 codes take, 6 are
 //     conversions (ALU, half rate) and 2 MMAs.  Hence 32 keys a step (645
@@ -46,10 +49,10 @@
 // more the merge.  (30 us while a tail unit's loads came a key after the other:
 // the last range's CTA ended late.)  Four CTAs an SM, with a ring of 12 KB a warp, took 37: each
 // has that cost, and a shorter range.
-// Tail units (bf16 rows: few) are scaled by a power of two per unit and
-// enter the same fragments.  A value row with a NaN or an infinity (a sealed
-// block of values that holds one) makes its key's score NaN, so that rows
-// which do not see it stay what they are.
+// Tail units (bf16 rows: few): a power of two per key is taken out of its row of K,
+// another out of its row of V, and they enter the same fragments.  A key with a NaN
+// or an infinity in either row (a sealed block that holds one) has a NaN score, so
+// that rows which do not see it stay what they are.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -96,16 +99,15 @@ struct Layout {
 };
 
 // A unit of tail rows as fp16 fragments in this thread's slots of `out`
-// ([K: key tiles x steps][V: halves x output tiles] of 32 lanes), scaled by
-// powers of two that are returned; zeros for keys from key_hi on.  First the
-// rows as they are, all on their way at once, then their magnitudes, then each
-// slot in place.  Bit k of
-// `bad`: key k of this thread (its two of each key tile) has a value that is
-// not finite.
+// ([K: key tiles x steps][V: halves x output tiles] of 32 lanes), each row scaled
+// by a power of two of its own; zeros for keys from key_hi on.  First the rows as
+// they are, all on their way at once, then their magnitudes, then each slot in
+// place.  For key i of the unit: kscale[i], the scale of its K row, NaN if that
+// holds a NaN or an infinity; vlog[i], log2 of its V row's, NaN likewise.
 template <int DT>
 __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bfloat16* vt, int key0, int sealed,
-                                          int key_hi, int d, int g, int c, int lane, uint2* out, float& kscale,
-                                          float& vscale, uint32_t& bad) {
+                                          int key_hi, int d, int g, int c, int lane, uint2* out, float* kscale,
+                                          float* vlog) {
   using L = Layout<DT>;
   constexpr int kKSlots = 2 * kHalves * L::kSteps;
   const uint32_t slots = smem_addr(out) + (uint32_t)lane * 8;
@@ -132,49 +134,86 @@ __device__ __forceinline__ void tail_unit(const __nv_bfloat16* kt, const __nv_bf
   }
   cp_commit();
   cp_wait<0>();
-  uint32_t ktop = 0, vtop = 0;
-#pragma unroll 8
-  for (int i = 0; i < kKSlots; ++i) {
-    const uint2 w = out[i * 32 + lane];
-    ktop = max(ktop, max(finite_top2(w.x), finite_top2(w.y)));
-  }
-#pragma unroll 8
-  for (int i = 0; i < kHalves * L::kTiles; ++i) {  // slot i: key (i / kTiles) * 4 + i % 4 of this thread
-    const uint2 x = out[(kKSlots + i) * 32 + lane];
-    vtop = max(vtop, max(finite_top2(x.x), finite_top2(x.y)));
-    if (any_nonfinite2(x.x) || any_nonfinite2(x.y)) bad |= 1u << (i / L::kTiles * 4 + (i & 3));
-  }
-  ktop = __reduce_max_sync(0xffffffffu, ktop);
-  vtop = __reduce_max_sync(0xffffffffu, vtop);
+  // Largest magnitudes (15-bit integers, two rows a register): of K rows t * 8 + g,
+  // whose dims a quad holds, and of V rows 2c, 2c + 1, 8 + 2c, 9 + 2c of a half,
+  // whose dims the eight lanes of a column hold.
+  uint32_t ktop[kHalves], vtop[2 * kHalves];
+  auto top_of = [](uint32_t t2) { return max(t2 & 0xffffu, t2 >> 16); };
 #pragma unroll
-  for (int off = 4; off < 32; off <<= 1) bad |= __shfl_xor_sync(0xffffffffu, bad, off);
-  const int ke = fit_exponent(ktop), ve = fit_exponent(vtop);
-  kscale = pow2f(ke);
-  vscale = pow2f(ve);
-  const float kinv = pow2f(-ke), vinv = pow2f(-ve);
-#pragma unroll 2
-  for (int i = 0; i < kKSlots; ++i) {
-    const uint2 w = out[i * 32 + lane];
-    out[i * 32 + lane] = make_uint2(pack_f16x2(bf_lo(w.x) * kinv, bf_hi(w.x) * kinv),
-                                    pack_f16x2(bf_lo(w.y) * kinv, bf_hi(w.y) * kinv));
+  for (int t = 0; t < kHalves; ++t) {
+    uint32_t a = 0, b = 0;
+#pragma unroll
+    for (int st = 0; st < L::kSteps; ++st) {
+      const uint2 x = out[((2 * t) * L::kSteps + st) * 32 + lane], y = out[((2 * t + 1) * L::kSteps + st) * 32 + lane];
+      a = __vmaxu2(__vmaxu2(a, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu);
+      b = __vmaxu2(__vmaxu2(b, y.x & 0x7fff7fffu), y.y & 0x7fff7fffu);
+    }
+    ktop[t] = top_of(a) | top_of(b) << 16;
   }
-#pragma unroll 1
-  for (int w = 0; w < kHalves * L::kTiles / 4; ++w) {
-    uint2* at = out + (kKSlots + 4 * w) * 32 + lane;
-    float f[4][4];
+#pragma unroll
+  for (int k = 0; k < 2 * kHalves; ++k) {
+    uint32_t a = 0, b = 0;
+#pragma unroll
+    for (int w = 0; w < L::kTiles / 4; ++w) {
+      const uint2* at = out + (kKSlots + (k >> 1) * L::kTiles + 4 * w + (k & 1) * 2) * 32 + lane;
+      const uint2 x = at[0], y = at[32];
+      a = __vmaxu2(__vmaxu2(a, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu);
+      b = __vmaxu2(__vmaxu2(b, y.x & 0x7fff7fffu), y.y & 0x7fff7fffu);
+    }
+    vtop[k] = top_of(a) | top_of(b) << 16;
+  }
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1)
+#pragma unroll
+    for (int t = 0; t < kHalves; ++t) ktop[t] = __vmaxu2(ktop[t], __shfl_xor_sync(0xffffffffu, ktop[t], off));
+#pragma unroll
+  for (int off = 4; off < 32; off <<= 1)
+#pragma unroll
+    for (int k = 0; k < 2 * kHalves; ++k) vtop[k] = __vmaxu2(vtop[k], __shfl_xor_sync(0xffffffffu, vtop[k], off));
+#pragma unroll
+  for (int t = 0; t < 2 * kHalves; ++t) {
+    const uint32_t top = (ktop[t >> 1] >> (16 * (t & 1))) & 0xffffu;
+    const bool bad = top >= 0x7f80u;
+    const int e = bad ? 0 : fit_exponent(top);
+    const float inv = pow2f(-e);
+    if (c == 0) kscale[t * 8 + g] = bad ? __int_as_float(0x7fc00000) : pow2f(e);
+#pragma unroll 4
+    for (int st = 0; st < L::kSteps; ++st) {
+      uint2* at = out + (t * L::kSteps + st) * 32 + lane;
+      const uint2 w = bad ? make_uint2(0, 0) : *at;
+      *at = make_uint2(pack_f16x2(bf_lo(w.x) * inv, bf_hi(w.x) * inv), pack_f16x2(bf_lo(w.y) * inv, bf_hi(w.y) * inv));
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h) {
+    float inv[4];
+    bool bad[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint2 u = at[k * 32];
-      f[k][0] = bf_lo(u.x);
-      f[k][1] = bf_hi(u.x);
-      f[k][2] = bf_lo(u.y);
-      f[k][3] = bf_hi(u.y);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[k][i] = fabsf(f[k][i]) < INFINITY ? f[k][i] * vinv : 0.f;
+      const uint32_t top = (vtop[2 * h + (k >> 1)] >> (16 * (k & 1))) & 0xffffu;
+      bad[k] = top >= 0x7f80u;
+      // Magnitudes below 2^9, like codes; a row of zeros counts as the smallest.
+      const int e = top == 0 ? -105 : fit_exponent(bad[k] ? 0 : top) + 5;
+      inv[k] = pow2f(-e);
+      if (g == 0) vlog[h * 16 + 2 * c + (k & 1) + (k >> 1) * 8] = bad[k] ? __int_as_float(0x7fc00000) : (float)e;
     }
+#pragma unroll 2
+    for (int w = 0; w < L::kTiles / 4; ++w) {
+      uint2* at = out + (kKSlots + h * L::kTiles + 4 * w) * 32 + lane;
+      float f[4][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) at[i * 32] = make_uint2(pack_f16x2(f[0][i], f[1][i]), pack_f16x2(f[2][i], f[3][i]));
+      for (int k = 0; k < 4; ++k) {
+        const uint2 u = bad[k] ? make_uint2(0, 0) : at[k * 32];
+        f[k][0] = bf_lo(u.x) * inv[k];
+        f[k][1] = bf_hi(u.x) * inv[k];
+        f[k][2] = bf_lo(u.y) * inv[k];
+        f[k][3] = bf_hi(u.y) * inv[k];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) at[i * 32] = make_uint2(pack_f16x2(f[0][i], f[1][i]), pack_f16x2(f[2][i], f[3][i]));
+    }
   }
+  __syncwarp();  // the scales, for the other lanes
 }
 
 // grid: (hkv, row tiles, splits * batch).  Full: D is DT.  Narrow: at most
@@ -189,6 +228,7 @@ kv8_attn_kernel(Kv8Attn p) {
   __shared__ float join_m[kWarps][kRows], join_l[kWarps][kRows];
   __shared__ float2 row_ml[kRows];  // of the CTA, for its cluster
   __shared__ __align__(16) uint4 q_frag[L::kSteps][32];
+  __shared__ float tail_k[kWarps][kUnit], tail_v[kWarps][kUnit];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -286,7 +326,6 @@ kv8_attn_kernel(Kv8Attn p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[t][i] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float unit = 0.f;  // o is in units of this V scale
 
   int stage = 0;
   for (int key0 = first; key0 < key_hi; key0 += kStep) {
@@ -308,16 +347,16 @@ kv8_attn_kernel(Kv8Attn p) {
     for (int t = 0; t < kSTiles; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
-    float kscale, vscale;
+    float kscale;
+    int v = 0;  // log2 of the V scale
     const bool coded = key0 < sealed;
-    uint32_t bad = 0;  // tail: bit k set when this thread's key k has a non-finite value
     if (coded) {
       kscale = ksc[key0 >> p.c.block_shift];
-      vscale = vsc[key0 >> p.c.block_shift];
-      if (vscale != vscale) {  // a block with a NaN among its values: its keys' scores are NaN
+      const float vscale = vsc[key0 >> p.c.block_shift];
+      if (vscale != vscale)  // a block with a NaN among its values: its keys' scores are NaN
         kscale = vscale;
-        vscale = unit;
-      }
+      else
+        v = scale_log2(vscale);
 #pragma unroll
       for (int j = 0; j < L::kKChunks; ++j) {
         uint32_t w[2 * kHalves][4];
@@ -349,7 +388,7 @@ kv8_attn_kernel(Kv8Attn p) {
         }
       }
     } else {
-      tail_unit<DT>(kt, vt, key0, sealed, key_hi, d, g, c, lane, tail_s, kscale, vscale, bad);
+      tail_unit<DT>(kt, vt, key0, sealed, key_hi, d, g, c, lane, tail_s, tail_k[warp], tail_v[warp]);
 #pragma unroll
       for (int st = 0; st < L::kSteps; ++st) {
         const uint4 qv = q_frag[st][lane];
@@ -368,41 +407,51 @@ kv8_attn_kernel(Kv8Attn p) {
           for (int t = 0; t < 2 * kHalves; ++t) mma_f16(s[t], qa, b[t].x, b[t].y);
         }
       }
-      // Bit i: this thread's key i (narrow: key g of key tile i, found by the quad's lane g / 2).
-      if constexpr (Narrow) {
-        const uint32_t w = __shfl_sync(0xffffffffu, bad, (lane & 28) | (g >> 1)) >> (g & 1);
-        bad = 0;
-#pragma unroll
-        for (int i = 0; i < kX; ++i) bad |= ((w >> (2 * i)) & 1u) << i;
-      }
     }
 
     // Scores in base 2, those not seen -infinity: keys 2c, 2c + 1 (narrow: g) of each key tile.
-    float x[2][kX], mx[2];
+    auto key_of = [&](int i) { return Narrow ? i * 8 + g : (i >> 1) * 8 + 2 * c + (i & 1); };
+    auto score = [&](int r, int i) { return s[i >> 1][Narrow ? 2 * (i & 1) + r : 2 * r + (i & 1)]; };
+    float x[2][kX], mx[2];  // mx: the largest, with log2 of its value's scale
     const bool open = key0 + kUnit <= p.prefix;  // no mask to read (prefix_len <= kv_len)
     bool grow = false;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float f = qs[r] * kscale;
-#pragma unroll
-      for (int i = 0; i < kX; ++i) x[r][i] = s[i >> 1][Narrow ? 2 * (i & 1) + r : 2 * r + (i & 1)] * f;
-    }
-    if (!open || bad) {
+    if (coded) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t w = open ? ~0u : (rok[r] ? (uint32_t)kv8_window(p, rbits[r], key0) : 0u);
+        const float f = qs[r] * kscale;
 #pragma unroll
-        for (int i = 0; i < kX; ++i) {
-          if ((bad >> i) & 1u) x[r][i] = __int_as_float(0x7fc00000);
-          if (!((w >> (Narrow ? i * 8 + g : (i >> 1) * 8 + 2 * c + (i & 1))) & 1u)) x[r][i] = -INFINITY;
-        }
+        for (int i = 0; i < kX; ++i) x[r][i] = score(r, i) * f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kX; ++i) {
+        const float vl = tail_v[warp][key_of(i)];
+        const float kf = vl == vl ? tail_k[warp][key_of(i)] : vl;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) x[r][i] = score(r, i) * (qs[r] * kf);
+      }
+    }
+    if (!open) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t w = rok[r] ? (uint32_t)kv8_window(p, rbits[r], key0) : 0u;
+#pragma unroll
+        for (int i = 0; i < kX; ++i)
+          if (!((w >> key_of(i)) & 1u)) x[r][i] = -INFINITY;
       }
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      mx[r] = x[r][0];
+      if (coded) {
+        mx[r] = x[r][0];
 #pragma unroll
-      for (int i = 1; i < kX; ++i) mx[r] = fmaxf(mx[r], x[r][i]);  // NaN is passed over
+        for (int i = 1; i < kX; ++i) mx[r] = fmaxf(mx[r], x[r][i]);  // NaN is passed over
+        mx[r] += (float)v;
+      } else {
+        mx[r] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kX; ++i) mx[r] = fmaxf(mx[r], x[r][i] + tail_v[warp][key_of(i)]);
+      }
       grow |= mx[r] > m[r] + kSlack;  // m -infinity: any score
     }
     float corr[2] = {1.f, 1.f};
@@ -420,18 +469,6 @@ kv8_attn_kernel(Kv8Attn p) {
         l[r] *= corr[r];
       }
     }
-    float pf = 1.f;  // this block's V scale in the accumulators' units
-    if (vscale != unit) {
-      if (vscale > unit) {  // a larger scale: the accumulators change units
-        const float f = unit / vscale;
-        corr[0] *= f;
-        corr[1] *= f;
-        unit = vscale;
-        rescale = true;
-      } else {
-        pf = vscale / unit;  // < 1
-      }
-    }
     if (rescale) {
 #pragma unroll
       for (int t = 0; t < kOTiles; ++t) {
@@ -442,27 +479,61 @@ kv8_attn_kernel(Kv8Attn p) {
       }
     }
     uint32_t pa[kHalves][4];
-    if constexpr (Narrow) {
-      const float base0 = (m[0] == -INFINITY ? 0.f : m[0]) - kPShift, base1 = (m[1] == -INFINITY ? 0.f : m[1]) - kPShift;
+    const float base0 = (m[0] == -INFINITY ? 0.f : m[0]) - kPShift, base1 = (m[1] == -INFINITY ? 0.f : m[1]) - kPShift;
+    if (coded) {
+      const float vh = (float)max(v, 0), pm = pow2f(min(v, 0)), em = pow2f(-max(v, 0));
+      float sum[2] = {0.f, 0.f};
+      if constexpr (Narrow) {
 #pragma unroll
-      for (int i = 0; i < kX; ++i) {
-        const float e0 = ex2(x[0][i] - base0), e1 = ex2(x[1][i] - base1);
-        l[0] += e0;
-        l[1] += e1;
-        // Key g, rows 2c and 2c + 1; turned: keys 2c and 2c + 1, row g.
-        pa[i >> 1][i & 1] = transpose_8x8(pack_f16x2(e0 * pf, e1 * pf));
+        for (int i = 0; i < kX; ++i) {
+          const float e0 = ex2(x[0][i] - (base0 - vh)), e1 = ex2(x[1][i] - (base1 - vh));
+          sum[0] += e0;
+          sum[1] += e1;
+          // Key g, rows 2c and 2c + 1; turned: keys 2c and 2c + 1, row g.
+          pa[i >> 1][i & 1] = transpose_8x8(pack_f16x2(e0 * pm, e1 * pm));
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float base = (r ? base1 : base0) - vh;
+#pragma unroll
+          for (int i = 0; i < kX; i += 2) {
+            const float e0 = ex2(x[r][i] - base), e1 = ex2(x[r][i + 1] - base);
+            sum[r] += e0 + e1;
+            pa[i >> 2][r + (i & 2)] = pack_f16x2(e0 * pm, e1 * pm);
+          }
+        }
       }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) l[r] = fmaf(sum[r], em, l[r]);
     } else {
+      auto weigh = [&](int i, float (&pr)[2]) {
+        const float vl = tail_v[warp][key_of(i)];
+        const int vi = vl == vl ? (int)vl : 0;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float base = (m[r] == -INFINITY ? 0.f : m[r]) - kPShift;
+        for (int r = 0; r < 2; ++r) {
+          const float y = ex2(x[r][i] - ((r ? base1 : base0) - (float)max(vi, 0)));
+          l[r] = fmaf(y, pow2f(-max(vi, 0)), l[r]);
+          pr[r] = y * pow2f(min(vi, 0));
+        }
+      };
+      if constexpr (Narrow) {
 #pragma unroll
-      for (int i = 0; i < kX; i += 2) {
-        const float e0 = ex2(x[r][i] - base), e1 = ex2(x[r][i + 1] - base);
-        l[r] += e0 + e1;
-        pa[i >> 2][r + (i & 2)] = pack_f16x2(e0 * pf, e1 * pf);
+        for (int i = 0; i < kX; ++i) {
+          float pr[2];
+          weigh(i, pr);
+          pa[i >> 1][i & 1] = transpose_8x8(pack_f16x2(pr[0], pr[1]));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kX; i += 2) {
+          float pr[2], pq[2];
+          weigh(i, pr);
+          weigh(i + 1, pq);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) pa[i >> 2][r + (i & 2)] = pack_f16x2(pr[r], pq[r]);
+        }
       }
-    }
     }
 
     // Output tile t, column g: dim g * kVBytes + t.
@@ -524,13 +595,18 @@ kv8_attn_kernel(Kv8Attn p) {
 
   // Join the four warps: rows' sums over the four threads of a quad, then
   // partial outputs through shared memory (the ring's space).
+  float unit[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
 #pragma unroll
     for (int off = Narrow ? 4 : 1; off < (Narrow ? 32 : 4); off <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], off);
+    // From here on in units in which a row's sum is about 1, wherever the scale of
+    // its values put the reference; P's 2^12 goes too.
+    const int lx = l[r] > 0.f && l[r] < INFINITY ? max(-100, min(100, scale_log2(l[r]) - (int)kPShift)) : 0;
+    unit[r] = pow2f(-(int)kPShift - lx);
     if (Narrow ? g == 0 : c == 0) {
-      join_m[warp][row_of(r)] = m[r];
-      join_l[warp][row_of(r)] = l[r];
+      join_m[warp][row_of(r)] = m[r] + (float)lx;
+      join_l[warp][row_of(r)] = l[r] * unit[r];
     }
   }
   __syncthreads();  // every warp is done with the ring
@@ -545,7 +621,7 @@ kv8_attn_kernel(Kv8Attn p) {
         // tile t: dim g * kVBytes + 2t + i.
         const float y = o[t][Narrow ? 2 * i + r : 2 * r + i];
         po[row_of(r) * DT + (Narrow ? g * L::kVBytes + 2 * t + i : (2 * c + i) * L::kVBytes + t)] =
-            unit > 0.f ? y * unit : y;
+            y * unit[r];
       }
   __syncthreads();
   constexpr int kPerRow = DT / 4, kJoinRows = Narrow ? 8 : kRows;
@@ -561,7 +637,7 @@ kv8_attn_kernel(Kv8Attn p) {
     *reinterpret_cast<uint2*>(p.out + req * p.out_bs + ((int64_t)t * p.heads + head) * d + col) = w;
     if (p.lse && col == 0)
       p.lse[((int64_t)req * p.heads + head) * p.q_len + t] =
-          sum == 0.f ? -INFINITY : (gm == -INFINITY ? sum : (gm - kPShift + log2f(sum)) * 0.69314718055994531f);
+          sum == 0.f ? -INFINITY : (gm == -INFINITY ? sum : (gm + log2f(sum)) * 0.69314718055994531f);
   };
   for (int i = threadIdx.x; i < kJoinRows * kPerRow; i += kWarps * 32) {
     const int row = i / kPerRow, col = (i % kPerRow) * 4;
@@ -594,7 +670,7 @@ kv8_attn_kernel(Kv8Attn p) {
       const int64_t idx = (((int64_t)req * p.splits + split) * p.heads + head) * p.q_len + t;
       *reinterpret_cast<float4*>(p.part_o + idx * d + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (col == 0) {
-        p.part_ml[idx * 2] = gm == -INFINITY ? gm : gm - kPShift;  // sums carry the 2^12
+        p.part_ml[idx * 2] = gm;
         p.part_ml[idx * 2 + 1] = sum;
       }
     }

@@ -138,8 +138,6 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 __device__ __forceinline__ uint4 decode8(const uint2& c) {
   return make_uint4(e4m3x2_to_f16x2(c.x), e4m3x2_hi_to_f16x2(c.x), e4m3x2_to_f16x2(c.y), e4m3x2_hi_to_f16x2(c.y));
 }
-// log2 of a power of two.
-__device__ __forceinline__ int log2_scale(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }
 // Eight bf16 values as fp16, times a power of two.
 __device__ __forceinline__ uint32_t tail2(uint32_t w, float inv) {
   return pack_f16x2(__uint_as_float(w << 16) * inv, __uint_as_float(w & 0xffff0000u) * inv);
@@ -586,7 +584,7 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       // Ring of four: block b - 4's softmax is over.  (The scores that freed this
       // stage, block b - 2's, were issued after P V of the lane's block before.)
       const float kf = ks * p.scale_log2;
-      const int v = log2_scale(vs) + (int)kPShift;
+      const int v = scale_log2(vs) + (int)kPShift;
       tail->key[b & 3][ct] = make_float4(kf, (float)v, pow2f(min(v, 0)), pow2f(-max(v, 0)));
       if (lane == 0) tail->group[b & 3][ct >> 5] = make_float4(kf, (float)v, pow2f(-v), 0.f);
       warp_arrive(&tail->k_full[s]);
@@ -793,7 +791,7 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       const int64_t idx = (((int64_t)req * p.splits + part) * p.heads + head) * p.q_len + row;
       // P carries 2^7.  Partial results are in units in which the row's sum is about
       // 1, wherever the scale of its values put the reference.
-      const int lx = !direct && l > 0.f && l < INFINITY ? max(-100, min(100, log2_scale(l))) : 0;
+      const int lx = !direct && l > 0.f && l < INFINITY ? max(-100, min(100, scale_log2(l))) : 0;
       const float f = direct ? (l == 0.f ? 0.f : 0x1p-7f / l) : pow2f(-7 - lx);
       // Rows leave in whole lines: 32 rows x 32 columns at a time through this
       // warp's part of the K and V stages, which no MMA reads any more.

@@ -53,9 +53,6 @@ __device__ __forceinline__ uint32_t finite_top2(uint32_t w) {
   const uint32_t lo = m & 0xffffu, hi = m >> 16;
   return max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u);
 }
-__device__ __forceinline__ bool any_nonfinite2(uint32_t w) {
-  return (w & 0x7fffu) >= 0x7f80u || (w & 0x7fff0000u) >= 0x7f800000u;
-}
 // Exponent of the power of two that brings magnitudes up to `top` (bf16
 // bits) below 2^14, bounded so that both it and its inverse are normal.
 __device__ __forceinline__ int fit_exponent(uint32_t top) {

@@ -68,6 +68,47 @@ def compare(ops, q, cache, vis):
 MANY = [(8, 9, 128), (8, 33, 128)]
 
 
+# What the forms for few take: at most eight packed rows, sixteen, more than one tile of them.
+FEW = [(8, 1, 128), (2, 3, 112), (1, 2, 64), (4, 3, 128), (5, 7, 48), (8, 9, 64)]
+
+
+@pytest.mark.parametrize("hq,rows,d", FEW)
+@pytest.mark.parametrize("where", ["tail", "codes"])
+@pytest.mark.parametrize("size", [1e4, 1e12, 1e30])
+def test_large_keys_and_values_of_an_unseen_key_stay_out(ops, hq, rows, d, where, size):
+    unseen_large(ops, hq, rows, d, where, size, keys=True)
+
+
+@pytest.mark.parametrize("hq,rows,d", [f for f in FEW if f[1] > 1])
+def test_rows_that_see_small_values_only(ops, hq, rows, d):
+    small_beside_large(ops, hq, rows, d)
+
+
+@pytest.mark.parametrize("hq,rows,d", FEW)
+def test_values_that_shrink_while_scores_grow(ops, hq, rows, d):
+    shrinking(ops, hq, rows, d)
+
+
+@pytest.mark.parametrize("hq,hkv,rows,sealed,tail,d", [(32, 4, 1, 65536, 33, 128), (32, 4, 8, 4096, 55, 128),
+                                                       (4, 1, 3, 1024, 20, 64), (16, 2, 40, 8192, 40, 64),
+                                                       (8, 8, 1, 2048, 90, 128)])
+def test_long_caches(ops, hq, hkv, rows, sealed, tail, d):
+    long_cache(ops, hq, hkv, rows, sealed, tail, d)
+
+
+def test_rows_of_zeros_and_tail_keys_far_apart(ops):
+    """Tail rows of quite different sizes, seen: rows of zeros, keys 2^20 apart."""
+    for hq, rows, d in FEW + MANY:
+        q, k, v = draw(1, hq, 1, rows, 150, d, 14)
+        k[:, :, 100::5] = (k[:, :, 100::5].float() * 2.0 ** -20).to(torch.bfloat16)
+        v[:, :, 96::3] = (v[:, :, 96::3].float() * 2.0 ** -50).to(torch.bfloat16)
+        k[:, :, 98], v[:, :, 99] = 0, 0
+        vis = torch.ones(1, rows, 150, dtype=torch.bool)
+        vis[:, -1] = False
+        vis[:, -1, 96::3] = True  # small values and a row of zeros only
+        compare(ops, q, sealed_cache(ops, k, v, 96, 32), vis)
+
+
 @pytest.mark.parametrize("hq,rows,d", MANY)
 @pytest.mark.parametrize("where", ["tail", "codes"])
 @pytest.mark.parametrize("size", [1e3, 1e9, 1e30])
