@@ -44,7 +44,7 @@ kv8_mass_kernel(MassParams mp) {
   const Kv8Attn& p = mp.a;
   constexpr int kSteps = DT / 16, kChunks = DT / 64;
   __shared__ __align__(16) uint4 qs_frag[kWarps][kSteps][32];
-  __shared__ float row_f[kChunkRows], row_lse[kChunkRows];
+  __shared__ float row_f[kChunkRows], row_lse[kChunkRows], tail_k[kWarps][kKeys];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.y % p.c.hkv, req = blockIdx.y / p.c.hkv;
@@ -84,8 +84,9 @@ kv8_mass_kernel(MassParams mp) {
     const int key0 = tile * kTileKeys + warp * kKeys;
     // This warp's keys as fp16 B fragments.
     uint32_t kf[2][kSteps][2];
-    float kscale = 1.f;
-    if (key0 < sealed) {
+    const bool coded = key0 < sealed;
+    float kscale = 1.f;  // of the codes; tail keys have theirs in shared memory
+    if (coded) {
       kscale = next_scale;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -100,30 +101,36 @@ kv8_mass_kernel(MassParams mp) {
           }
         }
     } else {
-      uint2 x[2][kSteps];
-      uint32_t top = 0;
+      // Tail rows: a power of two of its own for each, so that one which no row sees
+      // leaves the others what they are; NaN for one with a NaN or an infinity.
+      __syncwarp();  // the tile before has been read
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int key = key0 + t * 8 + g;
         const __nv_bfloat16* row = kt + (int64_t)(key - sealed) * d;
+        uint2 x[kSteps];
+        uint32_t top2 = 0;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
           const int dim = (s >> 2) * 64 + c * 16 + (s & 3) * 4;
-          x[t][s] = key < p.kv_len && dim < d ? *reinterpret_cast<const uint2*>(row + dim) : make_uint2(0, 0);
-          top = max(top, max(finite_top2(x[t][s].x), finite_top2(x[t][s].y)));
+          x[s] = key < p.kv_len && dim < d ? *reinterpret_cast<const uint2*>(row + dim) : make_uint2(0, 0);
+          top2 = __vmaxu2(__vmaxu2(top2, x[s].x & 0x7fff7fffu), x[s].y & 0x7fff7fffu);
         }
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const int e = fit_exponent(top);
-      kscale = pow2f(e);
-      const float inv = pow2f(-e);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
+        top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, 1));
+        top2 = __vmaxu2(top2, __shfl_xor_sync(0xffffffffu, top2, 2));
+        const uint32_t top = max(top2 & 0xffffu, top2 >> 16);
+        const bool bad = top >= 0x7f80u;
+        const int e = bad ? 0 : fit_exponent(top);
+        const float inv = pow2f(-e);
+        if (c == 0) tail_k[warp][t * 8 + g] = bad ? __int_as_float(0x7fc00000) : pow2f(e);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-          kf[t][s][0] = pack_f16x2(bf_lo(x[t][s].x) * inv, bf_hi(x[t][s].x) * inv);
-          kf[t][s][1] = pack_f16x2(bf_lo(x[t][s].y) * inv, bf_hi(x[t][s].y) * inv);
+          if (bad) x[s] = make_uint2(0, 0);
+          kf[t][s][0] = pack_f16x2(bf_lo(x[s].x) * inv, bf_hi(x[s].x) * inv);
+          kf[t][s][1] = pack_f16x2(bf_lo(x[s].y) * inv, bf_hi(x[s].y) * inv);
         }
+      }
+      __syncwarp();
     }
 
     float before[4];
@@ -177,10 +184,17 @@ kv8_mass_kernel(MassParams mp) {
             const uint32_t w = pr < packed ? (uint32_t)kv8_window(p, rbits, key0) : 0u;
             vis = ((w >> (2 * c)) & 3u) | (((w >> (8 + 2 * c)) & 3u) << 2);
           }
-          const float f = row_f[at] * kscale, lse = row_lse[at];  // rows past the last: lse +infinity
+          const float rf = row_f[at], lse = row_lse[at];  // rows past the last: lse +infinity
+          if (coded) {
+            const float f = rf * kscale;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if ((vis >> k) & 1u) acc[k] += ex2(s[k >> 1][2 * r + (k & 1)] * f - lse);
+            for (int k = 0; k < 4; ++k)
+              if ((vis >> k) & 1u) acc[k] += ex2(s[k >> 1][2 * r + (k & 1)] * f - lse);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if ((vis >> k) & 1u) acc[k] += ex2(s[k >> 1][2 * r + (k & 1)] * (rf * tail_k[warp][(k >> 1) * 8 + 2 * c + (k & 1)]) - lse);
+          }
         }
       }
     }

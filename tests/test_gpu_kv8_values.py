@@ -54,7 +54,7 @@ def draw(b, hq, hkv, rows, total, d, seed, k_size=1.0):
 
 
 def compare(ops, q, cache, vis):
-    """Attention of one call against the definition."""
+    """Attention and weights of one call against the definition."""
     d = q.shape[-1]
     k, v = opened(cache)
     bits = pack(vis)
@@ -62,6 +62,14 @@ def compare(ops, q, cache, vis):
     want = kb.attention(q, k, v, vis.to(DEV), d ** -0.5)
     assert kb.off(out, want) is None, kb.off(out, want)
     assert kb.lse_off(lse, want) is None, kb.lse_off(lse, want)
+    check_weights(ops, q, cache, vis, lse, want)
+
+
+def check_weights(ops, q, cache, vis, lse, want):
+    b, hkv = cache.shape[:2]
+    mass = ops.kv8_attention_mass(q, lse, cache, pack(vis), 0, torch.zeros(b, hkv, cache.length, device=DEV)).double()
+    bad = (mass - want["mass"]).abs() > 4e-4 * want["mass"] + 2.0 ** -100
+    assert not bool(bad.any()), (int(bad.sum()), mass[bad][:4], want["mass"][bad][:4])
 
 
 # Query heads of one KV head, rows, head_dim: what the form for many query rows takes.
@@ -94,6 +102,19 @@ def test_values_that_shrink_while_scores_grow(ops, hq, rows, d):
                                                        (8, 8, 1, 2048, 90, 128)])
 def test_long_caches(ops, hq, hkv, rows, sealed, tail, d):
     long_cache(ops, hq, hkv, rows, sealed, tail, d)
+
+
+@pytest.mark.parametrize("hq,rows,d", FEW + MANY)
+def test_weights_beside_a_large_unseen_key(ops, hq, rows, d):
+    """The weights alone, by the definition's log-sum-exp."""
+    sealed, tail = 128, 37
+    q, k, v = draw(1, hq, 1, rows, sealed + tail, d, 15)
+    k[:, :, sealed + 5] = 1e12
+    vis = torch.ones(1, rows, sealed + tail, dtype=torch.bool)
+    vis[:, :, sealed + 5] = False
+    cache = sealed_cache(ops, k, v, sealed, 64)
+    want = kb.attention(q, *opened(cache), vis.to(DEV), d ** -0.5)
+    check_weights(ops, q, cache, vis, want["lse"].float(), want)
 
 
 def test_rows_of_zeros_and_tail_keys_far_apart(ops):
