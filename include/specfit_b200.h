@@ -806,8 +806,9 @@ SF_API int sf_kv8_read(const sf_kv8_rows* rows, int64_t first, int64_t count, vo
  * tree_bits [batch, q_len, bit_words].  out [batch, q_len, num_heads,
  * head_dim] bf16; lse (nullable) [batch, num_heads, q_len]: the natural
  * log-sum-exp of a row's scaled scores.  A row that sees no key answers zeros
- * and -infinity.  A key with a NaN (or, in its value row, an infinity)
- * answers NaN to the rows that see it and to no other.  workspace (16-byte
+ * and -infinity.  A key whose row of K or of V holds a NaN or an infinity
+ * (sealed: whose block does) answers NaN to the rows that see it and to no other;
+ * a query row that holds one answers NaN.  workspace (16-byte
  * aligned): sf_kv8_attention_workspace_bytes(...) bytes, perhaps 0.
  */
 SF_API size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim,
@@ -822,7 +823,8 @@ SF_API int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int64_t 
  * weight that each cached token received in a pass: the sum over the query
  * heads of its KV head and the rows that see it of exp(scale * q . k - lse),
  * lse [batch, num_heads, q_len] as sf_kv8_tree_attention returned it.  Rows
- * with lse -infinity add nothing (but NaN to a visible key that holds one).
+ * with lse -infinity add nothing (but NaN to a visible key that holds a NaN or an
+ * infinity).
  * Only the key side of `rows` is read; requests and heads of mass lie apart.
  * workspace (16-byte aligned): sf_kv8_mass_workspace_bytes(...) bytes, perhaps 0.
  */

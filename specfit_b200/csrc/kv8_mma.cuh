@@ -47,12 +47,6 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-// Largest finite magnitude (15-bit integers) of two bf16; non-finite ones count as 0.
-__device__ __forceinline__ uint32_t finite_top2(uint32_t w) {
-  const uint32_t m = w & 0x7fff7fffu;
-  const uint32_t lo = m & 0xffffu, hi = m >> 16;
-  return max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u);
-}
 // Exponent of the power of two that brings magnitudes up to `top` (bf16
 // bits) below 2^14, bounded so that both it and its inverse are normal.
 __device__ __forceinline__ int fit_exponent(uint32_t top) {
@@ -64,28 +58,32 @@ __device__ __forceinline__ int fit_exponent(uint32_t top) {
 // of two that is returned: rows r = 0 (row g of the tile) and 1 (row g + 8).
 // The dims of k-step s are (s / 4) * 64 + c * 16 + (s % 4) * 4 + {0, 1, 2, 3},
 // the order in which a thread's 16-byte pieces of a key hold them.  `row`
-// null: zeros.  The four threads of a quad call this together.
+// null: zeros.  A row with a NaN or an infinity: zeros, and NaN is returned.  The
+// four threads of a quad call this together.
 template <int Steps>
 __device__ __forceinline__ float q_row_fragments(const __nv_bfloat16* row, int d, int c, uint32_t (&qf)[Steps][4],
                                                  int r) {
   uint2 x[Steps];
-  uint32_t top = 0;
+  uint32_t top2 = 0;  // two 15-bit magnitudes
 #pragma unroll
   for (int s = 0; s < Steps; ++s) {
     const int dim = (s >> 2) * 64 + c * 16 + (s & 3) * 4;
     x[s] = row && dim < d ? *reinterpret_cast<const uint2*>(row + dim) : make_uint2(0, 0);
-    top = max(top, max(finite_top2(x[s].x), finite_top2(x[s].y)));
+    top2 = __vmaxu2(__vmaxu2(top2, x[s].x & 0x7fff7fffu), x[s].y & 0x7fff7fffu);
   }
+  uint32_t top = max(top2 & 0xffffu, top2 >> 16);
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const int e = fit_exponent(top);
+  const bool bad = top >= 0x7f80u;
+  const int e = bad ? 0 : fit_exponent(top);
   const float inv = pow2f(-e);
 #pragma unroll
   for (int s = 0; s < Steps; ++s) {
+    if (bad) x[s] = make_uint2(0, 0);
     qf[s][r] = pack_f16x2(bf_lo(x[s].x) * inv, bf_hi(x[s].x) * inv);
     qf[s][r + 2] = pack_f16x2(bf_lo(x[s].y) * inv, bf_hi(x[s].y) * inv);
   }
-  return pow2f(e);
+  return bad ? __int_as_float(0x7fc00000) : pow2f(e);
 }
 
 }  // namespace sf

@@ -212,3 +212,40 @@ def long_cache(ops, hq, hkv, rows, sealed, tail, d):
     if tail >= rows:
         vis[:, :, total - rows:] = torch.ones(rows, rows, dtype=torch.bool).tril()
     compare(ops, q, cache, vis)
+
+
+@pytest.mark.parametrize("hq,rows,d", FEW + MANY)
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+def test_not_a_number_in_queries_and_keys(ops, hq, rows, d, what):
+    """A tail key whose K or V row holds one answers NaN to the rows that see it
+    (whatever the sign of the product), a query row that holds one answers NaN, and
+    the others stay what they are."""
+    sealed, tail = 64, 38
+    total = sealed + tail
+    q, k, v = draw(1, hq, 1, rows, total, d, 16)
+    clean = sealed_cache(ops, k, v, sealed, 32)
+    key, value = sealed + 7, sealed + 33
+    vis = torch.ones(1, rows, total, dtype=torch.bool)
+    vis[:, :, [key, value]] = False
+    want, wlse = ops.kv8_tree_attention(q, clean, pack(vis), 0, return_lse=True)
+    k[:, :, key, 3], v[:, :, value, d - 1] = what, what
+    cache = sealed_cache(ops, k, v, sealed, 32)
+    out, lse = ops.kv8_tree_attention(q, cache, pack(vis), 0, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, wlse)
+    for at in (key, value):
+        on = vis.clone()
+        on[:, 0, at] = True
+        out, lse = ops.kv8_tree_attention(q, cache, pack(on), 0, return_lse=True)
+        assert bool(torch.isnan(out[:, 0]).all()) and bool(torch.isnan(lse[:, :, 0]).all())
+        assert torch.equal(out[:, 1:], want[:, 1:]) and torch.equal(lse[:, :, 1:], wlse[:, :, 1:])
+    if rows > 1:
+        some = q.clone()
+        some[:, :, -1, d // 2] = what
+        out, lse = ops.kv8_tree_attention(some, cache, pack(vis), 0, return_lse=True)
+        assert bool(torch.isnan(out[:, -1]).all()) and bool(torch.isnan(lse[:, :, -1]).all())
+        assert torch.equal(out[:, :-1], want[:, :-1]) and torch.equal(lse[:, :, :-1], wlse[:, :, :-1])
+    # A weight per key: NaN for the seen key, none for those that no row sees.
+    on = vis.clone()
+    on[:, :, key] = True
+    mass = ops.kv8_attention_mass(q, wlse, cache, pack(on), 0, torch.zeros(1, 1, total, device=DEV))[0, 0]
+    assert bool(torch.isnan(mass[key])) and bool(torch.isfinite(mass[:key]).all()) and float(mass[value]) == 0
