@@ -96,6 +96,11 @@ class Kv8Layer(DynamicLayer):
         """Tokens that fit without a larger buffer."""
         return self._codes[0].shape[2] + self._kt.shape[2] if self._kt is not None else self._reserve
 
+    def layout(self):
+        """What a captured pass over this layer reads and writes by address: its
+        buffers, and how many rows are codes and tail."""
+        return (*self._codes, self._kt, self._vt), self.sealed, self.tail
+
     # --------------------------------------------------------------- a pass
     def begin(self, rows: int) -> None:
         """Makes room for ``rows`` more rows at tail row ``self.tail``.  What is

@@ -12,7 +12,10 @@ eager Hugging Face forward.
 The KV cache's committed prefix is not modified by a replay.  With a
 ``ReservedCache`` (or a ``Kv8Cache`` without a budget) the captured forward
 writes the tree's keys/values into the reserved rows after the prefix (the
-same rows on every replay) and the rollback is ``crop``.  With a plain ``DynamicCache`` the captured forward
+same rows on every replay) and the rollback is ``crop``.  An 8-bit cache replaces
+its buffers when a pass does not fit them and seals blocks as it grows: the
+graph keeps those that it was captured over, and ``replay`` refuses a cache that
+is not laid out as it was then.  With a plain ``DynamicCache`` the captured forward
 concatenates the prefix with the tree's keys/values into graph-owned
 buffers, exactly as an eager ``update`` followed by a rollback would; the
 prefix tensors are then kept alive for the graph's lifetime, and the cache
@@ -45,6 +48,7 @@ class VerifyGraph:
         if any(getattr(layer, "scored", False) for layer in kv_cache.layers):
             raise RuntimeError("VerifyGraph replays a pass at will: a cache that scores its passes cannot be captured")
         self._prefix = [(layer.keys, layer.values) for layer in kv_cache.layers]
+        self._held = []  # (layer, its layout) of the layers whose buffers may be replaced
         self.graph = None
         self.logits = None
         self.argmax = None
@@ -109,9 +113,15 @@ class VerifyGraph:
             self.logits, self.argmax = self._forward()
         clear_mask_cache()
         self._restore_prefix()
+        self._held = [(layer, layer.layout()) for layer in self.cache.layers if hasattr(layer, "layout")]
 
     def replay(self) -> torch.Tensor:
         """Runs the captured pass on the loaded inputs; returns the device
         argmax over the vocabulary per verification position."""
+        for layer, (buffers, *rows) in self._held:
+            now, *rows_now = layer.layout()
+            if rows_now != rows or any(a is not b for a, b in zip(now, buffers)):
+                raise RuntimeError("the cache is not laid out as it was captured: roll it back to the captured "
+                                   "length, or, if a pass has replaced its buffers, capture anew")
         self.graph.replay()
         return self.argmax

@@ -199,3 +199,26 @@ def test_speculative_decoding_over_the_8_bit_cache(target, budget):
         assert cache.dropped == 0 and cache.get_seq_length() == cache.next_position
     else:
         assert cache.get_seq_length() == budget and max(s[1] for s in seen[1:]) <= budget + 8
+
+
+def test_a_replay_over_replaced_buffers_is_refused(target):
+    cfg, m, state = target
+    fwd = LeanQwen3Forward(m.model)
+    ids = torch.randint(0, 512, (1, 100), generator=torch.Generator().manual_seed(3)).to(DEV)
+    cache = Kv8Cache(config=cfg, capacity=256, tail_room=16)
+    fwd(input_ids=ids, past_key_values=cache, use_cache=True)
+    inputs = tree_inputs(1, 100, 1)
+    g = VerifyGraph(m.model, cache, q_len=8, device=DEV, forward=fwd)
+    g.capture(*inputs)
+    want = g.replay().clone()
+    run(fwd, state, cache, ids[:, :70])  # wider than the tail
+    cache.crop(100)
+    with pytest.raises(RuntimeError, match="laid out"):
+        g.replay()
+    run(fwd, state, cache, ids[:, :1])
+    with pytest.raises(RuntimeError, match="laid out"):
+        g.replay()
+    cache.crop(100)
+    again = VerifyGraph(m.model, cache, q_len=8, device=DEV, forward=fwd)
+    again.capture(*inputs)
+    assert torch.equal(again.replay(), want)
