@@ -14,6 +14,10 @@
 // Compaction of 16 heads to 8,192 tokens each: 25 us, 2.7 TB/s; there the chain of a
 // CTA is what bounds it (indices, rows, the block's maximum, codes), of which
 // six fit on an SM, so its threads hold few registers and load all at once.
+#include <algorithm>
+#include <memory>
+#include <new>
+
 #include "kv8.cuh"
 
 namespace sf {
@@ -296,6 +300,81 @@ Target make_target(const sf_kv8_rows& r, int64_t first_block, int64_t full_block
   return t;
 }
 
+// Memory of one buffer: `extent` bytes for each of count[0] * count[1] * count[2]
+// pieces (requests, heads, rows that do not follow each other), stride bytes apart.
+struct Region {
+  const void* at = nullptr;
+  int64_t extent = 0, count[3] = {1, 1, 1}, stride[3] = {0, 0, 0};
+  int64_t pieces() const { return at == nullptr || extent <= 0 ? 0 : count[0] * count[1] * count[2]; }
+  uintptr_t start(int64_t n) const {
+    const int64_t k = n % count[2], j = n / count[2] % count[1], i = n / count[2] / count[1];
+    return reinterpret_cast<uintptr_t>(at) + (uintptr_t)(i * stride[0] + j * stride[1] + k * stride[2]);
+  }
+  // From the first byte to behind the last.
+  void span(uintptr_t& lo, uintptr_t& hi) const {
+    lo = hi = reinterpret_cast<uintptr_t>(at);
+    for (int i = 0; i < 3; ++i) (stride[i] < 0 ? lo : hi) += (uintptr_t)((count[i] - 1) * stride[i]);
+    hi += (uintptr_t)extent;
+  }
+};
+
+// Whether two buffers share memory.  Views of one buffer may lie between each
+// other, so where their spans meet the pieces are compared (and taken to share
+// memory if there is none to compare them in: no exception leaves a C entry).
+bool meet(const Region& x, const Region& y) {
+  const int64_t nx = x.pieces(), ny = y.pieces();
+  if (nx == 0 || ny == 0) return false;
+  uintptr_t xlo, xhi, ylo, yhi;
+  x.span(xlo, xhi);
+  y.span(ylo, yhi);
+  if (xhi <= ylo || yhi <= xlo) return false;
+  const std::unique_ptr<uintptr_t[]> at(new (std::nothrow) uintptr_t[nx]);
+  if (!at) return true;
+  for (int64_t i = 0; i < nx; ++i) at[i] = x.start(i);
+  std::sort(at.get(), at.get() + nx);
+  for (int64_t i = 0; i < ny; ++i) {
+    const uintptr_t lo = y.start(i), hi = lo + (uintptr_t)y.extent;
+    // The first piece of x that ends behind lo: they are all as long.
+    const uintptr_t* p = std::upper_bound(at.get(), at.get() + nx, lo, [&](uintptr_t l, uintptr_t a) {
+      return a + (uintptr_t)x.extent > l;
+    });
+    if (p != at.get() + nx && *p < hi) return true;
+  }
+  return false;
+}
+
+// Up to eight buffers.
+struct Regions {
+  Region r[8];
+  int n = 0;
+  void add(const void* at, int64_t extent, int64_t b, int64_t bs, int64_t h, int64_t hs, int64_t rows = 1,
+           int64_t rs = 0) {
+    r[n++] = Region{at, extent, {b, h, rows}, {bs, hs, rs}};
+  }
+  // The buffers of a cache: codes and scales of `tokens` tokens from token `first` on, and `tail` rows.
+  void add_cache(const sf_kv8_rows& c, int64_t first, int64_t tokens, int64_t tail) {
+    const int64_t b = c.batch, h = c.num_kv_heads, d = c.head_dim, blocks = tokens / c.block_tokens;
+    for (int v = 0; v < 2; ++v) {
+      const char* codes = static_cast<const char*>(v ? c.v_codes : c.k_codes);
+      const float* scale = v ? c.v_scale : c.k_scale;
+      if (codes) add(codes + first * d, tokens * d, b, c.code_batch_stride, h, c.code_head_stride);
+      if (scale) add(scale + first / c.block_tokens, blocks * 4, b, c.scale_batch_stride * 4, h, c.scale_head_stride * 4);
+      add(v ? c.v_tail : c.k_tail, tail * d * 2, b, c.tail_batch_stride * 2, h, c.tail_head_stride * 2);
+    }
+  }
+};
+
+// Whether anything written shares memory with anything else written or read.
+bool overlap(const Regions& written, const Regions& read) {
+  for (int i = 0; i < written.n; ++i) {
+    for (int j = i + 1; j < written.n; ++j)
+      if (meet(written.r[i], written.r[j])) return true;
+    for (int j = 0; j < read.n; ++j)
+      if (meet(written.r[i], read.r[j])) return true;
+  }
+  return false;
+}
+
 bool target_apart(const sf_kv8_rows& r) {
   auto apart = [&](int64_t bs, int64_t hs, int64_t extent) {
     return kv8_apart(r.batch, bs, r.num_kv_heads, hs, extent);
@@ -321,6 +400,12 @@ extern "C" int sf_kv8_seal(const void* k, const void* v, int64_t batch_stride, i
   SF_CHECK_ARG(target_apart(*rows), "requests and heads of the target must not overlap");
   SF_CHECK_ARG(aligned16(k) && aligned16(v) && batch_stride % 8 == 0 && head_stride % 8 == 0 && row_stride % 8 == 0,
                "k/v rows must be 16-byte aligned");
+  Regions to, from;
+  to.add_cache(*rows, first_block * rows->block_tokens, blocks * rows->block_tokens, 0);
+  for (const void* p : {k, v})
+    from.add(p, rows->head_dim * 2, rows->batch, batch_stride * 2, rows->num_kv_heads, head_stride * 2,
+             blocks * rows->block_tokens, row_stride * 2);
+  SF_CHECK_ARG(!overlap(to, from), "the blocks to seal and their rows must not overlap");
   const SourceRows src{static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), batch_stride,
                        head_stride, row_stride};
   const dim3 grid((unsigned)blocks, (unsigned)(rows->batch * rows->num_kv_heads), 2);
@@ -363,13 +448,17 @@ extern "C" int sf_kv8_compact(const sf_kv8_rows* rows, const int32_t* keep, int6
   SF_CHECK_ARG((mass == nullptr) == (mass_out == nullptr), "pass both mass and mass_out or neither");
   if (n == 0) return SF_OK;
   SF_CHECK_ARG(keep, "null pointer argument");
-  SF_CHECK_ARG((out->sealed == 0 || (out->k_codes != rows->k_codes && out->v_codes != rows->v_codes)) &&
-                   (out->tail == 0 || (out->k_tail != rows->k_tail && out->v_tail != rows->v_tail)) &&
-                   (mass == nullptr || mass != mass_out),
-               "compaction writes to buffers of its own");
   SF_CHECK_ARG(target_apart(*out) && (mass == nullptr || kv8_apart(out->batch, mass_out_batch_stride, out->num_kv_heads,
                                                                    mass_out_head_stride, n)),
                "requests and heads of the target must not overlap");
+  Regions to, from;
+  to.add_cache(*out, 0, out->sealed, out->tail);
+  to.add(mass_out, n * 4, out->batch, mass_out_batch_stride * 4, out->num_kv_heads, mass_out_head_stride * 4);
+  from.add_cache(*rows, 0, rows->sealed, rows->tail);
+  from.add(mass, (rows->sealed + rows->tail) * 4, out->batch, mass_batch_stride * 4, out->num_kv_heads,
+           mass_head_stride * 4);
+  from.add(keep, (int64_t)out->batch * out->num_kv_heads * n * 4, 1, 0, 1, 0);
+  SF_CHECK_ARG(!overlap(to, from), "compaction writes to buffers of its own: they must not overlap others");
   SourceKept src{kv8_view(*rows), keep, n, mass, mass_out, mass_batch_stride, mass_head_stride,
                  mass_out_batch_stride, mass_out_head_stride};
   const int64_t full = out->sealed / out->block_tokens;
