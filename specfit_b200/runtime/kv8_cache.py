@@ -132,10 +132,10 @@ class Kv8Layer(DynamicLayer):
         if self._kt.shape[2] > self.block + self.tail_room:
             self._new_tail(self.block + self.tail_room)
 
-    def rows(self) -> "ops.Kv8Rows":
-        """The cache as the kernels read it."""
-        return ops.Kv8Rows(*self._codes, self.sealed, self._kt[:, :, : self.tail], self._vt[:, :, : self.tail],
-                           self.block)
+    def rows(self, end: int | None = None) -> "ops.Kv8Rows":
+        """The cache, or its rows before ``end`` (in the tail), as the kernels read it."""
+        tail = self.tail if end is None else end - self.sealed
+        return ops.Kv8Rows(*self._codes, self.sealed, self._kt[:, :, :tail], self._vt[:, :, :tail], self.block)
 
     # ---------------------------------------------- transformers' interface
     @property

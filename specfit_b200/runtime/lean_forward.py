@@ -48,6 +48,34 @@ from .qwen3_offloaded_experts import Qwen3OffloadedExperts
 from .tree_attention import _causal_bits, _packed_bits
 
 
+# Rows of a call over an 8-bit cache: the operators take fewer than 2^20 query
+# rows of one KV head (its query heads x rows), and a causal pass has a
+# visibility bit for each pair of its rows, 32 MB for so many.
+KV8_ROWS = 16384
+
+
+def attend_kv8(cl, q: torch.Tensor, bits: torch.Tensor | None, out: torch.Tensor) -> None:
+    """Attention of the pass that ended at layer ``cl``'s last row, and its
+    weights where the layer adds them up; ``bits``: visibility words over every
+    row, None for a causal pass, whose chunks then end at their own last row."""
+    T, total = q.shape[2], cl.length
+    step = min(KV8_ROWS, ((1 << 20) - 1) // (q.shape[1] // cl._h))
+    for lo in range(0, T, step):
+        hi = min(T, lo + step)
+        if bits is None:
+            end, prefix = total - T + hi, total - T + lo
+            words = _causal_bits(hi - lo, q.device).unsqueeze(0).expand(q.shape[0], -1, -1)
+        else:
+            end, prefix, words = total, 0, bits[:, lo:hi]
+        rows = cl.rows(end)
+        part, to = q[:, :, lo:hi], out[:, lo:hi]
+        if cl.scored:
+            _, lse = ops.kv8_tree_attention(part, rows, words, prefix, out=to, return_lse=True)
+            ops.kv8_attention_mass(part, lse, rows, words, prefix, cl.mass)
+        else:
+            ops.kv8_tree_attention(part, rows, words, prefix, out=to)
+
+
 class LeanQwen3Forward:
     # Several requests' attention runs as one tcgen05 launch where a single
     # request would take that kernel too (sf_tree_attention's AUTO rule):
@@ -124,10 +152,15 @@ class LeanQwen3Forward:
 
     def _kv8_attention(self, cl, L, hn, cos, sin, B, T, attention_mask, attention_words, bits, stream):
         """One layer's attention over an 8-bit cache layer: (rows' outputs,
-        (visibility words, first masked column))."""
+        visibility words over every row, None for a causal pass)."""
         if (cl._b, cl._h, cl._d) != (B, self.hkv, self.D):
             raise ValueError("batch or head count differs from the 8-bit cache")
         dev = hn.device
+        total = cl.length + T
+        causal = attention_mask is None and attention_words is None
+        if bits is None and not causal:  # every layer holds the same number of rows
+            bits = attention_words if attention_words is not None else torch.stack(
+                [m.reshape(T, -1) for m in _packed_bits(attention_mask, T, total, B)])
         cl.begin(T)
         room = cl._kt.shape[2]
         qkv = ops.linear(hn, L.wqkv)
@@ -138,22 +171,8 @@ class LeanQwen3Forward:
                                       cl.tail, None, stream), "sf_qk_norm_rope")
         ops._launched(1)
         cl.end(T)
-        total = cl.length
-        causal = attention_mask is None and attention_words is None
-        if bits is None:  # every layer holds the same number of rows
-            if attention_words is not None:
-                bits = (attention_words, 0)
-            elif causal:
-                bits = (_causal_bits(T, dev).unsqueeze(0).expand(B, -1, -1), total - T)
-            else:
-                bits = (torch.stack([m.reshape(T, -1) for m in _packed_bits(attention_mask, T, total, B)]), 0)
         attn = torch.empty(B, T, self.hq, self.D, dtype=hn.dtype, device=dev)
-        rows = cl.rows()
-        if cl.scored:
-            _, lse = ops.kv8_tree_attention(q, rows, bits[0], bits[1], out=attn, return_lse=True)
-            ops.kv8_attention_mass(q, lse, rows, bits[0], bits[1], cl.mass)
-        else:
-            ops.kv8_tree_attention(q, rows, bits[0], bits[1], out=attn)
+        attend_kv8(cl, q, bits, attn)
         if causal and T > 1:
             cl.seal()  # a prompt's rows stay: no layer keeps them in bf16 through the pass
         return attn, bits
@@ -184,7 +203,7 @@ class LeanQwen3Forward:
         hn = torch.empty_like(x)
         self._norm(x, None, res, self.layers[0].ln_in, hn, stream)
         static = not kv8 and cache.layers[0].static_offset is not None
-        kv8_bits = None  # [B, T, words] and the prefix, one for all layers
+        kv8_bits = None  # [B, T, words], one for all layers
         stacked_bits = None  # (kv_len, [B, T, words]) built once per pass for the batched attention
         for li, L in enumerate(self.layers):
             layer = L.layer

@@ -222,3 +222,33 @@ def test_a_replay_over_replaced_buffers_is_refused(target):
     again = VerifyGraph(m.model, cache, q_len=8, device=DEV, forward=fwd)
     again.capture(*inputs)
     assert torch.equal(again.replay(), want)
+
+
+@pytest.mark.parametrize("budget", [None, 96])
+def test_a_long_pass_goes_through_in_parts(target, monkeypatch, budget):
+    """A causal pass and a masked one, whole and in parts of 48 rows."""
+    import specfit_b200.runtime.lean_forward as lf
+
+    cfg, m, state = target
+    fwd = LeanQwen3Forward(m.model)
+    ids = torch.randint(0, 512, (2, 170), generator=torch.Generator().manual_seed(8)).to(DEV)
+    outs, weights = [], []
+    for rows in (lf.KV8_ROWS, 48):
+        monkeypatch.setattr(lf, "KV8_ROWS", rows)
+        cache = Kv8Cache(config=cfg, capacity=512, budget=budget, recent=16)
+        got = [run(fwd, state, cache, ids), run(fwd, state, cache, ids[:, :101])]
+        total = 170 + 101 + 60
+        mask = torch.ones(2, 1, 60, total, dtype=torch.bool, device=DEV)
+        mask[:, :, :, 271:] = torch.ones(60, 60, dtype=torch.bool, device=DEV).tril()
+        pos = torch.arange(271, 331, device=DEV).expand(2, 60)
+        got.append(run(fwd, state, cache, ids[:, :60], attention_mask=mask, position_ids=pos))
+        outs.append(got)
+        if budget:
+            weights.append([l.mass[:, :, :total].double() for l in cache.layers])
+    for a, b in zip(*outs):
+        near(a, b)
+    if budget:
+        # Every row's weights sum to one; layer 0 sees the same inputs both times.
+        for w in weights:
+            assert all(float((x.sum(-1) - 4 * 331).abs().max()) <= 4 * 331 * 1e-3 for x in w)
+        assert bool(((weights[0][0] - weights[1][0]).abs() <= 1e-3 * weights[0][0] + 1e-3).all())
