@@ -703,8 +703,9 @@ class _Here:
 
 
 _HERE = _Here()
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# A torch built without CUDA has neither; there every call refuses its tensors first.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _on(index: int):

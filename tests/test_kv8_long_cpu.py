@@ -1,5 +1,9 @@
-"""Long passes over an 8-bit cache: the calls that a pass is made of, on the CPU."""
+"""Long passes over an 8-bit cache: the calls that a pass is made of, on the CPU; and
+importing the package where torch has no CUDA."""
+import subprocess
+import sys
 import types
+from pathlib import Path
 
 import pytest
 import torch
@@ -69,3 +73,20 @@ def test_a_masked_pass_keeps_its_words(calls):
     lf.attend_kv8(Layer(2, 50000, False), q, words, out)
     assert [c[3:5] for c in calls] == [(50000, 0)] * len(calls) and len(calls) > 1
     assert torch.equal(torch.cat([c[5] for c in calls], 1), words)
+
+
+def test_the_package_imports_where_torch_has_no_cuda():
+    code = ("import torch\n"
+            "for name in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, name)\n"
+            "import specfit_b200.runtime\n"
+            "from specfit_b200 import ops\n"
+            "try:\n"
+            "    ops.kv_keep_heaviest(torch.zeros(1, 1, 4), 4, 2)\n"
+            "except ValueError as e:\n"
+            "    assert 'CUDA' in str(e)\n"
+            "else:\n"
+            "    raise SystemExit('not refused')\n")
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True,
+                          text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
