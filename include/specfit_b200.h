@@ -836,6 +836,9 @@ SF_API int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int64_t 
                                  int64_t bits_batch_stride, int64_t prefix_len, float scale, float* mass,
                                  int64_t mass_batch_stride, int64_t mass_head_stride, void* workspace,
                                  size_t workspace_bytes, void* stream);
+/* Kernels that the calling thread's last sf_kv8_tree_attention or
+ * sf_kv8_attention_mass launched: 0 (nothing to do, refused) to 3. */
+SF_API int sf_kv8_launches(void);
 /*
  * The tokens an eviction keeps: keep [batch, num_kv_heads, budget] int32,
  * ascending: the first `sinks`, the last `recent`, and the heaviest of the

@@ -215,6 +215,7 @@ SIGNATURES = {
     "sf_kv8_attention_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64, _i64, _i64]),
     "sf_kv8_tree_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _i64, _kv8_p, _vp, _i32, _i64, _i64, _f32, _vp,
                                      _i64, _vp, _vp, _sz, _vp]),
+    "sf_kv8_launches": (_i32, []),
     "sf_kv8_mass_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i64, _i64, _i64]),
     "sf_kv8_attention_mass": (_i32, [_vp, _i64, _i64, _i64, _i32, _i64, _vp, _kv8_p, _vp, _i32, _i64, _i64, _f32,
                                      _vp, _i64, _i64, _vp, _sz, _vp]),

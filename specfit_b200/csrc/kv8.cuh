@@ -27,6 +27,9 @@ constexpr int kKv8MinExponent = -100;
 // Checks shared by every entry point that reads a sf_kv8_rows.
 int kv8_check(const sf_kv8_rows* r, bool need_values);
 
+// Kernels that this thread's last attention or weight call launched so far.
+int& kv8_launches();
+
 // Whether the requests and heads of something to be written lie apart: each
 // is `extent` elements, `b` of them bs apart, `h` hs apart.
 inline bool kv8_apart(int64_t b, int64_t bs, int64_t h, int64_t hs, int64_t extent) {

@@ -837,6 +837,7 @@ int launch_merge_few(const Kv8Attn& p, cudaStream_t stream) {
   const int64_t pairs = (int64_t)p.batch * p.heads * p.q_len;
   SF_CHECK_CUDA(launch_pdl(kv8_merge_few_kernel<N>, dim3((unsigned)((pairs + 7) / 8)), dim3(256), 0, stream, p));
   SF_CHECK_LAUNCH();
+  ++kv8_launches();
   return SF_OK;
 }
 
@@ -845,6 +846,7 @@ int launch_merge(const Kv8Attn& p, cudaStream_t stream) {
   const int64_t pairs = (int64_t)p.batch * p.heads * p.q_len;
   SF_CHECK_CUDA(launch_pdl(kv8_merge_kernel<W>, dim3((unsigned)((pairs * W + 7) / 8)), dim3(256), 0, stream, p));
   SF_CHECK_LAUNCH();
+  ++kv8_launches();
   return SF_OK;
 }
 
@@ -866,6 +868,7 @@ int launch_mma(const Kv8Attn& p, cudaStream_t stream) {
   else
     SF_CHECK_CUDA(launch_pdl(kv8_attn_kernel<DT, Full, Narrow>, grid, dim3(kWarps * 32), Layout<DT>::kSmem, stream, p));
   SF_CHECK_LAUNCH();
+  ++kv8_launches();
   return SF_OK;
 }
 
@@ -919,6 +922,7 @@ extern "C" int sf_kv8_tree_attention(const void* q, int64_t q_batch_stride, int6
                                      int64_t prefix_len, float scale, void* out, int64_t out_batch_stride, float* lse,
                                      void* workspace, size_t workspace_bytes, void* stream) {
   using namespace sf;
+  kv8_launches() = 0;
   if (int rc = kv8_check(rows, true)) return rc;
   const int64_t kv_len = rows->sealed + rows->tail;
   SF_CHECK_ARG(num_heads > 0 && num_heads % rows->num_kv_heads == 0,

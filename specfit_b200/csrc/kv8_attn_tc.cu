@@ -946,6 +946,7 @@ int kv8_prep(const Kv8Attn& p, const Kv8Prep& w, cudaStream_t stream) {
   const dim3 grid((unsigned)(w.tiles + w.blocks), (unsigned)(p.batch * p.c.hkv));
   SF_CHECK_CUDA(launch_pdl(kv8_prep_kernel, grid, dim3(256), 0, stream, p, w));
   SF_CHECK_LAUNCH();
+  ++kv8_launches();
   return SF_OK;
 }
 
@@ -981,6 +982,7 @@ int kv8_attention_tc(const Kv8Attn& p, void* prep, cudaStream_t stream) {
   SF_CHECK_CUDA(launch_pdl(kv8_attn_tc_kernel, grid, dim3(kThreads), kSmemBytes, stream, tm_k, p, w, sh.dual ? 1 : 0,
                            ranges));
   SF_CHECK_LAUNCH();
+  ++kv8_launches();
   return SF_OK;
 }
 

@@ -220,6 +220,7 @@ int launch_mass(const MassParams& p, cudaStream_t stream) {
   const dim3 grid((unsigned)std::min<int64_t>(want, p.tiles), (unsigned)heads);
   SF_CHECK_CUDA(launch_pdl(kv8_mass_kernel<DT>, grid, dim3(kWarps * 32), 0, stream, p));
   SF_CHECK_LAUNCH();
+  ++kv8_launches();
   return SF_OK;
 }
 
@@ -245,6 +246,7 @@ extern "C" int sf_kv8_attention_mass(const void* q, int64_t q_batch_stride, int6
                                      int64_t mass_batch_stride, int64_t mass_head_stride, void* workspace,
                                      size_t workspace_bytes, void* stream) {
   using namespace sf;
+  kv8_launches() = 0;
   if (int rc = kv8_check(rows, false)) return rc;
   const int64_t kv_len = rows->sealed + rows->tail;
   SF_CHECK_ARG(num_heads > 0 && num_heads % rows->num_kv_heads == 0,

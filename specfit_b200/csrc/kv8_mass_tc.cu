@@ -416,11 +416,13 @@ int kv8_mass_tc(const Kv8Attn& p, float* mass, int64_t m_bs, int64_t m_hs, void*
                            dim3(kThreads), kSmemBytes, stream, tm_k, p, w, mass, m_bs, m_hs, (int)nblocks, (int)per,
                            parts.tiles, sums));
   SF_CHECK_LAUNCH();
+  ++kv8_launches();
   if (sums) {
     SF_CHECK_CUDA(launch_pdl(kv8_mass_add_kernel, dim3((unsigned)((p.kv_len + 255) / 256), (unsigned)heads), dim3(256),
                              0, stream, static_cast<const float*>(sums), parts.count, mass, m_bs, m_hs, p.c.hkv,
                              p.kv_len));
     SF_CHECK_LAUNCH();
+    ++kv8_launches();
   }
   return SF_OK;
 }

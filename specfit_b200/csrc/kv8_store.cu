@@ -22,6 +22,11 @@
 
 namespace sf {
 
+int& kv8_launches() {
+  static thread_local int n = 0;
+  return n;
+}
+
 int kv8_check(const sf_kv8_rows* r, bool need_values) {
   SF_CHECK_ARG(r != nullptr, "null pointer argument");
   SF_CHECK_ARG(r->batch > 0 && r->num_kv_heads > 0 && (int64_t)r->batch * r->num_kv_heads <= 65535,
@@ -386,6 +391,8 @@ bool target_apart(const sf_kv8_rows& r) {
 
 }  // namespace
 }  // namespace sf
+
+extern "C" int sf_kv8_launches(void) { return sf::kv8_launches(); }
 
 extern "C" int sf_kv8_seal(const void* k, const void* v, int64_t batch_stride, int64_t head_stride,
                            int64_t row_stride, const sf_kv8_rows* rows, int64_t first_block, int64_t blocks,

@@ -835,7 +835,7 @@ def kv8_tree_attention(q: torch.Tensor, rows: Kv8Rows, tree_bits: torch.Tensor |
                                          None if ws is None else ws.data_ptr(), nbytes, _raw_stream(index))
     if rc:
         N.check(rc, "sf_kv8_tree_attention")
-    _launched((2 if nbytes else 1) if tq else 0)
+    _launched(N.lib.sf_kv8_launches())
     return (out, lse) if return_lse else out
 
 
@@ -864,7 +864,7 @@ def kv8_attention_mass(q: torch.Tensor, lse: torch.Tensor, rows: Kv8Rows, tree_b
                                          None if ws is None else ws.data_ptr(), nbytes, _raw_stream(index))
     if rc:
         N.check(rc, "sf_kv8_attention_mass")
-    _launched((2 if nbytes else 1) if tq and rows.shape[2] else 0)
+    _launched(N.lib.sf_kv8_launches())
     return mass
 
 

@@ -249,3 +249,46 @@ def test_not_a_number_in_queries_and_keys(ops, hq, rows, d, what):
     on[:, :, key] = True
     mass = ops.kv8_attention_mass(q, wlse, cache, pack(on), 0, torch.zeros(1, 1, total, device=DEV))[0, 0]
     assert bool(torch.isnan(mass[key])) and bool(torch.isfinite(mass[:key]).all()) and float(mass[value]) == 0
+
+
+def nodes_of(call):
+    """Kernels of a captured call."""
+    import ctypes
+
+    for _ in range(2):
+        call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    n = ctypes.c_size_t()
+    assert ctypes.CDLL("libcuda.so.1").cuGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None,
+                                                       ctypes.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("b,hq,hkv,rows,sealed,tail,shared", [
+    (1, 8, 1, 1, 64, 5, False),       # one range
+    (1, 32, 4, 1, 512, 17, False),    # ranges joined by a cluster
+    (1, 32, 4, 1, 16384, 17, False),  # and by a second kernel
+    (2, 8, 8, 100, 64, 70, False),    # many rows, one range
+    (1, 32, 4, 65, 4096, 65, False),  # many rows, many ranges; weights in one part
+    (1, 8, 1, 65, 640, 65, False),    # weights of a short cache in parts
+    (1, 16, 2, 65, 320, 70, True),    # heads that share memory: the form for few rows
+    (1, 8, 1, 0, 64, 5, False),       # nothing to do
+])
+def test_launches_are_counted(ops, b, hq, hkv, rows, sealed, tail, shared):
+    total = sealed + tail
+    q, k, v = draw(b, hq, hkv, rows, total, 128, 17)
+    cache = sealed_cache(ops, k, v, sealed, 64)
+    if shared:
+        parts = [t[:, :1].expand(b, hkv, *t.shape[2:]) for t in (cache.k_codes, cache.v_codes, cache.k_scale,
+                                                                  cache.v_scale)]
+        cache = ops.Kv8Rows(*parts, sealed, cache.k_tail, cache.v_tail, 64)
+    _, lse = ops.kv8_tree_attention(q, cache, None, total, return_lse=True)
+    mass = torch.zeros(b, hkv, total, device=DEV)
+    for call in (lambda: ops.kv8_tree_attention(q, cache, None, total),
+                 lambda: ops.kv8_attention_mass(q, lse, cache, None, total, mass)):
+        before = ops.LAUNCHES[0]
+        call()
+        assert ops.LAUNCHES[0] - before == (nodes_of(call) if rows else 0)
