@@ -16,11 +16,16 @@ to bf16, exactly what attention saw.
 With ``budget`` every pass also adds up the attention weight that each cached
 token received, per KV head (``ops.kv8_attention_mass``), and ``evict()`` keeps
 the first ``sinks`` tokens, the last ``recent``, and the heaviest of the others
-(``ops.kv_keep_heaviest``, ``ops.kv8_compact``).  Keys carry their rotary
-positions, so what stays is not recomputed; ``next_position`` is the position
+(``ops.kv_keep_heaviest``, ``ops.kv8_compact``).  A weight stays added when the
+row that gave it is taken back (a rejected tree row has looked at the context
+too).  Only ``LeanQwen3Forward`` adds weights: ``update`` does not see the queries,
+and ``evict()`` warns when rows came that way, since zeros decide nothing but age.
+Keys carry their rotary positions, so what stays is not recomputed; ``next_position`` is the position
 of the next token, ``get_seq_length`` the number of rows held.
 """
 from __future__ import annotations
+
+import warnings
 
 import torch
 from transformers.cache_utils import DynamicCache, DynamicLayer
@@ -40,6 +45,7 @@ class Kv8Layer(DynamicLayer):
         self.sealed = 0
         self.tail = 0
         self.mass = None
+        self.unscored = False       # rows came through ``update``, which adds no weights
         self._kt = None
 
     # ------------------------------------------------------------- buffers
@@ -153,6 +159,7 @@ class Kv8Layer(DynamicLayer):
         if key_states.shape[:2] != (self._b, self._h) or key_states.shape != value_states.shape:
             raise ValueError("batch or head count differs from the cache")
         n = key_states.shape[2]
+        self.unscored = self.scored
         self.begin(n)
         self._kt[:, :, self.tail: self.tail + n].copy_(key_states)
         self._vt[:, :, self.tail: self.tail + n].copy_(value_states)
@@ -207,6 +214,7 @@ class Kv8Layer(DynamicLayer):
 
     def reset(self) -> None:
         self.sealed = self.tail = 0
+        self.unscored = False
 
     def offload(self) -> None:
         raise RuntimeError("the 8-bit cache stays on its device")
@@ -275,6 +283,10 @@ class Kv8Cache(DynamicCache):
             raise RuntimeError("this cache was made without a budget")
         if not self.layers or not self.layers[0].is_initialized:
             return 0
+        if any(layer.unscored and layer.length > self.budget for layer in self.layers):
+            warnings.warn("rows appended by update() brought no attention weights: the eviction ranks by what the "
+                          "lean forward's passes added, and among equal weights keeps the earlier rows",
+                          RuntimeWarning, stacklevel=2)
         gone = [layer.evict(self.budget, self.sinks, self.recent) for layer in self.layers]
         if any(g != gone[0] for g in gone):
             raise RuntimeError("the cache's layers differ in length")

@@ -94,3 +94,19 @@ def test_a_graph_keeps_the_buffers_that_it_writes(captured):
     feed(c, 200, 3)
     feed(c, 1, 4)
     assert all(r() is not None for r in held)
+
+
+def test_an_eviction_without_weights_says_so(plain):  # noqa: F811
+    import warnings
+
+    c = cache(budget=40, sinks=2, recent=8)
+    feed(c, 90, 1)
+    with pytest.warns(RuntimeWarning, match="weights"):
+        assert c.evict() == 50
+    c.reset()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        for l in c.layers:  # as the lean forward appends
+            l.begin(60)
+            l.end(60)
+        assert c.evict() == 20
