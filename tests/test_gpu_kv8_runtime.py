@@ -252,3 +252,23 @@ def test_a_long_pass_goes_through_in_parts(target, monkeypatch, budget):
         for w in weights:
             assert all(float((x.sum(-1) - 4 * 331).abs().max()) <= 4 * 331 * 1e-3 for x in w)
         assert bool(((weights[0][0] - weights[1][0]).abs() <= 1e-3 * weights[0][0] + 1e-3).all())
+
+
+def test_batches_grow_shrink_and_change_order(target):
+    cfg, m, state = target
+    fwd = LeanQwen3Forward(m.model)
+    ids = torch.randint(0, 512, (2, 90), generator=torch.Generator().manual_seed(4)).to(DEV)
+    cache = Kv8Cache(config=cfg, capacity=256, budget=64, recent=16)
+    run(fwd, state, cache, ids)
+    before = [(ops.kv8_read(l.rows()), l.mass.clone()) for l in cache.layers]
+    cache.batch_repeat_interleave(3)
+    cache.reorder_cache(torch.tensor([5, 0, 2], device=DEV))  # requests 1, 0, 0
+    cache.batch_select_indices(torch.tensor([0, 1], device=DEV))
+    for l, ((k, v), mass) in zip(cache.layers, before):
+        nk, nv = ops.kv8_read(l.rows())
+        assert torch.equal(nk, k.flip(0)) and torch.equal(nv, v.flip(0)) and torch.equal(l.mass, mass.flip(0))
+    one = torch.tensor([[3], [4]], device=DEV)
+    flipped = run(fwd, state, cache, one.flip(0))
+    again = Kv8Cache(config=cfg, capacity=256, budget=64, recent=16)
+    run(fwd, state, again, ids)
+    near(flipped.flip(0), run(fwd, state, again, one))
