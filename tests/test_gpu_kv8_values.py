@@ -9,6 +9,7 @@ import torch
 
 import kv8_bounds as kb
 import kv8_reference as ref
+import test_gpu_kv8 as shapes
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -249,6 +250,19 @@ def test_not_a_number_in_queries_and_keys(ops, hq, rows, d, what):
     on[:, :, key] = True
     mass = ops.kv8_attention_mass(q, wlse, cache, pack(on), 0, torch.zeros(1, 1, total, device=DEV))[0, 0]
     assert bool(torch.isnan(mass[key])) and bool(torch.isfinite(mass[:key]).all()) and float(mass[value]) == 0
+
+
+@pytest.mark.parametrize("b,hq,hkv,d,block,sealed,tail,rows,mask", shapes.ATTENTION)
+def test_every_shape_to_the_row(ops, b, hq, hkv, d, block, sealed, tail, rows, mask):
+    """The operators' shapes, held to bounds that a row of zeros does not meet."""
+    seed = hq + d + sealed + rows + 1
+    cache = shapes.make_rows(ops, b, hkv, d, block, sealed, tail, seed, room=block)
+    q = shapes.queries(b, hq, rows, d, seed)
+    bits, prefix, vis = shapes.masks(mask, b, rows, sealed + tail, seed)
+    out, lse = ops.kv8_tree_attention(q, cache, bits, prefix, return_lse=True)
+    want = kb.attention(q, *opened(cache), vis.to(DEV), d ** -0.5)
+    assert kb.off(out, want) is None, kb.off(out, want)
+    assert kb.lse_off(lse, want) is None, kb.lse_off(lse, want)
 
 
 def nodes_of(call):
