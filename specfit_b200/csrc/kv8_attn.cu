@@ -446,11 +446,11 @@ kv8_attn_kernel(Kv8Attn p) {
         mx[r] = x[r][0];
 #pragma unroll
         for (int i = 1; i < kX; ++i) mx[r] = fmaxf(mx[r], x[r][i]);  // NaN is passed over
-        mx[r] += (float)v;
+        mx[r] += (float)max(v, kMinValueScale);
       } else {
         mx[r] = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kX; ++i) mx[r] = fmaxf(mx[r], x[r][i] + tail_v[warp][key_of(i)]);
+        for (int i = 0; i < kX; ++i) mx[r] = fmaxf(mx[r], x[r][i] + fmaxf(tail_v[warp][key_of(i)], (float)kMinValueScale));
       }
       grow |= mx[r] > m[r] + kSlack;  // m -infinity: any score
     }
@@ -464,9 +464,11 @@ kv8_attn_kernel(Kv8Attn p) {
 #pragma unroll
         for (int off = Narrow ? 4 : 1; off < (Narrow ? 32 : 4); off <<= 1)  // the threads of a row
           y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, off));
-        corr[r] = m[r] == -INFINITY ? 0.f : ex2(m[r] - y);
+        // In two steps: l may be far from 1, and one factor below what fp32 holds.
+        const float half = m[r] == -INFINITY ? 0.f : ex2(0.5f * (m[r] - y));
         m[r] = y;
-        l[r] *= corr[r];
+        l[r] = l[r] * half * half;
+        corr[r] = half * half;
       }
     }
     if (rescale) {

@@ -45,6 +45,12 @@ __device__ __forceinline__ uint64_t kv8_window(const Kv8Attn& p, const uint32_t*
   return w;
 }
 
+// A row's reference is the largest of a score plus log2 of its value's scale, or
+// this where that is less: sums of probabilities, in units of the reference,
+// then stay below 2^(75 + log2 of the keys), and only values below 2^-75 or so, where
+// a row sees no larger ones, lose digits.
+constexpr int kMinValueScale = -60;
+
 // Key ranges per (request, KV head, row tile) for `units` such units of work.
 struct Kv8Split {
   int splits, keys_per_split;

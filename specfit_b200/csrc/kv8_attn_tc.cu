@@ -96,8 +96,8 @@ struct __align__(16) Tail {
   float red[2][2][kBM], sum[2][2][kBM];  // per lane, half and row: maxima and final sums, for the other half
   int pair_ok[kSoftmaxWarps];
   // Per block (ring of 4) and key: scale * log2(e) * K scale (NaN for a key that
-  // holds one), v = log2 of the V scale times 2^7, 2^min(v, 0), 2^-max(v, 0); per 32
-  // keys, of the first: the first two, and 2^-v.
+  // holds one), v = log2 of the V scale times 2^7 (kMinValueScale if less), 2^min(v, 0),
+  // 2^-max(v, 0); per 32 keys, of the first: the first two, and 2^-v.
   float4 key[4][kKB], group[4][kKB / 32];
   uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t raw_full, raw_empty;
@@ -585,7 +585,7 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       // stage, block b - 2's, were issued after P V of the lane's block before.)
       const float kf = ks * p.scale_log2;
       const int v = scale_log2(vs) + (int)kPShift;
-      tail->key[b & 3][ct] = make_float4(kf, (float)v, pow2f(min(v, 0)), pow2f(-max(v, 0)));
+      tail->key[b & 3][ct] = make_float4(kf, (float)max(v, kMinValueScale), pow2f(min(v, 0)), pow2f(-max(v, 0)));
       if (lane == 0) tail->group[b & 3][ct >> 5] = make_float4(kf, (float)v, pow2f(-v), 0.f);
       warp_arrive(&tail->k_full[s]);
       return true;
@@ -689,7 +689,7 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
                 if (plain) {
                   const float y = scaled_max(sc, group[c >> 1].x * qf);
                   mx = fmaxf(mx, y);
-                  mv = fmaxf(mv, y + group[c >> 1].y);
+                  mv = fmaxf(mv, y + fmaxf(group[c >> 1].y, (float)kMinValueScale));
                 } else {
                   masked_max(sc, key + c * 16, qf, (uint32_t)(win >> (c * 16)), mx, mv);
                 }
@@ -708,9 +708,11 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
             }
             close = both & 2;
             const float mnew = fmaxf(m, fmaxf(mv, tail->red[t][half ^ 1][r]) - kPShift);
-            const float alpha = m == -INFINITY ? 1.f : ex2(m - mnew);  // nothing summed yet: O and l are 0
+            // Nothing summed yet: O and l are 0.  In two steps: l may be far from 1, and one
+            // factor below what fp32 holds.
+            const float step = m == -INFINITY ? 1.f : ex2(0.5f * (m - mnew)), alpha = step * step;
             m = mnew;
-            l *= alpha;
+            l = l * step * step;
             if (i > 0) {  // P V of the block before is complete, as its successor's scores are
 #pragma unroll 1
               for (int c = 0; c < 4; ++c) {

@@ -306,3 +306,35 @@ def test_launches_are_counted(ops, b, hq, hkv, rows, sealed, tail, shared):
         before = ops.LAUNCHES[0]
         call()
         assert ops.LAUNCHES[0] - before == (nodes_of(call) if rows else 0)
+
+
+# (KV heads so many that one range holds all keys, or few: ranges are joined.)
+@pytest.mark.parametrize("hq,hkv,rows,d", [(8, 1, 1, 128), (4, 1, 3, 64), (8, 1, 9, 128), (224, 224, 2, 128),
+                                           (128, 128, 40, 64), (148, 148, 70, 128)])
+@pytest.mark.parametrize("first", [0.0, 2.0 ** -60])
+def test_values_of_zeros_before_large_ones(ops, hq, hkv, rows, d, first):
+    """Blocks of zeros (or of 2^-60), then values of 2^60, all seen: the first blocks'
+    share of the weights stays when the reference moves by more than fp32's exponents."""
+    sealed, tail, block = 512, 40, 64
+    total = sealed + tail
+    q, k, v = draw(1, hq, hkv, rows, total, d, 18)
+    v[:, :, :256] = (v[:, :, :256].float() * first).to(torch.bfloat16)
+    v[:, :, 256:] = (v[:, :, 256:].float() * 2.0 ** 60).to(torch.bfloat16)
+    vis = torch.ones(1, rows, total, dtype=torch.bool)
+    compare(ops, q, sealed_cache(ops, k, v, sealed, block), vis)
+
+
+@pytest.mark.parametrize("hq,hkv,rows,d", [(8, 1, 1, 128), (224, 224, 2, 128), (444, 444, 1, 64), (8, 1, 16, 128)])
+def test_values_of_zeros_alone(ops, hq, hkv, rows, d):
+    """A long cache of zero values answers zeros and its log-sum-exp."""
+    sealed = 4096
+    g = torch.Generator(device=DEV).manual_seed(19)
+    q = torch.randn(1, hq, rows, d, generator=g, device=DEV).to(torch.bfloat16)
+    k = torch.randn(1, hkv, sealed, d, generator=g, device=DEV).to(ref.E4M3)
+    scale = torch.full((1, hkv, sealed // 64), 2.0 ** -100, device=DEV)
+    none = torch.zeros(1, hkv, 0, d, dtype=torch.bfloat16, device=DEV)
+    cache = ops.Kv8Rows(k, torch.zeros_like(k), torch.ones_like(scale), scale, sealed, none, none, 64)
+    out, lse = ops.kv8_tree_attention(q, cache, None, sealed, return_lse=True)
+    x = torch.einsum("bhgrd,bhkd->bhgrk", q.double().view(1, hkv, -1, rows, d), k.double()) * d ** -0.5
+    assert float(out.abs().max()) == 0
+    assert float((lse.double() - torch.logsumexp(x, -1).view_as(lse)).abs().max()) <= 2e-4
