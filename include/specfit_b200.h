@@ -791,7 +791,7 @@ typedef struct sf_kv8_rows {
  * Seals `blocks` blocks of bf16 rows k, v [batch, num_kv_heads, blocks *
  * block_tokens, head_dim] (strides in elements, multiples of 8) into the
  * cache's blocks first_block, first_block + 1, ...; rows->sealed is the number
- * of tokens its code buffers hold.
+ * of tokens its code buffers hold.  What is written shares memory with nothing else.
  */
 SF_API int sf_kv8_seal(const void* k, const void* v, int64_t batch_stride, int64_t head_stride,
                        int64_t row_stride, const sf_kv8_rows* rows, int64_t first_block, int64_t blocks,
@@ -808,8 +808,15 @@ SF_API int sf_kv8_read(const sf_kv8_rows* rows, int64_t first, int64_t count, vo
  * log-sum-exp of a row's scaled scores.  A row that sees no key answers zeros
  * and -infinity.  A key whose row of K or of V holds a NaN or an infinity
  * (sealed: whose block does) answers NaN to the rows that see it and to no other;
- * a query row that holds one answers NaN.  workspace (16-byte
- * aligned): sf_kv8_attention_workspace_bytes(...) bytes, perhaps 0.
+ * a query row that holds one answers NaN.
+ * Rounding: scores, maxima and sums are fp32.  A probability times its value's
+ * scale is fp16 (half a step, 2^-11 relative, down to 2^-21 of the row's largest); with
+ * more than 64 query rows of a KV head and head_dim 128, queries and tail keys
+ * are two e4m3 numbers, exact down to 2^-17 of a row's largest element.  With
+ * scores below 64: |error| <= 2^-8 |out| + 2^-10 sum p |v|, the first term the
+ * bf16 output's own.
+ * workspace (16-byte aligned): sf_kv8_attention_workspace_bytes(...) bytes,
+ * perhaps 0.
  */
 SF_API size_t sf_kv8_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim,
                                                int64_t q_len, int64_t sealed, int64_t tail);
@@ -849,8 +856,8 @@ SF_API int sf_kv_keep_heaviest(const float* mass, int64_t mass_batch_stride, int
                                int batch, int num_kv_heads, int64_t length, int64_t budget, int64_t sinks,
                                int64_t recent, int32_t* keep, void* stream);
 /*
- * Moves rows keep[b, h, 0 .. n) of `rows` into the cache `out` (buffers of its
- * own; out->sealed = n / block_tokens * block_tokens, out->tail = the rest):
+ * Moves rows keep[b, h, 0 .. n) of `rows` into the cache `out` (what is written
+ * shares memory with nothing else; out->sealed = n / block_tokens * block_tokens, out->tail = the rest):
  * whole blocks are sealed anew, the last n % block_tokens rows become its bf16
  * tail.  mass / mass_out (nullable, both or neither): the kept tokens' mass
  * moves along.  An index outside the cache moves a row of zeros.

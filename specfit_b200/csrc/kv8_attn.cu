@@ -44,10 +44,10 @@
 //     instructions for 16 keys were 43 us at 131,072 tokens), Q's fragments from
 //     shared memory (one 16-byte load for four MMAs), tail units converted there
 //     too, and addresses that are constants where D is the tile's width.
-// What it measured: one token, 32 heads over 131,113 tokens, 26 us, 5.1 TB/s, of
+// What it measured: one token, 32 heads over 131,113 tokens, 27 us, 5.0 TB/s, of
 // which about five are the launch, Q, the join and the partial results, and 7
-// more the merge.  (30 us while a tail unit's loads came a key after the other:
-// the last range's CTA ended late.)  Four CTAs an SM, with a ring of 12 KB a warp, took 37: each
+// more the merge; over 529 tokens 8.8.  (30 us while a tail unit's loads came a key
+// after the other: the last range's CTA ended late.)  Four CTAs an SM, with a ring of 12 KB a warp, took 37: each
 // has that cost, and a shorter range.
 // Tail units (bf16 rows: few): a power of two per key is taken out of its row of K,
 // another out of its row of V, and they enter the same fragments.  A key with a NaN
@@ -73,9 +73,10 @@ constexpr int kStep = kWarps * kUnit;
 constexpr int kMaxSplits = 128;
 constexpr int kMaxCluster = 8; // key ranges that a cluster joins itself
 // Up to so many steps of a CTA the ranges are at most a cluster's: a token
-// over 545 / 1,569 tokens 10.9 / 11.5 us against 12.5 / 14.3 with a range a step
-// and the merge kernel (8 rows: 13.1 / 15.2 against 14.7 / 18.9), and one launch
-// less; at 2,593 tokens they are equal, at 4,129 the merge is faster.
+// over 545 / 1,569 tokens 8.8 / 9.5 us against 10.0 / 10.0 with a range a step and
+// the merge kernel (8 rows: 11.0 / 12.6 against 11.9 / 14.1), and one launch less;
+// at 2,593 tokens they are equal (11.5 / 10.8; 15.5 / 17.2), at 4,129 the merge is
+// faster (11.5 / 11.0; 16.6 / 14.7).
 constexpr int kClusterSteps = 24;
 constexpr float kPShift = 12.f;  // probabilities are kept times 2^12
 constexpr float kSlack = 3.f;    // a row's reference maximum may lag by this (base 2)

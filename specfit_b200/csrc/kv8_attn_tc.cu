@@ -49,13 +49,19 @@
 //     scores late and at once, and then fight for the exponentials; one after
 //     the other, a lane's softmax runs under the other's products.
 //   * Waiting warps sleep in the barrier (up to 20 us a try): as they polled they
-//     took issue slots from the softmax warps (455 to 436 us in the case below).
-// What it measured: 1,000 rows of 32 heads over 17,391 tokens 421 us, 680
-// TFLOP/s; 8 requests of 65 rows over 4,161 tokens 88 us.  A block of two lanes
-// takes about 5,700 clocks, the MMAs 2,050 and the exponentials 2,050 of them;
+//     took issue slots from the softmax warps.
+//   * What a softmax thread spills matters: shared memory leaves 28 KB of L1, and the
+//     512 threads' stacks stop fitting at 56 bytes each (48 now; forms of this code
+//     with 64, 72 and 96 bytes took 410, 519 and 657 us in the case below).  Hence one path of little code for
+//     whole blocks of codes, and a rolled one, key by key, for what is masked, tail
+//     or far apart in scale; half a block that no row of a warp sees is passed over.
+// What it measured: 1,000 rows of 32 heads over 17,391 tokens 395 us, 700
+// TFLOP/s; 8 requests of 65 rows over 4,161 tokens 85 us.  A block of two lanes
+// takes about 5,400 clocks, the MMAs 2,050 and the exponentials 2,050 of them;
 // what bounds it is the chain of one lane (scores, 64 exponentials a thread,
 // probabilities to TMEM, two products), of which two fit beside each other.
-// P is rounded to fp16 (2^-12 relative); sums are fp32 of the unrounded values.
+// P is rounded to fp16 (half a step, 2^-11 relative; the bf16 output's is 2^-8, and 32
+// bits would be four times the tensor time); sums are fp32 of the unrounded values.
 // TMEM: S / P of lane t in columns [128 t, 128 t + 128), O in [256 + 128 t, ...).
 //
 // Every wait is bounded (sm100_ptx.cuh); one that gives up records its site
@@ -878,10 +884,10 @@ Shape shape_of(int64_t packed) {
 
 // Microseconds a call, this kernel's against the warp-level one's, four KV heads
 // (4,159 tokens; 32,831; eight requests of 4,159):
-//   48 packed rows: 22 / 34 / 36 against 21 / 29 / 31
-//   64:             23 / 34 / 36 against 18 / 35 / 39
-//   96:             23 / 34 / 38 against 21 / 42 / 49
-//   128:            24 / 34 / 40 against 26 / 55 / 74
+//   48 packed rows: 22 / 30 / 31 against 18 / 27 / 28
+//   64:             22 / 31 / 32 against 15 / 33 / 36
+//   80:             22 / 31 / 33 against 18 / 37 / 46
+//   128:            23 / 32 / 36 against 21 / 53 / 75
 bool kv8_use_tc(int head_dim, int64_t packed, int64_t kv_len) { return head_dim == kD && packed > 64 && kv_len > 0; }
 
 // Heads and requests of their own rows: what a tensor map can describe.

@@ -9,7 +9,7 @@
 // codes are read and decoded once whatever the number of rows, and a key's
 // sum never leaves its warp (no atomics: the same inputs give the same bits).
 // The tile after the present one is on its way to registers, with the mass so
-// far: one token over 65,569 tokens, 32 heads, takes 15 us (25 without), 2.3
+// far: one token over 65,569 tokens, 32 heads, takes 14 us (25 without), 2.5
 // TB/s; four to five of them are the launch, Q and the first tile.
 // Query rows are staged in shared memory in MMA fragment order, 64 at a time,
 // as fp16 with a power of two taken out of each (kv8_attn.cu has the reasons).

@@ -17,7 +17,7 @@
 //     sums a second kernel adds to the mass, again in one order.
 //   * At a block's end one warp adds the four partial sums of a key, in one
 //     order, so the same inputs give the same bits.
-// What it measured: 8 requests of 65 rows, 32 heads, over 4,161 tokens 47 us (the
+// What it measured: 8 requests of 65 rows, 32 heads, over 4,161 tokens 46 us (the
 // warp-level kernel 265), 2.3 times the exponentials' 20; a CTA's last block, the
 // one with a mask, takes twice a full one's time.
 // Every wait is bounded; a warp whose wait gave up skips the work but still
