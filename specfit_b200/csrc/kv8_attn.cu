@@ -349,7 +349,8 @@ kv8_attn_kernel(Kv8Attn p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
     float kscale;
-    int v = 0;  // log2 of the V scale
+    int v = 0;  // log2 of the V scale, rounded down, and what it lacks (1 for a power of two)
+    float vrest = 1.f;
     const bool coded = key0 < sealed;
     if (coded) {
       kscale = ksc[key0 >> p.c.block_shift];
@@ -357,7 +358,7 @@ kv8_attn_kernel(Kv8Attn p) {
       if (vscale != vscale)  // a block with a NaN among its values: its keys' scores are NaN
         kscale = vscale;
       else
-        v = scale_log2(vscale);
+        v = scale_log2(vscale), vrest = vscale * pow2f(-v);
 #pragma unroll
       for (int j = 0; j < L::kKChunks; ++j) {
         uint32_t w[2 * kHalves][4];
@@ -447,7 +448,7 @@ kv8_attn_kernel(Kv8Attn p) {
         mx[r] = x[r][0];
 #pragma unroll
         for (int i = 1; i < kX; ++i) mx[r] = fmaxf(mx[r], x[r][i]);  // NaN is passed over
-        mx[r] += (float)max(v, kMinValueScale);
+        mx[r] += (float)max(v + (vrest > 1.f ? 1 : 0), kMinValueScale);
       } else {
         mx[r] = -INFINITY;
 #pragma unroll
@@ -484,7 +485,7 @@ kv8_attn_kernel(Kv8Attn p) {
     uint32_t pa[kHalves][4];
     const float base0 = (m[0] == -INFINITY ? 0.f : m[0]) - kPShift, base1 = (m[1] == -INFINITY ? 0.f : m[1]) - kPShift;
     if (coded) {
-      const float vh = (float)max(v, 0), pm = pow2f(min(v, 0)), em = pow2f(-max(v, 0));
+      const float vh = (float)max(v, 0), pm = pow2f(min(v, 0)) * vrest, em = pow2f(-max(v, 0));
       float sum[2] = {0.f, 0.f};
       if constexpr (Narrow) {
 #pragma unroll

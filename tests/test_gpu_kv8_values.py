@@ -265,6 +265,27 @@ def test_every_shape_to_the_row(ops, b, hq, hkv, d, block, sealed, tail, rows, m
     assert kb.lse_off(lse, want) is None, kb.lse_off(lse, want)
 
 
+@pytest.mark.parametrize("hq,rows,d", FEW + MANY)
+def test_scales_that_are_no_powers_of_two(ops, hq, rows, d):
+    """Codes of another maker, scaled by their largest value over 448."""
+    sealed, block = 512, 64
+    g = torch.Generator().manual_seed(21)
+    q = torch.randn(1, hq, rows, d, generator=g).to(torch.bfloat16).to(DEV)
+    codes, scales = [], []
+    for _ in range(2):
+        x = torch.randn(1, 1, sealed // block, block, d, generator=g) * torch.rand(1, 1, sealed // block, 1, 1, generator=g)
+        s = x.abs().amax((3, 4)) / 448
+        codes.append((x / s[..., None, None]).reshape(1, 1, sealed, d).to(ref.E4M3).to(DEV))
+        scales.append(s.to(DEV))
+    none = torch.zeros(1, 1, 0, d, dtype=torch.bfloat16, device=DEV)
+    cache = ops.Kv8Rows(*codes, *scales, sealed, none, none, block)
+    vis = torch.rand(1, rows, sealed, generator=g) < 0.8
+    compare(ops, q, cache, vis)
+    out, lse = ops.kv8_tree_attention(q, cache, None, sealed, return_lse=True)
+    want = kb.attention(q, *opened(cache), torch.ones_like(vis).to(DEV), d ** -0.5)
+    assert kb.off(out, want) is None and kb.lse_off(lse, want) is None
+
+
 def nodes_of(call):
     """Kernels of a captured call."""
     import ctypes
