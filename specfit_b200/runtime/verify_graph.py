@@ -118,9 +118,9 @@ class VerifyGraph:
     def replay(self) -> torch.Tensor:
         """Runs the captured pass on the loaded inputs; returns the device
         argmax over the vocabulary per verification position."""
-        for layer, (buffers, *rows) in self._held:
-            now, *rows_now = layer.layout()
-            if rows_now != rows or any(a is not b for a, b in zip(now, buffers)):
+        for layer, (buffers, sealed, tail) in self._held:  # rows behind the captured ones are written over
+            now, sealed_now, tail_now = layer.layout()
+            if sealed_now != sealed or tail_now < tail or any(a is not b for a, b in zip(now, buffers)):
                 raise RuntimeError("the cache is not laid out as it was captured: roll it back to the captured "
                                    "length, or, if a pass has replaced its buffers, capture anew")
         self.graph.replay()

@@ -219,8 +219,12 @@ def test_a_replay_over_replaced_buffers_is_refused(target):
     with pytest.raises(RuntimeError, match="laid out"):
         g.replay()
     cache.crop(100)
+    run(fwd, state, cache, ids[:, :1])  # the tail is the usual one again
+    cache.crop(100)
     again = VerifyGraph(m.model, cache, q_len=8, device=DEV, forward=fwd)
     again.capture(*inputs)
+    assert torch.equal(again.replay(), want)
+    run(fwd, state, cache, ids[:, :5])  # rows that the replay writes over
     assert torch.equal(again.replay(), want)
 
 
