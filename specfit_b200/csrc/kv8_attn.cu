@@ -452,7 +452,8 @@ kv8_attn_kernel(Kv8Attn p) {
       } else {
         mx[r] = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kX; ++i) mx[r] = fmaxf(mx[r], x[r][i] + fmaxf(tail_v[warp][key_of(i)], (float)kMinValueScale));
+        for (int i = 0; i < kX; ++i)
+          mx[r] = fmaxf(mx[r], x[r][i] + fmaxf(tail_v[warp][key_of(i)], (float)kMinValueScale));
       }
       grow |= mx[r] > m[r] + kSlack;  // m -infinity: any score
     }

@@ -357,15 +357,21 @@ struct Regions {
            int64_t rs = 0) {
     r[n++] = Region{at, extent, {b, h, rows}, {bs, hs, rs}};
   }
-  // The buffers of a cache: codes and scales of `tokens` tokens from token `first` on, and `tail` rows.
-  void add_cache(const sf_kv8_rows& c, int64_t first, int64_t tokens, int64_t tail) {
+  // The buffers of a cache: codes and scales of `tokens` tokens from token `first` on, and
+  // `tail` rows.  `one`: keys and values are the same data, so their buffers may be
+  // the same too (written twice with one content).
+  void add_cache(const sf_kv8_rows& c, int64_t first, int64_t tokens, int64_t tail, bool one = false) {
     const int64_t b = c.batch, h = c.num_kv_heads, d = c.head_dim, blocks = tokens / c.block_tokens;
     for (int v = 0; v < 2; ++v) {
       const char* codes = static_cast<const char*>(v ? c.v_codes : c.k_codes);
       const float* scale = v ? c.v_scale : c.k_scale;
-      if (codes) add(codes + first * d, tokens * d, b, c.code_batch_stride, h, c.code_head_stride);
-      if (scale) add(scale + first / c.block_tokens, blocks * 4, b, c.scale_batch_stride * 4, h, c.scale_head_stride * 4);
-      add(v ? c.v_tail : c.k_tail, tail * d * 2, b, c.tail_batch_stride * 2, h, c.tail_head_stride * 2);
+      const void* rows = v ? c.v_tail : c.k_tail;
+      const bool again = one && v;
+      if (codes && !(again && codes == c.k_codes))
+        add(codes + first * d, tokens * d, b, c.code_batch_stride, h, c.code_head_stride);
+      if (scale && !(again && scale == c.k_scale))
+        add(scale + first / c.block_tokens, blocks * 4, b, c.scale_batch_stride * 4, h, c.scale_head_stride * 4);
+      if (!(again && rows == c.k_tail)) add(rows, tail * d * 2, b, c.tail_batch_stride * 2, h, c.tail_head_stride * 2);
     }
   }
 };
@@ -409,7 +415,7 @@ extern "C" int sf_kv8_seal(const void* k, const void* v, int64_t batch_stride, i
   SF_CHECK_ARG(aligned16(k) && aligned16(v) && batch_stride % 8 == 0 && head_stride % 8 == 0 && row_stride % 8 == 0,
                "k/v rows must be 16-byte aligned");
   Regions to, from;
-  to.add_cache(*rows, first_block * rows->block_tokens, blocks * rows->block_tokens, 0);
+  to.add_cache(*rows, first_block * rows->block_tokens, blocks * rows->block_tokens, 0, k == v);
   for (const void* p : {k, v})
     from.add(p, rows->head_dim * 2, rows->batch, batch_stride * 2, rows->num_kv_heads, head_stride * 2,
              blocks * rows->block_tokens, row_stride * 2);
@@ -460,7 +466,9 @@ extern "C" int sf_kv8_compact(const sf_kv8_rows* rows, const int32_t* keep, int6
                                                                    mass_out_head_stride, n)),
                "requests and heads of the target must not overlap");
   Regions to, from;
-  to.add_cache(*out, 0, out->sealed, out->tail);
+  to.add_cache(*out, 0, out->sealed, out->tail,
+               (rows->sealed == 0 || (rows->k_codes == rows->v_codes && rows->k_scale == rows->v_scale)) &&
+                   (rows->tail == 0 || rows->k_tail == rows->v_tail));
   to.add(mass_out, n * 4, out->batch, mass_out_batch_stride * 4, out->num_kv_heads, mass_out_head_stride * 4);
   from.add_cache(*rows, 0, rows->sealed, rows->tail);
   from.add(mass, (rows->sealed + rows->tail) * 4, out->batch, mass_batch_stride * 4, out->num_kv_heads,

@@ -744,7 +744,8 @@ def kv8_seal(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, v_codes: t
     st = k.stride()
     kp, vp = k.data_ptr(), v.data_ptr()
     if st[3] != 1 or (st[0] | st[1] | st[2]) & 7 or (kp | vp) & 15 or v.stride() != st:
-        k, v = k.contiguous(), v.contiguous()
+        one, k = v is k, k.contiguous()
+        v = k if one else v.contiguous()
         st, kp, vp = k.stride(), k.data_ptr(), v.data_ptr()
     n = ks[2] // block
     with _on(index):

@@ -359,3 +359,26 @@ def test_values_of_zeros_alone(ops, hq, hkv, rows, d):
     x = torch.einsum("bhgrd,bhkd->bhgrk", q.double().view(1, hkv, -1, rows, d), k.double()) * d ** -0.5
     assert float(out.abs().max()) == 0
     assert float((lse.double() - torch.logsumexp(x, -1).view_as(lse)).abs().max()) <= 2e-4
+
+
+def test_keys_that_are_the_values(ops):
+    """One content in one place: sealed, compacted and read back."""
+    g = torch.Generator().manual_seed(22)
+    x = torch.randn(1, 96, 2, 64, generator=g).to(torch.bfloat16).to(DEV).permute(0, 2, 1, 3)[:, :, :, ::1]
+    codes = torch.zeros(1, 2, 96, 64, device=DEV).to(ref.E4M3)
+    scale = torch.zeros(1, 2, 3, device=DEV)
+    for rows in (x, torch.stack([x, x], -1)[..., 0]):  # in place, and copied to be contiguous
+        ops.kv8_seal(rows, rows, codes, codes, scale, scale)
+        want, wscale = ref.seal(x.cpu(), 32)
+        assert torch.equal(codes.cpu().double(), want) and torch.equal(scale.cpu().double(), wscale)
+    none = torch.zeros(1, 2, 0, 64, dtype=torch.bfloat16, device=DEV)
+    cache = ops.Kv8Rows(codes, codes, scale, scale, 96, none, none, 32)
+    keep = torch.arange(0, 96, 2, dtype=torch.int32, device=DEV).expand(1, 2, 48).contiguous()
+    oc, os = torch.zeros(1, 2, 32, 64, device=DEV).to(ref.E4M3), torch.zeros(1, 2, 1, device=DEV)
+    ot = torch.zeros(1, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    new, _ = ops.kv8_compact(cache, keep, out=ops.Kv8Rows(oc, oc, os, os, 32, ot, ot, 32))
+    k, v = ops.kv8_read(new)
+    old, _ = ops.kv8_read(cache)
+    kept = old[:, :, ::2]
+    assert torch.equal(k, v) and torch.equal(k[:, :, 32:], kept[:, :, 32:])
+    assert float((k[:, :, :32].float() - kept[:, :, :32].float()).abs().max()) <= 2.0 ** -10 * float(os.max())

@@ -135,3 +135,18 @@ def test_sealing():
     assert refused(seal(wide[:, :, :64], other, one, 0, 2))
     assert refused(seal(wide[:, :, 31:95], other, one, 0, 2))
     assert not refused(seal(wide[:, :, 32:96], other, one, 0, 2))
+
+
+def test_keys_that_are_the_values_may_share_their_buffers():
+    """One content, written twice: both sides must be one."""
+    k, v = (torch.zeros(B, H, 64, D, dtype=torch.bfloat16) for _ in range(2))
+    one = Buffers(128, 10)
+    one.codes[1], one.scales[1], one.tails[1] = one.codes[0], one.scales[0], one.tails[0]
+    assert not refused(seal(k, k, one, 0, 2))
+    assert refused(seal(k, v, one, 0, 2))
+    keep = torch.zeros(B, H, 70, dtype=torch.int32)
+    out = Buffers(64, 10)
+    out.codes[1], out.scales[1], out.tails[1] = out.codes[0], out.scales[0], out.tails[0]
+    assert not refused(compact(one.of(128, 10), out.of(64, 6), 70, keep))
+    one.tails[1] = torch.zeros_like(one.tails[0])
+    assert refused(compact(one.of(128, 10), out.of(64, 6), 70, keep))
