@@ -590,9 +590,13 @@ kv8_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_k, Kv8Attn p, Kv8Prep 
       // Ring of four: block b - 4's softmax is over.  (The scores that freed this
       // stage, block b - 2's, were issued after P V of the lane's block before.)
       const float kf = ks * p.scale_log2;
-      // log2 of a power of two is exact, the inverse too.
-      const float mantissa = __uint_as_float((__float_as_uint(vs) & 0x7fffffu) | 0x3f800000u);
-      const float v = (float)(scale_log2(vs) + (int)kPShift) + log2f(mantissa), s128 = vs * 0x1p7f, inv = 1.f / s128;
+      float v = (float)(scale_log2(vs) + (int)kPShift), s128 = vs * 0x1p7f, inv;
+      if (const uint32_t mantissa = __float_as_uint(vs) & 0x7fffffu) {
+        v += log2f(__uint_as_float(mantissa | 0x3f800000u));
+        inv = 1.f / s128;
+      } else {
+        inv = pow2f(-(int)v);
+      }
       tail->key[b & 3][ct] =
           make_float4(kf, fmaxf(v, (float)kMinValueScale), v < 0.f ? s128 : 1.f, v > 0.f ? inv : 1.f);
       if (lane == 0) tail->group[b & 3][ct >> 5] = make_float4(kf, v, inv, 0.f);
