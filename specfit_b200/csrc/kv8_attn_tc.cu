@@ -55,7 +55,7 @@
 //     with 64, 72 and 96 bytes took 410, 519 and 657 us in the case below).  Hence one path of little code for
 //     whole blocks of codes, and a rolled one, key by key, for what is masked, tail
 //     or far apart in scale; half a block that no row of a warp sees is passed over.
-// What it measured: 1,000 rows of 32 heads over 17,391 tokens 395 us, 700
+// What it measured: 1,000 rows of 32 heads over 17,391 tokens 396 us, 700
 // TFLOP/s; 8 requests of 65 rows over 4,161 tokens 85 us.  A block of two lanes
 // takes about 5,400 clocks, the MMAs 2,050 and the exponentials 2,050 of them;
 // what bounds it is the chain of one lane (scores, 64 exponentials a thread,
