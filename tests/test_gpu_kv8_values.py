@@ -382,3 +382,40 @@ def test_keys_that_are_the_values(ops):
     kept = old[:, :, ::2]
     assert torch.equal(k, v) and torch.equal(k[:, :, 32:], kept[:, :, 32:])
     assert float((k[:, :, :32].float() - kept[:, :, :32].float()).abs().max()) <= 2.0 ** -10 * float(os.max())
+
+
+@pytest.mark.parametrize("hq,hkv,rows,sealed,tail", [(16, 2, 65, 1024, 65), (8, 1, 9, 320, 33)])
+def test_many_rows_replayed_and_on_several_streams(ops, hq, hkv, rows, sealed, tail):
+    """Captured once, replayed with other queries; and on three streams at once."""
+    total = sealed + tail
+    q, k, v = draw(2, hq, hkv, rows, total, 128, 23)
+    cache = sealed_cache(ops, k, v, sealed, 64)
+    vis = torch.ones(2, rows, total, dtype=torch.bool)
+    vis[:, :, total - rows:] = torch.ones(rows, rows, dtype=torch.bool).tril()
+    bits = pack(vis)
+    inputs = [q, q.flip(2).contiguous(), -q]
+
+    def call(x):
+        out, lse = ops.kv8_tree_attention(x, cache, bits, 0, return_lse=True)
+        return out, lse, ops.kv8_attention_mass(x, lse, cache, bits, 0, torch.zeros(2, hkv, total, device=DEV))
+
+    want = [call(x) for x in inputs]
+    x = q.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call(x)
+    for i in (1, 0, 2, 1):
+        x.copy_(inputs[i])
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(held, want[i])), i
+    streams = [torch.cuda.Stream() for _ in inputs]
+    got = [[] for _ in inputs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(inputs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in range(3) for g in got[i] for a, b in zip(g, want[i]))
